@@ -242,6 +242,99 @@ int mlpk_peer_free(void* buf);
 int mlpk_peer_allreduce(void* const* bufs, int world, int rank, int64_t n, float* dW_out,
                         mlpk_stream_t stream);
 
+/* ---- Operators of a block around the MLP.  No counterpart in the reference,
+ * whose users leave it for these: the norm before the MLP, the rows of a
+ * mixture of MLPs sorted by expert and back, and the optimizer's step.  Types
+ * of values: MLPK_DT_F16, MLPK_DT_F32, MLPK_DT_BF16.  Pointers are 16-byte
+ * aligned unless said otherwise, tensors contiguous. */
+#define MLPK_DT_BF16 2
+
+/* Root-mean-square norm of each row, with the residual's addition:
+ * h = x + residual, y = h / sqrt(mean(h^2) + eps) * weight, in fp32 from the
+ * loads on.  x, residual, y, h: [rows][width] of dtype; weight: [width] of dtype
+ * or fp32 (NULL: ones); residual NULL: h = x, and h may be NULL; rstd: [rows],
+ * what the backward needs, or NULL.  width is 1 to 32768. */
+int mlpk_rms_norm(int64_t rows, int width, int dtype, const void* x, const void* residual, const void* weight,
+                  int w_dtype, float eps, void* y, void* h, float* rstd, mlpk_stream_t stream);
+/* The same with an 8-bit output: q = e4m3(y / scale), scale = max|y| / 448 over
+ * the row (group 0) or over each 128 columns (group 128; the last may be
+ * shorter).  q: [rows][width]; scale: fp32 [rows][1 or ceil(width / 128)].  A
+ * group whose scale would be below the smallest normal number is all zeros. */
+int mlpk_rms_norm_fp8(int64_t rows, int width, int dtype, const void* x, const void* residual, const void* weight,
+                      int w_dtype, float eps, int group, void* q, float* scale, void* h, mlpk_stream_t stream);
+/* Backward of mlpk_rms_norm: from h, rstd and the gradients of y and h (grad_h
+ * NULL: none), dx (the gradient of x and of the residual) and dw ([width] of
+ * w_dtype, summed over the rows in fp32 in a fixed order; NULL: not wanted).
+ * workspace: mlpk_rms_norm_bwd_workspace_size bytes, only for dw
+ * (MLPK_ERR_SCRATCH if smaller). */
+int64_t mlpk_rms_norm_bwd_workspace_size(int64_t rows, int width, int dtype);
+int mlpk_rms_norm_bwd(int64_t rows, int width, int dtype, const void* h, const float* rstd, const void* weight,
+                      int w_dtype, const void* grad_y, const void* grad_h, void* dx, void* dw, void* workspace,
+                      int64_t workspace_bytes, mlpk_stream_t stream);
+
+/* Stable order of slots by expert: ids[slots] (int32 or int64, id_bytes 4 or
+ * 8), row_of[i] = the place of slot i when the slots are ordered by expert and
+ * then by i, offsets[experts + 1]: the first row of each expert, and at last the
+ * number of rows kept.  A slot whose id is outside [0, experts) is dropped: its
+ * place is behind the rows kept.  experts is 1 to 1024, slots below 2^31. */
+int64_t mlpk_expert_sort_workspace_size(int64_t slots, int experts);
+int mlpk_expert_sort(int64_t slots, int experts, const void* ids, int id_bytes, int32_t* row_of, int32_t* offsets,
+                     void* workspace, int64_t workspace_bytes, mlpk_stream_t stream);
+/* Slot t * top + k is token t's k-th choice; kept points to offsets[experts]
+ * (device memory).  xs[row_of[t, k]] = x[t]; rows of dropped slots are zero.
+ * x: [tokens][width], xs: [tokens * top][width] of dtype. */
+int mlpk_expert_dispatch(int64_t tokens, int top, int width, int dtype, const void* x, const int32_t* row_of,
+                         const int32_t* kept, void* xs, mlpk_stream_t stream);
+/* out[t] = sum over k of weights[t, k] * y[row_of[t, k]], in fp32 in the order
+ * of k; dropped slots add nothing and their rows of y are not read.  weights:
+ * [tokens][top] of dtype or fp32, any alignment (NULL: ones; with y the
+ * gradient of xs this is the backward of mlpk_expert_dispatch). */
+int mlpk_expert_combine(int64_t tokens, int top, int width, int dtype, const void* y, const void* weights, int w_dtype,
+                        const int32_t* row_of, const int32_t* kept, void* out, mlpk_stream_t stream);
+/* Backward of mlpk_expert_combine: dy[row_of[t, k]] = weights[t, k] *
+ * grad_out[t] (zero in the dropped slots' rows), dw[t, k] = <grad_out[t],
+ * y[row_of[t, k]]> (zero for dropped slots), of w_dtype.  Either may be NULL. */
+int mlpk_expert_combine_bwd(int64_t tokens, int top, int width, int dtype, const void* grad_out, const void* y,
+                            const void* weights, int w_dtype, const int32_t* row_of, const int32_t* kept, void* dy,
+                            void* dw, mlpk_stream_t stream);
+
+/* One AdamW step over `count` tensors (one launch for each 768 of them):
+ *   m = beta1 m + (1 - beta1) g; v = beta2 v + (1 - beta2) g^2;
+ *   p = p (1 - lr weight_decay)
+ *       - lr / (1 - beta1^t) * m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
+ * in fp32.  The state of all tensors lies in flat buffers; tensor i's begins at
+ * element state_off[i], a multiple of MLPK_ADAMW_BLOCK, and is padded to a
+ * multiple of it (the padding is zero and stays so).  bits 32: exp_avg and
+ * exp_avg_sq are fp32.  bits 8: exp_avg is e4m3 m and exp_avg_sq e4m3 sqrt(v),
+ * each block of MLPK_ADAMW_BLOCK elements times its scale (max / 448).  master:
+ * fp32 copies of 16-bit parameters, which the step reads and writes beside
+ * them, or NULL.  Parameters and gradients: p_dtype and g_dtype (p_dtype or
+ * fp32), of any alignment (16 bytes are fastest).  ticks[tick[i]]: tensor i's
+ * step count, times ceil(numel / MLPK_ADAMW_CHUNK); the step adds to it on the
+ * device.  Device scalars, each may be NULL: lr_ptr replaces lr; the gradients
+ * are divided by grad_scale; a found_inf that is not 0 skips the whole step. */
+#define MLPK_ADAMW_BLOCK 256
+#define MLPK_ADAMW_CHUNK 4096
+typedef struct mlpk_adamw_state {
+  int32_t bits;
+  void* exp_avg;
+  void* exp_avg_sq;
+  float* exp_avg_scale;
+  float* exp_avg_sq_scale;
+  float* master;
+  int64_t* ticks;
+} mlpk_adamw_state;
+typedef struct mlpk_adamw_args {
+  double lr, beta1, beta2, eps, weight_decay;
+  int32_t maximize;
+  const float* lr_ptr;
+  const float* grad_scale;
+  const float* found_inf;
+} mlpk_adamw_args;
+int mlpk_adamw_step(int count, const int64_t* numel, void* const* params, const void* const* grads,
+                    const int64_t* state_off, const int32_t* tick, int p_dtype, int g_dtype,
+                    const mlpk_adamw_state* state, const mlpk_adamw_args* args, mlpk_stream_t stream);
+
 /* Text of the CUDA runtime / driver failure behind the calling thread's most
  * recent MLPK_ERR_CUDA ("no error" if none).  The reference reports failures as
  * Python exceptions carrying the CUDA message (cutile_mlp.py:388); this is the

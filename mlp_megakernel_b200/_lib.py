@@ -39,6 +39,20 @@ class MlpkShape(ctypes.Structure):
 _SHAPE_P = ctypes.POINTER(MlpkShape)
 _VPP = ctypes.POINTER(ctypes.c_void_p)
 
+
+class MlpkAdamwState(ctypes.Structure):
+    _fields_ = [("bits", ctypes.c_int32), ("exp_avg", _vp), ("exp_avg_sq", _vp), ("exp_avg_scale", _vp),
+                ("exp_avg_sq_scale", _vp), ("master", _vp), ("ticks", _vp)]
+
+
+class MlpkAdamwArgs(ctypes.Structure):
+    _fields_ = [("lr", ctypes.c_double), ("beta1", ctypes.c_double), ("beta2", ctypes.c_double),
+                ("eps", ctypes.c_double), ("weight_decay", ctypes.c_double), ("maximize", ctypes.c_int32),
+                ("lr_ptr", _vp), ("grad_scale", _vp), ("found_inf", _vp)]
+
+
+_i32, _i64, _f32 = ctypes.c_int, ctypes.c_int64, ctypes.c_float
+
 SIGNATURES = {
     "mlpk_status_string": (ctypes.c_char_p, [ctypes.c_int]),
     "mlpk_shape_supported": (ctypes.c_int, [_SHAPE_P]),
@@ -70,12 +84,29 @@ SIGNATURES = {
     "mlpk_fwd_host_workspace_size": (ctypes.c_int64, [_SHAPE_P, ctypes.c_int64]),
     "mlpk_fwd_host": (ctypes.c_int, [_SHAPE_P, ctypes.c_int64, _vp, _VPP, _vp, ctypes.c_int64, _vp,
                                      ctypes.c_int64, _vp]),
+    "mlpk_rms_norm": (_i32, [_i64, _i32, _i32, _vp, _vp, _vp, _i32, _f32, _vp, _vp, _vp, _vp]),
+    "mlpk_rms_norm_fp8": (_i32, [_i64, _i32, _i32, _vp, _vp, _vp, _i32, _f32, _i32, _vp, _vp, _vp, _vp]),
+    "mlpk_rms_norm_bwd_workspace_size": (_i64, [_i64, _i32, _i32]),
+    "mlpk_rms_norm_bwd": (_i32, [_i64, _i32, _i32, _vp, _vp, _vp, _i32, _vp, _vp, _vp, _vp, _vp, _i64, _vp]),
+    "mlpk_expert_sort_workspace_size": (_i64, [_i64, _i32]),
+    "mlpk_expert_sort": (_i32, [_i64, _i32, _vp, _i32, _vp, _vp, _vp, _i64, _vp]),
+    "mlpk_expert_dispatch": (_i32, [_i64, _i32, _i32, _i32, _vp, _vp, _vp, _vp, _vp]),
+    "mlpk_expert_combine": (_i32, [_i64, _i32, _i32, _i32, _vp, _vp, _i32, _vp, _vp, _vp, _vp]),
+    "mlpk_expert_combine_bwd": (_i32, [_i64, _i32, _i32, _i32, _vp, _vp, _vp, _i32, _vp, _vp, _vp, _vp, _vp]),
+    "mlpk_adamw_step": (_i32, [_i32, _vp, _vp, _vp, _vp, _vp, _i32, _i32, ctypes.POINTER(MlpkAdamwState),
+                               ctypes.POINTER(MlpkAdamwArgs), _vp]),
 }
 FWD_HOST_CHUNK_ROWS = 131072
 H_F16 = 0  # MLPK_H_F16: saved activations in fp16
 H_F32 = 1  # MLPK_H_F32: saved activations in fp32 (the reference's storage)
 DT_F16 = 0  # MLPK_DT_F16: fp16 operands
 DT_F32 = 1  # MLPK_DT_F32: fp32 operands on tf32 tensor cores
+DT_BF16 = 2  # MLPK_DT_BF16: bf16 values (the block operators)
+ADAMW_BLOCK = 256  # MLPK_ADAMW_BLOCK: elements that share a scale of the 8-bit state
+ADAMW_CHUNK = 4096  # MLPK_ADAMW_CHUNK: elements of a tensor's step-count unit
+EXPERT_MAX = 1024
+NORM_MAX_WIDTH = 32768
+NORM_GROUP = 128  # columns that share a scale of the 8-bit norm
 PEER_HANDLE_BYTES = 64
 PEER_MAX_RANKS = 8
 

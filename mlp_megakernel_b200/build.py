@@ -6,6 +6,7 @@ with the source tree; nothing is installed into site-packages.
 """
 from __future__ import annotations
 
+import concurrent.futures
 import os
 import shutil
 import subprocess
@@ -17,15 +18,20 @@ CSRC = os.path.join(HERE, "csrc")
 LIBDIR = os.path.join(HERE, "lib")
 LIB = os.path.join(LIBDIR, "libmlpk.so")
 
-SOURCES = ["mlpk_api.cu"]
-DEPS = ["ptx.cuh", "layout.cuh", "softplus.cuh", "fwd_kernel.cuh",
-        "bwd_kernel.cuh", "wn_kernel.cuh", "stream_kernel.cuh", "wgrad_kernel.cuh", "peer_kernel.cuh", "cast_kernel.cuh"]
+# Each translation unit with the headers it is built from.
+SOURCES = {
+    "mlpk_api.cu": ["host.cuh", "pdl.cuh", "ptx.cuh", "layout.cuh", "softplus.cuh", "fwd_kernel.cuh", "bwd_kernel.cuh",
+                    "wn_kernel.cuh", "stream_kernel.cuh", "wgrad_kernel.cuh", "peer_kernel.cuh", "cast_kernel.cuh"],
+    "norm_api.cu": ["host.cuh", "pdl.cuh", "vec.cuh", "norm_kernel.cuh"],
+    "expert_api.cu": ["host.cuh", "pdl.cuh", "vec.cuh", "expert_kernel.cuh"],
+    "adamw_api.cu": ["host.cuh", "pdl.cuh", "vec.cuh", "adamw_kernel.cuh"],
+}
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-O3", "-lineinfo", "-std=c++17",
     "--expt-relaxed-constexpr",
-    "-Xcompiler", "-fPIC", "-shared",
+    "-Xcompiler", "-fPIC",
     "-diag-suppress", "20013",
 ]
 
@@ -37,14 +43,25 @@ def nvcc_path() -> str:
     raise RuntimeError("nvcc not found; the CUDA library cannot be built")
 
 
-def _stale() -> bool:
-    if not os.path.exists(LIB):
+def _inputs(source: str) -> list:
+    return [os.path.join(CSRC, f) for f in [source, *SOURCES[source]]] + \
+        [os.path.join(ROOT, "include", "mlpk.h"), os.path.abspath(__file__)]
+
+
+def _object(source: str) -> str:
+    return os.path.join(LIBDIR, source[:-3] + ".o")
+
+
+def _newer(files, target: str) -> bool:
+    """Whether the target is missing or older than one of the files."""
+    if not os.path.exists(target):
         return True
-    t = os.path.getmtime(LIB)
-    files = [os.path.join(CSRC, f) for f in SOURCES + DEPS]
-    files.append(os.path.join(ROOT, "include", "mlpk.h"))
-    files.append(os.path.abspath(__file__))
+    t = os.path.getmtime(target)
     return any(os.path.getmtime(f) > t for f in files if os.path.exists(f))
+
+
+def _stale() -> bool:
+    return any(_newer(_inputs(s), LIB) for s in SOURCES)
 
 
 DEVTEST_SRC = os.path.join(ROOT, "tests", "device_api", "devtest.cu")
@@ -55,12 +72,12 @@ def build_devtest(force: bool = False, verbose: bool = False) -> str:
     """Compile the device-API test kernels (tests/device_api/devtest.cu, a
     user kernel calling include/mlpk_device.cuh) if missing or stale."""
     deps = [DEVTEST_SRC, os.path.join(ROOT, "include", "mlpk_device.cuh")] + \
-        [os.path.join(CSRC, f) for f in DEPS + ["device_mlp.cuh"]]
+        [os.path.join(CSRC, f) for f in SOURCES["mlpk_api.cu"] + ["device_mlp.cuh"]]
     if not force and os.path.exists(DEVTEST_LIB) and \
             all(os.path.getmtime(f) <= os.path.getmtime(DEVTEST_LIB) for f in deps if os.path.exists(f)):
         return DEVTEST_LIB
     tmp = DEVTEST_LIB + ".tmp"
-    cmd = [nvcc_path(), *NVCC_FLAGS, "-o", tmp, DEVTEST_SRC]
+    cmd = [nvcc_path(), *NVCC_FLAGS, "-shared", "-o", tmp, DEVTEST_SRC]
     if verbose:
         print(" ".join(cmd), file=sys.stderr)
     res = subprocess.run(cmd, capture_output=True, text=True)
@@ -70,24 +87,37 @@ def build_devtest(force: bool = False, verbose: bool = False) -> str:
     return DEVTEST_LIB
 
 
-def build(force: bool = False, verbose: bool = False, ptxas_info: bool = False) -> str:
-    """Compile libmlpk.so if missing or older than its sources; return its path."""
-    if not force and not _stale():
-        return LIB
-    os.makedirs(LIBDIR, exist_ok=True)
-    tmp = LIB + ".tmp"
-    cmd = [nvcc_path(), *NVCC_FLAGS]
-    if ptxas_info:
-        cmd += ["-Xptxas", "-v"]
-    cmd += ["-o", tmp] + [os.path.join(CSRC, s) for s in SOURCES]
+def _run(cmd, verbose: bool) -> str:
     if verbose:
         print(" ".join(cmd), file=sys.stderr)
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         raise RuntimeError("nvcc failed:\n" + res.stdout + res.stderr)
+    return res.stdout + res.stderr
+
+
+def _compile(source: str, verbose: bool, ptxas_info: bool) -> str:
+    obj = _object(source)
+    cmd = [nvcc_path(), *NVCC_FLAGS, *(["-Xptxas", "-v"] if ptxas_info else []), "-c",
+           "-o", obj + ".tmp", os.path.join(CSRC, source)]
+    said = _run(cmd, verbose)
+    os.replace(obj + ".tmp", obj)
+    return said
+
+
+def build(force: bool = False, verbose: bool = False, ptxas_info: bool = False) -> str:
+    """Compile the translation units of libmlpk.so that are older than their
+    sources, side by side, link the library if any was; return its path."""
+    if not force and not _stale():
+        return LIB
+    os.makedirs(LIBDIR, exist_ok=True)
+    todo = [s for s in SOURCES if force or _newer(_inputs(s), _object(s))]
+    with concurrent.futures.ThreadPoolExecutor(len(SOURCES)) as pool:
+        said = "".join(pool.map(lambda s: _compile(s, verbose, ptxas_info), todo))
+    said += _run([nvcc_path(), *NVCC_FLAGS, "-shared", "-o", LIB + ".tmp"] + [_object(s) for s in SOURCES], verbose)
     if verbose or ptxas_info:
-        sys.stderr.write(res.stdout + res.stderr)
-    os.replace(tmp, LIB)
+        sys.stderr.write(said)
+    os.replace(LIB + ".tmp", LIB)
     return LIB
 
 

@@ -17,6 +17,7 @@
 #include "../../include/mlpk.h"
 #include "bwd_kernel.cuh"
 #include "cast_kernel.cuh"
+#include "host.cuh"
 #include "stream_kernel.cuh"
 #include "peer_kernel.cuh"
 #include "wgrad_kernel.cuh"
@@ -27,15 +28,16 @@ namespace {
 using mlpk::FwdCfg;
 using mlpk::FwdMaps;
 using mlpk::Net;
+using mlpk::host::aligned16;
+using mlpk::host::cuda_status;
+using mlpk::host::current_device_info;
+using mlpk::host::DevInfo;
+using mlpk::host::launch_kernel;
+using mlpk::host::launch_kernel_cfg;
+using mlpk::host::launch_kernel_early;
 
 // ------------------------------------------------------------------ device
 constexpr int kMaxDevices = 64;
-struct DevInfo {
-  int sm_count = 0;
-  int major = 0;
-  int minor = 0;
-  bool valid = false;
-};
 DevInfo g_dev[kMaxDevices];
 std::mutex g_dev_mu;
 
@@ -43,52 +45,16 @@ std::mutex g_dev_mu;
 // mlpk_last_cuda_error).
 thread_local char t_last_cuda_error[160] = "no error";
 
+}  // namespace
+
+namespace mlpk {
+namespace host {
+
 int cuda_status(cudaError_t e) {
   if (e == cudaSuccess) return MLPK_OK;
   std::snprintf(t_last_cuda_error, sizeof(t_last_cuda_error), "%s: %s", cudaGetErrorName(e),
                 cudaGetErrorString(e));
   return MLPK_ERR_CUDA;
-}
-
-int driver_status(const char* what, int result) {
-  if (result == 0) return MLPK_OK;
-  std::snprintf(t_last_cuda_error, sizeof(t_last_cuda_error), "%s returned CUresult %d", what, result);
-  return MLPK_ERR_CUDA;
-}
-
-// Launch through cudaLaunchKernelEx so that the status returned is that of
-// THIS launch, not an error left earlier on the calling thread.  With `early`
-// the kernel is launched with programmatic stream serialization: it may start
-// while the kernel before it on the stream is still running (every kernel of
-// the library calls pdl_enter() before touching global memory, ptx.cuh), so
-// its setup overlaps that kernel's tail.  The inference forward launches this
-// way (back-to-back small calls: 6.0 -> 5.2 us per call at 64 rows); the
-// training kernels do not (the config-3 step measured 40.8 us at 16,384 rows
-// without it, 42.4 with it).
-template <typename... KArgs, typename... Args>
-int launch_kernel_cfg(bool early, void (*kern)(KArgs...), dim3 grid, unsigned block, size_t smem,
-                      cudaStream_t st, Args&&... args) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
-  cfg.blockDim = dim3(block, 1, 1);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = early ? 1 : 0;
-  return cuda_status(cudaLaunchKernelEx(&cfg, kern, std::forward<Args>(args)...));
-}
-template <typename... KArgs, typename... Args>
-int launch_kernel(void (*kern)(KArgs...), dim3 grid, unsigned block, size_t smem, cudaStream_t st,
-                  Args&&... args) {
-  return launch_kernel_cfg(false, kern, grid, block, smem, st, std::forward<Args>(args)...);
-}
-template <typename... KArgs, typename... Args>
-int launch_kernel_early(void (*kern)(KArgs...), dim3 grid, unsigned block, size_t smem, cudaStream_t st,
-                        Args&&... args) {
-  return launch_kernel_cfg(true, kern, grid, block, smem, st, std::forward<Args>(args)...);
 }
 
 int current_device_info(DevInfo* out, int* dev_out) {
@@ -117,6 +83,17 @@ int current_device_info(DevInfo* out, int* dev_out) {
   *out = d;
   if (dev_out) *dev_out = dev;
   return d.major == 10 ? MLPK_OK : MLPK_ERR_ARCH;
+}
+
+}  // namespace host
+}  // namespace mlpk
+
+namespace {
+
+int driver_status(const char* what, int result) {
+  if (result == 0) return MLPK_OK;
+  std::snprintf(t_last_cuda_error, sizeof(t_last_cuda_error), "%s returned CUresult %d", what, result);
+  return MLPK_ERR_CUDA;
 }
 
 // ------------------------------------------------------------------ TMA maps
@@ -158,8 +135,6 @@ int make_map_2d(CUtensorMap* map, const void* ptr, uint64_t inner, uint64_t oute
                    CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return driver_status("cuTensorMapEncodeTiled", static_cast<int>(r));
 }
-
-bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 // Raise a kernel's dynamic shared-memory limit once per (kernel, device).
 template <class Kern>

@@ -11,6 +11,8 @@
 #include <cuda.h>
 #include <cuda_fp16.h>
 
+#include "pdl.cuh"
+
 #ifndef MLPK_WAIT_TIMEOUT_NS
 #define MLPK_WAIT_TIMEOUT_NS 1000000000ull  // 1 s
 #endif
@@ -18,8 +20,8 @@
 namespace mlpk {
 
 // Device-global status word (0 = ok).  Set by bounded waits that expire.
-// The library is one translation unit (mlpk_api.cu includes every kernel), so
-// this is the single definition.
+// mlpk_api.cu is the one translation unit that includes this header (the
+// kernels of block_api.cu have no waits), so this is the single definition.
 __device__ int g_device_status = 0;
 
 enum DeviceStatus : int {
@@ -95,20 +97,6 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
       return false;
     }
   }
-}
-
-// ---------------------------------------------------------------- programmatic dependent launch
-// A kernel launched with programmatic stream serialization may start while
-// the kernel before it on the stream is still running, so every kernel of the
-// library calls pdl_enter() after its own setup (barrier init, TMEM
-// allocation: shared memory and TMEM only) and before its first access to
-// global memory.  griddepcontrol.wait returns once the grids it depends on
-// have completed and their memory operations are visible (at once when there
-// are none); launch_dependents lets the next kernel's CTAs start their own
-// setup as SMs free up (they wait in turn before touching memory).
-__device__ __forceinline__ void pdl_enter() {
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
 // ---------------------------------------------------------------- fences

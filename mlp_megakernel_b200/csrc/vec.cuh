@@ -1,0 +1,91 @@
+// Element types and vector access of the block kernels (norm, experts,
+// AdamW): fp16, bf16 and fp32 values are held as fp32 in registers; a vector
+// is 16 bytes where the row allows it, else one element.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+
+#include <cstdint>
+
+namespace mlpk {
+
+__device__ __forceinline__ float to_float(float v) { return v; }
+__device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+
+// Round to nearest even.
+template <class T>
+__device__ __forceinline__ T from_float(float v);
+template <>
+__device__ __forceinline__ float from_float<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+// Elements of a 16-byte vector.
+template <class T>
+constexpr int kVecOf = 16 / static_cast<int>(sizeof(T));
+
+// VEC elements as they lie in memory.  VEC is 1, or any count whose bytes are
+// a multiple of 8 (the access is aligned to min(16, bytes)).
+template <class T, int VEC>
+struct alignas(VEC * sizeof(T) >= 16 ? 16 : VEC * sizeof(T)) Raw {
+  T v[VEC];
+};
+
+template <class T, int VEC>
+__device__ __forceinline__ Raw<T, VEC> load_raw(const T* p) {
+  return *reinterpret_cast<const Raw<T, VEC>*>(p);
+}
+
+template <class T, int VEC>
+__device__ __forceinline__ void unpack(const Raw<T, VEC>& r, float (&f)[VEC]) {
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) f[e] = to_float(r.v[e]);
+}
+
+template <class T, int VEC>
+__device__ __forceinline__ void store_vec(T* p, const float (&f)[VEC]) {
+  Raw<T, VEC> r;
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) r.v[e] = from_float<T>(f[e]);
+  *reinterpret_cast<Raw<T, VEC>*>(p) = r;
+}
+
+// The 8-bit type: 4 exponent bits, 3 of mantissa (e4m3), largest value 448,
+// smallest positive one 2^-9.
+constexpr float kFp8Max = 448.0f;
+constexpr float kFp8Tiny = 0.001953125f;
+
+// f rounded to e4m3 (to nearest even, NaN kept, |f| above 448 clipped).
+template <int VEC>
+__device__ __forceinline__ void store_fp8(uint8_t* p, const float (&f)[VEC]) {
+  if constexpr (VEC == 1) {
+    *p = __nv_cvt_float_to_fp8(f[0], __NV_SATFINITE, __NV_E4M3);
+  } else {
+    Raw<uint16_t, VEC / 2> r;
+#pragma unroll
+    for (int e = 0; e < VEC / 2; ++e)
+      r.v[e] = __nv_cvt_float2_to_fp8x2(make_float2(f[2 * e], f[2 * e + 1]), __NV_SATFINITE, __NV_E4M3);
+    *reinterpret_cast<Raw<uint16_t, VEC / 2>*>(p) = r;
+  }
+}
+
+// |v| as an unsigned whole number: ordered like |v|, with a NaN above
+// infinity, so a maximum over it keeps a NaN.
+__device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+
+// The scale of a group of 8-bit values whose largest magnitude has these
+// bits, and what to multiply by before the rounding.  A scale below the
+// smallest normal number has no finite reciprocal (and zero times infinity
+// would put NaN into the group's zeros): such a group is all zeros.
+__device__ __forceinline__ float fp8_scale(uint32_t amax_bits, float* inv) {
+  float scale = __uint_as_float(amax_bits) * (1.0f / kFp8Max);
+  if (scale < 1.17549435e-38f) scale = 0.0f;
+  *inv = scale > 0.0f ? 1.0f / scale : 0.0f;
+  return scale;
+}
+
+}  // namespace mlpk

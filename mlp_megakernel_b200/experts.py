@@ -1,0 +1,296 @@
+"""Rows sorted by expert and back, with weights applied, and a block of fused
+MLP experts (no counterpart in the reference, which has one MLP).
+
+* ``expert_sort(ids, num_experts)`` -- the plan of a batch: where each slot
+  (token, choice) lies when the slots are ordered by expert;
+* ``expert_dispatch(x, plan)`` -- each token's row copied to its slots' rows;
+* ``expert_combine(y, weights, plan)`` -- the weighted sum of its slots' rows
+  back at each token;
+* ``FusedMLPExperts`` -- norm, router, dispatch, a FusedMLPSoftplus for each
+  expert, combine.
+
+Rows are fp16, bf16 or fp32 of any width; sums are fp32 in a fixed order, so
+results are the same from run to run.  Everything runs on the current CUDA
+stream without a wait of the host; there is no CPU path.  Under torch.compile
+the calls are the operators ``torch.ops.mlpk.expert_*``; eager calls go straight
+to the C ABI.
+"""
+from __future__ import annotations
+
+import math
+from typing import NamedTuple, Optional
+
+import torch
+import torch.nn as nn
+from torch import Tensor
+
+from . import _lib
+from .functional import _current_stream, _is_fake
+from .modules import FusedMLPSoftplus
+from .norm import DTYPES, FusedRMSNorm, _needs_grad, _on_device, _ptr
+from .ops import _aligned
+
+
+class ExpertPlan(NamedTuple):
+    """Where the slots of a batch lie in the order by expert (int32, on the
+    GPU).  ``row_of[t, k]`` is the row of token t's k-th choice;
+    ``offsets[e]`` is expert e's first row and ``offsets[-1]`` the number of
+    rows kept.  Slots without an expert lie behind those."""
+
+    row_of: Tensor
+    offsets: Tensor
+
+    @property
+    def num_experts(self) -> int:
+        return self.offsets.shape[0] - 1
+
+    @property
+    def counts(self) -> Tensor:
+        """Rows of each expert."""
+        return self.offsets.diff()
+
+
+# ------------------------------------------------------------ kernels
+@_on_device
+def _sort(ids, num_experts):
+    ids = _aligned(ids)
+    slots = ids.numel()
+    lib = _lib.lib()
+    size = lib.mlpk_expert_sort_workspace_size(slots, num_experts)
+    row_of = torch.empty(ids.shape, device=ids.device, dtype=torch.int32)
+    offsets = torch.empty(num_experts + 1, device=ids.device, dtype=torch.int32)
+    work = torch.empty(max(size, 16), device=ids.device, dtype=torch.uint8)
+    _lib.check("mlpk_expert_sort", lib.mlpk_expert_sort(
+        slots, num_experts, ids.data_ptr(), ids.element_size(), row_of.data_ptr(), offsets.data_ptr(),
+        work.data_ptr(), work.numel(), _current_stream(ids.get_device())))
+    return row_of, offsets
+
+
+def _kept(offsets: Tensor) -> int:
+    return offsets.data_ptr() + 4 * (offsets.shape[0] - 1)
+
+
+@_on_device
+def _dispatch(x, row_of, offsets):
+    x, row_of = _aligned(x), _aligned(row_of)
+    T, K = row_of.shape
+    xs = torch.empty((T * K, x.shape[1]), device=x.device, dtype=x.dtype)
+    _lib.check("mlpk_expert_dispatch", _lib.lib().mlpk_expert_dispatch(
+        T, K, x.shape[1], DTYPES[x.dtype], x.data_ptr(), row_of.data_ptr(), _kept(offsets), xs.data_ptr(),
+        _current_stream(x.get_device())))
+    return xs
+
+
+@_on_device
+def _combine(y, weights, row_of, offsets):
+    y, row_of = _aligned(y), _aligned(row_of)
+    weights = None if weights is None else weights.contiguous()
+    T, K = row_of.shape
+    out = torch.empty((T, y.shape[1]), device=y.device, dtype=y.dtype)
+    _lib.check("mlpk_expert_combine", _lib.lib().mlpk_expert_combine(
+        T, K, y.shape[1], DTYPES[y.dtype], y.data_ptr(), _ptr(weights),
+        DTYPES[y.dtype if weights is None else weights.dtype], row_of.data_ptr(), _kept(offsets), out.data_ptr(),
+        _current_stream(y.get_device())))
+    return out
+
+
+@_on_device
+def _combine_bwd(grad_out, y, weights, row_of, offsets, want_dy, want_dw):
+    grad_out, y, row_of = _aligned(grad_out), _aligned(y), _aligned(row_of)
+    weights = None if weights is None else weights.contiguous()
+    T, K = row_of.shape
+    dy = torch.empty_like(y) if want_dy else None
+    dw = torch.empty_like(weights) if want_dw else None
+    _lib.check("mlpk_expert_combine_bwd", _lib.lib().mlpk_expert_combine_bwd(
+        T, K, y.shape[1], DTYPES[y.dtype], grad_out.data_ptr(), y.data_ptr(), _ptr(weights),
+        DTYPES[y.dtype if weights is None else weights.dtype], row_of.data_ptr(), _kept(offsets), _ptr(dy), _ptr(dw),
+        _current_stream(y.get_device())))
+    return dy, dw
+
+
+# ------------------------------------------------------------ torch.ops.mlpk
+def _require_cuda(*ts):
+    for t in ts:
+        if t is not None and not t.is_cuda:
+            raise RuntimeError("the expert operators run on CUDA (sm_100) only; got a CPU tensor")
+
+
+@torch.library.custom_op("mlpk::expert_sort", mutates_args=())
+def _sort_op(ids: Tensor, num_experts: int) -> list[Tensor]:
+    _require_cuda(ids)
+    return list(_sort(ids, num_experts))
+
+
+@_sort_op.register_fake
+def _sort_fake(ids, num_experts):
+    return [ids.new_empty(ids.shape, dtype=torch.int32), ids.new_empty((num_experts + 1,), dtype=torch.int32)]
+
+
+@torch.library.custom_op("mlpk::expert_dispatch", mutates_args=())
+def _dispatch_op(x: Tensor, row_of: Tensor, offsets: Tensor) -> Tensor:
+    _require_cuda(x, row_of, offsets)
+    return _dispatch(x, row_of, offsets)
+
+
+@_dispatch_op.register_fake
+def _dispatch_fake(x, row_of, offsets):
+    return x.new_empty((row_of.shape[0] * row_of.shape[1], x.shape[1]))
+
+
+@torch.library.custom_op("mlpk::expert_combine", mutates_args=())
+def _combine_op(y: Tensor, weights: Optional[Tensor], row_of: Tensor, offsets: Tensor) -> Tensor:
+    _require_cuda(y, weights, row_of, offsets)
+    return _combine(y, weights, row_of, offsets)
+
+
+@_combine_op.register_fake
+def _combine_fake(y, weights, row_of, offsets):
+    return y.new_empty((row_of.shape[0], y.shape[1]))
+
+
+@torch.library.custom_op("mlpk::expert_combine_bwd", mutates_args=())
+def _combine_bwd_op(grad_out: Tensor, y: Tensor, weights: Optional[Tensor], row_of: Tensor, offsets: Tensor,
+                    want_dy: bool, want_dw: bool) -> list[Tensor]:
+    """[dy] and / or [dw], as wanted."""
+    _require_cuda(grad_out, y, weights, row_of, offsets)
+    return [t for t in _combine_bwd(grad_out, y, weights, row_of, offsets, want_dy, want_dw) if t is not None]
+
+
+@_combine_bwd_op.register_fake
+def _combine_bwd_fake(grad_out, y, weights, row_of, offsets, want_dy, want_dw):
+    return ([y.new_empty(y.shape)] if want_dy else []) + ([weights.new_empty(weights.shape)] if want_dw else [])
+
+
+def _traced(t: Tensor) -> bool:
+    return torch.compiler.is_compiling() or _is_fake(t)
+
+
+# ------------------------------------------------------------ autograd
+class _DispatchFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, row_of, offsets):
+        ctx.save_for_backward(row_of, offsets)
+        return (torch.ops.mlpk.expert_dispatch if _traced(x) else _dispatch)(x, row_of, offsets)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        row_of, offsets = ctx.saved_tensors
+        return (torch.ops.mlpk.expert_combine if _traced(grad) else _combine)(grad, None, row_of, offsets), None, None
+
+
+class _CombineFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, y, weights, row_of, offsets):
+        ctx.has_weights = weights is not None
+        ctx.save_for_backward(y, row_of, offsets, *([weights] if ctx.has_weights else []))
+        return (torch.ops.mlpk.expert_combine if _traced(y) else _combine)(y, weights, row_of, offsets)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        y, row_of, offsets, *rest = ctx.saved_tensors
+        weights = rest[0] if rest else None
+        want_dy, want_dw = ctx.needs_input_grad[0], ctx.has_weights and ctx.needs_input_grad[1]
+        if _traced(grad):
+            got = torch.ops.mlpk.expert_combine_bwd(grad, y, weights, row_of, offsets, want_dy, want_dw)
+            dy, dw = (got[0] if want_dy else None), (got[-1] if want_dw else None)
+        else:
+            dy, dw = _combine_bwd(grad, y, weights, row_of, offsets, want_dy, want_dw)
+        return dy, dw, None, None
+
+
+# ------------------------------------------------------------ public calls
+def expert_sort(ids: Tensor, num_experts: int) -> ExpertPlan:
+    """The plan of a batch from the experts its tokens chose.
+
+    ``ids`` is an int32 or int64 CUDA tensor ``[tokens, choices]``; the order is
+    stable (by expert, then by token and choice).  A slot whose id is outside
+    ``[0, num_experts)`` -- -1 for a choice over its expert's capacity, say -- is
+    dropped: dispatch gives it a row of zeros behind the kept rows, combine
+    leaves it out.  At most 1024 experts and 2^31 - 1 slots.
+    """
+    if not isinstance(ids, Tensor) or ids.dim() != 2:
+        raise ValueError("ids must be a 2-D tensor [tokens, choices]")
+    _require_cuda(ids)
+    if ids.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"ids must be int32 or int64, got {ids.dtype}")
+    if not 1 <= num_experts <= _lib.EXPERT_MAX:
+        raise ValueError(f"num_experts must be 1 to {_lib.EXPERT_MAX}, got {num_experts}")
+    if ids.shape[1] < 1 or ids.numel() > 2 ** 31 - 1:
+        raise ValueError(f"ids must have at least one choice a token and at most 2^31 - 1 slots, got {tuple(ids.shape)}")
+    return ExpertPlan(*(torch.ops.mlpk.expert_sort if _traced(ids) else _sort)(ids, num_experts))
+
+
+def _check_rows(what: str, t: Tensor, rows: int, plan: ExpertPlan) -> None:
+    if plan.row_of.dtype != torch.int32 or plan.offsets.dtype != torch.int32 or not plan.offsets.is_contiguous():
+        raise ValueError("plan must be what expert_sort returned")
+    if not isinstance(t, Tensor) or t.dim() != 2 or t.shape[0] != rows or t.shape[1] < 1:
+        raise ValueError(f"{what} must be a 2-D tensor of {rows} rows")
+    _require_cuda(t)
+    if t.dtype not in DTYPES:
+        raise TypeError(f"{what} must be fp16, bf16 or fp32, got {t.dtype}")
+    if t.device != plan.row_of.device:
+        raise ValueError(f"{what} is on {t.device}, the plan on {plan.row_of.device}")
+
+
+def expert_dispatch(x: Tensor, plan: ExpertPlan) -> Tensor:
+    """``[tokens * choices, width]``: row ``plan.row_of[t, k]`` is ``x[t]``, rows
+    of dropped slots are zero.  Differentiable in x (a sum over the kept slots)."""
+    _check_rows("x", x, plan.row_of.shape[0], plan)
+    if _needs_grad(x):
+        return _DispatchFn.apply(x, *plan)
+    return (torch.ops.mlpk.expert_dispatch if _traced(x) else _dispatch)(x, *plan)
+
+
+def expert_combine(y: Tensor, weights: Optional[Tensor], plan: ExpertPlan) -> Tensor:
+    """``[tokens, width]``: the sum over k of ``weights[t, k] * y[plan.row_of[t, k]]``
+    in fp32; dropped slots add nothing, whatever their rows and weights hold.
+    ``weights`` is ``[tokens, choices]`` in y's dtype or fp32, or None for ones.
+    Differentiable in y and weights."""
+    _check_rows("y", y, plan.row_of.numel(), plan)
+    if weights is not None and (weights.shape != plan.row_of.shape or weights.device != y.device
+                                or (weights.dtype != y.dtype and weights.dtype != torch.float32)):
+        raise ValueError(f"weights must be a {tuple(plan.row_of.shape)} tensor of {y.dtype} or float32 on {y.device}")
+    if _needs_grad(y, weights):
+        return _CombineFn.apply(y, weights, *plan)
+    return (torch.ops.mlpk.expert_combine if _traced(y) else _combine)(y, weights, *plan)
+
+
+class FusedMLPExperts(nn.Module):
+    """A residual block of fused MLP experts: ``h = x + residual``, an RMS norm of
+    h, a router that takes each row's ``top`` best experts, a FusedMLPSoftplus
+    ``D -> H -> .. -> D`` for each expert, and the weighted sum of their rows.
+
+    ``forward(x, residual=None)`` returns ``(out, h)``, the next block's x and
+    residual.  ``capacity`` (rows an expert takes, the first of a batch; None:
+    all) drops the choices above it.  Each expert runs on its own rows: their
+    numbers are read by the host, once a call.
+    """
+
+    def __init__(self, D: int = 128, H: int = 128, num_experts: int = 8, top: int = 2, num_layers: int = 3,
+                 capacity: Optional[int] = None, eps: float = 1e-6):
+        super().__init__()
+        if not 1 <= top <= num_experts:
+            raise ValueError(f"top must be 1 to num_experts, got {top}")
+        if capacity is not None and capacity < 1:
+            raise ValueError(f"capacity must be positive, got {capacity}")
+        self.top, self.capacity = top, capacity
+        self.norm = FusedRMSNorm(D, eps)
+        self.router = nn.Parameter(torch.empty(D, num_experts).uniform_(-1 / math.sqrt(D), 1 / math.sqrt(D)))
+        self.experts = nn.ModuleList(FusedMLPSoftplus(D=D, H=H, out_features=D, num_layers=num_layers)
+                                     for _ in range(num_experts))
+
+    def forward(self, x: Tensor, residual: Optional[Tensor] = None):
+        y, h = self.norm(x, residual) if residual is not None else (self.norm(x), x)
+        scores, ids = (y.float() @ self.router.float()).topk(self.top, dim=1)
+        weights = torch.softmax(scores, dim=1)
+        plan = expert_sort(ids, len(self.experts))
+        if self.capacity is not None:
+            rank = plan.row_of - plan.offsets[:-1][ids]
+            plan = expert_sort(torch.where(rank < self.capacity, ids, -1), len(self.experts))
+        rows = expert_dispatch(y, plan)
+        counts = plan.counts.tolist()
+        *parts, dropped = rows.split([*counts, rows.shape[0] - sum(counts)])
+        parts = [expert(part).to(rows.dtype) if len(part) else part for expert, part in zip(self.experts, parts)]
+        return expert_combine(torch.cat([*parts, dropped]), weights, plan), h

@@ -1,0 +1,262 @@
+"""Root-mean-square norm with the residual's addition (no counterpart in the
+reference, whose MLP takes its rows as they come).
+
+* ``fused_rms_norm(x, weight, residual=r)`` -- ``h = x + r`` and
+  ``y = h / sqrt(mean(h^2) + eps) * weight`` in one pass, differentiable;
+* ``fused_rms_norm_fp8(...)`` -- the same with an 8-bit (e4m3) output and its
+  fp32 scales, for inference;
+* ``FusedRMSNorm`` -- the module.
+
+x is fp16, bf16 or fp32 of shape ``[..., width]`` with width up to 32768; all
+arithmetic is fp32.  The kernels run on the current CUDA stream; there is no
+CPU path.  Under torch.compile the calls are the operators
+``torch.ops.mlpk.rms_norm`` / ``rms_norm_bwd`` / ``rms_norm_fp8``; eager calls
+go straight to the C ABI.
+"""
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+import torch.nn as nn
+from torch import Tensor
+
+from . import _lib
+from .functional import _current_stream, _is_fake
+from .ops import _aligned
+
+DTYPES = {torch.float16: _lib.DT_F16, torch.float32: _lib.DT_F32, torch.bfloat16: _lib.DT_BF16}
+
+
+def _on_device(fn):
+    """fn(x, ...) with x's device current, as the C ABI launches on it."""
+    def call(x, *args):
+        dev = x.get_device()
+        if dev == torch.cuda.current_device():
+            return fn(x, *args)
+        with torch.cuda.device(dev):
+            return fn(x, *args)
+    return call
+
+
+def _ptr(t: Optional[Tensor]):
+    return None if t is None else t.data_ptr()
+
+
+def _check(x, weight, residual, eps):
+    if not isinstance(x, Tensor) or x.dim() < 1:
+        raise ValueError("x must be a tensor [..., width]")
+    if not x.is_cuda:
+        raise RuntimeError("fused_rms_norm runs on CUDA (sm_100) only; got a CPU tensor")
+    if x.dtype not in DTYPES:
+        raise TypeError(f"fused_rms_norm takes fp16, bf16 or fp32; got {x.dtype}")
+    width = x.shape[-1]
+    if not 1 <= width <= _lib.NORM_MAX_WIDTH:
+        raise ValueError(f"the width must be 1 to {_lib.NORM_MAX_WIDTH}, got {width}")
+    if weight is not None and (weight.shape != (width,) or weight.device != x.device
+                               or (weight.dtype != x.dtype and weight.dtype != torch.float32)):
+        raise ValueError(f"weight must be a [{width}] tensor of {x.dtype} or float32 on {x.device}")
+    if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype or residual.device != x.device):
+        raise ValueError(f"residual must be a {tuple(x.shape)} {x.dtype} tensor on {x.device}")
+    if not eps >= 0.0:
+        raise ValueError(f"eps must not be negative, got {eps}")
+
+
+def _w_dtype(weight, x) -> int:
+    return DTYPES[x.dtype if weight is None else weight.dtype]
+
+
+@_on_device
+def _forward(x, weight, residual, eps, want_rstd):
+    """(y, h, rstd): h is x itself without a residual, rstd None unless wanted."""
+    x = _aligned(x)
+    width = x.shape[-1]
+    rows = x.numel() // width
+    y = torch.empty_like(x)
+    rstd = torch.empty(rows, device=x.device, dtype=torch.float32) if want_rstd else None
+    if residual is not None:
+        residual, h = _aligned(residual), torch.empty_like(x)
+    else:
+        h = None
+    weight = None if weight is None else _aligned(weight)
+    _lib.check("mlpk_rms_norm", _lib.lib().mlpk_rms_norm(
+        rows, width, DTYPES[x.dtype], x.data_ptr(), _ptr(residual), _ptr(weight), _w_dtype(weight, x), eps,
+        y.data_ptr(), _ptr(h), _ptr(rstd), _current_stream(x.get_device())))
+    return y, x if h is None else h, rstd
+
+
+@_on_device
+def _backward(h, weight, rstd, grad_y, grad_h, want_dw):
+    """(dx, dw): dw in weight's dtype, None unless wanted."""
+    h, grad_y = _aligned(h), _aligned(grad_y)
+    grad_h = None if grad_h is None else _aligned(grad_h)
+    weight = None if weight is None else _aligned(weight)
+    width = h.shape[-1]
+    rows = h.numel() // width
+    dx = torch.empty_like(h)
+    dw = work = None
+    lib = _lib.lib()
+    if want_dw:
+        dw = torch.empty_like(weight)
+        size = lib.mlpk_rms_norm_bwd_workspace_size(rows, width, DTYPES[h.dtype])
+        work = torch.empty(max(size, 16), device=h.device, dtype=torch.uint8)
+    _lib.check("mlpk_rms_norm_bwd", lib.mlpk_rms_norm_bwd(
+        rows, width, DTYPES[h.dtype], h.data_ptr(), rstd.data_ptr(), _ptr(weight), _w_dtype(weight, h),
+        grad_y.data_ptr(), _ptr(grad_h), dx.data_ptr(), _ptr(dw), _ptr(work), 0 if work is None else work.numel(),
+        _current_stream(h.get_device())))
+    return dx, dw
+
+
+@_on_device
+def _forward_fp8(x, weight, residual, eps, group):
+    x = _aligned(x)
+    width = x.shape[-1]
+    rows = x.numel() // width
+    q = torch.empty(x.shape, device=x.device, dtype=torch.float8_e4m3fn)
+    groups = -(-width // group) if group else 1
+    scale = torch.empty((*x.shape[:-1], groups), device=x.device, dtype=torch.float32)
+    h = None
+    if residual is not None:
+        residual, h = _aligned(residual), torch.empty_like(x)
+    weight = None if weight is None else _aligned(weight)
+    _lib.check("mlpk_rms_norm_fp8", _lib.lib().mlpk_rms_norm_fp8(
+        rows, width, DTYPES[x.dtype], x.data_ptr(), _ptr(residual), _ptr(weight), _w_dtype(weight, x), eps, group,
+        q.data_ptr(), scale.data_ptr(), _ptr(h), _current_stream(x.get_device())))
+    return q, scale, h
+
+
+# ------------------------------------------------------------ torch.ops.mlpk
+@torch.library.custom_op("mlpk::rms_norm", mutates_args=())
+def rms_norm(x: Tensor, weight: Optional[Tensor], residual: Optional[Tensor], eps: float) -> list[Tensor]:
+    """[y, rstd], and h with a residual."""
+    _check(x, weight, residual, eps)
+    y, h, rstd = _forward(x, weight, residual, eps, True)
+    return [y, rstd] if residual is None else [y, rstd, h]
+
+
+@rms_norm.register_fake
+def _rms_norm_fake(x, weight, residual, eps):
+    rstd = x.new_empty((x.numel() // x.shape[-1],), dtype=torch.float32)
+    return [x.new_empty(x.shape), rstd] + ([] if residual is None else [x.new_empty(x.shape)])
+
+
+@torch.library.custom_op("mlpk::rms_norm_bwd", mutates_args=())
+def rms_norm_bwd(h: Tensor, weight: Optional[Tensor], rstd: Tensor, grad_y: Tensor, grad_h: Optional[Tensor],
+                 want_dw: bool) -> list[Tensor]:
+    """[dx], and dw if wanted."""
+    dx, dw = _backward(h, weight, rstd, grad_y, grad_h, want_dw)
+    return [dx] if dw is None else [dx, dw]
+
+
+@rms_norm_bwd.register_fake
+def _rms_norm_bwd_fake(h, weight, rstd, grad_y, grad_h, want_dw):
+    return [h.new_empty(h.shape)] + ([weight.new_empty(weight.shape)] if want_dw else [])
+
+
+@torch.library.custom_op("mlpk::rms_norm_fp8", mutates_args=())
+def rms_norm_fp8(x: Tensor, weight: Optional[Tensor], residual: Optional[Tensor], eps: float,
+                 group: int) -> list[Tensor]:
+    """[q, scale], and h with a residual."""
+    _check(x, weight, residual, eps)
+    q, scale, h = _forward_fp8(x, weight, residual, eps, group)
+    return [q, scale] if h is None else [q, scale, h]
+
+
+@rms_norm_fp8.register_fake
+def _rms_norm_fp8_fake(x, weight, residual, eps, group):
+    groups = -(-x.shape[-1] // group) if group else 1
+    return [x.new_empty(x.shape, dtype=torch.float8_e4m3fn),
+            x.new_empty((*x.shape[:-1], groups), dtype=torch.float32)] + \
+        ([] if residual is None else [x.new_empty(x.shape)])
+
+
+# ------------------------------------------------------------ autograd
+class _RMSNormFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, residual, eps):
+        if torch.compiler.is_compiling() or _is_fake(x):
+            y, rstd, *rest = torch.ops.mlpk.rms_norm(x, weight, residual, eps)
+            h = rest[0] if rest else x
+        else:
+            y, h, rstd = _forward(x, weight, residual, eps, True)
+        ctx.has_weight = weight is not None
+        ctx.has_residual = residual is not None
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(h, rstd, *([weight] if ctx.has_weight else []))
+        return (y, h) if ctx.has_residual else y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_y, grad_h=None):
+        h, rstd, *rest = ctx.saved_tensors
+        weight = rest[0] if rest else None
+        want_dw = ctx.has_weight and ctx.needs_input_grad[1]
+        if grad_y is None:  # y was not used: the norm adds nothing
+            dx, dw = grad_h, torch.zeros_like(weight) if want_dw and grad_h is not None else None
+        elif torch.compiler.is_compiling() or _is_fake(h):
+            dx, *dws = torch.ops.mlpk.rms_norm_bwd(h, weight, rstd, grad_y, grad_h, want_dw)
+            dw = dws[0] if dws else None
+        else:
+            dx, dw = _backward(h, weight, rstd, grad_y, grad_h, want_dw)
+        return (dx if ctx.needs_input_grad[0] else None, dw,
+                dx if ctx.has_residual and ctx.needs_input_grad[2] else None, None)
+
+
+def _needs_grad(*ts) -> bool:
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
+
+
+def fused_rms_norm(x: Tensor, weight: Optional[Tensor] = None, *, residual: Optional[Tensor] = None,
+                   eps: float = 1e-6):
+    """``y = h * rsqrt(mean(h^2) + eps) * weight`` with ``h = x + residual``.
+
+    Returns ``y``, or ``(y, h)`` with a residual (h is the next residual); both
+    new tensors of x's dtype.  ``weight`` is ``[width]`` in x's dtype or fp32
+    (None: ones).  y is computed from the unrounded sum; h is rounded once.
+    Differentiable in x, weight and residual; the weight's gradient is summed
+    over the rows in fp32 in a fixed order.  A row that holds an infinity or a
+    NaN gives NaN where it stands, as the formula does.
+    """
+    _check(x, weight, residual, eps)
+    if _needs_grad(x, weight, residual):
+        return _RMSNormFn.apply(x, weight, residual, eps)
+    if torch.compiler.is_compiling() or _is_fake(x):
+        y, _, *rest = torch.ops.mlpk.rms_norm(x, weight, residual, eps)
+        return (y, rest[0]) if rest else y
+    y, h, _ = _forward(x, weight, residual, eps, False)
+    return y if residual is None else (y, h)
+
+
+def fused_rms_norm_fp8(x: Tensor, weight: Optional[Tensor] = None, *, residual: Optional[Tensor] = None,
+                       eps: float = 1e-6, group: int = 0):
+    """The norm with an 8-bit output: ``(q, scale)``, or ``(q, scale, h)`` with a
+    residual; ``q.float() * scale`` (each scale over its columns) is y.
+
+    ``q`` is float8_e4m3fn of x's shape, ``scale`` fp32 ``[..., groups]``:
+    max|y| / 448 over the row (``group=0``) or over each 128 columns
+    (``group=128``, the last group may be shorter).  A NaN makes its group's
+    scale NaN.  For inference: raises where a gradient would be needed.
+    """
+    _check(x, weight, residual, eps)
+    if group not in (0, _lib.NORM_GROUP):
+        raise ValueError(f"group must be 0 (the row) or {_lib.NORM_GROUP}, got {group}")
+    if _needs_grad(x, weight, residual):
+        raise RuntimeError("fused_rms_norm_fp8 has no gradient: call it under torch.no_grad()")
+    if torch.compiler.is_compiling() or _is_fake(x):
+        return tuple(torch.ops.mlpk.rms_norm_fp8(x, weight, residual, eps, group))
+    q, scale, h = _forward_fp8(x, weight, residual, eps, group)
+    return (q, scale) if h is None else (q, scale, h)
+
+
+class FusedRMSNorm(nn.Module):
+    """RMS norm with a learned weight ``[width]``, initialised to ones."""
+
+    def __init__(self, width: int, eps: float = 1e-6):
+        super().__init__()
+        if not 1 <= width <= _lib.NORM_MAX_WIDTH:
+            raise ValueError(f"the width must be 1 to {_lib.NORM_MAX_WIDTH}, got {width}")
+        self.eps = eps
+        self.weight = nn.Parameter(torch.ones(width))
+
+    def forward(self, x, residual=None):
+        return fused_rms_norm(x, self.weight, residual=residual, eps=self.eps)

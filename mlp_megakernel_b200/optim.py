@@ -1,0 +1,306 @@
+"""AdamW over many tensors in one launch, with the state in 32 bits or in 8
+(no counterpart in the reference, which leaves the step to its caller).
+
+``FusedAdamW`` is a ``torch.optim.Optimizer``: learning-rate schedulers,
+parameter groups, ``state_dict`` and GradScaler work as with torch's AdamW.
+All tensors of a parameter group that share their types are stepped by one
+kernel launch on the current CUDA stream (768 tensors at most each); there is
+no CPU path.
+"""
+from __future__ import annotations
+
+import contextlib
+import ctypes
+
+import torch
+from torch import Tensor
+
+from . import _lib
+from .functional import _current_stream
+from .norm import DTYPES
+
+BLOCK = _lib.ADAMW_BLOCK
+
+
+def _blocks(n: int) -> int:
+    return -(-n // BLOCK)
+
+
+def _dense(t: Tensor) -> bool:
+    """Whether the elements fill one stretch of memory, in any order of the
+    dimensions."""
+    if t.is_contiguous():
+        return True
+    want = 1
+    for size, stride in sorted(((n, s) for n, s in zip(t.shape, t.stride()) if n != 1), key=lambda d: d[1]):
+        if stride != want:
+            return False
+        want *= size
+    return True
+
+
+class _Bucket:
+    """The flat state of some tensors of one parameter group: each begins at a
+    multiple of BLOCK elements, and what pads it is zero."""
+
+    def __init__(self, params, bits: int, master: bool):
+        self.params, self.bits = list(params), bits
+        self.index = {p: i for i, p in enumerate(self.params)}
+        self.numel = [p.numel() for p in self.params]
+        self.off, total = [], 0
+        for n in self.numel:
+            self.off.append(total)
+            total += _blocks(n) * BLOCK
+        self.device = dev = self.params[0].device
+        self.dtype = self.params[0].dtype
+        self.strides = {p: p.stride() for p in self.params}
+
+        total = max(total, BLOCK)  # tensors of no elements have a state too
+
+        def zeros(n, dtype):
+            return torch.zeros(n, device=dev, dtype=dtype)
+
+        if bits == 8:
+            self.flat = {"exp_avg": zeros(total, torch.float8_e4m3fn), "exp_avg_scale": zeros(total // BLOCK, torch.float32),
+                         "exp_avg_rms": zeros(total, torch.float8_e4m3fn),
+                         "exp_avg_rms_scale": zeros(total // BLOCK, torch.float32)}
+        else:
+            self.flat = {"exp_avg": zeros(total, torch.float32), "exp_avg_sq": zeros(total, torch.float32)}
+        if master:
+            self.flat["master_param"] = zeros(total, torch.float32)
+        self.ticks = torch.zeros(len(self.params), device=dev, dtype=torch.int64)
+        self.chunks = [max(1, -(-n // _lib.ADAMW_CHUNK)) for n in self.numel]
+        if master:
+            for i, p in enumerate(self.params):
+                self.view(i, "master_param").copy_(p.detach())
+        sq = self.flat["exp_avg_rms" if bits == 8 else "exp_avg_sq"]
+        self.struct = _lib.MlpkAdamwState(
+            bits, self.flat["exp_avg"].data_ptr(), sq.data_ptr(),
+            self.flat["exp_avg_scale"].data_ptr() if bits == 8 else None,
+            self.flat["exp_avg_rms_scale"].data_ptr() if bits == 8 else None,
+            self.flat["master_param"].data_ptr() if master else None, self.ticks.data_ptr())
+        self.arrays = self.arrays_of(range(len(self.params)))
+
+    def arrays_of(self, which):
+        """The parts of the C call's table that stay: sizes, places, counters."""
+        n = len(which)
+        return ((ctypes.c_int64 * n)(*[self.numel[i] for i in which]),
+                (ctypes.c_int64 * n)(*[self.off[i] for i in which]), (ctypes.c_int32 * n)(*which))
+
+    def view(self, i: int, name: str) -> Tensor:
+        """Tensor i's part of a flat buffer: of its own shape and strides, or
+        [blocks] for a scale."""
+        flat = self.flat[name]
+        if name.endswith("_scale"):
+            return flat[self.off[i] // BLOCK:self.off[i] // BLOCK + _blocks(self.numel[i])]
+        p = self.params[i]
+        return flat[self.off[i]:self.off[i] + self.numel[i]].as_strided(p.shape, p.stride(),
+                                                                         flat.storage_offset() + self.off[i])
+
+    def steps(self) -> list:
+        return [int(t) // c for t, c in zip(self.ticks.tolist(), self.chunks)]
+
+
+class FusedAdamW(torch.optim.Optimizer):
+    """AdamW (decoupled weight decay) for CUDA parameters in fp32, fp16 or bf16.
+
+    ``state_bits=32`` keeps m and v in fp32.  ``state_bits=8`` keeps m and sqrt(v)
+    as e4m3 in blocks of 256 elements with an fp32 scale each: 2.03 bytes an
+    element instead of 8.  (Blocks are of a tensor's elements in memory order.  A
+    gradient that is not finite makes its whole block's state NaN: use GradScaler
+    or clip.)  ``master_weights=True`` keeps an fp32 copy of each 16-bit
+    parameter, made when its state is, which is stepped and rounded into the
+    parameter; without it a 16-bit parameter is stepped in fp32 and rounded to
+    itself, as in torch.  ``lr`` is a number or a CUDA tensor of one element.
+
+    A parameter whose ``grad`` is None is left as it is.  Gradients are in the
+    parameter's dtype or fp32.  The step count is on the device, so ``step()``
+    can be captured in a CUDA graph after one ordinary step, and a step that
+    GradScaler's ``found_inf`` skips does not count.
+    """
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 1e-2, *,
+                 state_bits: int = 32, master_weights: bool = False, maximize: bool = False):
+        if state_bits not in (8, 32):
+            raise ValueError(f"state_bits must be 8 or 32, got {state_bits}")
+        defaults = dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay, maximize=maximize)
+        self._state_bits, self._master = state_bits, master_weights
+        self._buckets: list = []  # lists of buckets, a list for each parameter group
+        self._step_supports_amp_scaling = True
+        super().__init__(params, defaults)
+
+    def add_param_group(self, group) -> None:
+        super().add_param_group(group)
+        group = self.param_groups[-1]
+        try:
+            self._check_group(group)
+        except Exception:
+            self.param_groups.pop()
+            raise
+        self._buckets.append([])
+
+    @staticmethod
+    def _check_group(group) -> None:
+        lr, (b1, b2) = group["lr"], group["betas"]
+        if isinstance(lr, Tensor):
+            if lr.numel() != 1 or lr.dtype != torch.float32 or not lr.is_cuda:
+                raise ValueError("a tensor lr must be one float32 value on the GPU")
+        elif not lr >= 0.0:
+            raise ValueError(f"lr must not be negative, got {lr}")
+        if not (0.0 < b1 < 1.0 and 0.0 < b2 < 1.0):
+            raise ValueError(f"betas must lie between 0 and 1, got {(b1, b2)}")
+        if not group["eps"] >= 0.0 or not group["weight_decay"] >= 0.0:
+            raise ValueError("eps and weight_decay must not be negative")
+        for p in group["params"]:
+            if not p.is_cuda:
+                raise RuntimeError("FusedAdamW runs on CUDA (sm_100) only; got a CPU parameter")
+            if p.dtype not in DTYPES:
+                raise TypeError(f"FusedAdamW takes fp16, bf16 or fp32 parameters; got {p.dtype}")
+            if not _dense(p):
+                raise ValueError(f"a parameter of shape {tuple(p.shape)} and strides {p.stride()} does not fill its memory")
+
+    def _bucket(self, g: int, params) -> None:
+        """State for parameters of group g that have none, a bucket for each type
+        and device."""
+        kinds: dict = {}
+        for p in params:
+            kinds.setdefault((p.dtype, p.device), []).append(p)
+        for (dtype, dev), ps in kinds.items():
+            with torch.cuda.device(dev):
+                b = _Bucket(ps, self._state_bits, self._master and dtype != torch.float32)
+            self._buckets[g].append(b)
+            for i, p in enumerate(ps):
+                self.state[p] = {name: b.view(i, name) for name in b.flat}
+
+    @torch.no_grad()
+    def step(self, closure=None, *, grad_scale=None, found_inf=None):
+        """One step.  ``grad_scale`` and ``found_inf`` (fp32 values on the GPU, as
+        GradScaler passes them): the gradients are divided by the one; a
+        ``found_inf`` that is not 0 leaves parameters, state and step count as
+        they were."""
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        grad_scale = getattr(self, "grad_scale", None) if grad_scale is None else grad_scale
+        found_inf = getattr(self, "found_inf", None) if found_inf is None else found_inf
+        for g, group in enumerate(self.param_groups):
+            new = [p for p in group["params"] if p.grad is not None and p not in self.state]
+            if new:
+                self._bucket(g, new)
+            for b in self._buckets[g]:
+                self._step_bucket(b, group, grad_scale, found_inf)
+        return loss
+
+    @staticmethod
+    def _step_bucket(b: _Bucket, group, grad_scale, found_inf) -> None:
+        params, arrays = b.params, b.arrays
+        grads = [p.grad for p in params]
+        if any(g is None for g in grads):
+            which = [i for i, g in enumerate(grads) if g is not None]
+            if not which:
+                return
+            params, grads, arrays = [params[i] for i in which], [grads[i] for i in which], b.arrays_of(which)
+        kinds = {g.dtype for g in grads}
+        if len(kinds) == 1:
+            FusedAdamW._launch(b, params, grads, arrays, group, grad_scale, found_inf)
+            return
+        for kind in kinds:  # fp32 gradients beside 16-bit ones: a launch for each
+            part = [(p, g) for p, g in zip(params, grads) if g.dtype == kind]
+            FusedAdamW._launch(b, [p for p, _ in part], [g for _, g in part],
+                               b.arrays_of([b.index[p] for p, _ in part]), group, grad_scale, found_inf)
+
+    @staticmethod
+    def _launch(b: _Bucket, params, grads, arrays, group, grad_scale, found_inf) -> None:
+        dev, dtype, g_dtype = b.device, b.dtype, grads[0].dtype
+        if g_dtype != dtype and g_dtype != torch.float32:
+            raise TypeError(f"gradients must be {dtype} or float32, got {g_dtype}")
+        for i, (p, g) in enumerate(zip(params, grads)):
+            if p.dtype != dtype or p.device != dev or p.stride() != b.strides[p]:
+                raise RuntimeError("a parameter changed its type, device or strides after its first step")
+            if g.device != dev or g.is_sparse:
+                raise ValueError(f"a gradient must be a dense tensor on {dev}")
+            if g.stride() != p.stride():  # the elements are taken in the parameter's order of memory
+                grads[i] = torch.empty_like(p, dtype=g_dtype).copy_(g)
+        lr = group["lr"]
+        scalars = [lr if isinstance(lr, Tensor) else None, grad_scale, found_inf]
+        for t in scalars:
+            if t is not None and (t.dtype != torch.float32 or t.device != dev):
+                raise ValueError(f"lr, grad_scale and found_inf must be float32 values on {dev}")
+        b1, b2 = group["betas"]
+        args = _lib.MlpkAdamwArgs(0.0 if scalars[0] is not None else lr, b1, b2, group["eps"], group["weight_decay"],
+                                  int(group["maximize"]), *[None if t is None else t.data_ptr() for t in scalars])
+        n = len(params)
+        pointers = ctypes.c_void_p * n
+        with contextlib.nullcontext() if dev.index == torch.cuda.current_device() else torch.cuda.device(dev):
+            _lib.check("mlpk_adamw_step", _lib.lib().mlpk_adamw_step(
+                n, arrays[0], pointers(*[p.data_ptr() for p in params]), pointers(*[g.data_ptr() for g in grads]),
+                arrays[1], arrays[2], DTYPES[dtype], DTYPES[g_dtype], ctypes.byref(b.struct), ctypes.byref(args),
+                _current_stream(dev.index)))
+        torch.autograd.graph.increment_version(params)
+
+    def __reduce__(self):
+        raise TypeError("FusedAdamW is saved and copied by its state_dict()")
+
+    # ------------------------------------------------------------ state
+    def flat_state(self) -> list:
+        """The state's own buffers, a dict for each group and type of tensors in
+        the order they got their state: ``exp_avg`` and ``exp_avg_sq`` (32 bits), or
+        ``exp_avg``, ``exp_avg_scale``, ``exp_avg_rms`` and ``exp_avg_rms_scale``
+        (8 bits), and ``master_param``.  A tensor's part begins at a multiple of
+        256 elements; what pads it is zero."""
+        return [b.flat for buckets in self._buckets for b in buckets]
+
+    def state_dict(self) -> dict:
+        """As torch's: ``state[i]`` has ``step`` (a number; the host waits for the
+        GPU) and the tensors of parameter i, ``param_groups`` the rest."""
+        place, groups = {}, []
+        for group in self.param_groups:
+            packed = {k: v for k, v in group.items() if k != "params"}
+            packed["params"] = [place.setdefault(p, len(place)) for p in group["params"]]
+            groups.append(packed)
+        state = {}
+        for buckets in self._buckets:
+            for b in buckets:
+                for i, (p, step) in enumerate(zip(b.params, b.steps())):
+                    state[place[p]] = {"step": step, **{name: b.view(i, name) for name in b.flat}}
+        return {"state": state, "param_groups": groups}
+
+    @torch.no_grad()
+    def load_state_dict(self, state_dict) -> None:
+        """Takes what ``state_dict`` gave, of the same ``state_bits`` and
+        ``master_weights``; the values are copied."""
+        groups, state = state_dict["param_groups"], state_dict["state"]
+        if len(groups) != len(self.param_groups) or \
+                any(len(a["params"]) != len(b["params"]) for a, b in zip(groups, self.param_groups)):
+            raise ValueError("the state is of other parameter groups")
+        plans = []
+        for g, (saved, group) in enumerate(zip(groups, self.param_groups)):
+            found = [(p, state[i]) for i, p in zip(saved["params"], group["params"]) if i in state]
+            for p, s in found:
+                names = {"exp_avg", "exp_avg_scale", "exp_avg_rms", "exp_avg_rms_scale"} if self._state_bits == 8 else \
+                    {"exp_avg", "exp_avg_sq"}
+                names |= {"master_param"} if self._master and p.dtype != torch.float32 else set()
+                if set(s) != names | {"step"}:
+                    raise ValueError(f"the state of a parameter holds {sorted(s)}, expected {sorted(names | {'step'})}")
+                for name in names:
+                    n = _blocks(p.numel()) if name.endswith("_scale") else p.numel()
+                    kind = torch.float8_e4m3fn if self._state_bits == 8 and name in ("exp_avg", "exp_avg_rms") else \
+                        torch.float32
+                    if s[name].numel() != n or s[name].dtype != kind:
+                        raise ValueError(f"{name} must hold {n} values of {kind}")
+            plans.append(found)
+        self.state.clear()
+        self._buckets = [[] for _ in self.param_groups]
+        for g, found in enumerate(plans):
+            self.param_groups[g].update({k: v.clone() if isinstance(v, Tensor) else v
+                                         for k, v in groups[g].items() if k != "params"})
+            self._check_group(self.param_groups[g])
+            self._bucket(g, [p for p, _ in found])
+            saved = dict(found)
+            for b in self._buckets[g]:
+                for i, p in enumerate(b.params):
+                    for name in b.flat:
+                        v = b.view(i, name)
+                        v.copy_(saved[p][name].reshape(v.shape))
+                b.ticks.copy_(torch.tensor([int(saved[p]["step"]) * c for p, c in zip(b.params, b.chunks)]))
