@@ -262,15 +262,15 @@ int mlpk_rms_norm(int64_t rows, int width, int dtype, const void* x, const void*
  * group whose scale would be below the smallest normal number is all zeros. */
 int mlpk_rms_norm_fp8(int64_t rows, int width, int dtype, const void* x, const void* residual, const void* weight,
                       int w_dtype, float eps, int group, void* q, float* scale, void* h, mlpk_stream_t stream);
-/* Backward of mlpk_rms_norm: from h, rstd and the gradients of y and h (grad_h
- * NULL: none), dx (the gradient of x and of the residual) and dw ([width] of
+/* Backward of mlpk_rms_norm: from its x, residual (NULL: none) and rstd and the
+ * gradients of y and h (grad_h NULL: none), dx (the gradient of x and of the residual) and dw ([width] of
  * w_dtype, summed over the rows in fp32 in a fixed order; NULL: not wanted).
  * workspace: mlpk_rms_norm_bwd_workspace_size bytes, only for dw
  * (MLPK_ERR_SCRATCH if smaller). */
 int64_t mlpk_rms_norm_bwd_workspace_size(int64_t rows, int width, int dtype);
-int mlpk_rms_norm_bwd(int64_t rows, int width, int dtype, const void* h, const float* rstd, const void* weight,
-                      int w_dtype, const void* grad_y, const void* grad_h, void* dx, void* dw, void* workspace,
-                      int64_t workspace_bytes, mlpk_stream_t stream);
+int mlpk_rms_norm_bwd(int64_t rows, int width, int dtype, const void* x, const void* residual, const float* rstd,
+                      const void* weight, int w_dtype, const void* grad_y, const void* grad_h, void* dx, void* dw,
+                      void* workspace, int64_t workspace_bytes, mlpk_stream_t stream);
 
 /* Stable order of slots by expert: ids[slots] (int32 or int64, id_bytes 4 or
  * 8), row_of[i] = the place of slot i when the slots are ordered by expert and

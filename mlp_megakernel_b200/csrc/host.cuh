@@ -26,6 +26,13 @@ __attribute__((visibility("hidden"))) int cuda_status(cudaError_t e);
 // The current device's properties; MLPK_ERR_ARCH if it is not sm_100.
 __attribute__((visibility("hidden"))) int current_device_info(DevInfo* out, int* dev_out);
 
+constexpr int kMaxBlockSmem = 227 * 1024;  // dynamic shared memory of a block
+
+// Blocks of a kernel that an SM holds at a time (found once for each size; also
+// lets the kernel have that much dynamic shared memory); 0 on a failure, whose
+// status is kept for mlpk_last_cuda_error.
+__attribute__((visibility("hidden"))) int blocks_per_sm(const void* kern, int threads, size_t smem, int dev);
+
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 // Launch through cudaLaunchKernelEx so that the status returned is that of

@@ -10,8 +10,10 @@
 #include <cstdint>
 #include <cstdio>
 #include <cstring>
+#include <map>
 #include <mutex>
 #include <set>
+#include <tuple>
 #include <utility>
 
 #include "../../include/mlpk.h"
@@ -83,6 +85,20 @@ int current_device_info(DevInfo* out, int* dev_out) {
   *out = d;
   if (dev_out) *dev_out = dev;
   return d.major == 10 ? MLPK_OK : MLPK_ERR_ARCH;
+}
+
+int blocks_per_sm(const void* kern, int threads, size_t smem, int dev) {
+  static std::mutex mu;
+  static std::map<std::tuple<const void*, int, size_t, int>, int> known;
+  std::lock_guard<std::mutex> lk(mu);
+  int& n = known[{kern, threads, smem, dev}];
+  if (n == 0) {
+    if (smem > 48 * 1024 && cuda_status(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                             kMaxBlockSmem)))
+      return 0;
+    if (cuda_status(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, threads, smem))) n = 0;
+  }
+  return n;
 }
 
 }  // namespace host

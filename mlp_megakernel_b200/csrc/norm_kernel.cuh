@@ -5,16 +5,29 @@
 //   h = x + r;   s = rsqrt(mean_j h_j^2 + eps);   y_j = h_j s w_j
 // y is computed from the unrounded h; h is rounded once, as it is stored.  The
 // 8-bit output stores e4m3(y / scale) with scale = max|y| / 448 over the row
-// or over each 128 columns.  Backward, from the stored h and s (G = dL/dy):
+// or over each 128 columns.  Backward, from x, r and s (G = dL/dy):
 //   n_j = h_j s;   c = mean_j G_j w_j n_j
 //   dx_j = dr_j = s (G_j w_j - n_j c) + dL/dh_j;   dw_j = sum_rows G_j n_j
-// (c uses the norm of the rounded h: it differs from the forward's by the
-// rounding of h alone.)
+// It adds x and r again: from the rounded h, dw would be half as exact again
+// (its own rounding and h's are of the same size), and h costs 2 bytes less of
+// 20 an element.
 //
-// Layout: TPR threads share a row and hold it in registers (NV vectors each,
-// vector i of lane l is the row's vector i * TPR + l), so every value is read
-// once.  Up to 32 threads a row's sum is a warp shuffle and several rows share
-// a block; above, a block has one row and sums through shared memory.
+// What bounds it: memory; every value is read once and written once.
+//
+// Layout: TPR threads share a row, NV 16-byte vectors each (vector i of lane l
+// is the row's vector i * TPR + l).  Up to 32 threads a row's sum is a warp
+// shuffle and several rows share a block; above, a block has one row and sums
+// through shared memory.  Blocks stay and loop over rows.  A thread copies its
+// vectors of the next rows to its own slots of shared memory (cp.async) and
+// reads them back itself: enough bytes are in flight whatever the registers
+// hold, and no barrier guards the slots.  Rows whose slots do not fit (PIPE
+// false) are read directly.
+//
+// A width that no vector divides (RAGGED): a row begins `shift` elements into
+// an aligned vector of the tensor, its first and last vectors are shared with
+// its neighbours, and a thread leaves out the elements that are not its row's.
+// Blocks step by a multiple of VEC rows, so that `shift`, and with it each
+// thread's columns, are the same in all rows of a block's row group.
 #pragma once
 #include "pdl.cuh"
 #include "vec.cuh"
@@ -24,10 +37,11 @@ namespace mlpk {
 constexpr int kNormThreads = 256;  // threads of a block of several rows
 constexpr int kNormGroup = 128;    // columns that share a scale
 constexpr int kNormMaxWidth = 32768;
+constexpr int kNormStages = 4;     // rows that a thread has under way, at most
 
-// Sum of v over the row's threads.  TPR > 32: `red` is one float per warp;
-// two calls in a row take different halves of it (`half`), so one barrier
-// separates a write from the reads of the call before the last.
+// Sum of v over the row's threads.  TPR > 32: `red` has two halves of a float
+// per warp, used in turn (`half`), so one barrier separates a write from the
+// reads of the call before the last.
 __device__ __forceinline__ float norm_row_sum(float v, int tpr, float* red, int half) {
   if (tpr <= 32) {
     for (int o = tpr / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
@@ -38,9 +52,11 @@ __device__ __forceinline__ float norm_row_sum(float v, int tpr, float* red, int 
   red += half * 32;
   if (threadIdx.x % 32 == 0) red[threadIdx.x / 32] = v;
   __syncthreads();
-  float t = 0.0f;
-  for (int k = 0; k < tpr / 32; ++k) t += red[k];  // the same order in every thread
-  return t;
+  // Each warp adds the warps' sums the same way.
+  v = threadIdx.x % 32 < tpr / 32 ? red[threadIdx.x % 32] : 0.0f;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
 }
 
 __device__ __forceinline__ uint32_t norm_row_max(uint32_t v, int tpr, float* red, int half) {
@@ -49,10 +65,69 @@ __device__ __forceinline__ uint32_t norm_row_max(uint32_t v, int tpr, float* red
   uint32_t* r = reinterpret_cast<uint32_t*>(red) + half * 32;
   if (threadIdx.x % 32 == 0) r[threadIdx.x / 32] = v;
   __syncthreads();
-  uint32_t t = 0;
-  for (int k = 0; k < tpr / 32; ++k) t = max(t, r[k]);
-  return t;
+  v = threadIdx.x % 32 < tpr / 32 ? r[threadIdx.x % 32] : 0u;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
 }
+
+// A thread's vectors of the rows of its block's row group.
+template <class T, int NV, bool RAGGED>
+struct RowSpan {
+  static constexpr int VEC = kVecOf<T>;
+  int64_t total;  // elements of the tensor
+  int width, tpr, lane, shift, nvec;
+
+  // first_row: any row of the row group
+  __device__ RowSpan(int64_t rows, int width_, int tpr_, int lane_, int64_t first_row)
+      : total(rows * width_), width(width_), tpr(tpr_), lane(lane_) {
+    shift = RAGGED ? static_cast<int>((first_row % VEC) * (width % VEC) % VEC) : 0;
+    nvec = (width + shift + VEC - 1) / VEC;
+  }
+  __device__ bool has(int i) const { return i * tpr + lane < nvec; }
+  __device__ int col(int i) const { return (i * tpr + lane) * VEC - shift; }  // of element 0; may be below 0
+  __device__ int64_t at(int64_t row, int i) const { return row * width + col(i); }  // a multiple of VEC
+  __device__ bool owns(int i, int e) const {
+    return !RAGGED || static_cast<unsigned>(col(i) + e) < static_cast<unsigned>(width);
+  }
+  __device__ bool whole(int i) const { return !RAGGED || (col(i) >= 0 && col(i) + VEC <= width); }
+  // Bytes of the vector that lie inside the tensor.
+  __device__ int bytes(int64_t row, int i) const {
+    if (!RAGGED) return 16;
+    const int64_t left = total - at(row, i);
+    return left >= VEC ? 16 : static_cast<int>(left) * static_cast<int>(sizeof(T));
+  }
+  __device__ Raw<T, VEC> load(const T* p, int64_t row, int i) const {
+    if constexpr (RAGGED) {
+      if (total - at(row, i) < VEC) {
+        Raw<T, VEC> r;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) r.v[e] = at(row, i) + e < total ? p[at(row, i) + e] : from_float<T>(0.0f);
+        return r;
+      }
+    }
+    return load_raw<T, VEC>(p + at(row, i));
+  }
+  __device__ void store(T* p, int64_t row, int i, const float (&f)[VEC]) const {
+    if (whole(i)) {
+      store_vec<T, VEC>(p + at(row, i), f);
+      return;
+    }
+#pragma unroll
+    for (int e = 0; e < VEC; ++e)
+      if (owns(i, e)) p[at(row, i) + e] = from_float<T>(f[e]);
+  }
+  // The weight's values of the vector's columns; ones without a weight.
+  template <class W>
+  __device__ void weights(const W* w, int i, Raw<W, VEC>& r) const {
+    if (!RAGGED && w) {
+      r = load_raw<W, VEC>(w + col(i));
+      return;
+    }
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) r.v[e] = w && owns(i, e) ? w[col(i) + e] : from_float<W>(1.0f);
+  }
+};
 
 struct NormArgs {
   int64_t rows;
@@ -69,125 +144,181 @@ struct NormArgs {
   int group;      // FP8: columns that share a scale: 128, or 0 for the row
 };
 
-template <class T, class W, int VEC, int NV, bool FP8>
-__global__ void __launch_bounds__(1024) rms_norm_fwd_kernel(const NormArgs a) {
-  extern __shared__ float smem[];  // 64 floats, then with FP8 and VEC 1 a maximum per group
+// Shared memory: 128 floats for the row sums, then with FP8, RAGGED and groups
+// a maximum per group and row group, then the slots [stage][x, r][i][thread].
+template <class T, class W, int NV, bool RAGGED, bool PIPE, int MAXT, bool FP8>
+__global__ void __launch_bounds__(MAXT) rms_norm_fwd_kernel(const NormArgs a, int stages, int slots_at) {
+  using Span = RowSpan<T, NV, RAGGED>;
+  constexpr int VEC = Span::VEC;
+  extern __shared__ __align__(16) uint8_t smem_raw[];
+  float* red = reinterpret_cast<float*>(smem_raw);
   pdl_enter();
-  const int lane = threadIdx.x % a.tpr;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * (blockDim.x / a.tpr) + threadIdx.x / a.tpr;
-  const bool live = row < a.rows;  // whole rows: the other threads take part in the shuffles and barriers
-  const int64_t base = row * a.width;
-  const T* x = static_cast<const T*>(a.x) + base;
-  const T* r = a.r ? static_cast<const T*>(a.r) + base : nullptr;
-  const W* w = static_cast<const W*>(a.w);
-  const int nvec = a.width / VEC;
+  const int lane = threadIdx.x % a.tpr, sub = threadIdx.x / a.tpr, subs = blockDim.x / a.tpr;
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * subs + sub;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * subs;
+  const Span span(a.rows, a.width, a.tpr, lane, first);
+  const T* x = static_cast<const T*>(a.x);
+  const T* r = static_cast<const T*>(a.r);
+  const int streams = r ? 2 : 1;
+  Raw<T, VEC>* slots = reinterpret_cast<Raw<T, VEC>*>(smem_raw + slots_at) + threadIdx.x;
+  auto slot = [&](int stage, int stream, int i) { return slots + ((stage * streams + stream) * NV + i) * blockDim.x; };
+  auto fetch = [&](int64_t row, int stage) {
+    if (row < a.rows) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+        if (span.has(i)) {
+          cp_async16(slot(stage, 0, i), x + span.at(row, i), span.bytes(row, i));
+          if (r) cp_async16(slot(stage, 1, i), r + span.at(row, i), span.bytes(row, i));
+        }
+    }
+    cp_async_commit();
+  };
+  if constexpr (PIPE)
+    for (int k = 0; k < stages; ++k) fetch(first + k * step, k);
+  Raw<W, VEC> w[NV];
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+    if (span.has(i)) span.weights(static_cast<const W*>(a.w), i, w[i]);
 
-  float h[NV][VEC];
-  float sum = 0.0f;
+  int stage = 0, half = 0;
+  // Whole blocks loop together: the last rows' missing ones take part in the
+  // shuffles and barriers.
+  for (int64_t row0 = first - sub; row0 < a.rows; row0 += step, half ^= 1) {
+    const int64_t row = row0 + sub;
+    const bool live = row < a.rows;
+    if constexpr (PIPE) cp_async_wait_upto(stages - 1);
+    float h[NV][VEC];
+    float sum = 0.0f;
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int v = i * a.tpr + lane;
+    for (int i = 0; i < NV; ++i) {
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) h[i][e] = 0.0f;
-    if (live && v < nvec) {
-      unpack(load_raw<T, VEC>(x + v * VEC), h[i]);
-      if (r) {
+      for (int e = 0; e < VEC; ++e) h[i][e] = 0.0f;
+      if (live && span.has(i)) {
+        unpack(PIPE ? *slot(stage, 0, i) : span.load(x, row, i), h[i]);
+        if (r) {
+          float f[VEC];
+          unpack(PIPE ? *slot(stage, 1, i) : span.load(r, row, i), f);
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) h[i][e] += f[e];
+        }
+        if (RAGGED) {
+#pragma unroll
+          for (int e = 0; e < VEC; ++e)
+            if (!span.owns(i, e)) h[i][e] = 0.0f;
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) sum += h[i][e] * h[i][e];
+    }
+    if constexpr (PIPE) {
+      fetch(row + stages * step, stage);
+      stage = stage + 1 == stages ? 0 : stage + 1;
+    }
+    const float s = rsqrtf(norm_row_sum(sum, a.tpr, red, half) / static_cast<float>(a.width) + a.eps);
+    if (a.rstd && live && lane == 0) a.rstd[row] = s;
+    uint32_t amax = 0;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      if (live && span.has(i)) {
+        if (a.h) span.store(static_cast<T*>(a.h), row, i, h[i]);
         float f[VEC];
-        unpack(load_raw<T, VEC>(r + v * VEC), f);
+        unpack(w[i], f);
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) h[i][e] += f[e];
-      }
-      if (a.h) store_vec<T, VEC>(static_cast<T*>(a.h) + base + v * VEC, h[i]);
-    }
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) sum += h[i][e] * h[i][e];
-  }
-  const float s = rsqrtf(norm_row_sum(sum, a.tpr, smem, 0) / static_cast<float>(a.width) + a.eps);
-  if (a.rstd && live && lane == 0) a.rstd[row] = s;
-
-  uint32_t amax = 0;
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int v = i * a.tpr + lane;
-    if (live && v < nvec) {
-      float f[VEC];
-      if (w) {
-        unpack(load_raw<W, VEC>(w + v * VEC), f);
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) h[i][e] = h[i][e] * s * f[e];
-      } else {
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) h[i][e] *= s;
-      }
-      if constexpr (FP8) {
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) amax = max(amax, abs_bits(h[i][e]));
-      } else {
-        store_vec<T, VEC>(static_cast<T*>(a.y) + base + v * VEC, h[i]);
-      }
-    }
-  }
-  if constexpr (FP8) {
-    uint8_t* q = static_cast<uint8_t*>(a.y) + base;
-    if (a.group == 0) {
-      float inv;
-      const float scale = fp8_scale(norm_row_max(amax, a.tpr, smem, 1), &inv);
-      if (live && lane == 0) a.scale[row] = scale;
-#pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        const int v = i * a.tpr + lane;
-        if (live && v < nvec) {
-#pragma unroll
-          for (int e = 0; e < VEC; ++e) h[i][e] *= inv;
-          store_fp8<VEC>(q + v * VEC, h[i]);
+        for (int e = 0; e < VEC; ++e) {
+          h[i][e] = h[i][e] * s * f[e];
+          if (FP8) amax = max(amax, abs_bits(h[i][e]));
         }
+        if constexpr (!FP8) span.store(static_cast<T*>(a.y), row, i, h[i]);
       }
-      return;
     }
-    const int groups = (a.width + kNormGroup - 1) / kNormGroup;
-    if constexpr (VEC > 1) {
-      // The 128 / VEC lanes of a group are neighbours: a power of two, and a
-      // divisor of tpr unless the row is narrower than a group.
-      const int gl = min(kNormGroup / VEC, a.tpr);
+    if constexpr (FP8) {
+      auto store = [&](int i) {
+        uint8_t* q = static_cast<uint8_t*>(a.y) + span.at(row, i);
+        if (span.whole(i)) {
+          store_fp8<VEC>(q, h[i]);
+          return;
+        }
 #pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        const int v = i * a.tpr + lane;
-        uint32_t m = 0;
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) m = max(m, abs_bits(h[i][e]));
-        for (int o = gl / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+        for (int e = 0; e < VEC; ++e) {
+          const float f[1] = {h[i][e]};
+          if (span.owns(i, e)) store_fp8<1>(q + e, f);
+        }
+      };
+      const int groups = (a.width + kNormGroup - 1) / kNormGroup;
+      if (a.group == 0) {
         float inv;
-        const float scale = fp8_scale(m, &inv);
-        if (live && v < nvec) {
-          if (v % gl == 0) a.scale[row * groups + v / gl] = scale;
+        const float scale = fp8_scale(norm_row_max(amax, a.tpr, red + 64, half), &inv);
+        if (live && lane == 0) a.scale[row] = scale;
 #pragma unroll
-          for (int e = 0; e < VEC; ++e) h[i][e] *= inv;
-          store_fp8<VEC>(q + v * VEC, h[i]);
+        for (int i = 0; i < NV; ++i) {
+          if (live && span.has(i)) {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) h[i][e] *= inv;
+            store(i);
+          }
         }
-      }
-    } else {
-      // One element per lane: 32 neighbours lie in one group (32 divides both
-      // 128 and every offset i * tpr, or the whole row is one group), and the
-      // warps of a group meet in shared memory.  A maximum does not depend on
-      // the order.
-      uint32_t* gmax = reinterpret_cast<uint32_t*>(smem + 64) + (threadIdx.x / a.tpr) * groups;
-      for (int k = lane; k < groups; k += a.tpr) gmax[k] = 0;
-      __syncthreads();
+      } else if constexpr (!RAGGED) {
+        // The 128 / VEC lanes of a group are neighbours: a power of two, and a
+        // divisor of tpr unless the row is narrower than a group.
+        const int gl = min(kNormGroup / VEC, a.tpr);
 #pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        const int v = i * a.tpr + lane;
-        if (live && v < nvec) atomicMax(gmax + v / kNormGroup, abs_bits(h[i][0]));
-      }
-      __syncthreads();
+        for (int i = 0; i < NV; ++i) {
+          uint32_t m = 0;
 #pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        const int v = i * a.tpr + lane;
-        if (live && v < nvec) {
+          for (int e = 0; e < VEC; ++e) m = max(m, abs_bits(h[i][e]));
+          for (int o = gl / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
           float inv;
-          const float scale = fp8_scale(gmax[v / kNormGroup], &inv);
-          if (v % kNormGroup == 0) a.scale[row * groups + v / kNormGroup] = scale;
-          h[i][0] *= inv;
-          store_fp8<1>(q + v, h[i]);
+          const float scale = fp8_scale(m, &inv);
+          if (live && span.has(i)) {
+            const int v = i * a.tpr + lane;
+            if (v % gl == 0) a.scale[row * groups + v / gl] = scale;
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) h[i][e] *= inv;
+            store(i);
+          }
+        }
+      } else {
+        // A vector may reach into two groups, and groups do not begin at a
+        // lane: the maxima meet in shared memory (they do not depend on the
+        // order).
+        uint32_t* gmax = reinterpret_cast<uint32_t*>(smem_raw + 512) + sub * groups;
+        __syncthreads();
+        for (int k = lane; k < groups; k += a.tpr) gmax[k] = 0;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+          if (live && span.has(i)) {
+            const int lo = max(span.col(i), 0) / kNormGroup, hi = (min(span.col(i) + VEC, a.width) - 1) / kNormGroup;
+            const int edge = (lo + 1) * kNormGroup - span.col(i);  // elements from here on are of the next group
+            uint32_t m0 = 0, m1 = 0;
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+              const uint32_t m = span.owns(i, e) ? abs_bits(h[i][e]) : 0u;
+              if (e < edge) m0 = max(m0, m);
+              else m1 = max(m1, m);
+            }
+            atomicMax(gmax + lo, m0);
+            if (hi != lo) atomicMax(gmax + hi, m1);
+          }
+        }
+        __syncthreads();
+        if (live)
+          for (int k = lane; k < groups; k += a.tpr) {
+            float inv;
+            a.scale[row * groups + k] = fp8_scale(gmax[k], &inv);
+          }
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+          if (live && span.has(i)) {
+            const int lo = max(span.col(i), 0) / kNormGroup, hi = (min(span.col(i) + VEC, a.width) - 1) / kNormGroup;
+            const int edge = (lo + 1) * kNormGroup - span.col(i);
+            float inv0, inv1;
+            fp8_scale(gmax[lo], &inv0);
+            fp8_scale(gmax[hi], &inv1);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) h[i][e] *= e < edge ? inv0 : inv1;
+            store(i);
+          }
         }
       }
     }
@@ -198,7 +329,8 @@ struct NormBwdArgs {
   int64_t rows;
   int width;
   int tpr;
-  const void* h;
+  const void* x;
+  const void* r;  // null: no residual
   const float* rstd;
   const void* w;   // null: ones
   const void* gy;
@@ -207,86 +339,136 @@ struct NormBwdArgs {
   float* part;     // null: no weight gradient; else [gridDim.x][width]
 };
 
-// A block takes rows blockIdx.x * rows-per-block + k * gridDim.x * ..., its
-// threads keep their columns' share of dw in registers, and the block's sum
-// over its row groups (through shared memory, in order) is one row of `part`.
-template <class T, class W, int VEC, int NV>
-__global__ void __launch_bounds__(1024) rms_norm_bwd_kernel(const NormBwdArgs a) {
-  extern __shared__ float smem[];  // 64 floats, then [row groups][width] if there are several
+// A block's threads keep their columns' share of dw in registers; the block's
+// sum over its row groups (through shared memory, in order) is one row of
+// `part`.  A row's vectors are read from their slots twice (before and after
+// the row's sum) instead of being kept in registers.  PIPE false, for rows whose
+// slots do not fit: they are read from global memory, the second time from L2.
+// Shared memory: 64 floats, then the slots [stage][x, gy, r, gh][i][thread], which
+// the sum over the row groups takes over at the end.
+template <class T, class W, int NV, bool RAGGED, bool PIPE, int MAXT>
+__global__ void __launch_bounds__(MAXT, MAXT == 256 ? 2 : 1) rms_norm_bwd_kernel(const NormBwdArgs a, int stages) {
+  using Span = RowSpan<T, NV, RAGGED>;
+  constexpr int VEC = Span::VEC;
+  extern __shared__ __align__(16) uint8_t smem_raw[];
+  float* red = reinterpret_cast<float*>(smem_raw);
   pdl_enter();
-  const int lane = threadIdx.x % a.tpr;
-  const int sub = threadIdx.x / a.tpr, subs = blockDim.x / a.tpr;
-  const int nvec = a.width / VEC;
-  const W* w = static_cast<const W*>(a.w);
-  float dw[NV][VEC];
+  const int lane = threadIdx.x % a.tpr, sub = threadIdx.x / a.tpr, subs = blockDim.x / a.tpr;
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * subs + sub;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * subs;
+  const Span span(a.rows, a.width, a.tpr, lane, first);
+  const T* in[4] = {static_cast<const T*>(a.x), static_cast<const T*>(a.gy), static_cast<const T*>(a.r),
+                    static_cast<const T*>(a.gh)};
+  const int streams = 2 + (a.r != nullptr) + (a.gh != nullptr);
+  const int gh_slot = a.r ? 3 : 2;
+  Raw<T, VEC>* slots = reinterpret_cast<Raw<T, VEC>*>(smem_raw + 256) + threadIdx.x;
+  auto slot = [&](int stage, int stream, int i) { return slots + ((stage * streams + stream) * NV + i) * blockDim.x; };
+  auto fetch = [&](int64_t row, int stage) {
+    if (row < a.rows) {
 #pragma unroll
-  for (int i = 0; i < NV; ++i)
+      for (int i = 0; i < NV; ++i)
+        if (span.has(i)) {
+          const int n = span.bytes(row, i);
+          cp_async16(slot(stage, 0, i), in[0] + span.at(row, i), n);
+          cp_async16(slot(stage, 1, i), in[1] + span.at(row, i), n);
+          if (in[2]) cp_async16(slot(stage, 2, i), in[2] + span.at(row, i), n);
+          if (in[3]) cp_async16(slot(stage, gh_slot, i), in[3] + span.at(row, i), n);
+        }
+    }
+    cp_async_commit();
+  };
+  float dw[NV][VEC];
+  Raw<W, VEC> w[NV];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
 #pragma unroll
     for (int e = 0; e < VEC; ++e) dw[i][e] = 0.0f;
+    if (span.has(i)) span.weights(static_cast<const W*>(a.w), i, w[i]);
+  }
+  if constexpr (PIPE)
+    for (int k = 0; k < stages; ++k) fetch(first + k * step, k);
 
-  int half = 0;
-  for (int64_t row0 = static_cast<int64_t>(blockIdx.x) * subs; row0 < a.rows;
-       row0 += static_cast<int64_t>(gridDim.x) * subs, half ^= 1) {
+  int half = 0, stage = 0;
+  for (int64_t row0 = first - sub; row0 < a.rows; row0 += step, half ^= 1) {
     const int64_t row = row0 + sub;
     const bool live = row < a.rows;
-    const int64_t base = row * a.width;
     const float s = live ? a.rstd[row] : 0.0f;
-    float n[NV][VEC], g[NV][VEC];
+    if constexpr (PIPE) cp_async_wait_upto(stages - 1);
+    // n and G w of vector i, and G
+    auto terms = [&](int i, float (&n)[VEC], float (&gw)[VEC], float (&g)[VEC]) {
+      unpack(PIPE ? *slot(stage, 0, i) : span.load(in[0], row, i), n);
+      unpack(PIPE ? *slot(stage, 1, i) : span.load(in[1], row, i), g);
+      if (in[2]) {
+        float f[VEC];
+        unpack(PIPE ? *slot(stage, 2, i) : span.load(in[2], row, i), f);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) n[e] += f[e];
+      }
+      float f[VEC];
+      unpack(w[i], f);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        if (RAGGED && !span.owns(i, e)) n[e] = g[e] = 0.0f;
+        n[e] *= s;
+        gw[e] = g[e] * f[e];
+      }
+    };
     float sum = 0.0f;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int v = i * a.tpr + lane;
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) n[i][e] = g[i][e] = 0.0f;
-      if (live && v < nvec) {
-        unpack(load_raw<T, VEC>(static_cast<const T*>(a.h) + base + v * VEC), n[i]);
-        unpack(load_raw<T, VEC>(static_cast<const T*>(a.gy) + base + v * VEC), g[i]);
-        float f[VEC];
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) f[e] = 1.0f;
-        if (w) unpack(load_raw<W, VEC>(w + v * VEC), f);
+    for (int i = 0; i < NV; ++i)
+      if (live && span.has(i)) {
+        float n[VEC], gw[VEC], g[VEC];
+        terms(i, n, gw, g);
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
-          n[i][e] *= s;
-          dw[i][e] += g[i][e] * n[i][e];
-          g[i][e] *= f[e];
-          sum += g[i][e] * n[i][e];
+          dw[i][e] += g[e] * n[e];
+          sum += gw[e] * n[e];
         }
       }
-    }
-    const float c = norm_row_sum(sum, a.tpr, smem, half) / static_cast<float>(a.width);
+    const float c = norm_row_sum(sum, a.tpr, red, half) / static_cast<float>(a.width);
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int v = i * a.tpr + lane;
-      if (live && v < nvec) {
-        float f[VEC];
+    for (int i = 0; i < NV; ++i)
+      if (live && span.has(i)) {
+        float n[VEC], gw[VEC], g[VEC];
+        terms(i, n, gw, g);
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) f[e] = 0.0f;
-        if (a.gh) unpack(load_raw<T, VEC>(static_cast<const T*>(a.gh) + base + v * VEC), f);
+        for (int e = 0; e < VEC; ++e) g[e] = 0.0f;
+        if (in[3]) unpack(PIPE ? *slot(stage, gh_slot, i) : span.load(in[3], row, i), g);
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) f[e] += s * (g[i][e] - n[i][e] * c);
-        store_vec<T, VEC>(static_cast<T*>(a.dx) + base + v * VEC, f);
+        for (int e = 0; e < VEC; ++e) g[e] += s * (gw[e] - n[e] * c);
+        span.store(static_cast<T*>(a.dx), row, i, g);
       }
+    if constexpr (PIPE) {
+      fetch(row + stages * step, stage);
+      stage = stage + 1 == stages ? 0 : stage + 1;
     }
   }
   if (!a.part) return;
   float* out = a.part + static_cast<int64_t>(blockIdx.x) * a.width;
   if (subs == 1) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int v = i * a.tpr + lane;
-      if (v < nvec) store_vec<float, VEC>(out + v * VEC, dw[i]);
-    }
+    for (int i = 0; i < NV; ++i)
+      if (span.has(i)) {
+        if (!RAGGED) {
+          store_vec<float, VEC>(out + span.col(i), dw[i]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < VEC; ++e)
+            if (span.owns(i, e)) out[span.col(i) + e] = dw[i][e];
+        }
+      }
     return;
   }
-  float* acc = smem + 64;
+  float* acc = red + 64;  // [row groups][width]
+  cp_async_wait<0>();
+  __syncthreads();  // the slots are free
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int v = i * a.tpr + lane;
-    if (v < nvec)
+  for (int i = 0; i < NV; ++i)
+    if (span.has(i)) {
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) acc[sub * a.width + v * VEC + e] = dw[i][e];
-  }
+      for (int e = 0; e < VEC; ++e)
+        if (span.owns(i, e)) acc[sub * a.width + span.col(i) + e] = dw[i][e];
+    }
   __syncthreads();
   for (int j = threadIdx.x; j < a.width; j += blockDim.x) {
     float t = 0.0f;

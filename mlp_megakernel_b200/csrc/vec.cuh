@@ -54,6 +54,28 @@ __device__ __forceinline__ void store_vec(T* p, const float (&f)[VEC]) {
   *reinterpret_cast<Raw<T, VEC>*>(p) = r;
 }
 
+// A 16-byte copy from global to shared memory that the thread waits for later;
+// `bytes` of it are read, the rest are zeros.  A thread that reads back only
+// what it copied itself needs no barrier, just cp_async_wait.
+__device__ __forceinline__ void cp_async16(void* smem, const void* global, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
+                   static_cast<uint32_t>(__cvta_generic_to_shared(smem))),
+               "l"(global), "r"(bytes)
+               : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// Until all but the N youngest groups of this thread have arrived.
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void cp_async_wait_upto(int n) {  // n from 0 to 3
+  if (n >= 3) cp_async_wait<3>();
+  else if (n == 2) cp_async_wait<2>();
+  else if (n == 1) cp_async_wait<1>();
+  else cp_async_wait<0>();
+}
+
 // The 8-bit type: 4 exponent bits, 3 of mantissa (e4m3), largest value 448,
 // smallest positive one 2^-9.
 constexpr float kFp8Max = 448.0f;

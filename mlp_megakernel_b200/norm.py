@@ -86,24 +86,25 @@ def _forward(x, weight, residual, eps, want_rstd):
 
 
 @_on_device
-def _backward(h, weight, rstd, grad_y, grad_h, want_dw):
+def _backward(x, residual, weight, rstd, grad_y, grad_h, want_dw):
     """(dx, dw): dw in weight's dtype, None unless wanted."""
-    h, grad_y = _aligned(h), _aligned(grad_y)
+    x, grad_y = _aligned(x), _aligned(grad_y)
+    residual = None if residual is None else _aligned(residual)
     grad_h = None if grad_h is None else _aligned(grad_h)
     weight = None if weight is None else _aligned(weight)
-    width = h.shape[-1]
-    rows = h.numel() // width
-    dx = torch.empty_like(h)
+    width = x.shape[-1]
+    rows = x.numel() // width
+    dx = torch.empty_like(x)
     dw = work = None
     lib = _lib.lib()
     if want_dw:
         dw = torch.empty_like(weight)
-        size = lib.mlpk_rms_norm_bwd_workspace_size(rows, width, DTYPES[h.dtype])
-        work = torch.empty(max(size, 16), device=h.device, dtype=torch.uint8)
+        size = lib.mlpk_rms_norm_bwd_workspace_size(rows, width, DTYPES[x.dtype])
+        work = torch.empty(max(size, 16), device=x.device, dtype=torch.uint8)
     _lib.check("mlpk_rms_norm_bwd", lib.mlpk_rms_norm_bwd(
-        rows, width, DTYPES[h.dtype], h.data_ptr(), rstd.data_ptr(), _ptr(weight), _w_dtype(weight, h),
-        grad_y.data_ptr(), _ptr(grad_h), dx.data_ptr(), _ptr(dw), _ptr(work), 0 if work is None else work.numel(),
-        _current_stream(h.get_device())))
+        rows, width, DTYPES[x.dtype], x.data_ptr(), _ptr(residual), rstd.data_ptr(), _ptr(weight),
+        _w_dtype(weight, x), grad_y.data_ptr(), _ptr(grad_h), dx.data_ptr(), _ptr(dw), _ptr(work),
+        0 if work is None else work.numel(), _current_stream(x.get_device())))
     return dx, dw
 
 
@@ -141,16 +142,16 @@ def _rms_norm_fake(x, weight, residual, eps):
 
 
 @torch.library.custom_op("mlpk::rms_norm_bwd", mutates_args=())
-def rms_norm_bwd(h: Tensor, weight: Optional[Tensor], rstd: Tensor, grad_y: Tensor, grad_h: Optional[Tensor],
-                 want_dw: bool) -> list[Tensor]:
+def rms_norm_bwd(x: Tensor, residual: Optional[Tensor], weight: Optional[Tensor], rstd: Tensor, grad_y: Tensor,
+                 grad_h: Optional[Tensor], want_dw: bool) -> list[Tensor]:
     """[dx], and dw if wanted."""
-    dx, dw = _backward(h, weight, rstd, grad_y, grad_h, want_dw)
+    dx, dw = _backward(x, residual, weight, rstd, grad_y, grad_h, want_dw)
     return [dx] if dw is None else [dx, dw]
 
 
 @rms_norm_bwd.register_fake
-def _rms_norm_bwd_fake(h, weight, rstd, grad_y, grad_h, want_dw):
-    return [h.new_empty(h.shape)] + ([weight.new_empty(weight.shape)] if want_dw else [])
+def _rms_norm_bwd_fake(x, residual, weight, rstd, grad_y, grad_h, want_dw):
+    return [x.new_empty(x.shape)] + ([weight.new_empty(weight.shape)] if want_dw else [])
 
 
 @torch.library.custom_op("mlpk::rms_norm_fp8", mutates_args=())
@@ -176,28 +177,26 @@ class _RMSNormFn(torch.autograd.Function):
     def forward(ctx, x, weight, residual, eps):
         if torch.compiler.is_compiling() or _is_fake(x):
             y, rstd, *rest = torch.ops.mlpk.rms_norm(x, weight, residual, eps)
-            h = rest[0] if rest else x
+            h = rest[0] if rest else None
         else:
             y, h, rstd = _forward(x, weight, residual, eps, True)
-        ctx.has_weight = weight is not None
         ctx.has_residual = residual is not None
         ctx.set_materialize_grads(False)
-        ctx.save_for_backward(h, rstd, *([weight] if ctx.has_weight else []))
+        ctx.save_for_backward(x, residual, weight, rstd)
         return (y, h) if ctx.has_residual else y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad_y, grad_h=None):
-        h, rstd, *rest = ctx.saved_tensors
-        weight = rest[0] if rest else None
-        want_dw = ctx.has_weight and ctx.needs_input_grad[1]
+        x, residual, weight, rstd = ctx.saved_tensors
+        want_dw = weight is not None and ctx.needs_input_grad[1]
         if grad_y is None:  # y was not used: the norm adds nothing
             dx, dw = grad_h, torch.zeros_like(weight) if want_dw and grad_h is not None else None
-        elif torch.compiler.is_compiling() or _is_fake(h):
-            dx, *dws = torch.ops.mlpk.rms_norm_bwd(h, weight, rstd, grad_y, grad_h, want_dw)
+        elif torch.compiler.is_compiling() or _is_fake(x):
+            dx, *dws = torch.ops.mlpk.rms_norm_bwd(x, residual, weight, rstd, grad_y, grad_h, want_dw)
             dw = dws[0] if dws else None
         else:
-            dx, dw = _backward(h, weight, rstd, grad_y, grad_h, want_dw)
+            dx, dw = _backward(x, residual, weight, rstd, grad_y, grad_h, want_dw)
         return (dx if ctx.needs_input_grad[0] else None, dw,
                 dx if ctx.has_residual and ctx.needs_input_grad[2] else None, None)
 

@@ -123,8 +123,8 @@ def test_c_calls_refuse_before_they_touch_the_device(built_lib):
         assert lib.mlpk_rms_norm(*args) == want
     assert lib.mlpk_rms_norm_fp8(4, 8, 0, a, None, None, 0, 1e-6, 64, a, a, None, None) == un
     assert lib.mlpk_rms_norm_fp8(4, 8, 0, a, None, None, 0, 1e-6, 0, a, None, None, None) == nu
-    assert lib.mlpk_rms_norm_bwd(4, 8, 0, a, a, None, 0, a, None, a, a, a, 1 << 20, None) == nu  # dw without a weight
-    assert lib.mlpk_rms_norm_bwd(4, 8, 0, a, a, a, 0, a, None, a, a, None, 0, None) == nu
+    assert lib.mlpk_rms_norm_bwd(4, 8, 0, a, None, a, None, 0, a, None, a, a, a, 1 << 20, None) == nu  # no weight for dw
+    assert lib.mlpk_rms_norm_bwd(4, 8, 0, a, None, a, a, 0, a, None, a, a, None, 0, None) == nu
     assert lib.mlpk_expert_sort(-1, 4, a, 8, a, a, a, 1 << 20, None) == sh
     assert lib.mlpk_expert_sort(8, 2000, a, 8, a, a, a, 1 << 20, None) == un
     assert lib.mlpk_expert_sort(8, 4, a, 2, a, a, a, 1 << 20, None) == un
