@@ -22,7 +22,8 @@ LIB = os.path.join(LIBDIR, "libmlpk.so")
 SOURCES = {
     "mlpk_api.cu": ["host.cuh", "pdl.cuh", "ptx.cuh", "layout.cuh", "softplus.cuh", "fwd_kernel.cuh", "bwd_kernel.cuh",
                     "wn_kernel.cuh", "stream_kernel.cuh", "wgrad_kernel.cuh", "peer_kernel.cuh", "cast_kernel.cuh"],
-    "norm_api.cu": ["host.cuh", "pdl.cuh", "vec.cuh", "norm_kernel.cuh"],
+    **{f"norm_{part}.cu": ["host.cuh", "pdl.cuh", "vec.cuh", "norm_kernel.cuh", "norm_launch.cuh"]
+       for part in ("api", "f16", "bf16", "f32")},
     "expert_api.cu": ["host.cuh", "pdl.cuh", "vec.cuh", "expert_kernel.cuh"],
     "adamw_api.cu": ["host.cuh", "pdl.cuh", "vec.cuh", "adamw_kernel.cuh"],
 }

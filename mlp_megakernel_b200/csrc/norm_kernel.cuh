@@ -39,9 +39,14 @@ constexpr int kNormGroup = 128;    // columns that share a scale
 constexpr int kNormMaxWidth = 32768;
 constexpr int kNormStages = 4;     // rows that a thread has under way, at most
 
-// Sum of v over the row's threads.  TPR > 32: `red` has two halves of a float
-// per warp, used in turn (`half`), so one barrier separates a write from the
-// reads of the call before the last.
+// Sum of v over the row's threads.  TPR > 32: `red` has two halves of 32 floats,
+// one a warp (the others zero, norm_row_init), used in turn (`half`), so one
+// barrier separates a write from the reads of the call before the last.
+__device__ __forceinline__ void norm_row_init(float* red, int n, int tpr) {
+  if (tpr <= 32) return;
+  for (int k = threadIdx.x; k < n; k += blockDim.x) red[k] = 0.0f;
+  __syncthreads();
+}
 __device__ __forceinline__ float norm_row_sum(float v, int tpr, float* red, int half) {
   if (tpr <= 32) {
     for (int o = tpr / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
@@ -52,10 +57,12 @@ __device__ __forceinline__ float norm_row_sum(float v, int tpr, float* red, int 
   red += half * 32;
   if (threadIdx.x % 32 == 0) red[threadIdx.x / 32] = v;
   __syncthreads();
-  // Each warp adds the warps' sums the same way.
-  v = threadIdx.x % 32 < tpr / 32 ? red[threadIdx.x % 32] : 0.0f;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  // Every thread adds the warps' sums in the same order.
+  v = 0.0f;
+  for (int k = 0; k < tpr / 32; k += 4) {
+    const float4 t = *reinterpret_cast<const float4*>(red + k);  // 32 floats a half: those of no warp stay zero
+    v += (t.x + t.y) + (t.z + t.w);
+  }
   return v;
 }
 
@@ -65,9 +72,11 @@ __device__ __forceinline__ uint32_t norm_row_max(uint32_t v, int tpr, float* red
   uint32_t* r = reinterpret_cast<uint32_t*>(red) + half * 32;
   if (threadIdx.x % 32 == 0) r[threadIdx.x / 32] = v;
   __syncthreads();
-  v = threadIdx.x % 32 < tpr / 32 ? r[threadIdx.x % 32] : 0u;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, o));
+  v = 0;
+  for (int k = 0; k < tpr / 32; k += 4) {
+    const uint4 t = *reinterpret_cast<const uint4*>(r + k);
+    v = max(v, max(max(t.x, t.y), max(t.z, t.w)));
+  }
   return v;
 }
 
@@ -86,36 +95,36 @@ struct RowSpan {
   }
   __device__ bool has(int i) const { return i * tpr + lane < nvec; }
   __device__ int col(int i) const { return (i * tpr + lane) * VEC - shift; }  // of element 0; may be below 0
-  __device__ int64_t at(int64_t row, int i) const { return row * width + col(i); }  // a multiple of VEC
+  __device__ int64_t at(int64_t begin, int i) const { return begin + col(i); }  // begin = row * width; a multiple of VEC
   __device__ bool owns(int i, int e) const {
     return !RAGGED || static_cast<unsigned>(col(i) + e) < static_cast<unsigned>(width);
   }
   __device__ bool whole(int i) const { return !RAGGED || (col(i) >= 0 && col(i) + VEC <= width); }
   // Bytes of the vector that lie inside the tensor.
-  __device__ int bytes(int64_t row, int i) const {
+  __device__ int bytes(int64_t begin, int i) const {
     if (!RAGGED) return 16;
-    const int64_t left = total - at(row, i);
+    const int64_t left = total - at(begin, i);
     return left >= VEC ? 16 : static_cast<int>(left) * static_cast<int>(sizeof(T));
   }
-  __device__ Raw<T, VEC> load(const T* p, int64_t row, int i) const {
+  __device__ Raw<T, VEC> load(const T* p, int64_t begin, int i) const {
     if constexpr (RAGGED) {
-      if (total - at(row, i) < VEC) {
+      if (total - at(begin, i) < VEC) {
         Raw<T, VEC> r;
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) r.v[e] = at(row, i) + e < total ? p[at(row, i) + e] : from_float<T>(0.0f);
+        for (int e = 0; e < VEC; ++e) r.v[e] = at(begin, i) + e < total ? p[at(begin, i) + e] : from_float<T>(0.0f);
         return r;
       }
     }
-    return load_raw<T, VEC>(p + at(row, i));
+    return load_raw<T, VEC>(p + at(begin, i));
   }
-  __device__ void store(T* p, int64_t row, int i, const float (&f)[VEC]) const {
+  __device__ void store(T* p, int64_t begin, int i, const float (&f)[VEC]) const {
     if (whole(i)) {
-      store_vec<T, VEC>(p + at(row, i), f);
+      store_vec<T, VEC>(p + at(begin, i), f);
       return;
     }
 #pragma unroll
     for (int e = 0; e < VEC; ++e)
-      if (owns(i, e)) p[at(row, i) + e] = from_float<T>(f[e]);
+      if (owns(i, e)) p[at(begin, i) + e] = from_float<T>(f[e]);
   }
   // The weight's values of the vector's columns; ones without a weight.
   template <class W>
@@ -126,6 +135,32 @@ struct RowSpan {
     }
 #pragma unroll
     for (int e = 0; e < VEC; ++e) r.v[e] = w && owns(i, e) ? w[col(i) + e] : from_float<W>(1.0f);
+  }
+};
+
+// A thread's weights: as floats where the registers allow it, else as they lie
+// in memory.
+template <class T, class W, int NV, bool FLOATS>
+struct NormWeights {
+  static constexpr int VEC = kVecOf<T>;
+  Raw<W, VEC> raw[FLOATS ? 1 : NV];
+  float f32[FLOATS ? NV : 1][VEC];
+  template <class Span>
+  __device__ void load(const Span& span, const W* w) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      if (span.has(i)) {
+        span.weights(w, i, raw[FLOATS ? 0 : i]);
+        if constexpr (FLOATS) unpack(raw[0], f32[i]);
+      }
+  }
+  __device__ void get(int i, float (&f)[VEC]) const {
+    if constexpr (FLOATS) {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) f[e] = f32[i][e];
+    } else {
+      unpack(raw[i], f);
+    }
   }
 };
 
@@ -161,30 +196,33 @@ __global__ void __launch_bounds__(MAXT) rms_norm_fwd_kernel(const NormArgs a, in
   const T* r = static_cast<const T*>(a.r);
   const int streams = r ? 2 : 1;
   Raw<T, VEC>* slots = reinterpret_cast<Raw<T, VEC>*>(smem_raw + slots_at) + threadIdx.x;
-  auto slot = [&](int stage, int stream, int i) { return slots + ((stage * streams + stream) * NV + i) * blockDim.x; };
-  auto fetch = [&](int64_t row, int stage) {
-    if (row < a.rows) {
+  const int stage_slots = streams * NV * blockDim.x;  // `stage` counts them
+  auto slot = [&](int stage, int stream, int i) { return slots + (stage + (stream * NV + i) * blockDim.x); };
+  auto fetch = [&](int64_t begin, int stage) {
+    if (begin < span.total) {
 #pragma unroll
       for (int i = 0; i < NV; ++i)
         if (span.has(i)) {
-          cp_async16(slot(stage, 0, i), x + span.at(row, i), span.bytes(row, i));
-          if (r) cp_async16(slot(stage, 1, i), r + span.at(row, i), span.bytes(row, i));
+          cp_async16(slot(stage, 0, i), x + span.at(begin, i), span.bytes(begin, i));
+          if (r) cp_async16(slot(stage, 1, i), r + span.at(begin, i), span.bytes(begin, i));
         }
     }
     cp_async_commit();
   };
+  const int64_t begin_step = step * a.width;
+  int64_t begin = first * a.width;
   if constexpr (PIPE)
-    for (int k = 0; k < stages; ++k) fetch(first + k * step, k);
-  Raw<W, VEC> w[NV];
-#pragma unroll
-  for (int i = 0; i < NV; ++i)
-    if (span.has(i)) span.weights(static_cast<const W*>(a.w), i, w[i]);
+    for (int k = 0; k < stages; ++k) fetch(begin + k * begin_step, k * stage_slots);
+  NormWeights<T, W, NV, (NV <= 2)> w;
+  w.load(span, static_cast<const W*>(a.w));
+  norm_row_init(red, 128, a.tpr);
 
   int stage = 0, half = 0;
+  const float inv_width = 1.0f / static_cast<float>(a.width);
   // Whole blocks loop together: the last rows' missing ones take part in the
   // shuffles and barriers.
-  for (int64_t row0 = first - sub; row0 < a.rows; row0 += step, half ^= 1) {
-    const int64_t row = row0 + sub;
+  int64_t row = first;
+  for (int64_t row0 = first - sub; row0 < a.rows; row0 += step, row += step, begin += begin_step, half ^= 1) {
     const bool live = row < a.rows;
     if constexpr (PIPE) cp_async_wait_upto(stages - 1);
     float h[NV][VEC];
@@ -194,10 +232,10 @@ __global__ void __launch_bounds__(MAXT) rms_norm_fwd_kernel(const NormArgs a, in
 #pragma unroll
       for (int e = 0; e < VEC; ++e) h[i][e] = 0.0f;
       if (live && span.has(i)) {
-        unpack(PIPE ? *slot(stage, 0, i) : span.load(x, row, i), h[i]);
+        unpack(PIPE ? *slot(stage, 0, i) : span.load(x, begin, i), h[i]);
         if (r) {
           float f[VEC];
-          unpack(PIPE ? *slot(stage, 1, i) : span.load(r, row, i), f);
+          unpack(PIPE ? *slot(stage, 1, i) : span.load(r, begin, i), f);
 #pragma unroll
           for (int e = 0; e < VEC; ++e) h[i][e] += f[e];
         }
@@ -211,29 +249,29 @@ __global__ void __launch_bounds__(MAXT) rms_norm_fwd_kernel(const NormArgs a, in
       for (int e = 0; e < VEC; ++e) sum += h[i][e] * h[i][e];
     }
     if constexpr (PIPE) {
-      fetch(row + stages * step, stage);
-      stage = stage + 1 == stages ? 0 : stage + 1;
+      fetch(begin + stages * begin_step, stage);
+      stage = stage + stage_slots == stages * stage_slots ? 0 : stage + stage_slots;
     }
-    const float s = rsqrtf(norm_row_sum(sum, a.tpr, red, half) / static_cast<float>(a.width) + a.eps);
+    const float s = rsqrtf(norm_row_sum(sum, a.tpr, red, half) * inv_width + a.eps);
     if (a.rstd && live && lane == 0) a.rstd[row] = s;
     uint32_t amax = 0;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       if (live && span.has(i)) {
-        if (a.h) span.store(static_cast<T*>(a.h), row, i, h[i]);
+        if (a.h) span.store(static_cast<T*>(a.h), begin, i, h[i]);
         float f[VEC];
-        unpack(w[i], f);
+        w.get(i, f);
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
           h[i][e] = h[i][e] * s * f[e];
           if (FP8) amax = max(amax, abs_bits(h[i][e]));
         }
-        if constexpr (!FP8) span.store(static_cast<T*>(a.y), row, i, h[i]);
+        if constexpr (!FP8) span.store(static_cast<T*>(a.y), begin, i, h[i]);
       }
     }
     if constexpr (FP8) {
       auto store = [&](int i) {
-        uint8_t* q = static_cast<uint8_t*>(a.y) + span.at(row, i);
+        uint8_t* q = static_cast<uint8_t*>(a.y) + span.at(begin, i);
         if (span.whole(i)) {
           store_fp8<VEC>(q, h[i]);
           return;
@@ -341,15 +379,17 @@ struct NormBwdArgs {
 
 // A block's threads keep their columns' share of dw in registers; the block's
 // sum over its row groups (through shared memory, in order) is one row of
-// `part`.  A row's vectors are read from their slots twice (before and after
-// the row's sum) instead of being kept in registers.  PIPE false, for rows whose
-// slots do not fit: they are read from global memory, the second time from L2.
+// `part`.  With 4 or more vectors a thread, a row's vectors are read from their
+// slots twice (before and after the row's sum) instead of being kept in
+// registers; rows without slots (PIPE false) are read from global memory, the
+// second time from L2.
 // Shared memory: 64 floats, then the slots [stage][x, gy, r, gh][i][thread], which
 // the sum over the row groups takes over at the end.
 template <class T, class W, int NV, bool RAGGED, bool PIPE, int MAXT>
 __global__ void __launch_bounds__(MAXT, MAXT == 256 ? 2 : 1) rms_norm_bwd_kernel(const NormBwdArgs a, int stages) {
   using Span = RowSpan<T, NV, RAGGED>;
   constexpr int VEC = Span::VEC;
+  constexpr bool KEEP = NV <= 2;
   extern __shared__ __align__(16) uint8_t smem_raw[];
   float* red = reinterpret_cast<float*>(smem_raw);
   pdl_enter();
@@ -362,50 +402,56 @@ __global__ void __launch_bounds__(MAXT, MAXT == 256 ? 2 : 1) rms_norm_bwd_kernel
   const int streams = 2 + (a.r != nullptr) + (a.gh != nullptr);
   const int gh_slot = a.r ? 3 : 2;
   Raw<T, VEC>* slots = reinterpret_cast<Raw<T, VEC>*>(smem_raw + 256) + threadIdx.x;
-  auto slot = [&](int stage, int stream, int i) { return slots + ((stage * streams + stream) * NV + i) * blockDim.x; };
-  auto fetch = [&](int64_t row, int stage) {
-    if (row < a.rows) {
+  const int stage_slots = streams * NV * blockDim.x;  // `stage` counts them
+  auto slot = [&](int stage, int stream, int i) { return slots + (stage + (stream * NV + i) * blockDim.x); };
+  auto fetch = [&](int64_t begin, int stage) {
+    if (begin < span.total) {
 #pragma unroll
       for (int i = 0; i < NV; ++i)
         if (span.has(i)) {
-          const int n = span.bytes(row, i);
-          cp_async16(slot(stage, 0, i), in[0] + span.at(row, i), n);
-          cp_async16(slot(stage, 1, i), in[1] + span.at(row, i), n);
-          if (in[2]) cp_async16(slot(stage, 2, i), in[2] + span.at(row, i), n);
-          if (in[3]) cp_async16(slot(stage, gh_slot, i), in[3] + span.at(row, i), n);
+          const int n = span.bytes(begin, i);
+          cp_async16(slot(stage, 0, i), in[0] + span.at(begin, i), n);
+          cp_async16(slot(stage, 1, i), in[1] + span.at(begin, i), n);
+          if (in[2]) cp_async16(slot(stage, 2, i), in[2] + span.at(begin, i), n);
+          if (in[3]) cp_async16(slot(stage, gh_slot, i), in[3] + span.at(begin, i), n);
         }
     }
     cp_async_commit();
   };
+  const int64_t begin_step = step * a.width;
+  int64_t begin = first * a.width;
+  if constexpr (PIPE)
+    for (int k = 0; k < stages; ++k) fetch(begin + k * begin_step, k * stage_slots);
   float dw[NV][VEC];
-  Raw<W, VEC> w[NV];
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
+  for (int i = 0; i < NV; ++i)
 #pragma unroll
     for (int e = 0; e < VEC; ++e) dw[i][e] = 0.0f;
-    if (span.has(i)) span.weights(static_cast<const W*>(a.w), i, w[i]);
-  }
-  if constexpr (PIPE)
-    for (int k = 0; k < stages; ++k) fetch(first + k * step, k);
+  NormWeights<T, W, NV, KEEP> w;
+  w.load(span, static_cast<const W*>(a.w));
+  norm_row_init(red, 64, a.tpr);
 
   int half = 0, stage = 0;
-  for (int64_t row0 = first - sub; row0 < a.rows; row0 += step, half ^= 1) {
-    const int64_t row = row0 + sub;
+  int64_t row = first;
+  const float inv_width = 1.0f / static_cast<float>(a.width);
+  float s_next = row < a.rows ? a.rstd[row] : 0.0f;
+  for (int64_t row0 = first - sub; row0 < a.rows; row0 += step, row += step, begin += begin_step, half ^= 1) {
     const bool live = row < a.rows;
-    const float s = live ? a.rstd[row] : 0.0f;
+    const float s = s_next;  // the next row's is on its way while this one is worked on
+    s_next = row + step < a.rows ? a.rstd[row + step] : 0.0f;
     if constexpr (PIPE) cp_async_wait_upto(stages - 1);
     // n and G w of vector i, and G
     auto terms = [&](int i, float (&n)[VEC], float (&gw)[VEC], float (&g)[VEC]) {
-      unpack(PIPE ? *slot(stage, 0, i) : span.load(in[0], row, i), n);
-      unpack(PIPE ? *slot(stage, 1, i) : span.load(in[1], row, i), g);
+      unpack(PIPE ? *slot(stage, 0, i) : span.load(in[0], begin, i), n);
+      unpack(PIPE ? *slot(stage, 1, i) : span.load(in[1], begin, i), g);
       if (in[2]) {
         float f[VEC];
-        unpack(PIPE ? *slot(stage, 2, i) : span.load(in[2], row, i), f);
+        unpack(PIPE ? *slot(stage, 2, i) : span.load(in[2], begin, i), f);
 #pragma unroll
         for (int e = 0; e < VEC; ++e) n[e] += f[e];
       }
       float f[VEC];
-      unpack(w[i], f);
+      w.get(i, f);
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
         if (RAGGED && !span.owns(i, e)) n[e] = g[e] = 0.0f;
@@ -413,34 +459,35 @@ __global__ void __launch_bounds__(MAXT, MAXT == 256 ? 2 : 1) rms_norm_bwd_kernel
         gw[e] = g[e] * f[e];
       }
     };
+    float n[KEEP ? NV : 1][VEC], gw[KEEP ? NV : 1][VEC], g[VEC];
     float sum = 0.0f;
 #pragma unroll
     for (int i = 0; i < NV; ++i)
       if (live && span.has(i)) {
-        float n[VEC], gw[VEC], g[VEC];
-        terms(i, n, gw, g);
+        const int k = KEEP ? i : 0;
+        terms(i, n[k], gw[k], g);
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
-          dw[i][e] += g[e] * n[e];
-          sum += gw[e] * n[e];
+          dw[i][e] += g[e] * n[k][e];
+          sum += gw[k][e] * n[k][e];
         }
       }
-    const float c = norm_row_sum(sum, a.tpr, red, half) / static_cast<float>(a.width);
+    const float c = norm_row_sum(sum, a.tpr, red, half) * inv_width;
 #pragma unroll
     for (int i = 0; i < NV; ++i)
       if (live && span.has(i)) {
-        float n[VEC], gw[VEC], g[VEC];
-        terms(i, n, gw, g);
+        const int k = KEEP ? i : 0;
+        if constexpr (!KEEP) terms(i, n[k], gw[k], g);
 #pragma unroll
         for (int e = 0; e < VEC; ++e) g[e] = 0.0f;
-        if (in[3]) unpack(PIPE ? *slot(stage, gh_slot, i) : span.load(in[3], row, i), g);
+        if (in[3]) unpack(PIPE ? *slot(stage, gh_slot, i) : span.load(in[3], begin, i), g);
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) g[e] += s * (gw[e] - n[e] * c);
-        span.store(static_cast<T*>(a.dx), row, i, g);
+        for (int e = 0; e < VEC; ++e) g[e] += s * (gw[k][e] - n[k][e] * c);
+        span.store(static_cast<T*>(a.dx), begin, i, g);
       }
     if constexpr (PIPE) {
-      fetch(row + stages * step, stage);
-      stage = stage + 1 == stages ? 0 : stage + 1;
+      fetch(begin + stages * begin_step, stage);
+      stage = stage + stage_slots == stages * stage_slots ? 0 : stage + stage_slots;
     }
   }
   if (!a.part) return;

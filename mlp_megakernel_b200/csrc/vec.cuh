@@ -40,17 +40,49 @@ __device__ __forceinline__ Raw<T, VEC> load_raw(const T* p) {
   return *reinterpret_cast<const Raw<T, VEC>*>(p);
 }
 
+// Two values at a time: one instruction a value to widen, one for two to round.
+__device__ __forceinline__ float2 to_float2(__half2 v) { return __half22float2(v); }
+__device__ __forceinline__ float2 to_float2(__nv_bfloat162 v) { return __bfloat1622float2(v); }
+template <class T>
+struct Pair;
+template <>
+struct Pair<__half> {
+  using type = __half2;
+  static __device__ __forceinline__ type round(float a, float b) { return __floats2half2_rn(a, b); }
+};
+template <>
+struct Pair<__nv_bfloat16> {
+  using type = __nv_bfloat162;
+  static __device__ __forceinline__ type round(float a, float b) { return __floats2bfloat162_rn(a, b); }
+};
+
 template <class T, int VEC>
 __device__ __forceinline__ void unpack(const Raw<T, VEC>& r, float (&f)[VEC]) {
+  if constexpr (sizeof(T) == 2 && VEC % 2 == 0) {
+    const typename Pair<T>::type* p = reinterpret_cast<const typename Pair<T>::type*>(r.v);
 #pragma unroll
-  for (int e = 0; e < VEC; ++e) f[e] = to_float(r.v[e]);
+    for (int e = 0; e < VEC / 2; ++e) {
+      const float2 v = to_float2(p[e]);
+      f[2 * e] = v.x;
+      f[2 * e + 1] = v.y;
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) f[e] = to_float(r.v[e]);
+  }
 }
 
 template <class T, int VEC>
 __device__ __forceinline__ void store_vec(T* p, const float (&f)[VEC]) {
   Raw<T, VEC> r;
+  if constexpr (sizeof(T) == 2 && VEC % 2 == 0) {
+    typename Pair<T>::type* q = reinterpret_cast<typename Pair<T>::type*>(r.v);
 #pragma unroll
-  for (int e = 0; e < VEC; ++e) r.v[e] = from_float<T>(f[e]);
+    for (int e = 0; e < VEC / 2; ++e) q[e] = Pair<T>::round(f[2 * e], f[2 * e + 1]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) r.v[e] = from_float<T>(f[e]);
+  }
   *reinterpret_cast<Raw<T, VEC>*>(p) = r;
 }
 
