@@ -314,7 +314,7 @@ int mlpk_expert_combine_bwd(int64_t tokens, int top, int width, int dtype, const
  * device.  Device scalars, each may be NULL: lr_ptr replaces lr; the gradients
  * are divided by grad_scale; a found_inf that is not 0 skips the whole step. */
 #define MLPK_ADAMW_BLOCK 256
-#define MLPK_ADAMW_CHUNK 4096
+#define MLPK_ADAMW_CHUNK 2048
 typedef struct mlpk_adamw_state {
   int32_t bits;
   void* exp_avg;

@@ -103,7 +103,7 @@ DT_F16 = 0  # MLPK_DT_F16: fp16 operands
 DT_F32 = 1  # MLPK_DT_F32: fp32 operands on tf32 tensor cores
 DT_BF16 = 2  # MLPK_DT_BF16: bf16 values (the block operators)
 ADAMW_BLOCK = 256  # MLPK_ADAMW_BLOCK: elements that share a scale of the 8-bit state
-ADAMW_CHUNK = 4096  # MLPK_ADAMW_CHUNK: elements of a tensor's step-count unit
+ADAMW_CHUNK = 2048  # MLPK_ADAMW_CHUNK: the unit of the step counts, in elements
 EXPERT_MAX = 1024
 NORM_MAX_WIDTH = 32768
 NORM_GROUP = 128  # columns that share a scale of the 8-bit norm

@@ -16,24 +16,47 @@ using namespace mlpk::host;
 constexpr int kFewTensors = 32;
 constexpr int kManyTensors = 768;
 
+int64_t chunks_of(int64_t n) { return (n + kAdamChunk - 1) / kAdamChunk; }
+
 template <class P, class G, bool BITS8, bool MASTER, int CAP>
 int launch_step(int count, const int64_t* numel, void* const* p, const void* const* g, const int64_t* off,
                 const int32_t* tick, AdamArgs a, cudaStream_t st) {
+  DevInfo di;
+  int dev;
+  int rc = current_device_info(&di, &dev);
+  if (rc) return rc;
+  void (*kern)(AdamTable<CAP>, AdamArgs);
+  size_t smem = 0;
+  if constexpr (BITS8) {
+    kern = adamw8_kernel<P, G, MASTER, CAP>;
+    smem = AdamSlots<P, G, MASTER>::BYTES;
+    if (blocks_per_sm(reinterpret_cast<const void*>(kern), kAdamThreads, smem, dev) == 0) return MLPK_ERR_CUDA;
+    // 1 chunk a thread block until the step has 12 of them an SM (four waves),
+    // then more, up to 16.
+    int64_t all = 0;
+    for (int i = 0; i < count; ++i) all += chunks_of(numel[i]);
+    a.per = static_cast<int>(std::min<int64_t>(std::max<int64_t>(all / (di.sm_count * 12), 1), 16));
+  } else {
+    kern = adamw32_kernel<P, G, MASTER, CAP>;
+    a.per = kAdamChunks32;
+  }
   for (int i = 0; i < count;) {
     AdamTable<CAP> table;
-    int64_t chunks = 0;
+    int64_t ctas = 0;
     int k = 0;
     for (; i < count && k < CAP; ++i) {
       if (numel[i] == 0) continue;
-      const int64_t c = (numel[i] + kAdamChunk - 1) / kAdamChunk;
-      if (chunks + c > 0x7fffffff) break;
-      table.t[k++] = {p[i], g[i], numel[i], off[i], static_cast<int32_t>(chunks), tick[i]};
-      chunks += c;
+      const int64_t n = (chunks_of(numel[i]) + a.per - 1) / a.per;
+      if (ctas + n > 0x7fffffff) break;
+      table.t[k++] = {p[i], g[i], numel[i], off[i], static_cast<int32_t>(ctas), tick[i]};
+      ctas += n;
     }
-    if (k == 0) break;
+    if (k == 0) {
+      if (i < count) return MLPK_ERR_SHAPE;  // a tensor of 2^43 elements
+      break;
+    }
     a.count = k;
-    const int rc = launch_kernel_early(adamw_kernel<P, G, BITS8, MASTER, CAP>, dim3(static_cast<unsigned>(chunks)),
-                                       kAdamThreads, 0, st, table, a);
+    rc = launch_kernel_early(kern, dim3(static_cast<unsigned>(ctas)), kAdamThreads, smem, st, table, a);
     if (rc) return rc;
   }
   return MLPK_OK;
@@ -80,18 +103,16 @@ int mlpk_adamw_step(int count, const int64_t* numel, void* const* params, const 
     if (state_off[i] % kAdamBlock) return MLPK_ERR_ALIGN;
     if (numel[i] > 0 && (!params[i] || !grads[i])) return MLPK_ERR_NULL;
   }
-  DevInfo di;
-  const int rc = current_device_info(&di, nullptr);
-  if (rc) return rc;
   AdamArgs a = {};
   a.lr = static_cast<float>(args->lr);
-  a.b1 = static_cast<float>(args->beta1);
-  a.b1c = static_cast<float>(1.0 - args->beta1);
-  a.b2 = static_cast<float>(args->beta2);
-  a.b2c = static_cast<float>(1.0 - args->beta2);
+  const auto twice = [](double v) { return make_float2(static_cast<float>(v), static_cast<float>(v)); };
+  a.b1 = twice(args->beta1);
+  a.b1c = twice(1.0 - args->beta1);
+  a.b2 = twice(args->beta2);
+  a.b2c = twice(1.0 - args->beta2);
+  a.eps = twice(args->eps);
   a.lnb1 = static_cast<float>(std::log(args->beta1));
   a.lnb2 = static_cast<float>(std::log(args->beta2));
-  a.eps = static_cast<float>(args->eps);
   a.wd = static_cast<float>(args->weight_decay);
   a.maximize = args->maximize;
   a.lr_ptr = args->lr_ptr;

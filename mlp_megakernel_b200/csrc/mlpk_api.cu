@@ -90,12 +90,16 @@ int current_device_info(DevInfo* out, int* dev_out) {
 int blocks_per_sm(const void* kern, int threads, size_t smem, int dev) {
   static std::mutex mu;
   static std::map<std::tuple<const void*, int, size_t, int>, int> known;
+  static std::map<std::pair<const void*, int>, size_t> allowed;  // dynamic shared memory that the kernel may have
   std::lock_guard<std::mutex> lk(mu);
   int& n = known[{kern, threads, smem, dev}];
   if (n == 0) {
-    if (smem > 48 * 1024 && cuda_status(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                             kMaxBlockSmem)))
-      return 0;
+    size_t& most = allowed[{kern, dev}];
+    if (smem > most && smem > 32 * 1024) {  // beside static shared memory, of 48 KB in all
+      if (cuda_status(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem))))
+        return 0;
+      most = smem;
+    }
     if (cuda_status(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, threads, smem))) n = 0;
   }
   return n;

@@ -239,7 +239,7 @@ __global__ void __launch_bounds__(MAXT) rms_norm_fwd_kernel(const NormArgs a, in
 #pragma unroll
           for (int e = 0; e < VEC; ++e) h[i][e] += f[e];
         }
-        if (RAGGED) {
+        if (!span.whole(i)) {
 #pragma unroll
           for (int e = 0; e < VEC; ++e)
             if (!span.owns(i, e)) h[i][e] = 0.0f;
@@ -328,12 +328,11 @@ __global__ void __launch_bounds__(MAXT) rms_norm_fwd_kernel(const NormArgs a, in
           if (live && span.has(i)) {
             const int lo = max(span.col(i), 0) / kNormGroup, hi = (min(span.col(i) + VEC, a.width) - 1) / kNormGroup;
             const int edge = (lo + 1) * kNormGroup - span.col(i);  // elements from here on are of the next group
-            uint32_t m0 = 0, m1 = 0;
+            uint32_t m0 = 0, m1 = 0;  // what is not the row's is zero
 #pragma unroll
             for (int e = 0; e < VEC; ++e) {
-              const uint32_t m = span.owns(i, e) ? abs_bits(h[i][e]) : 0u;
-              if (e < edge) m0 = max(m0, m);
-              else m1 = max(m1, m);
+              if (e < edge) m0 = max(m0, abs_bits(h[i][e]));
+              else m1 = max(m1, abs_bits(h[i][e]));
             }
             atomicMax(gmax + lo, m0);
             if (hi != lo) atomicMax(gmax + hi, m1);
@@ -450,11 +449,15 @@ __global__ void __launch_bounds__(MAXT, MAXT == 256 ? 2 : 1) rms_norm_bwd_kernel
 #pragma unroll
         for (int e = 0; e < VEC; ++e) n[e] += f[e];
       }
+      if (!span.whole(i)) {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e)
+          if (!span.owns(i, e)) n[e] = g[e] = 0.0f;
+      }
       float f[VEC];
       w.get(i, f);
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
-        if (RAGGED && !span.owns(i, e)) n[e] = g[e] = 0.0f;
         n[e] *= s;
         gw[e] = g[e] * f[e];
       }

@@ -95,6 +95,13 @@ __device__ __forceinline__ void cp_async16(void* smem, const void* global, int b
                "l"(global), "r"(bytes)
                : "memory");
 }
+template <int BYTES>  // 4 or 8
+__device__ __forceinline__ void cp_async_small(void* smem, const void* global) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(
+                   static_cast<uint32_t>(__cvta_generic_to_shared(smem))),
+               "l"(global), "n"(BYTES)
+               : "memory");
+}
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 // Until all but the N youngest groups of this thread have arrived.
 template <int N>
@@ -108,12 +115,46 @@ __device__ __forceinline__ void cp_async_wait_upto(int n) {  // n from 0 to 3
   else cp_async_wait<0>();
 }
 
+// Two products in one instruction, each rounded on its own.
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  unsigned long long d;
+  asm("mul.rn.f32x2 %0, %1, %2;"
+      : "=l"(d)
+      : "l"(*reinterpret_cast<unsigned long long*>(&a)), "l"(*reinterpret_cast<unsigned long long*>(&b)));
+  return *reinterpret_cast<float2*>(&d);
+}
+// Two sums, one at a time: a sum of pairs behind products of pairs came out
+// contracted (a product not rounded).
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  return make_float2(__fadd_rn(a.x, b.x), __fadd_rn(a.y, b.y));
+}
+
+// The values of a vector as pairs.
+template <class T, int VEC>
+__device__ __forceinline__ void unpack2(const Raw<T, VEC>& r, float2 (&f)[VEC / 2]) {
+  float v[VEC];
+  unpack(r, v);
+#pragma unroll
+  for (int e = 0; e < VEC / 2; ++e) f[e] = make_float2(v[2 * e], v[2 * e + 1]);
+}
+template <class T, int VEC>
+__device__ __forceinline__ void store_vec2(T* p, const float2 (&f)[VEC / 2]) {
+  float v[VEC];
+#pragma unroll
+  for (int e = 0; e < VEC / 2; ++e) {
+    v[2 * e] = f[e].x;
+    v[2 * e + 1] = f[e].y;
+  }
+  store_vec<T, VEC>(p, v);
+}
+
 // The 8-bit type: 4 exponent bits, 3 of mantissa (e4m3), largest value 448,
 // smallest positive one 2^-9.
 constexpr float kFp8Max = 448.0f;
 constexpr float kFp8Tiny = 0.001953125f;
 
-// f rounded to e4m3 (to nearest even, NaN kept, |f| above 448 clipped).
+// Rounded to e4m3 (to nearest even, NaN kept, magnitudes above 448 clipped).
+__device__ __forceinline__ uint16_t to_fp8x2(float2 f) { return __nv_cvt_float2_to_fp8x2(f, __NV_SATFINITE, __NV_E4M3); }
 template <int VEC>
 __device__ __forceinline__ void store_fp8(uint8_t* p, const float (&f)[VEC]) {
   if constexpr (VEC == 1) {
@@ -121,10 +162,35 @@ __device__ __forceinline__ void store_fp8(uint8_t* p, const float (&f)[VEC]) {
   } else {
     Raw<uint16_t, VEC / 2> r;
 #pragma unroll
-    for (int e = 0; e < VEC / 2; ++e)
-      r.v[e] = __nv_cvt_float2_to_fp8x2(make_float2(f[2 * e], f[2 * e + 1]), __NV_SATFINITE, __NV_E4M3);
+    for (int e = 0; e < VEC / 2; ++e) r.v[e] = to_fp8x2(make_float2(f[2 * e], f[2 * e + 1]));
     *reinterpret_cast<Raw<uint16_t, VEC / 2>*>(p) = r;
   }
+}
+
+// VEC values of the 8-bit type as fp32 (exact).
+template <int VEC>
+__device__ __forceinline__ void unpack_fp8(const Raw<uint16_t, VEC / 2>& r, float2 (&f)[VEC / 2]) {
+#pragma unroll
+  for (int e = 0; e < VEC / 2; ++e)
+    f[e] = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(r.v[e], __NV_E4M3)));
+}
+
+// The largest magnitude of a, b and c; a NaN stays.
+__device__ __forceinline__ float max_abs(float a, float b, float c) {
+  float m;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(m) : "f"(a), "f"(b), "f"(c));
+  return m;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float m;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(a), "f"(b));
+  return m;
+}
+// 1 / v to within a unit of the last place; v is 0 or a normal number.
+__device__ __forceinline__ float fast_reciprocal(float v) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
 }
 
 // |v| as an unsigned whole number: ordered like |v|, with a NaN above
