@@ -302,7 +302,7 @@ int mlpk_expert_combine_bwd(int64_t tokens, int top, int width, int dtype, const
  *   m = beta1 m + (1 - beta1) g; v = beta2 v + (1 - beta2) g^2;
  *   p = p (1 - lr weight_decay)
  *       - lr / (1 - beta1^t) * m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
- * in fp32.  The state of all tensors lies in flat buffers; tensor i's begins at
+ * in fp32.  The state of all tensors lies in flat buffers, 32-byte aligned; tensor i's begins at
  * element state_off[i], a multiple of MLPK_ADAMW_BLOCK, and is padded to a
  * multiple of it (the padding is zero and stays so).  bits 32: exp_avg and
  * exp_avg_sq are fp32.  bits 8: exp_avg is e4m3 m and exp_avg_sq e4m3 sqrt(v),

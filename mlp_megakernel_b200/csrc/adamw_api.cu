@@ -97,7 +97,8 @@ int mlpk_adamw_step(int count, const int64_t* numel, void* const* params, const 
   if (!numel || !params || !grads || !state_off || !tick || !state->exp_avg || !state->exp_avg_sq || !state->ticks)
     return MLPK_ERR_NULL;
   if (state->bits == 8 && (!state->exp_avg_scale || !state->exp_avg_sq_scale)) return MLPK_ERR_NULL;
-  if (!aligned16(state->exp_avg) || !aligned16(state->exp_avg_sq) || !aligned16(state->master)) return MLPK_ERR_ALIGN;
+  for (const void* p : {state->exp_avg, state->exp_avg_sq, static_cast<void*>(state->master)})
+    if (reinterpret_cast<uintptr_t>(p) & 31u) return MLPK_ERR_ALIGN;
   for (int i = 0; i < count; ++i) {
     if (numel[i] < 0 || state_off[i] < 0 || tick[i] < 0) return MLPK_ERR_SHAPE;
     if (state_off[i] % kAdamBlock) return MLPK_ERR_ALIGN;

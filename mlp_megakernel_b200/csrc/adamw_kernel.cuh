@@ -21,16 +21,18 @@
 // need shuffles alone; 8 warps have a chunk of 2048.  Products are taken two at
 // a time.
 //
-// 32-bit state: memory bounds it.  A thread block has two chunks and issues
-// all its loads first; those of the SM's other thread blocks overlap its
-// arithmetic.  113 million fp16 parameters with fp32 copies: 470 us, 6.7 TB/s.
+// 32-bit state: memory bounds it.  A thread block has two chunks, one after
+// the other; 4 thread blocks an SM overlap each other's loads, and fp32 values
+// move 32 bytes a lane.  113 million fp16 parameters with fp32 copies: 477 us,
+// 6.65 TB/s.  Measured against it: all loads of both chunks first, 3 thread
+// blocks an SM, 536 us; 16-byte accesses 506; 5 thread blocks 503; 8 chunks 493.
 //
 // 8-bit state: 10 bytes an element and 54 instructions (a root, a quotient,
 // four conversions), so memory bounds it only while the warps hardly wait.  A
 // thread block has up to 16 chunks, one after the other, and each thread copies
 // its part of the next ones to its own slots of shared memory (cp.async): 3
 // under way.  233 million bf16 parameters: 438 us, 5.4 TB/s.  Measured against
-// it: loads first as in 32 bits 516 us; one chunk ahead in registers 760 (the
+// it: all loads of two chunks first 516 us; one chunk ahead in registers 760 (the
 // loads were put off behind the work they were to overlap); 4 thread blocks an
 // SM with their registers spilling 516, 3 without 438; 4 copies under way 442.
 #pragma once
@@ -186,7 +188,7 @@ __device__ __forceinline__ void adam_store(T* p, const float2 (&f)[4], bool whol
 }
 
 template <class P, class G, bool MASTER, int CAP>
-__global__ void __launch_bounds__(kAdamThreads, 3)
+__global__ void __launch_bounds__(kAdamThreads, 4)
     adamw32_kernel(const __grid_constant__ AdamTable<CAP> table, const __grid_constant__ AdamArgs a) {
   using Param = typename std::conditional<MASTER, float, P>::type;
   constexpr int N = kAdamChunks32;
@@ -200,38 +202,29 @@ __global__ void __launch_bounds__(kAdamThreads, 3)
   float* sm = static_cast<float*>(a.m) + t.off + part.i0;
   float* sv = static_cast<float*>(a.v) + t.off + part.i0;
   float* master = MASTER ? a.master + t.off + part.i0 : nullptr;
-
-  Raw<Param, 8> rp[N];
-  Raw<G, 8> rg[N];
-  Raw<float, 8> rm[N], rv[N];
-#pragma unroll
-  for (int k = 0; k < N; ++k) {
-    const int ahead = k * kAdamChunk, here = part.left - ahead;
-    if (here + lane * 8 <= 0) break;  // the whole warp
-    const bool whole = part.aligned && here >= 8;
-    rg[k] = adam_load(g + ahead, whole, here);
-    if constexpr (MASTER) rp[k] = load_raw<float, 8>(master + ahead);
-    else rp[k] = adam_load(p + ahead, whole, here);
-    rm[k] = load_raw<float, 8>(sm + ahead);
-    rv[k] = load_raw<float, 8>(sv + ahead);
-  }
   AdamFactors f;
   if (adam_factors(a, t, part, ticks, f)) return;
-#pragma unroll
+#pragma unroll 1
   for (int k = 0; k < N; ++k) {
     const int ahead = k * kAdamChunk, here = part.left - ahead;
-    if (here + lane * 8 <= 0) break;
+    if (here + lane * 8 <= 0) break;  // the whole warp, at the tensor's end
+    const bool whole = part.aligned && here >= 8;
+    Raw<Param, 8> rp;
+    const Raw<G, 8> rg = adam_load(g + ahead, whole, here);
+    if constexpr (MASTER) rp = load_32b(master + ahead);
+    else rp = adam_load(p + ahead, whole, here);
+    const Raw<float, 8> rm = load_32b(sm + ahead), rv = load_32b(sv + ahead);
     float2 pf[4], gf[4], m[4], v[4], r;
-    unpack2(rp[k], pf);
-    unpack2(rg[k], gf);
-    unpack2(rm[k], m);
-    unpack2(rv[k], v);
+    unpack2(rp, pf);
+    unpack2(rg, gf);
+    unpack2(rm, m);
+    unpack2(rv, v);
 #pragma unroll
     for (int e = 0; e < 4; ++e) adam_update(a, f, pf[e], gf[e], m[e], v[e], r);
-    adam_store(p + ahead, pf, part.aligned && here >= 8, here);
-    if constexpr (MASTER) store_vec2<float, 8>(master + ahead, pf);
-    store_vec2<float, 8>(sm + ahead, m);
-    store_vec2<float, 8>(sv + ahead, v);
+    adam_store(p + ahead, pf, whole, here);
+    if constexpr (MASTER) store_32b(master + ahead, pf);
+    store_32b(sm + ahead, m);
+    store_32b(sv + ahead, v);
   }
 }
 

@@ -86,6 +86,23 @@ __device__ __forceinline__ void store_vec(T* p, const float (&f)[VEC]) {
   *reinterpret_cast<Raw<T, VEC>*>(p) = r;
 }
 
+// 8 fp32 values in one access (p is 32-byte aligned): two of 16 bytes each
+// touch every sector of a warp's values twice.
+__device__ __forceinline__ Raw<float, 8> load_32b(const float* p) {
+  Raw<float, 8> r;
+  asm volatile("ld.global.v8.f32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=f"(r.v[0]), "=f"(r.v[1]), "=f"(r.v[2]), "=f"(r.v[3]), "=f"(r.v[4]), "=f"(r.v[5]), "=f"(r.v[6]),
+                 "=f"(r.v[7])
+               : "l"(p)
+               : "memory");
+  return r;
+}
+__device__ __forceinline__ void store_32b(float* p, const float2 (&f)[4]) {
+  asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "f"(f[0].x), "f"(f[0].y),
+               "f"(f[1].x), "f"(f[1].y), "f"(f[2].x), "f"(f[2].y), "f"(f[3].x), "f"(f[3].y)
+               : "memory");
+}
+
 // A 16-byte copy from global to shared memory that the thread waits for later;
 // `bytes` of it are read, the rest are zeros.  A thread that reads back only
 // what it copied itself needs no barrier, just cp_async_wait.
