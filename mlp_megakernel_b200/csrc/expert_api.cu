@@ -1,6 +1,8 @@
 // C-ABI entry points of the rows sorted by expert and back (declared in
 // include/mlpk.h).
 #include <algorithm>
+#include <mutex>
+#include <type_traits>
 
 #include "expert_kernel.cuh"
 #include "host.cuh"
@@ -12,46 +14,66 @@ using namespace mlpk::host;
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-constexpr int kMaxChunks = 148;
-
-// Slots of a chunk (a multiple of 32 a warp) and the number of chunks.
-void sort_chunks(int64_t slots, int64_t* chunk, int* chunks) {
-  const int64_t unit = 32 * kSortWarps;
-  *chunk = std::max<int64_t>(ceil_div(ceil_div(slots, kMaxChunks), unit), 1) * unit;
-  *chunks = static_cast<int>(std::max<int64_t>(ceil_div(slots, *chunk), 1));
-}
-
 int check_rows(int64_t tokens, int top, int width, int dtype) {
   if (tokens < 0 || top < 1 || width < 1 || tokens > 0x7fffffff / top) return MLPK_ERR_SHAPE;
-  if (dtype != MLPK_DT_F16 && dtype != MLPK_DT_BF16 && dtype != MLPK_DT_F32) return MLPK_ERR_UNSUPPORTED;
+  if ((dtype != MLPK_DT_F16 && dtype != MLPK_DT_BF16 && dtype != MLPK_DT_F32) || width > kRowWidthMax)
+    return MLPK_ERR_UNSUPPORTED;
   return MLPK_OK;
 }
 
+// Thread blocks of the sort's cluster: as many as have 4096 slots each, up to
+// 16 (one SM each; above 8 a kernel has to ask).
 template <class I>
-int sort_slots(int64_t slots, int experts, const void* ids, int* row_of, int* offsets, int* hist, cudaStream_t st) {
-  int64_t chunk;
-  int chunks;
-  sort_chunks(slots, &chunk, &chunks);
-  const size_t bins = experts + 1;
-  int rc = launch_kernel_early(expert_count_kernel<I>, dim3(chunks), kSortThreads, bins * 4, st,
-                               static_cast<const I*>(ids), slots, experts, chunk, hist);
+int sort_slots(int64_t slots, int experts, const void* ids, int* row_of, int* offsets, cudaStream_t st) {
+  int dev = 0;
+  int rc = cuda_status(cudaGetDevice(&dev));
   if (rc) return rc;
-  return launch_kernel_early(expert_place_kernel<I>, dim3(chunks), kSortThreads, bins * 4 * (kSortWarps + 2), st,
-                             static_cast<const I*>(ids), slots, experts, chunk, static_cast<const int*>(hist), row_of,
-                             offsets);
+  const auto kern = expert_sort_kernel<I>;
+  int blocks = 1;
+  while (blocks < 16 && slots > blocks * 4096) blocks *= 2;
+  const int64_t part = ceil_div(ceil_div(slots, static_cast<int64_t>(blocks) * kSortWarps), 32) * 32;
+  const size_t smem = sizeof(int) * (kSortWarps + static_cast<size_t>(kSortWarps + 1) * (experts + 1));
+  if (blocks_per_sm(reinterpret_cast<const void*>(kern), kSortThreads, smem, dev) == 0) return MLPK_ERR_CUDA;
+  static std::once_flag wide[2][64];  // by type and device
+  if (blocks > 8 && dev < 64)
+    std::call_once(wide[sizeof(I) == 8][dev], [&] {
+      rc = cuda_status(cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    });
+  if (rc) return rc;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(blocks);
+  cfg.blockDim = dim3(kSortThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = blocks;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  return cuda_status(cudaLaunchKernelEx(&cfg, kern, static_cast<const I*>(ids), slots, experts, part, row_of, offsets));
 }
 
-// Blocks for `items` pieces of work of one thread each: at most 16 blocks of
-// 256 an SM, which loop.
-unsigned blocks_for(int64_t items, int sm_count) {
-  return static_cast<unsigned>(std::min<int64_t>(ceil_div(items, 256), static_cast<int64_t>(sm_count) * 16));
+// Threads of a token's row of `items` words or vectors, `each` a thread.
+int threads_of_row(int64_t items, int each) {
+  int tpr = 1;
+  while (tpr < kRowThreads && static_cast<int64_t>(tpr) * each < items) tpr *= 2;
+  return tpr;
+}
+dim3 row_grid(int64_t tokens, int64_t items, int tpr, int each) {
+  return dim3(static_cast<unsigned>(ceil_div(tokens, kRowThreads / tpr)),
+              static_cast<unsigned>(ceil_div(items, static_cast<int64_t>(tpr) * each)));
 }
 
 template <class U>
 int dispatch_words(int64_t tokens, int top, int64_t words, const void* x, const int* row_of, const int* kept, void* xs,
-                   int sm_count, cudaStream_t st) {
-  return launch_kernel_early(expert_dispatch_kernel<U>, dim3(blocks_for(tokens * words, sm_count)), 256, 0, st,
-                             static_cast<const U*>(x), tokens, top, static_cast<int>(words), row_of, kept,
+                   cudaStream_t st) {
+  constexpr int NW = 2;
+  const int tpr = threads_of_row(words, NW);
+  return launch_kernel_early(expert_dispatch_kernel<U, NW>, row_grid(tokens, words, tpr, NW), kRowThreads, 0, st,
+                             static_cast<const U*>(x), tokens, top, static_cast<int>(words), tpr, row_of, kept,
                              static_cast<U*>(xs));
 }
 
@@ -74,29 +96,18 @@ int with_types(int dtype, int w_dtype, int width, F&& f) {
 
 extern "C" {
 
-int64_t mlpk_expert_sort_workspace_size(int64_t slots, int experts) {
-  if (slots < 0 || slots > 0x7fffffff || experts < 1) return -1;
-  if (experts > kExpertMax) return -1;
-  int64_t chunk;
-  int chunks;
-  sort_chunks(slots, &chunk, &chunks);
-  return static_cast<int64_t>(chunks) * (experts + 1) * 4;
-}
-
 int mlpk_expert_sort(int64_t slots, int experts, const void* ids, int id_bytes, int32_t* row_of, int32_t* offsets,
-                     void* workspace, int64_t workspace_bytes, mlpk_stream_t stream) {
+                     mlpk_stream_t stream) {
   if (slots < 0 || slots > 0x7fffffff || experts < 1) return MLPK_ERR_SHAPE;
   if (experts > kExpertMax || (id_bytes != 4 && id_bytes != 8)) return MLPK_ERR_UNSUPPORTED;
-  if (!offsets || !workspace || (slots > 0 && (!ids || !row_of))) return MLPK_ERR_NULL;
-  if (!aligned16(ids) || !aligned16(row_of) || !aligned16(offsets) || !aligned16(workspace)) return MLPK_ERR_ALIGN;
-  if (workspace_bytes < mlpk_expert_sort_workspace_size(slots, experts)) return MLPK_ERR_SCRATCH;
+  if (!offsets || (slots > 0 && (!ids || !row_of))) return MLPK_ERR_NULL;
+  if (!aligned16(ids) || !aligned16(row_of) || !aligned16(offsets)) return MLPK_ERR_ALIGN;
   DevInfo di;
   int rc = current_device_info(&di, nullptr);
   if (rc) return rc;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  int* hist = static_cast<int*>(workspace);
-  return id_bytes == 8 ? sort_slots<int64_t>(slots, experts, ids, row_of, offsets, hist, st)
-                       : sort_slots<int32_t>(slots, experts, ids, row_of, offsets, hist, st);
+  return id_bytes == 8 ? sort_slots<int64_t>(slots, experts, ids, row_of, offsets, st)
+                       : sort_slots<int32_t>(slots, experts, ids, row_of, offsets, st);
 }
 
 int mlpk_expert_dispatch(int64_t tokens, int top, int width, int dtype, const void* x, const int32_t* row_of,
@@ -111,10 +122,10 @@ int mlpk_expert_dispatch(int64_t tokens, int top, int width, int dtype, const vo
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int64_t bytes = static_cast<int64_t>(width) * (dtype == MLPK_DT_F32 ? 4 : 2);
   if (bytes % 16 == 0)
-    return dispatch_words<uint4>(tokens, top, bytes / 16, x, row_of, kept, xs, di.sm_count, st);
-  if (bytes % 8 == 0) return dispatch_words<uint2>(tokens, top, bytes / 8, x, row_of, kept, xs, di.sm_count, st);
-  if (bytes % 4 == 0) return dispatch_words<uint32_t>(tokens, top, bytes / 4, x, row_of, kept, xs, di.sm_count, st);
-  return dispatch_words<uint16_t>(tokens, top, bytes / 2, x, row_of, kept, xs, di.sm_count, st);
+    return dispatch_words<uint4>(tokens, top, bytes / 16, x, row_of, kept, xs, st);
+  if (bytes % 8 == 0) return dispatch_words<uint2>(tokens, top, bytes / 8, x, row_of, kept, xs, st);
+  if (bytes % 4 == 0) return dispatch_words<uint32_t>(tokens, top, bytes / 4, x, row_of, kept, xs, st);
+  return dispatch_words<uint16_t>(tokens, top, bytes / 2, x, row_of, kept, xs, st);
 }
 
 int mlpk_expert_combine(int64_t tokens, int top, int width, int dtype, const void* y, const void* weights, int w_dtype,
@@ -130,10 +141,12 @@ int mlpk_expert_combine(int64_t tokens, int top, int width, int dtype, const voi
   return with_types(dtype, weights ? w_dtype : dtype, width, [&](auto t, auto w, auto vec) {
     using T = decltype(t);
     using W = decltype(w);
-    constexpr int V = decltype(vec)::value;
-    return launch_kernel_early(expert_combine_kernel<T, W, V>, dim3(blocks_for(tokens * (width / V), di.sm_count)), 256,
-                               0, static_cast<cudaStream_t>(stream), static_cast<const T*>(y),
-                               static_cast<const W*>(weights), tokens, top, width, row_of, kept, static_cast<T*>(out));
+    constexpr int V = decltype(vec)::value, NW = V == 1 ? 4 : 1;
+    const int tpr = threads_of_row(width / V, NW);
+    return launch_kernel_early(expert_combine_kernel<T, W, V, NW>, row_grid(tokens, width / V, tpr, NW), kRowThreads, 0,
+                               static_cast<cudaStream_t>(stream), static_cast<const T*>(y),
+                               static_cast<const W*>(weights), tokens, top, width, tpr, row_of, kept,
+                               static_cast<T*>(out));
   });
 }
 
@@ -151,11 +164,12 @@ int mlpk_expert_combine_bwd(int64_t tokens, int top, int width, int dtype, const
   return with_types(dtype, weights || dw ? w_dtype : dtype, width, [&](auto t, auto w, auto vec) {
     using T = decltype(t);
     using W = decltype(w);
-    return launch_kernel_early(expert_combine_bwd_kernel<T, W, decltype(vec)::value>,
-                               dim3(blocks_for(tokens * top * 32, di.sm_count)), 256, 0,
-                               static_cast<cudaStream_t>(stream), static_cast<const T*>(grad_out),
-                               static_cast<const T*>(y), static_cast<const W*>(weights), tokens, top, width, row_of,
-                               kept, static_cast<T*>(dy), static_cast<W*>(dw));
+    constexpr int V = decltype(vec)::value;
+    const int tpr = threads_of_row(width / V, V == 1 ? 4 : 1);
+    return launch_kernel_early(expert_combine_bwd_kernel<T, W, V>, dim3(ceil_div(tokens, kRowThreads / tpr)),
+                               kRowThreads, 0, static_cast<cudaStream_t>(stream), static_cast<const T*>(grad_out),
+                               static_cast<const T*>(y), static_cast<const W*>(weights), tokens, top, width, tpr,
+                               row_of, kept, static_cast<T*>(dy), static_cast<W*>(dw));
   });
 }
 

@@ -12,210 +12,306 @@
 //   backward of the dispatch: the combine of dL/dxs with weights of 1.
 // Sums over k and over columns are fp32 in a fixed order.
 #pragma once
+#include <cooperative_groups.h>
+
 #include "pdl.cuh"
 #include "vec.cuh"
 
 namespace mlpk {
 
-constexpr int kSortThreads = 256;
+// ------------------------------------------------------------------ sort
+// One cluster of thread blocks does the whole sort, so it is one launch and
+// reads nothing back from another: each warp has a contiguous part of the
+// slots, each thread block contiguous warps.
+//   1. a warp takes 32 slots at a time; equal ids among them (a warp match)
+//      get consecutive ranks behind the warp's count of that id so far, kept in
+//      row_of for the time being;
+//   2. per id, the counts are summed over the block's warps, over the
+//      cluster's lower blocks (distributed shared memory) and over lower ids;
+//   3. row_of += that.
+// What bounds it: the latency of step 1's chain, some 100 cycles for 32 slots
+// of a warp.
+constexpr int kSortThreads = 1024;
 constexpr int kSortWarps = kSortThreads / 32;
 constexpr int kExpertMax = 1024;
+constexpr int kRowWidthMax = 1 << 24;  // columns; 65,535 parts of a row are the grid's limit
+constexpr int kSortAhead = 4;  // groups of 32 slots whose ids are loaded together
 
 template <class I>
-__device__ __forceinline__ int expert_of(const I* ids, int64_t i, int64_t n, int experts) {
-  if (i >= n) return -1;  // no slot
+__device__ __forceinline__ int expert_of(const I* ids, int64_t i, int64_t last, int experts) {
+  if (i >= last) return -1;  // no slot
   const I e = ids[i];
   return e >= 0 && e < experts ? static_cast<int>(e) : experts;
 }
 
-// Counts per chunk: hist[chunk][e], e = E for the dropped slots.
-template <class I>
-__global__ void __launch_bounds__(kSortThreads) expert_count_kernel(const I* __restrict__ ids, int64_t n, int experts,
-                                                                    int64_t chunk, int* __restrict__ hist) {
-  extern __shared__ int cnt[];  // [E + 1]
-  pdl_enter();
-  for (int e = threadIdx.x; e <= experts; e += kSortThreads) cnt[e] = 0;
-  __syncthreads();
-  const int64_t first = blockIdx.x * chunk, last = min(n, first + chunk);
-  for (int64_t i = first + threadIdx.x; i < last; i += kSortThreads)
-    atomicAdd(cnt + expert_of(ids, i, n, experts), 1);
-  __syncthreads();
-  for (int e = threadIdx.x; e <= experts; e += kSortThreads)
-    hist[static_cast<int64_t>(blockIdx.x) * (experts + 1) + e] = cnt[e];
-}
-
-// Each block places its chunk's slots: the first row of (chunk, e) is the
-// number of slots of smaller experts plus those of e in earlier chunks; inside
-// the chunk each warp takes a contiguous part, counts it, and places it 32
-// slots at a time (equal ids among the 32 by a warp match).
+// `part`: slots of a warp, a multiple of 32.
 template <class I>
 __global__ void __launch_bounds__(kSortThreads)
-    expert_place_kernel(const I* __restrict__ ids, int64_t n, int experts, int64_t chunk,
-                        const int* __restrict__ hist, int* __restrict__ row_of, int* __restrict__ offsets) {
+    expert_sort_kernel(const I* __restrict__ ids, int64_t n, int experts, int64_t part, int* __restrict__ row_of,
+                       int* __restrict__ offsets) {
   extern __shared__ int sm[];
-  int* next = sm;                                  // [warps][E + 1]: each warp's next row of e
-  int* total = sm + kSortWarps * (experts + 1);    // [E + 1]: slots of e, then the first row of e
-  int* before = total + (experts + 1);             // [E + 1]: slots of e in earlier chunks
-  __shared__ int wsum[kSortWarps];
+  const int bins = experts + 1;  // the last one for the dropped slots
+  int* mine = sm + kSortWarps;                         // [bins]: this block's slots of e; then the first row of e
+  int* count = mine + bins;                            // [warps][bins]
+  __shared__ int carry_total;
+  auto cluster = cooperative_groups::this_cluster();
+  const int blocks = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  for (int k = threadIdx.x; k < kSortWarps * bins; k += kSortThreads) count[k] = 0;
   pdl_enter();
-  const int bins = experts + 1, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  for (int e = threadIdx.x; e < bins; e += kSortThreads) {
-    int t = 0, b = 0;
-    for (int c = 0; c < gridDim.x; ++c) {
-      const int v = hist[static_cast<int64_t>(c) * bins + e];
-      if (c < blockIdx.x) b += v;
-      t += v;
-    }
-    total[e] = t;
-    before[e] = b;
-  }
-  for (int k = threadIdx.x; k < kSortWarps * bins; k += kSortThreads) next[k] = 0;
   __syncthreads();
-  // Exclusive sums of total[], kSortThreads bins at a time.
+
+  const int64_t first = (static_cast<int64_t>(rank) * kSortWarps + warp) * part, last = min(n, first + part);
+  int* own = count + warp * bins;
+  for (int64_t i0 = first; i0 < last; i0 += 32 * kSortAhead) {
+    int e[kSortAhead];
+#pragma unroll
+    for (int k = 0; k < kSortAhead; ++k) e[k] = expert_of(ids, i0 + k * 32 + lane, last, experts);
+#pragma unroll
+    for (int k = 0; k < kSortAhead; ++k) {
+      const uint32_t same = __match_any_sync(0xffffffffu, e[k]);
+      const int before = __popc(same & ((1u << lane) - 1u));
+      int at = 0;
+      if (e[k] >= 0) {
+        at = own[e[k]];
+        row_of[i0 + k * 32 + lane] = at + before;
+      }
+      __syncwarp();
+      if (e[k] >= 0 && before == 0) own[e[k]] = at + __popc(same);
+      __syncwarp();
+    }
+  }
+  __syncthreads();
+  // Sums over the block's warps: count becomes what lies before each warp.
+  for (int e = threadIdx.x; e < bins; e += kSortThreads) {
+    int t = 0;
+    for (int k = 0; k < kSortWarps; ++k) {
+      const int c = count[k * bins + e];
+      count[k * bins + e] = t;
+      t += c;
+    }
+    mine[e] = t;
+  }
+  if (blocks > 1) cluster.sync();
+  else __syncthreads();
+  // Sums over the cluster's blocks, then over lower ids, kSortThreads ids at a
+  // time; at most two rounds.
+  int base[(kExpertMax + kSortThreads) / kSortThreads];
   int carry = 0;
-  for (int e0 = 0; e0 < bins; e0 += kSortThreads) {
-    const int e = e0 + threadIdx.x;
-    const int v = e < bins ? total[e] : 0;
-    int s = v;
+#pragma unroll
+  for (int r = 0; r < (kExpertMax + kSortThreads) / kSortThreads; ++r) {
+    const int e = r * kSortThreads + threadIdx.x;
+    base[r] = 0;
+    if (r * kSortThreads >= bins) break;  // the whole block
+    int all = 0, lower = 0;
+    if (e < bins) {
+      if (blocks == 1) {
+        all = mine[e];
+      } else {
+#pragma unroll 8
+        for (int b = 0; b < blocks; ++b) {
+          const int c = *cluster.map_shared_rank(mine + e, b);
+          if (b < rank) lower += c;
+          all += c;
+        }
+      }
+    }
+    int s = all;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int u = __shfl_up_sync(0xffffffffu, s, o);
       if (lane >= o) s += u;
     }
-    if (lane == 31) wsum[warp] = s;
+    if (lane == 31) sm[warp] = s;
     __syncthreads();
-    int pre = carry, all = 0;
-    for (int k = 0; k < kSortWarps; ++k) {
-      if (k < warp) pre += wsum[k];
-      all += wsum[k];
+    int w = sm[lane];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, w, o);
+      if (lane >= o) w += u;
     }
-    if (e < bins) {
-      total[e] = pre + s - v;
-      if (blockIdx.x == 0) offsets[e] = pre + s - v;
-    }
-    carry += all;
+    const int pre = __shfl_sync(0xffffffffu, w, warp) - sm[warp];  // of lower warps
+    const int start = carry + pre + s - all;
+    if (e < bins && rank == 0) offsets[e] = start;
+    base[r] = start + lower;
+    if (threadIdx.x == kSortThreads - 1) carry_total = start + all;
     __syncthreads();
+    carry = carry_total;
   }
-  // Each warp's part of the chunk: a multiple of 32 slots.
-  const int64_t first = blockIdx.x * chunk, last = min(n, first + chunk);
-  const int64_t part = chunk / kSortWarps;
-  const int64_t w0 = first + warp * part, w1 = min(last, w0 + part);
-  int* mine = next + warp * bins;
-  for (int64_t i = w0 + lane; i < w1; i += 32) atomicAdd(mine + expert_of(ids, i, n, experts), 1);
-  __syncthreads();
-  for (int e = threadIdx.x; e < bins; e += kSortThreads) {
-    int at = total[e] + before[e];
-    for (int k = 0; k < kSortWarps; ++k) {
-      const int c = next[k * bins + e];
-      next[k * bins + e] = at;
-      at += c;
-    }
+  if (blocks > 1) cluster.sync();  // every block has read the others' `mine`
+#pragma unroll
+  for (int r = 0; r < (kExpertMax + kSortThreads) / kSortThreads; ++r) {
+    const int e = r * kSortThreads + threadIdx.x;
+    if (e < bins) mine[e] = base[r];
   }
   __syncthreads();
-  for (int64_t i0 = w0; i0 < w1; i0 += 32) {
-    const int64_t i = i0 + lane;
-    const int e = expert_of(ids, i < w1 ? i : n, n, experts);
-    const uint32_t same = __match_any_sync(0xffffffffu, e);
-    const int rank = __popc(same & ((1u << lane) - 1u));
-    int at = 0;
-    if (e >= 0) {
-      at = mine[e];
-      row_of[i] = at + rank;
+  for (int64_t i0 = first; i0 < last; i0 += 32 * kSortAhead) {
+#pragma unroll
+    for (int k = 0; k < kSortAhead; ++k) {
+      const int64_t i = i0 + k * 32 + lane;
+      const int e = expert_of(ids, i, last, experts);
+      if (e >= 0) row_of[i] += mine[e] + own[e];
     }
-    __syncwarp();
-    if (e >= 0 && rank == 0) mine[e] = at + __popc(same);
-    __syncwarp();
   }
 }
+
+// ------------------------------------------------------------------ rows
+// The kernels below give a token's row (or a part of it, blockIdx.y) to `tpr`
+// threads, a power of two up to 256; several tokens share a block of 256.
+// Memory bounds them: a token's row is read or written once, its K rows in the
+// order by expert once, each access as wide as a row allows.
+
+constexpr int kRowThreads = 256;
+constexpr int kTopGroup = 4;  // rows of a token that are under way together
 
 // Rows are moved as words of U (16, 8, 4 or 2 bytes: the widest that divides
-// a row); a thread takes one word of a token's row and stores it K times.
-template <class U>
-__global__ void __launch_bounds__(256) expert_dispatch_kernel(const U* __restrict__ x, int64_t tokens, int top,
-                                                              int words, const int* __restrict__ row_of,
-                                                              const int* __restrict__ kept, U* __restrict__ xs) {
+// a row), NW a thread.
+template <class U, int NW>
+__global__ void __launch_bounds__(kRowThreads)
+    expert_dispatch_kernel(const U* __restrict__ x, int64_t tokens, int top, int words, int tpr,
+                           const int* __restrict__ row_of, const int* __restrict__ kept, U* __restrict__ xs) {
   pdl_enter();
-  const int64_t total = tokens * words;
+  const int lane = threadIdx.x % tpr;
+  const int64_t t = static_cast<int64_t>(blockIdx.x) * (kRowThreads / tpr) + threadIdx.x / tpr;
+  if (t >= tokens) return;
+  const int c0 = blockIdx.y * tpr * NW + lane;
+  U v[NW];
+#pragma unroll
+  for (int i = 0; i < NW; ++i)
+    if (c0 + i * tpr < words) v[i] = x[t * words + c0 + i * tpr];
   const int rows_kept = *kept;
-  for (int64_t j = blockIdx.x * static_cast<int64_t>(blockDim.x) + threadIdx.x; j < total;
-       j += static_cast<int64_t>(gridDim.x) * blockDim.x) {
-    const int64_t t = j / words, c = j - t * words;
-    const U v = x[j];
-    for (int k = 0; k < top; ++k) {
-      const int row = row_of[t * top + k];
-      xs[static_cast<int64_t>(row) * words + c] = row < rows_kept ? v : U{};
-    }
+  for (int k = 0; k < top; ++k) {
+    const int row = row_of[t * top + k];
+    U* to = xs + static_cast<int64_t>(row) * words + c0;
+#pragma unroll
+    for (int i = 0; i < NW; ++i)
+      if (c0 + i * tpr < words) to[i * tpr] = row < rows_kept ? v[i] : U{};
   }
 }
 
-// out[t] = sum_k w[t,k] y[row_of[t,k]]; one vector of a token's row a thread.
-template <class T, class W, int VEC>
-__global__ void __launch_bounds__(256) expert_combine_kernel(const T* __restrict__ y, const W* __restrict__ w,
-                                                             int64_t tokens, int top, int width,
-                                                             const int* __restrict__ row_of,
-                                                             const int* __restrict__ kept, T* __restrict__ out) {
+// out[t] = sum_k w[t,k] y[row_of[t,k]], NW vectors of VEC elements a thread.
+template <class T, class W, int VEC, int NW>
+__global__ void __launch_bounds__(kRowThreads)
+    expert_combine_kernel(const T* __restrict__ y, const W* __restrict__ w, int64_t tokens, int top, int width, int tpr,
+                          const int* __restrict__ row_of, const int* __restrict__ kept, T* __restrict__ out) {
   pdl_enter();
+  const int lane = threadIdx.x % tpr;
+  const int64_t t = static_cast<int64_t>(blockIdx.x) * (kRowThreads / tpr) + threadIdx.x / tpr;
+  if (t >= tokens) return;
   const int nvec = width / VEC;
-  const int64_t total = tokens * nvec;
+  const int c0 = blockIdx.y * tpr * NW + lane;
   const int rows_kept = *kept;
-  for (int64_t j = blockIdx.x * static_cast<int64_t>(blockDim.x) + threadIdx.x; j < total;
-       j += static_cast<int64_t>(gridDim.x) * blockDim.x) {
-    const int64_t t = j / nvec, c = j - t * nvec;
-    float acc[VEC];
+  float acc[NW][VEC];
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) acc[e] = 0.0f;
-    for (int k = 0; k < top; ++k) {
-      const int row = row_of[t * top + k];
-      if (row >= rows_kept) continue;  // a dropped slot's row is not read: it may hold anything
-      const float wk = w ? to_float(w[t * top + k]) : 1.0f;
-      float f[VEC];
-      unpack(load_raw<T, VEC>(y + static_cast<int64_t>(row) * width + c * VEC), f);
+  for (int i = 0; i < NW; ++i)
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) acc[e] += wk * f[e];
+    for (int e = 0; e < VEC; ++e) acc[i][e] = 0.0f;
+  for (int k0 = 0; k0 < top; k0 += kTopGroup) {
+    // A dropped slot's row is not read (it may hold anything), nor its weight.
+    Raw<T, VEC> v[kTopGroup][NW];
+    float wk[kTopGroup];
+    bool on[kTopGroup];
+#pragma unroll
+    for (int k = 0; k < kTopGroup; ++k) {
+      const int row = k0 + k < top ? row_of[t * top + k0 + k] : rows_kept;
+      on[k] = row < rows_kept;
+      wk[k] = on[k] && w ? to_float(w[t * top + k0 + k]) : 1.0f;
+#pragma unroll
+      for (int i = 0; i < NW; ++i)
+        if (on[k] && c0 + i * tpr < nvec)
+          v[k][i] = load_raw<T, VEC>(y + static_cast<int64_t>(row) * width + (c0 + i * tpr) * VEC);
     }
-    store_vec<T, VEC>(out + j * VEC, acc);
+#pragma unroll
+    for (int k = 0; k < kTopGroup; ++k) {
+      if (!on[k]) continue;
+#pragma unroll
+      for (int i = 0; i < NW; ++i) {
+        float f[VEC];
+        unpack(v[k][i], f);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) acc[i][e] += wk[k] * f[e];
+      }
+    }
   }
+#pragma unroll
+  for (int i = 0; i < NW; ++i)
+    if (c0 + i * tpr < nvec) store_vec<T, VEC>(out + t * width + (c0 + i * tpr) * VEC, acc[i]);
 }
 
-// dy and dw of the combine; a warp takes one slot.
+// dy and dw of the combine.  The tpr threads of a token go over its columns; 4
+// choices at a time, whose dot products they sum by shuffles and, above a
+// warp, through shared memory.
 template <class T, class W, int VEC>
-__global__ void __launch_bounds__(256) expert_combine_bwd_kernel(const T* __restrict__ gout, const T* __restrict__ y,
-                                                                 const W* __restrict__ w, int64_t tokens, int top,
-                                                                 int width, const int* __restrict__ row_of,
-                                                                 const int* __restrict__ kept, T* __restrict__ dy,
-                                                                 W* __restrict__ dw) {
+__global__ void __launch_bounds__(kRowThreads)
+    expert_combine_bwd_kernel(const T* __restrict__ gout, const T* __restrict__ y, const W* __restrict__ w,
+                              int64_t tokens, int top, int width, int tpr, const int* __restrict__ row_of,
+                              const int* __restrict__ kept, T* __restrict__ dy, W* __restrict__ dw) {
+  __shared__ float red[2][kRowThreads / 32][kTopGroup];
   pdl_enter();
-  const int nvec = width / VEC, lane = threadIdx.x % 32;
-  const int64_t slots = tokens * top;
+  const int lane = threadIdx.x % tpr;
+  const int64_t t = static_cast<int64_t>(blockIdx.x) * (kRowThreads / tpr) + threadIdx.x / tpr;
+  const bool live = t < tokens;  // the others take part in the shuffles and barriers
+  const int nvec = width / VEC;
   const int rows_kept = *kept;
-  for (int64_t i = (blockIdx.x * static_cast<int64_t>(blockDim.x) + threadIdx.x) / 32; i < slots;
-       i += static_cast<int64_t>(gridDim.x) * (blockDim.x / 32)) {
-    const int row = row_of[i];
-    const bool on = row < rows_kept;
-    const float wk = on ? (w ? to_float(w[i]) : 1.0f) : 0.0f;
-    const T* g = gout + (i / top) * width;
-    const int64_t base = static_cast<int64_t>(row) * width;
-    float dot = 0.0f;
-    for (int v = lane; v < nvec; v += 32) {
-      float d[VEC];
+  int half = 0;
+  for (int k0 = 0; k0 < top; k0 += kTopGroup, half ^= 1) {
+    int row[kTopGroup];  // below 0: no such choice
+    float wk[kTopGroup], dot[kTopGroup];
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) d[e] = 0.0f;
-      if (on) {
-        unpack(load_raw<T, VEC>(g + v * VEC), d);
-        if (dw) {
-          float f[VEC];
-          unpack(load_raw<T, VEC>(y + base + v * VEC), f);
-#pragma unroll
-          for (int e = 0; e < VEC; ++e) dot += d[e] * f[e];
-        }
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) d[e] *= wk;
-      }
-      if (dy) store_vec<T, VEC>(dy + base + v * VEC, d);
+    for (int k = 0; k < kTopGroup; ++k) {
+      row[k] = live && k0 + k < top ? row_of[t * top + k0 + k] : -1;
+      wk[k] = row[k] >= 0 && row[k] < rows_kept ? (w ? to_float(w[t * top + k0 + k]) : 1.0f) : 0.0f;
+      dot[k] = 0.0f;
     }
+    if (live)
+      for (int v = lane; v < nvec; v += tpr) {
+        Raw<T, VEC> yr[kTopGroup];
+        if (dw) {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
-    if (dw && lane == 0) dw[i] = from_float<W>(dot);
+          for (int k = 0; k < kTopGroup; ++k)
+            if (row[k] >= 0 && row[k] < rows_kept)
+              yr[k] = load_raw<T, VEC>(y + static_cast<int64_t>(row[k]) * width + v * VEC);
+        }
+        float g[VEC];
+        unpack(load_raw<T, VEC>(gout + t * width + v * VEC), g);
+#pragma unroll
+        for (int k = 0; k < kTopGroup; ++k) {
+          if (row[k] < 0) continue;
+          const bool on = row[k] < rows_kept;
+          float f[VEC];
+          if (dw && on) {
+            unpack(yr[k], f);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) dot[k] += g[e] * f[e];
+          }
+          if (dy) {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) f[e] = on ? wk[k] * g[e] : 0.0f;
+            store_vec<T, VEC>(dy + static_cast<int64_t>(row[k]) * width + v * VEC, f);
+          }
+        }
+      }
+    if (!dw) continue;
+#pragma unroll
+    for (int k = 0; k < kTopGroup; ++k)
+      for (int o = (tpr < 32 ? tpr : 32) / 2; o > 0; o >>= 1) dot[k] += __shfl_xor_sync(0xffffffffu, dot[k], o);
+    if (tpr > 32) {
+      const int warps = tpr / 32, warp = threadIdx.x / 32;
+      if (threadIdx.x % 32 == 0) {
+#pragma unroll
+        for (int k = 0; k < kTopGroup; ++k) red[half][warp][k] = dot[k];
+      }
+      __syncthreads();
+      if (lane < kTopGroup) {
+        float s = 0.0f;
+        for (int k = 0; k < warps; ++k) s += red[half][warp + k][lane];
+        if (live && k0 + lane < top) dw[t * top + k0 + lane] = from_float<W>(s);
+      }
+    } else if (lane == 0 && live) {
+#pragma unroll
+      for (int k = 0; k < kTopGroup; ++k)
+        if (k0 + k < top) dw[t * top + k0 + k] = from_float<W>(dot[k]);
+    }
   }
 }
 

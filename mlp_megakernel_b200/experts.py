@@ -55,14 +55,11 @@ class ExpertPlan(NamedTuple):
 def _sort(ids, num_experts):
     ids = _aligned(ids)
     slots = ids.numel()
-    lib = _lib.lib()
-    size = lib.mlpk_expert_sort_workspace_size(slots, num_experts)
     row_of = torch.empty(ids.shape, device=ids.device, dtype=torch.int32)
     offsets = torch.empty(num_experts + 1, device=ids.device, dtype=torch.int32)
-    work = torch.empty(max(size, 16), device=ids.device, dtype=torch.uint8)
-    _lib.check("mlpk_expert_sort", lib.mlpk_expert_sort(
+    _lib.check("mlpk_expert_sort", _lib.lib().mlpk_expert_sort(
         slots, num_experts, ids.data_ptr(), ids.element_size(), row_of.data_ptr(), offsets.data_ptr(),
-        work.data_ptr(), work.numel(), _current_stream(ids.get_device())))
+        _current_stream(ids.get_device())))
     return row_of, offsets
 
 

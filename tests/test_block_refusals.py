@@ -110,7 +110,7 @@ def test_shapes_on_fake_tensors(fake, dtype):
 
 def test_c_calls_refuse_before_they_touch_the_device(built_lib):
     lib, a = built_lib, 256  # an aligned address that is never read
-    sh, un, al, nu, sc = (1, 2, 5, 6, 8)
+    sh, un, al, nu = (1, 2, 5, 6)
     for want, args in ((sh, (-1, 8, 0, a, None, None, 0, 1e-6, a, None, None, None)),
                        (sh, (4, 0, 0, a, None, None, 0, 1e-6, a, None, None, None)),
                        (un, (4, 32769, 0, a, None, None, 0, 1e-6, a, None, None, None)),
@@ -125,12 +125,11 @@ def test_c_calls_refuse_before_they_touch_the_device(built_lib):
     assert lib.mlpk_rms_norm_fp8(4, 8, 0, a, None, None, 0, 1e-6, 0, a, None, None, None) == nu
     assert lib.mlpk_rms_norm_bwd(4, 8, 0, a, None, a, None, 0, a, None, a, a, a, 1 << 20, None) == nu  # no weight for dw
     assert lib.mlpk_rms_norm_bwd(4, 8, 0, a, None, a, a, 0, a, None, a, a, None, 0, None) == nu
-    assert lib.mlpk_expert_sort(-1, 4, a, 8, a, a, a, 1 << 20, None) == sh
-    assert lib.mlpk_expert_sort(8, 2000, a, 8, a, a, a, 1 << 20, None) == un
-    assert lib.mlpk_expert_sort(8, 4, a, 2, a, a, a, 1 << 20, None) == un
-    assert lib.mlpk_expert_sort(8, 4, a, 8, None, a, a, 1 << 20, None) == nu
-    assert lib.mlpk_expert_sort(8, 4, a, 8, a, a, a, 0, None) == sc
-    assert lib.mlpk_expert_sort_workspace_size(8, 2000) == -1
+    assert lib.mlpk_expert_sort(-1, 4, a, 8, a, a, None) == sh
+    assert lib.mlpk_expert_sort(8, 2000, a, 8, a, a, None) == un
+    assert lib.mlpk_expert_sort(8, 4, a, 2, a, a, None) == un
+    assert lib.mlpk_expert_sort(8, 4, a, 8, None, a, None) == nu
+    assert lib.mlpk_expert_sort(8, 4, a, 8, a + 4, a, None) == al
     assert lib.mlpk_expert_dispatch(2 ** 30, 2, 8, 0, a, a, a, a, None) == sh
     assert lib.mlpk_expert_dispatch(4, 2, 8, 7, a, a, a, a, None) == un
     assert lib.mlpk_expert_dispatch(4, 2, 8, 0, a, a, None, a, None) == nu
