@@ -28,15 +28,16 @@ int sort_slots(int64_t slots, int experts, const void* ids, int* row_of, int* of
   int dev = 0;
   int rc = cuda_status(cudaGetDevice(&dev));
   if (rc) return rc;
-  const auto kern = expert_sort_kernel<I>;
   int blocks = 1;
   while (blocks < 16 && slots > blocks * 4096) blocks *= 2;
   const int64_t part = ceil_div(ceil_div(slots, static_cast<int64_t>(blocks) * kSortWarps), 32) * 32;
+  const bool held = part <= 32 * kSortGroups;
+  const auto kern = held ? expert_sort_kernel<I, true> : expert_sort_kernel<I, false>;
   const size_t smem = sizeof(int) * (kSortWarps + static_cast<size_t>(kSortWarps + 1) * (experts + 1));
   if (blocks_per_sm(reinterpret_cast<const void*>(kern), kSortThreads, smem, dev) == 0) return MLPK_ERR_CUDA;
-  static std::once_flag wide[2][64];  // by type and device
+  static std::once_flag wide[2][64];  // by kernel and device
   if (blocks > 8 && dev < 64)
-    std::call_once(wide[sizeof(I) == 8][dev], [&] {
+    std::call_once(wide[held][dev], [&] {
       rc = cuda_status(cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     });
   if (rc) return rc;
@@ -56,31 +57,42 @@ int sort_slots(int64_t slots, int experts, const void* ids, int* row_of, int* of
   return cuda_status(cudaLaunchKernelEx(&cfg, kern, static_cast<const I*>(ids), slots, experts, part, row_of, offsets));
 }
 
-// Threads of a token's row of `items` words or vectors, `each` a thread.
-int threads_of_row(int64_t items, int each) {
-  int tpr = 1;
-  while (tpr < kRowThreads && static_cast<int64_t>(tpr) * each < items) tpr *= 2;
-  return tpr;
-}
-dim3 row_grid(int64_t tokens, int64_t items, int tpr, int each) {
-  return dim3(static_cast<unsigned>(ceil_div(tokens, kRowThreads / tpr)),
-              static_cast<unsigned>(ceil_div(items, static_cast<int64_t>(tpr) * each)));
+// Threads of a token's row of `items` words or vectors, `each` a thread, and the
+// blocks for the tokens, `tokens_each` a thread.
+struct RowGrid {
+  int tpr, threads;
+  dim3 grid;
+};
+RowGrid row_grid(int64_t tokens, int tokens_each, int64_t items, int each, bool parts) {
+  RowGrid g;
+  const int64_t want = std::min<int64_t>(ceil_div(items, each), kRowThreads);
+  g.tpr = 1;
+  while (g.tpr < want && g.tpr < 32) g.tpr *= 2;
+  if (want > 32) g.tpr = static_cast<int>(ceil_div(want, 32)) * 32;
+  const int subs = kRowThreads / g.tpr;
+  g.threads = subs * g.tpr;
+  g.grid = dim3(static_cast<unsigned>(ceil_div(tokens, static_cast<int64_t>(subs) * tokens_each)),
+                parts ? static_cast<unsigned>(ceil_div(items, static_cast<int64_t>(g.tpr) * each)) : 1);
+  return g;
 }
 
 template <class U>
 int dispatch_words(int64_t tokens, int top, int64_t words, const void* x, const int* row_of, const int* kept, void* xs,
                    cudaStream_t st) {
-  constexpr int NW = 2;
-  const int tpr = threads_of_row(words, NW);
-  return launch_kernel_early(expert_dispatch_kernel<U, NW>, row_grid(tokens, words, tpr, NW), kRowThreads, 0, st,
-                             static_cast<const U*>(x), tokens, top, static_cast<int>(words), tpr, row_of, kept,
-                             static_cast<U*>(xs));
+  constexpr int NW = sizeof(U) == 16 ? 1 : sizeof(U) == 8 ? 2 : 4, NT = 2;
+  const RowGrid g = row_grid(tokens, NT, words, NW, true);
+  return launch_kernel_early(expert_dispatch_kernel<U, NT, NW>, g.grid, g.threads, 0, st, static_cast<const U*>(x),
+                             tokens, top, static_cast<int>(words), g.tpr, row_of, kept, static_cast<U*>(xs));
 }
 
-// f(T, W, VEC)
+// f(T, W, VEC): 16-byte vectors where the width allows them, else pairs of
+// 16-bit values, else single ones.
 template <class T, class W, class F>
 int with_vec(int width, F&& f) {
   if (width % kVecOf<T> == 0) return f(T{}, W{}, std::integral_constant<int, kVecOf<T>>{});
+  if constexpr (sizeof(T) == 2) {
+    if (width % 2 == 0) return f(T{}, W{}, std::integral_constant<int, 2>{});
+  }
   return f(T{}, W{}, std::integral_constant<int, 1>{});
 }
 template <class F>
@@ -90,6 +102,12 @@ int with_types(int dtype, int w_dtype, int width, F&& f) {
     return w_dtype == MLPK_DT_F32 ? with_vec<__half, float>(width, f) : with_vec<__half, __half>(width, f);
   return w_dtype == MLPK_DT_F32 ? with_vec<__nv_bfloat16, float>(width, f)
                                 : with_vec<__nv_bfloat16, __nv_bfloat16>(width, f);
+}
+// f(GROUP): choices of a token that are under way together.
+template <class F>
+int with_group(int top, F&& f) {
+  if (top <= 2) return f(std::integral_constant<int, 2>{});
+  return f(std::integral_constant<int, 4>{});
 }
 
 }  // namespace
@@ -141,12 +159,15 @@ int mlpk_expert_combine(int64_t tokens, int top, int width, int dtype, const voi
   return with_types(dtype, weights ? w_dtype : dtype, width, [&](auto t, auto w, auto vec) {
     using T = decltype(t);
     using W = decltype(w);
-    constexpr int V = decltype(vec)::value, NW = V == 1 ? 4 : 1;
-    const int tpr = threads_of_row(width / V, NW);
-    return launch_kernel_early(expert_combine_kernel<T, W, V, NW>, row_grid(tokens, width / V, tpr, NW), kRowThreads, 0,
-                               static_cast<cudaStream_t>(stream), static_cast<const T*>(y),
-                               static_cast<const W*>(weights), tokens, top, width, tpr, row_of, kept,
-                               static_cast<T*>(out));
+    constexpr int V = decltype(vec)::value, NW = V == kVecOf<T> ? 1 : 4;
+    return with_group(top, [&](auto group) {
+      constexpr int GROUP = decltype(group)::value;
+      const RowGrid g = row_grid(tokens, kRowsAhead / GROUP, width / V, NW, true);
+      return launch_kernel_early(expert_combine_kernel<T, W, V, NW, GROUP>, g.grid, g.threads, 0,
+                                 static_cast<cudaStream_t>(stream), static_cast<const T*>(y),
+                                 static_cast<const W*>(weights), tokens, top, width, g.tpr, row_of, kept,
+                                 static_cast<T*>(out));
+    });
   });
 }
 
@@ -165,11 +186,14 @@ int mlpk_expert_combine_bwd(int64_t tokens, int top, int width, int dtype, const
     using T = decltype(t);
     using W = decltype(w);
     constexpr int V = decltype(vec)::value;
-    const int tpr = threads_of_row(width / V, V == 1 ? 4 : 1);
-    return launch_kernel_early(expert_combine_bwd_kernel<T, W, V>, dim3(ceil_div(tokens, kRowThreads / tpr)),
-                               kRowThreads, 0, static_cast<cudaStream_t>(stream), static_cast<const T*>(grad_out),
-                               static_cast<const T*>(y), static_cast<const W*>(weights), tokens, top, width, tpr,
-                               row_of, kept, static_cast<T*>(dy), static_cast<W*>(dw));
+    return with_group(top, [&](auto group) {
+      constexpr int GROUP = decltype(group)::value;
+      const RowGrid g = row_grid(tokens, 4 / GROUP, width / V, V == kVecOf<T> ? 1 : 2, false);
+      return launch_kernel_early(expert_combine_bwd_kernel<T, W, V, GROUP>, g.grid, g.threads, 0,
+                                 static_cast<cudaStream_t>(stream), static_cast<const T*>(grad_out),
+                                 static_cast<const T*>(y), static_cast<const W*>(weights), tokens, top, width, g.tpr,
+                                 row_of, kept, static_cast<T*>(dy), static_cast<W*>(dw));
+    });
   });
 }
 
