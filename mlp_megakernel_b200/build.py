@@ -11,12 +11,15 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 LIBDIR = os.path.join(HERE, "lib")
 LIB = os.path.join(LIBDIR, "libmlpk.so")
+BINDING = os.path.join(LIBDIR, "mlpk_torch.so")
+BINDING_SRC = "torch_binding.cpp"
 
 # Each translation unit with the headers it is built from.
 SOURCES = {
@@ -106,10 +109,33 @@ def _compile(source: str, verbose: bool, ptxas_info: bool) -> str:
     return said
 
 
+def _torch_flags() -> list:
+    """What the binding's compiler needs to find torch, Python and the library."""
+    from torch.utils import cpp_extension
+
+    flags = [f"-I{p}" for p in cpp_extension.include_paths("cuda") + [sysconfig.get_paths()["include"]]]
+    flags += [f"-L{p}" for p in cpp_extension.library_paths("cuda") + [LIBDIR]]
+    return flags + ["-ltorch_python", "-ltorch_cuda", "-ltorch_cpu", "-ltorch", "-lc10_cuda", "-lc10", "-l:libmlpk.so",
+                    "-Wl,-rpath,$ORIGIN"]
+
+
+def build_binding(force: bool = False, verbose: bool = False) -> str:
+    """Compile the torch binding of the block operators (host code only) if it is
+    missing or older than its source; return its path."""
+    source = os.path.join(CSRC, BINDING_SRC)
+    if force or _newer([source, os.path.join(ROOT, "include", "mlpk.h"), os.path.abspath(__file__)], BINDING):
+        _run([os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-o",
+              BINDING + ".tmp", source, *_torch_flags()], verbose)
+        os.replace(BINDING + ".tmp", BINDING)
+    return BINDING
+
+
 def build(force: bool = False, verbose: bool = False, ptxas_info: bool = False) -> str:
     """Compile the translation units of libmlpk.so that are older than their
-    sources, side by side, link the library if any was; return its path."""
+    sources, side by side, link the library if any was, and see to the torch
+    binding; return the library's path."""
     if not force and not _stale():
+        build_binding(verbose=verbose)
         return LIB
     os.makedirs(LIBDIR, exist_ok=True)
     todo = [s for s in SOURCES if force or _newer(_inputs(s), _object(s))]
@@ -119,6 +145,7 @@ def build(force: bool = False, verbose: bool = False, ptxas_info: bool = False) 
     if verbose or ptxas_info:
         sys.stderr.write(said)
     os.replace(LIB + ".tmp", LIB)
+    build_binding(force, verbose)
     return LIB
 
 

@@ -11,9 +11,9 @@ MLP experts (no counterpart in the reference, which has one MLP).
 
 Rows are fp16, bf16 or fp32 of any width; sums are fp32 in a fixed order, so
 results are the same from run to run.  Everything runs on the current CUDA
-stream without a wait of the host; there is no CPU path.  Under torch.compile
-the calls are the operators ``torch.ops.mlpk.expert_*``; eager calls go straight
-to the C ABI.
+stream without a wait of the host; there is no CPU path.  Eager calls go through
+the native binding (_native.py); under torch.compile and on fake tensors the
+calls are the operators ``torch.ops.mlpk.expert_*``.
 """
 from __future__ import annotations
 
@@ -25,10 +25,9 @@ import torch.nn as nn
 from torch import Tensor
 
 from . import _lib
-from .functional import _current_stream, _is_fake
+from ._native import native
 from .modules import FusedMLPSoftplus
-from .norm import DTYPES, FusedRMSNorm, _needs_grad, _on_device, _ptr
-from .ops import _aligned
+from .norm import DTYPES, FusedRMSNorm, _eager, _needs_grad
 
 
 class ExpertPlan(NamedTuple):
@@ -50,61 +49,6 @@ class ExpertPlan(NamedTuple):
         return self.offsets.diff()
 
 
-# ------------------------------------------------------------ kernels
-@_on_device
-def _sort(ids, num_experts):
-    ids = _aligned(ids)
-    slots = ids.numel()
-    row_of = torch.empty(ids.shape, device=ids.device, dtype=torch.int32)
-    offsets = torch.empty(num_experts + 1, device=ids.device, dtype=torch.int32)
-    _lib.check("mlpk_expert_sort", _lib.lib().mlpk_expert_sort(
-        slots, num_experts, ids.data_ptr(), ids.element_size(), row_of.data_ptr(), offsets.data_ptr(),
-        _current_stream(ids.get_device())))
-    return row_of, offsets
-
-
-def _kept(offsets: Tensor) -> int:
-    return offsets.data_ptr() + 4 * (offsets.shape[0] - 1)
-
-
-@_on_device
-def _dispatch(x, row_of, offsets):
-    x, row_of = _aligned(x), _aligned(row_of)
-    T, K = row_of.shape
-    xs = torch.empty((T * K, x.shape[1]), device=x.device, dtype=x.dtype)
-    _lib.check("mlpk_expert_dispatch", _lib.lib().mlpk_expert_dispatch(
-        T, K, x.shape[1], DTYPES[x.dtype], x.data_ptr(), row_of.data_ptr(), _kept(offsets), xs.data_ptr(),
-        _current_stream(x.get_device())))
-    return xs
-
-
-@_on_device
-def _combine(y, weights, row_of, offsets):
-    y, row_of = _aligned(y), _aligned(row_of)
-    weights = None if weights is None else weights.contiguous()
-    T, K = row_of.shape
-    out = torch.empty((T, y.shape[1]), device=y.device, dtype=y.dtype)
-    _lib.check("mlpk_expert_combine", _lib.lib().mlpk_expert_combine(
-        T, K, y.shape[1], DTYPES[y.dtype], y.data_ptr(), _ptr(weights),
-        DTYPES[y.dtype if weights is None else weights.dtype], row_of.data_ptr(), _kept(offsets), out.data_ptr(),
-        _current_stream(y.get_device())))
-    return out
-
-
-@_on_device
-def _combine_bwd(grad_out, y, weights, row_of, offsets, want_dy, want_dw):
-    grad_out, y, row_of = _aligned(grad_out), _aligned(y), _aligned(row_of)
-    weights = None if weights is None else weights.contiguous()
-    T, K = row_of.shape
-    dy = torch.empty_like(y) if want_dy else None
-    dw = torch.empty_like(weights) if want_dw else None
-    _lib.check("mlpk_expert_combine_bwd", _lib.lib().mlpk_expert_combine_bwd(
-        T, K, y.shape[1], DTYPES[y.dtype], grad_out.data_ptr(), y.data_ptr(), _ptr(weights),
-        DTYPES[y.dtype if weights is None else weights.dtype], row_of.data_ptr(), _kept(offsets), _ptr(dy), _ptr(dw),
-        _current_stream(y.get_device())))
-    return dy, dw
-
-
 # ------------------------------------------------------------ torch.ops.mlpk
 def _require_cuda(*ts):
     for t in ts:
@@ -115,7 +59,7 @@ def _require_cuda(*ts):
 @torch.library.custom_op("mlpk::expert_sort", mutates_args=())
 def _sort_op(ids: Tensor, num_experts: int) -> list[Tensor]:
     _require_cuda(ids)
-    return list(_sort(ids, num_experts))
+    return list(native().expert_sort(ids, num_experts))
 
 
 @_sort_op.register_fake
@@ -126,7 +70,7 @@ def _sort_fake(ids, num_experts):
 @torch.library.custom_op("mlpk::expert_dispatch", mutates_args=())
 def _dispatch_op(x: Tensor, row_of: Tensor, offsets: Tensor) -> Tensor:
     _require_cuda(x, row_of, offsets)
-    return _dispatch(x, row_of, offsets)
+    return native().dispatch_rows(x, row_of, offsets)
 
 
 @_dispatch_op.register_fake
@@ -137,7 +81,7 @@ def _dispatch_fake(x, row_of, offsets):
 @torch.library.custom_op("mlpk::expert_combine", mutates_args=())
 def _combine_op(y: Tensor, weights: Optional[Tensor], row_of: Tensor, offsets: Tensor) -> Tensor:
     _require_cuda(y, weights, row_of, offsets)
-    return _combine(y, weights, row_of, offsets)
+    return native().combine_rows(y, weights, row_of, offsets)
 
 
 @_combine_op.register_fake
@@ -150,7 +94,8 @@ def _combine_bwd_op(grad_out: Tensor, y: Tensor, weights: Optional[Tensor], row_
                     want_dy: bool, want_dw: bool) -> list[Tensor]:
     """[dy] and / or [dw], as wanted."""
     _require_cuda(grad_out, y, weights, row_of, offsets)
-    return [t for t in _combine_bwd(grad_out, y, weights, row_of, offsets, want_dy, want_dw) if t is not None]
+    dy, dw = native().combine_backward(grad_out, y, weights, row_of, offsets, want_dy, want_dw)
+    return ([dy] if want_dy else []) + ([dw] if want_dw else [])
 
 
 @_combine_bwd_op.register_fake
@@ -158,43 +103,34 @@ def _combine_bwd_fake(grad_out, y, weights, row_of, offsets, want_dy, want_dw):
     return ([y.new_empty(y.shape)] if want_dy else []) + ([weights.new_empty(weights.shape)] if want_dw else [])
 
 
-def _traced(t: Tensor) -> bool:
-    return torch.compiler.is_compiling() or _is_fake(t)
-
-
 # ------------------------------------------------------------ autograd
 class _DispatchFn(torch.autograd.Function):
+    """The node that torch.compile traces (as _CombineFn)."""
+
     @staticmethod
     def forward(ctx, x, row_of, offsets):
         ctx.save_for_backward(row_of, offsets)
-        return (torch.ops.mlpk.expert_dispatch if _traced(x) else _dispatch)(x, row_of, offsets)
+        return torch.ops.mlpk.expert_dispatch(x, row_of, offsets)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
-        row_of, offsets = ctx.saved_tensors
-        return (torch.ops.mlpk.expert_combine if _traced(grad) else _combine)(grad, None, row_of, offsets), None, None
+        return torch.ops.mlpk.expert_combine(grad, None, *ctx.saved_tensors), None, None
 
 
 class _CombineFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, y, weights, row_of, offsets):
-        ctx.has_weights = weights is not None
-        ctx.save_for_backward(y, row_of, offsets, *([weights] if ctx.has_weights else []))
-        return (torch.ops.mlpk.expert_combine if _traced(y) else _combine)(y, weights, row_of, offsets)
+        ctx.save_for_backward(y, weights, row_of, offsets)
+        return torch.ops.mlpk.expert_combine(y, weights, row_of, offsets)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
-        y, row_of, offsets, *rest = ctx.saved_tensors
-        weights = rest[0] if rest else None
-        want_dy, want_dw = ctx.needs_input_grad[0], ctx.has_weights and ctx.needs_input_grad[1]
-        if _traced(grad):
-            got = torch.ops.mlpk.expert_combine_bwd(grad, y, weights, row_of, offsets, want_dy, want_dw)
-            dy, dw = (got[0] if want_dy else None), (got[-1] if want_dw else None)
-        else:
-            dy, dw = _combine_bwd(grad, y, weights, row_of, offsets, want_dy, want_dw)
-        return dy, dw, None, None
+        y, weights, row_of, offsets = ctx.saved_tensors
+        want_dy, want_dw = ctx.needs_input_grad[0], weights is not None and ctx.needs_input_grad[1]
+        got = torch.ops.mlpk.expert_combine_bwd(grad, y, weights, row_of, offsets, want_dy, want_dw)
+        return got[0] if want_dy else None, got[-1] if want_dw else None, None, None
 
 
 # ------------------------------------------------------------ public calls
@@ -207,6 +143,10 @@ def expert_sort(ids: Tensor, num_experts: int) -> ExpertPlan:
     dropped: dispatch gives it a row of zeros behind the kept rows, combine
     leaves it out.  At most 1024 experts and 2^31 - 1 slots.
     """
+    if _eager(ids):
+        got = native().expert_sort(ids, num_experts)
+        if got is not None:
+            return ExpertPlan(*got)
     if not isinstance(ids, Tensor) or ids.dim() != 2:
         raise ValueError("ids must be a 2-D tensor [tokens, choices]")
     _require_cuda(ids)
@@ -216,7 +156,7 @@ def expert_sort(ids: Tensor, num_experts: int) -> ExpertPlan:
         raise ValueError(f"num_experts must be 1 to {_lib.EXPERT_MAX}, got {num_experts}")
     if ids.shape[1] < 1 or ids.numel() > 2 ** 31 - 1:
         raise ValueError(f"ids must have at least one choice a token and at most 2^31 - 1 slots, got {tuple(ids.shape)}")
-    return ExpertPlan(*(torch.ops.mlpk.expert_sort if _traced(ids) else _sort)(ids, num_experts))
+    return ExpertPlan(*torch.ops.mlpk.expert_sort(ids, num_experts))
 
 
 def _check_rows(what: str, t: Tensor, rows: int, plan: ExpertPlan) -> None:
@@ -234,10 +174,14 @@ def _check_rows(what: str, t: Tensor, rows: int, plan: ExpertPlan) -> None:
 def expert_dispatch(x: Tensor, plan: ExpertPlan) -> Tensor:
     """``[tokens * choices, width]``: row ``plan.row_of[t, k]`` is ``x[t]``, rows
     of dropped slots are zero.  Differentiable in x (a sum over the kept slots)."""
+    if _eager(x):
+        got = native().expert_dispatch(x, *plan)
+        if got is not None:
+            return got
     _check_rows("x", x, plan.row_of.shape[0], plan)
     if _needs_grad(x):
         return _DispatchFn.apply(x, *plan)
-    return (torch.ops.mlpk.expert_dispatch if _traced(x) else _dispatch)(x, *plan)
+    return torch.ops.mlpk.expert_dispatch(x, *plan)
 
 
 def expert_combine(y: Tensor, weights: Optional[Tensor], plan: ExpertPlan) -> Tensor:
@@ -245,13 +189,17 @@ def expert_combine(y: Tensor, weights: Optional[Tensor], plan: ExpertPlan) -> Te
     in fp32; dropped slots add nothing, whatever their rows and weights hold.
     ``weights`` is ``[tokens, choices]`` in y's dtype or fp32, or None for ones.
     Differentiable in y and weights."""
+    if _eager(y):
+        got = native().expert_combine(y, weights, *plan)
+        if got is not None:
+            return got
     _check_rows("y", y, plan.row_of.numel(), plan)
     if weights is not None and (weights.shape != plan.row_of.shape or weights.device != y.device
                                 or (weights.dtype != y.dtype and weights.dtype != torch.float32)):
         raise ValueError(f"weights must be a {tuple(plan.row_of.shape)} tensor of {y.dtype} or float32 on {y.device}")
     if _needs_grad(y, weights):
         return _CombineFn.apply(y, weights, *plan)
-    return (torch.ops.mlpk.expert_combine if _traced(y) else _combine)(y, weights, *plan)
+    return torch.ops.mlpk.expert_combine(y, weights, *plan)
 
 
 class FusedMLPExperts(nn.Module):

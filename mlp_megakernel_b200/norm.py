@@ -9,9 +9,10 @@ reference, whose MLP takes its rows as they come).
 
 x is fp16, bf16 or fp32 of shape ``[..., width]`` with width up to 32768; all
 arithmetic is fp32.  The kernels run on the current CUDA stream; there is no
-CPU path.  Under torch.compile the calls are the operators
-``torch.ops.mlpk.rms_norm`` / ``rms_norm_bwd`` / ``rms_norm_fp8``; eager calls
-go straight to the C ABI.
+CPU path.  Eager calls go through the native binding (_native.py), whose
+autograd nodes are native too; under torch.compile and on fake tensors the
+calls are the operators ``torch.ops.mlpk.rms_norm`` / ``rms_norm_bwd`` /
+``rms_norm_fp8``.
 """
 from __future__ import annotations
 
@@ -22,25 +23,15 @@ import torch.nn as nn
 from torch import Tensor
 
 from . import _lib
-from .functional import _current_stream, _is_fake
-from .ops import _aligned
+from ._native import native
 
 DTYPES = {torch.float16: _lib.DT_F16, torch.float32: _lib.DT_F32, torch.bfloat16: _lib.DT_BF16}
 
 
-def _on_device(fn):
-    """fn(x, ...) with x's device current, as the C ABI launches on it."""
-    def call(x, *args):
-        dev = x.get_device()
-        if dev == torch.cuda.current_device():
-            return fn(x, *args)
-        with torch.cuda.device(dev):
-            return fn(x, *args)
-    return call
-
-
-def _ptr(t: Optional[Tensor]):
-    return None if t is None else t.data_ptr()
+def _eager(x) -> bool:
+    """Whether x is an ordinary tensor outside of tracing: the native calls take
+    it."""
+    return (type(x) is Tensor or type(x) is nn.Parameter) and not torch.compiler.is_compiling()
 
 
 def _check(x, weight, residual, eps):
@@ -62,76 +53,12 @@ def _check(x, weight, residual, eps):
         raise ValueError(f"eps must not be negative, got {eps}")
 
 
-def _w_dtype(weight, x) -> int:
-    return DTYPES[x.dtype if weight is None else weight.dtype]
-
-
-@_on_device
-def _forward(x, weight, residual, eps, want_rstd):
-    """(y, h, rstd): h is x itself without a residual, rstd None unless wanted."""
-    x = _aligned(x)
-    width = x.shape[-1]
-    rows = x.numel() // width
-    y = torch.empty_like(x)
-    rstd = torch.empty(rows, device=x.device, dtype=torch.float32) if want_rstd else None
-    if residual is not None:
-        residual, h = _aligned(residual), torch.empty_like(x)
-    else:
-        h = None
-    weight = None if weight is None else _aligned(weight)
-    _lib.check("mlpk_rms_norm", _lib.lib().mlpk_rms_norm(
-        rows, width, DTYPES[x.dtype], x.data_ptr(), _ptr(residual), _ptr(weight), _w_dtype(weight, x), eps,
-        y.data_ptr(), _ptr(h), _ptr(rstd), _current_stream(x.get_device())))
-    return y, x if h is None else h, rstd
-
-
-@_on_device
-def _backward(x, residual, weight, rstd, grad_y, grad_h, want_dw):
-    """(dx, dw): dw in weight's dtype, None unless wanted."""
-    x, grad_y = _aligned(x), _aligned(grad_y)
-    residual = None if residual is None else _aligned(residual)
-    grad_h = None if grad_h is None else _aligned(grad_h)
-    weight = None if weight is None else _aligned(weight)
-    width = x.shape[-1]
-    rows = x.numel() // width
-    dx = torch.empty_like(x)
-    dw = work = None
-    lib = _lib.lib()
-    if want_dw:
-        dw = torch.empty_like(weight)
-        size = lib.mlpk_rms_norm_bwd_workspace_size(rows, width, DTYPES[x.dtype])
-        work = torch.empty(max(size, 16), device=x.device, dtype=torch.uint8)
-    _lib.check("mlpk_rms_norm_bwd", lib.mlpk_rms_norm_bwd(
-        rows, width, DTYPES[x.dtype], x.data_ptr(), _ptr(residual), rstd.data_ptr(), _ptr(weight),
-        _w_dtype(weight, x), grad_y.data_ptr(), _ptr(grad_h), dx.data_ptr(), _ptr(dw), _ptr(work),
-        0 if work is None else work.numel(), _current_stream(x.get_device())))
-    return dx, dw
-
-
-@_on_device
-def _forward_fp8(x, weight, residual, eps, group):
-    x = _aligned(x)
-    width = x.shape[-1]
-    rows = x.numel() // width
-    q = torch.empty(x.shape, device=x.device, dtype=torch.float8_e4m3fn)
-    groups = -(-width // group) if group else 1
-    scale = torch.empty((*x.shape[:-1], groups), device=x.device, dtype=torch.float32)
-    h = None
-    if residual is not None:
-        residual, h = _aligned(residual), torch.empty_like(x)
-    weight = None if weight is None else _aligned(weight)
-    _lib.check("mlpk_rms_norm_fp8", _lib.lib().mlpk_rms_norm_fp8(
-        rows, width, DTYPES[x.dtype], x.data_ptr(), _ptr(residual), _ptr(weight), _w_dtype(weight, x), eps, group,
-        q.data_ptr(), scale.data_ptr(), _ptr(h), _current_stream(x.get_device())))
-    return q, scale, h
-
-
 # ------------------------------------------------------------ torch.ops.mlpk
 @torch.library.custom_op("mlpk::rms_norm", mutates_args=())
 def rms_norm(x: Tensor, weight: Optional[Tensor], residual: Optional[Tensor], eps: float) -> list[Tensor]:
     """[y, rstd], and h with a residual."""
     _check(x, weight, residual, eps)
-    y, h, rstd = _forward(x, weight, residual, eps, True)
+    y, h, rstd = native().norm_forward(x, weight, residual, eps)
     return [y, rstd] if residual is None else [y, rstd, h]
 
 
@@ -145,8 +72,8 @@ def _rms_norm_fake(x, weight, residual, eps):
 def rms_norm_bwd(x: Tensor, residual: Optional[Tensor], weight: Optional[Tensor], rstd: Tensor, grad_y: Tensor,
                  grad_h: Optional[Tensor], want_dw: bool) -> list[Tensor]:
     """[dx], and dw if wanted."""
-    dx, dw = _backward(x, residual, weight, rstd, grad_y, grad_h, want_dw)
-    return [dx] if dw is None else [dx, dw]
+    dx, dw = native().norm_backward(x, residual, weight, rstd, grad_y, grad_h, want_dw)
+    return [dx, dw] if want_dw else [dx]
 
 
 @rms_norm_bwd.register_fake
@@ -159,8 +86,8 @@ def rms_norm_fp8(x: Tensor, weight: Optional[Tensor], residual: Optional[Tensor]
                  group: int) -> list[Tensor]:
     """[q, scale], and h with a residual."""
     _check(x, weight, residual, eps)
-    q, scale, h = _forward_fp8(x, weight, residual, eps, group)
-    return [q, scale] if h is None else [q, scale, h]
+    with torch.no_grad():
+        return list(native().rms_norm_fp8(x, weight, residual, eps, group))
 
 
 @rms_norm_fp8.register_fake
@@ -173,17 +100,14 @@ def _rms_norm_fp8_fake(x, weight, residual, eps, group):
 
 # ------------------------------------------------------------ autograd
 class _RMSNormFn(torch.autograd.Function):
+    """The node that torch.compile traces."""
+
     @staticmethod
     def forward(ctx, x, weight, residual, eps):
-        if torch.compiler.is_compiling() or _is_fake(x):
-            y, rstd, *rest = torch.ops.mlpk.rms_norm(x, weight, residual, eps)
-            h = rest[0] if rest else None
-        else:
-            y, h, rstd = _forward(x, weight, residual, eps, True)
-        ctx.has_residual = residual is not None
+        y, rstd, *h = torch.ops.mlpk.rms_norm(x, weight, residual, eps)
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(x, residual, weight, rstd)
-        return (y, h) if ctx.has_residual else y
+        return (y, h[0]) if h else y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
@@ -192,13 +116,11 @@ class _RMSNormFn(torch.autograd.Function):
         want_dw = weight is not None and ctx.needs_input_grad[1]
         if grad_y is None:  # y was not used: the norm adds nothing
             dx, dw = grad_h, torch.zeros_like(weight) if want_dw and grad_h is not None else None
-        elif torch.compiler.is_compiling() or _is_fake(x):
+        else:
             dx, *dws = torch.ops.mlpk.rms_norm_bwd(x, residual, weight, rstd, grad_y, grad_h, want_dw)
             dw = dws[0] if dws else None
-        else:
-            dx, dw = _backward(x, residual, weight, rstd, grad_y, grad_h, want_dw)
         return (dx if ctx.needs_input_grad[0] else None, dw,
-                dx if ctx.has_residual and ctx.needs_input_grad[2] else None, None)
+                dx if residual is not None and ctx.needs_input_grad[2] else None, None)
 
 
 def _needs_grad(*ts) -> bool:
@@ -216,14 +138,15 @@ def fused_rms_norm(x: Tensor, weight: Optional[Tensor] = None, *, residual: Opti
     over the rows in fp32 in a fixed order.  A row that holds an infinity or a
     NaN gives NaN where it stands, as the formula does.
     """
+    if _eager(x):
+        got = native().rms_norm(x, weight, residual, eps)
+        if got is not None:
+            return got
     _check(x, weight, residual, eps)
     if _needs_grad(x, weight, residual):
         return _RMSNormFn.apply(x, weight, residual, eps)
-    if torch.compiler.is_compiling() or _is_fake(x):
-        y, _, *rest = torch.ops.mlpk.rms_norm(x, weight, residual, eps)
-        return (y, rest[0]) if rest else y
-    y, h, _ = _forward(x, weight, residual, eps, False)
-    return y if residual is None else (y, h)
+    y, _, *h = torch.ops.mlpk.rms_norm(x, weight, residual, eps)
+    return (y, h[0]) if h else y
 
 
 def fused_rms_norm_fp8(x: Tensor, weight: Optional[Tensor] = None, *, residual: Optional[Tensor] = None,
@@ -236,15 +159,16 @@ def fused_rms_norm_fp8(x: Tensor, weight: Optional[Tensor] = None, *, residual: 
     (``group=128``, the last group may be shorter).  A NaN makes its group's
     scale NaN.  For inference: raises where a gradient would be needed.
     """
+    if _eager(x):
+        got = native().rms_norm_fp8(x, weight, residual, eps, group)
+        if got is not None:
+            return got
     _check(x, weight, residual, eps)
     if group not in (0, _lib.NORM_GROUP):
         raise ValueError(f"group must be 0 (the row) or {_lib.NORM_GROUP}, got {group}")
     if _needs_grad(x, weight, residual):
         raise RuntimeError("fused_rms_norm_fp8 has no gradient: call it under torch.no_grad()")
-    if torch.compiler.is_compiling() or _is_fake(x):
-        return tuple(torch.ops.mlpk.rms_norm_fp8(x, weight, residual, eps, group))
-    q, scale, h = _forward_fp8(x, weight, residual, eps, group)
-    return (q, scale) if h is None else (q, scale, h)
+    return tuple(torch.ops.mlpk.rms_norm_fp8(x, weight, residual, eps, group))
 
 
 class FusedRMSNorm(nn.Module):

@@ -9,14 +9,11 @@ no CPU path.
 """
 from __future__ import annotations
 
-import contextlib
-import ctypes
-
 import torch
 from torch import Tensor
 
 from . import _lib
-from .functional import _current_stream
+from ._native import native
 from .norm import DTYPES
 
 BLOCK = _lib.ADAMW_BLOCK
@@ -45,16 +42,12 @@ class _Bucket:
 
     def __init__(self, params, bits: int, master: bool):
         self.params, self.bits = list(params), bits
-        self.index = {p: i for i, p in enumerate(self.params)}
         self.numel = [p.numel() for p in self.params]
         self.off, total = [], 0
         for n in self.numel:
             self.off.append(total)
             total += _blocks(n) * BLOCK
-        self.device = dev = self.params[0].device
-        self.dtype = self.params[0].dtype
-        self.strides = {p: p.stride() for p in self.params}
-
+        dev = self.params[0].device
         total = max(total, BLOCK)  # tensors of no elements have a state too
 
         def zeros(n, dtype):
@@ -74,18 +67,9 @@ class _Bucket:
             for i, p in enumerate(self.params):
                 self.view(i, "master_param").copy_(p.detach())
         sq = self.flat["exp_avg_rms" if bits == 8 else "exp_avg_sq"]
-        self.struct = _lib.MlpkAdamwState(
-            bits, self.flat["exp_avg"].data_ptr(), sq.data_ptr(),
-            self.flat["exp_avg_scale"].data_ptr() if bits == 8 else None,
-            self.flat["exp_avg_rms_scale"].data_ptr() if bits == 8 else None,
-            self.flat["master_param"].data_ptr() if master else None, self.ticks.data_ptr())
-        self.arrays = self.arrays_of(range(len(self.params)))
-
-    def arrays_of(self, which):
-        """The parts of the C call's table that stay: sizes, places, counters."""
-        n = len(which)
-        return ((ctypes.c_int64 * n)(*[self.numel[i] for i in which]),
-                (ctypes.c_int64 * n)(*[self.off[i] for i in which]), (ctypes.c_int32 * n)(*which))
+        self.native = native().AdamwBucket(
+            self.params, self.off, bits, self.flat["exp_avg"], sq, self.flat.get("exp_avg_scale"),
+            self.flat.get("exp_avg_rms_scale"), self.flat.get("master_param"), self.ticks)
 
     def view(self, i: int, name: str) -> Tensor:
         """Tensor i's part of a flat buffer: of its own shape and strides, or
@@ -185,59 +169,17 @@ class FusedAdamW(torch.optim.Optimizer):
         grad_scale = getattr(self, "grad_scale", None) if grad_scale is None else grad_scale
         found_inf = getattr(self, "found_inf", None) if found_inf is None else found_inf
         for g, group in enumerate(self.param_groups):
-            new = [p for p in group["params"] if p.grad is not None and p not in self.state]
-            if new:
-                self._bucket(g, new)
-            for b in self._buckets[g]:
-                self._step_bucket(b, group, grad_scale, found_inf)
+            buckets = self._buckets[g]
+            if sum(len(b.params) for b in buckets) < len(group["params"]):
+                new = [p for p in group["params"] if p.grad is not None and p not in self.state]
+                if new:
+                    self._bucket(g, new)
+            lr, (b1, b2) = group["lr"], group["betas"]
+            lr, lr_tensor = (0.0, lr) if isinstance(lr, Tensor) else (lr, None)
+            for b in buckets:
+                b.native.step(lr, lr_tensor, b1, b2, group["eps"], group["weight_decay"], group["maximize"], grad_scale,
+                              found_inf)
         return loss
-
-    @staticmethod
-    def _step_bucket(b: _Bucket, group, grad_scale, found_inf) -> None:
-        params, arrays = b.params, b.arrays
-        grads = [p.grad for p in params]
-        if any(g is None for g in grads):
-            which = [i for i, g in enumerate(grads) if g is not None]
-            if not which:
-                return
-            params, grads, arrays = [params[i] for i in which], [grads[i] for i in which], b.arrays_of(which)
-        kinds = {g.dtype for g in grads}
-        if len(kinds) == 1:
-            FusedAdamW._launch(b, params, grads, arrays, group, grad_scale, found_inf)
-            return
-        for kind in kinds:  # fp32 gradients beside 16-bit ones: a launch for each
-            part = [(p, g) for p, g in zip(params, grads) if g.dtype == kind]
-            FusedAdamW._launch(b, [p for p, _ in part], [g for _, g in part],
-                               b.arrays_of([b.index[p] for p, _ in part]), group, grad_scale, found_inf)
-
-    @staticmethod
-    def _launch(b: _Bucket, params, grads, arrays, group, grad_scale, found_inf) -> None:
-        dev, dtype, g_dtype = b.device, b.dtype, grads[0].dtype
-        if g_dtype != dtype and g_dtype != torch.float32:
-            raise TypeError(f"gradients must be {dtype} or float32, got {g_dtype}")
-        for i, (p, g) in enumerate(zip(params, grads)):
-            if p.dtype != dtype or p.device != dev or p.stride() != b.strides[p]:
-                raise RuntimeError("a parameter changed its type, device or strides after its first step")
-            if g.device != dev or g.is_sparse:
-                raise ValueError(f"a gradient must be a dense tensor on {dev}")
-            if g.stride() != p.stride():  # the elements are taken in the parameter's order of memory
-                grads[i] = torch.empty_like(p, dtype=g_dtype).copy_(g)
-        lr = group["lr"]
-        scalars = [lr if isinstance(lr, Tensor) else None, grad_scale, found_inf]
-        for t in scalars:
-            if t is not None and (t.dtype != torch.float32 or t.device != dev):
-                raise ValueError(f"lr, grad_scale and found_inf must be float32 values on {dev}")
-        b1, b2 = group["betas"]
-        args = _lib.MlpkAdamwArgs(0.0 if scalars[0] is not None else lr, b1, b2, group["eps"], group["weight_decay"],
-                                  int(group["maximize"]), *[None if t is None else t.data_ptr() for t in scalars])
-        n = len(params)
-        pointers = ctypes.c_void_p * n
-        with contextlib.nullcontext() if dev.index == torch.cuda.current_device() else torch.cuda.device(dev):
-            _lib.check("mlpk_adamw_step", _lib.lib().mlpk_adamw_step(
-                n, arrays[0], pointers(*[p.data_ptr() for p in params]), pointers(*[g.data_ptr() for g in grads]),
-                arrays[1], arrays[2], DTYPES[dtype], DTYPES[g_dtype], ctypes.byref(b.struct), ctypes.byref(args),
-                _current_stream(dev.index)))
-        torch.autograd.graph.increment_version(params)
 
     def __reduce__(self):
         raise TypeError("FusedAdamW is saved and copied by its state_dict()")
