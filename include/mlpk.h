@@ -276,9 +276,11 @@ int mlpk_rms_norm_bwd(int64_t rows, int width, int dtype, const void* x, const v
  * 8), row_of[i] = the place of slot i when the slots are ordered by expert and
  * then by i, offsets[experts + 1]: the first row of each expert, and at last the
  * number of rows kept.  A slot whose id is outside [0, experts) is dropped: its
- * place is behind the rows kept.  experts is 1 to 1024, slots below 2^31. */
+ * place is behind the rows kept.  experts is 1 to 1024, slots below 2^31.
+ * workspace: mlpk_expert_sort_workspace_size bytes (0 up to 65,536 slots). */
+int64_t mlpk_expert_sort_workspace_size(int64_t slots, int experts);
 int mlpk_expert_sort(int64_t slots, int experts, const void* ids, int id_bytes, int32_t* row_of, int32_t* offsets,
-                     mlpk_stream_t stream);
+                     void* workspace, int64_t workspace_bytes, mlpk_stream_t stream);
 /* Slot t * top + k is token t's k-th choice; kept points to offsets[experts]
  * (device memory).  xs[row_of[t, k]] = x[t]; rows of dropped slots are zero.
  * x: [tokens][width], xs: [tokens * top][width] of dtype. */

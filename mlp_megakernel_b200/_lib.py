@@ -88,7 +88,8 @@ SIGNATURES = {
     "mlpk_rms_norm_fp8": (_i32, [_i64, _i32, _i32, _vp, _vp, _vp, _i32, _f32, _i32, _vp, _vp, _vp, _vp]),
     "mlpk_rms_norm_bwd_workspace_size": (_i64, [_i64, _i32, _i32]),
     "mlpk_rms_norm_bwd": (_i32, [_i64, _i32, _i32, _vp, _vp, _vp, _vp, _i32, _vp, _vp, _vp, _vp, _vp, _i64, _vp]),
-    "mlpk_expert_sort": (_i32, [_i64, _i32, _vp, _i32, _vp, _vp, _vp]),
+    "mlpk_expert_sort_workspace_size": (_i64, [_i64, _i32]),
+    "mlpk_expert_sort": (_i32, [_i64, _i32, _vp, _i32, _vp, _vp, _vp, _i64, _vp]),
     "mlpk_expert_dispatch": (_i32, [_i64, _i32, _i32, _i32, _vp, _vp, _vp, _vp, _vp]),
     "mlpk_expert_combine": (_i32, [_i64, _i32, _i32, _i32, _vp, _vp, _i32, _vp, _vp, _vp, _vp]),
     "mlpk_expert_combine_bwd": (_i32, [_i64, _i32, _i32, _i32, _vp, _vp, _vp, _i32, _vp, _vp, _vp, _vp, _vp]),

@@ -21,28 +21,54 @@ int check_rows(int64_t tokens, int top, int width, int dtype) {
   return MLPK_OK;
 }
 
-// Thread blocks of the sort's cluster: as many as have 4096 slots each, up to
-// 16 (one SM each; above 8 a kernel has to ask).
+// Thread blocks of a sort and slots of a warp: a cluster's blocks up to 16,
+// above that (two launches) at most one an SM.
+struct SortPlan {
+  int blocks;
+  int64_t part;
+  bool cluster() const { return blocks <= 16; }
+};
+SortPlan sort_plan(int64_t slots, int sm_count) {
+  SortPlan p;
+  const int64_t want = ceil_div(slots, kSortBlockSlots);
+  if (want <= 16) {
+    p.blocks = 1;
+    while (p.blocks < want) p.blocks *= 2;
+  } else {
+    p.blocks = static_cast<int>(std::min<int64_t>(want, sm_count));
+  }
+  p.part = std::max<int64_t>(ceil_div(ceil_div(slots, static_cast<int64_t>(p.blocks) * kSortWarps), 32), 1) * 32;
+  return p;
+}
+
 template <class I>
-int sort_slots(int64_t slots, int experts, const void* ids, int* row_of, int* offsets, cudaStream_t st) {
-  int dev = 0;
-  int rc = cuda_status(cudaGetDevice(&dev));
-  if (rc) return rc;
-  int blocks = 1;
-  while (blocks < 16 && slots > blocks * 4096) blocks *= 2;
-  const int64_t part = ceil_div(ceil_div(slots, static_cast<int64_t>(blocks) * kSortWarps), 32) * 32;
-  const bool held = part <= 32 * kSortGroups;
-  const auto kern = held ? expert_sort_kernel<I, true> : expert_sort_kernel<I, false>;
+int sort_slots(int64_t slots, int experts, const void* ids_, int* row_of, int* offsets, int* hist, int dev,
+               const SortPlan& p, cudaStream_t st) {
+  const I* ids = static_cast<const I*>(ids_);
   const size_t smem = sizeof(int) * (kSortWarps + static_cast<size_t>(kSortWarps + 1) * (experts + 1));
+  if (!p.cluster()) {
+    const auto rank = p.part <= 32 * kSortGroups ? expert_rank_kernel<I, true> : expert_rank_kernel<I, false>;
+    if (blocks_per_sm(reinterpret_cast<const void*>(rank), kSortThreads, smem, dev) == 0) return MLPK_ERR_CUDA;
+    const int rc =
+        launch_kernel_early(rank, dim3(p.blocks), kSortThreads, smem, st, ids, slots, experts, p.part, row_of, hist);
+    if (rc) return rc;
+    return launch_kernel_early(expert_place_kernel<I>, dim3(p.blocks), kSortThreads,
+                               sizeof(int) * (2 * kSortThreads + experts + 1), st, ids, slots, experts, p.part, row_of,
+                               offsets, static_cast<const int*>(hist));
+  }
+  const auto kern = expert_sort_kernel<I>;
   if (blocks_per_sm(reinterpret_cast<const void*>(kern), kSortThreads, smem, dev) == 0) return MLPK_ERR_CUDA;
-  static std::once_flag wide[2][64];  // by kernel and device
-  if (blocks > 8 && dev < 64)
-    std::call_once(wide[held][dev], [&] {
-      rc = cuda_status(cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
-    });
-  if (rc) return rc;
+  if (p.blocks > 8) {  // more than a cluster has unasked
+    static std::once_flag asked[64];  // by device
+    int rc = MLPK_OK;
+    if (dev < 64)
+      std::call_once(asked[dev], [&] {
+        rc = cuda_status(cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+      });
+    if (rc) return rc;
+  }
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(blocks);
+  cfg.gridDim = dim3(p.blocks);
   cfg.blockDim = dim3(kSortThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
@@ -50,11 +76,11 @@ int sort_slots(int64_t slots, int experts, const void* ids, int* row_of, int* of
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = blocks;
+  attr[1].val.clusterDim.x = p.blocks;
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  return cuda_status(cudaLaunchKernelEx(&cfg, kern, static_cast<const I*>(ids), slots, experts, part, row_of, offsets));
+  return cuda_status(cudaLaunchKernelEx(&cfg, kern, ids, slots, experts, p.part, row_of, offsets));
 }
 
 // Threads of a token's row of `items` words or vectors, `each` a thread, and the
@@ -65,14 +91,16 @@ struct RowGrid {
 };
 RowGrid row_grid(int64_t tokens, int tokens_each, int64_t items, int each, bool parts) {
   RowGrid g;
-  const int64_t want = std::min<int64_t>(ceil_div(items, each), kRowThreads);
+  // Parts of a row of equal size, each at most what 256 threads take.
+  const int64_t n = parts ? ceil_div(items, static_cast<int64_t>(kRowThreads) * each) : 1;
+  const int64_t want = std::min<int64_t>(ceil_div(ceil_div(items, n), each), kRowThreads);
   g.tpr = 1;
   while (g.tpr < want && g.tpr < 32) g.tpr *= 2;
   if (want > 32) g.tpr = static_cast<int>(ceil_div(want, 32)) * 32;
   const int subs = kRowThreads / g.tpr;
   g.threads = subs * g.tpr;
   g.grid = dim3(static_cast<unsigned>(ceil_div(tokens, static_cast<int64_t>(subs) * tokens_each)),
-                parts ? static_cast<unsigned>(ceil_div(items, static_cast<int64_t>(g.tpr) * each)) : 1);
+                static_cast<unsigned>(n));
   return g;
 }
 
@@ -114,18 +142,33 @@ int with_group(int top, F&& f) {
 
 extern "C" {
 
+int64_t mlpk_expert_sort_workspace_size(int64_t slots, int experts) {
+  if (slots < 0 || slots > 0x7fffffff || experts < 1 || experts > kExpertMax) return -1;
+  if (slots <= 16 * kSortBlockSlots) return 0;
+  DevInfo di;
+  if (current_device_info(&di, nullptr)) return -1;
+  return sort_plan(slots, di.sm_count).blocks * (experts + 1) * static_cast<int64_t>(sizeof(int));
+}
+
 int mlpk_expert_sort(int64_t slots, int experts, const void* ids, int id_bytes, int32_t* row_of, int32_t* offsets,
-                     mlpk_stream_t stream) {
+                     void* workspace, int64_t workspace_bytes, mlpk_stream_t stream) {
   if (slots < 0 || slots > 0x7fffffff || experts < 1) return MLPK_ERR_SHAPE;
   if (experts > kExpertMax || (id_bytes != 4 && id_bytes != 8)) return MLPK_ERR_UNSUPPORTED;
   if (!offsets || (slots > 0 && (!ids || !row_of))) return MLPK_ERR_NULL;
-  if (!aligned16(ids) || !aligned16(row_of) || !aligned16(offsets)) return MLPK_ERR_ALIGN;
+  if (!aligned16(ids) || !aligned16(row_of) || !aligned16(offsets) || !aligned16(workspace)) return MLPK_ERR_ALIGN;
   DevInfo di;
-  int rc = current_device_info(&di, nullptr);
+  int dev;
+  int rc = current_device_info(&di, &dev);
   if (rc) return rc;
+  const SortPlan p = sort_plan(slots, di.sm_count);
+  if (!p.cluster()) {
+    if (!workspace) return MLPK_ERR_NULL;
+    if (workspace_bytes < p.blocks * (experts + 1) * static_cast<int64_t>(sizeof(int))) return MLPK_ERR_SCRATCH;
+  }
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return id_bytes == 8 ? sort_slots<int64_t>(slots, experts, ids, row_of, offsets, st)
-                       : sort_slots<int32_t>(slots, experts, ids, row_of, offsets, st);
+  int* hist = static_cast<int*>(workspace);
+  return id_bytes == 8 ? sort_slots<int64_t>(slots, experts, ids, row_of, offsets, hist, dev, p, st)
+                       : sort_slots<int32_t>(slots, experts, ids, row_of, offsets, hist, dev, p, st);
 }
 
 int mlpk_expert_dispatch(int64_t tokens, int top, int width, int dtype, const void* x, const int32_t* row_of,
@@ -162,7 +205,7 @@ int mlpk_expert_combine(int64_t tokens, int top, int width, int dtype, const voi
     constexpr int V = decltype(vec)::value, NW = V == kVecOf<T> ? 1 : 4;
     return with_group(top, [&](auto group) {
       constexpr int GROUP = decltype(group)::value;
-      const RowGrid g = row_grid(tokens, kRowsAhead / GROUP, width / V, NW, true);
+      const RowGrid g = row_grid(tokens, 1, width / V, NW, true);
       return launch_kernel_early(expert_combine_kernel<T, W, V, NW, GROUP>, g.grid, g.threads, 0,
                                  static_cast<cudaStream_t>(stream), static_cast<const T*>(y),
                                  static_cast<const W*>(weights), tokens, top, width, g.tpr, row_of, kept,
@@ -188,7 +231,7 @@ int mlpk_expert_combine_bwd(int64_t tokens, int top, int width, int dtype, const
     constexpr int V = decltype(vec)::value;
     return with_group(top, [&](auto group) {
       constexpr int GROUP = decltype(group)::value;
-      const RowGrid g = row_grid(tokens, 4 / GROUP, width / V, V == kVecOf<T> ? 1 : 2, false);
+      const RowGrid g = row_grid(tokens, 1, width / V, V == kVecOf<T> ? 2 : 8, false);
       return launch_kernel_early(expert_combine_bwd_kernel<T, W, V, GROUP>, g.grid, g.threads, 0,
                                  static_cast<cudaStream_t>(stream), static_cast<const T*>(grad_out),
                                  static_cast<const T*>(y), static_cast<const W*>(weights), tokens, top, width, g.tpr,

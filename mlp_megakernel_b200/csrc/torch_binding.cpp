@@ -213,9 +213,12 @@ py::object expert_sort(const Tensor& ids_in, int64_t experts) {
     const Tensor ids = aligned(ids_in);
     row_of = at::empty(ids.sizes(), ids.options().dtype(at::kInt));
     offsets = at::empty({experts + 1}, ids.options().dtype(at::kInt));
+    const int64_t bytes = mlpk_expert_sort_workspace_size(ids.numel(), static_cast<int>(experts));
+    const Tensor work = bytes > 0 ? at::empty({bytes}, ids.options().dtype(at::kByte)) : Tensor();
     check("mlpk_expert_sort",
           mlpk_expert_sort(ids.numel(), static_cast<int>(experts), ptr(ids), wide ? 8 : 4,
-                           static_cast<int32_t*>(ptr(row_of)), static_cast<int32_t*>(ptr(offsets)), stream_of(ids)));
+                           static_cast<int32_t*>(ptr(row_of)), static_cast<int32_t*>(ptr(offsets)), ptr(work), bytes,
+                           stream_of(ids)));
   }
   return py::make_tuple(row_of, offsets);
 }

@@ -125,11 +125,11 @@ def test_c_calls_refuse_before_they_touch_the_device(built_lib):
     assert lib.mlpk_rms_norm_fp8(4, 8, 0, a, None, None, 0, 1e-6, 0, a, None, None, None) == nu
     assert lib.mlpk_rms_norm_bwd(4, 8, 0, a, None, a, None, 0, a, None, a, a, a, 1 << 20, None) == nu  # no weight for dw
     assert lib.mlpk_rms_norm_bwd(4, 8, 0, a, None, a, a, 0, a, None, a, a, None, 0, None) == nu
-    assert lib.mlpk_expert_sort(-1, 4, a, 8, a, a, None) == sh
-    assert lib.mlpk_expert_sort(8, 2000, a, 8, a, a, None) == un
-    assert lib.mlpk_expert_sort(8, 4, a, 2, a, a, None) == un
-    assert lib.mlpk_expert_sort(8, 4, a, 8, None, a, None) == nu
-    assert lib.mlpk_expert_sort(8, 4, a, 8, a + 4, a, None) == al
+    assert lib.mlpk_expert_sort(-1, 4, a, 8, a, a, None, 0, None) == sh
+    assert lib.mlpk_expert_sort(8, 2000, a, 8, a, a, None, 0, None) == un
+    assert lib.mlpk_expert_sort(8, 4, a, 2, a, a, None, 0, None) == un
+    assert lib.mlpk_expert_sort(8, 4, a, 8, None, a, None, 0, None) == nu
+    assert lib.mlpk_expert_sort(8, 4, a, 8, a + 4, a, None, 0, None) == al
     assert lib.mlpk_expert_dispatch(2 ** 30, 2, 8, 0, a, a, a, a, None) == sh
     assert lib.mlpk_expert_dispatch(4, 2, 8, 7, a, a, a, a, None) == un
     assert lib.mlpk_expert_dispatch(4, 2, 8, 0, a, a, None, a, None) == nu
