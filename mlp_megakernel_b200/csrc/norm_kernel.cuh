@@ -66,16 +66,17 @@ __device__ __forceinline__ float norm_row_sum(float v, int tpr, float* red, int 
   return v;
 }
 
-__device__ __forceinline__ uint32_t norm_row_max(uint32_t v, int tpr, float* red, int half) {
-  for (int o = (tpr < 32 ? tpr : 32) / 2; o > 0; o >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, o));
+// The largest v (not below 0) of the row's threads; a NaN stays.
+__device__ __forceinline__ float norm_row_max(float v, int tpr, float* red, int half) {
+  for (int o = (tpr < 32 ? tpr : 32) / 2; o > 0; o >>= 1) v = max_nan(v, __shfl_xor_sync(0xffffffffu, v, o));
   if (tpr <= 32) return v;
-  uint32_t* r = reinterpret_cast<uint32_t*>(red) + half * 32;
-  if (threadIdx.x % 32 == 0) r[threadIdx.x / 32] = v;
+  red += half * 32;
+  if (threadIdx.x % 32 == 0) red[threadIdx.x / 32] = v;
   __syncthreads();
-  v = 0;
+  v = 0.0f;
   for (int k = 0; k < tpr / 32; k += 4) {
-    const uint4 t = *reinterpret_cast<const uint4*>(r + k);
-    v = max(v, max(max(t.x, t.y), max(t.z, t.w)));
+    const float4 t = *reinterpret_cast<const float4*>(red + k);
+    v = max_abs(max_abs(v, t.x, t.y), t.z, t.w);
   }
   return v;
 }
@@ -117,14 +118,25 @@ struct RowSpan {
     }
     return load_raw<T, VEC>(p + at(begin, i));
   }
-  __device__ void store(T* p, int64_t begin, int i, const float (&f)[VEC]) const {
+  __device__ void store(T* p, int64_t begin, int i, const float2 (&f)[VEC / 2]) const {
     if (whole(i)) {
-      store_vec<T, VEC>(p + at(begin, i), f);
+      store_vec2<T, VEC>(p + at(begin, i), f);
       return;
     }
 #pragma unroll
-    for (int e = 0; e < VEC; ++e)
-      if (owns(i, e)) p[at(begin, i) + e] = from_float<T>(f[e]);
+    for (int e = 0; e < VEC / 2; ++e) {
+      if (owns(i, 2 * e)) p[at(begin, i) + 2 * e] = from_float<T>(f[e].x);
+      if (owns(i, 2 * e + 1)) p[at(begin, i) + 2 * e + 1] = from_float<T>(f[e].y);
+    }
+  }
+  // Zeros in the place of what is not this row's.
+  __device__ void mask(int i, float2 (&f)[VEC / 2]) const {
+    if (whole(i)) return;
+#pragma unroll
+    for (int e = 0; e < VEC / 2; ++e) {
+      if (!owns(i, 2 * e)) f[e].x = 0.0f;
+      if (!owns(i, 2 * e + 1)) f[e].y = 0.0f;
+    }
   }
   // The weight's values of the vector's columns; ones without a weight.
   template <class W>
@@ -144,22 +156,22 @@ template <class T, class W, int NV, bool FLOATS>
 struct NormWeights {
   static constexpr int VEC = kVecOf<T>;
   Raw<W, VEC> raw[FLOATS ? 1 : NV];
-  float f32[FLOATS ? NV : 1][VEC];
+  float2 f32[FLOATS ? NV : 1][VEC / 2];
   template <class Span>
   __device__ void load(const Span& span, const W* w) {
 #pragma unroll
     for (int i = 0; i < NV; ++i)
       if (span.has(i)) {
         span.weights(w, i, raw[FLOATS ? 0 : i]);
-        if constexpr (FLOATS) unpack(raw[0], f32[i]);
+        if constexpr (FLOATS) unpack2(raw[0], f32[i]);
       }
   }
-  __device__ void get(int i, float (&f)[VEC]) const {
+  __device__ void get(int i, float2 (&f)[VEC / 2]) const {
     if constexpr (FLOATS) {
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) f[e] = f32[i][e];
+      for (int e = 0; e < VEC / 2; ++e) f[e] = f32[i][e];
     } else {
-      unpack(raw[i], f);
+      unpack2(raw[i], f);
     }
   }
 };
@@ -184,7 +196,7 @@ struct NormArgs {
 template <class T, class W, int NV, bool RAGGED, bool PIPE, int MAXT, bool FP8>
 __global__ void __launch_bounds__(MAXT) rms_norm_fwd_kernel(const NormArgs a, int stages, int slots_at) {
   using Span = RowSpan<T, NV, RAGGED>;
-  constexpr int VEC = Span::VEC;
+  constexpr int VEC = Span::VEC, HALF = VEC / 2;
   extern __shared__ __align__(16) uint8_t smem_raw[];
   float* red = reinterpret_cast<float*>(smem_raw);
   pdl_enter();
@@ -225,100 +237,93 @@ __global__ void __launch_bounds__(MAXT) rms_norm_fwd_kernel(const NormArgs a, in
   for (int64_t row0 = first - sub; row0 < a.rows; row0 += step, row += step, begin += begin_step, half ^= 1) {
     const bool live = row < a.rows;
     if constexpr (PIPE) cp_async_wait_upto(stages - 1);
-    float h[NV][VEC];
-    float sum = 0.0f;
+    float2 h[NV][HALF];
+    float2 sum2 = make_float2(0.0f, 0.0f);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) h[i][e] = 0.0f;
+      for (int e = 0; e < HALF; ++e) h[i][e] = make_float2(0.0f, 0.0f);
       if (live && span.has(i)) {
-        unpack(PIPE ? *slot(stage, 0, i) : span.load(x, begin, i), h[i]);
+        unpack2(PIPE ? *slot(stage, 0, i) : span.load(x, begin, i), h[i]);
         if (r) {
-          float f[VEC];
-          unpack(PIPE ? *slot(stage, 1, i) : span.load(r, begin, i), f);
+          float2 f[HALF];
+          unpack2(PIPE ? *slot(stage, 1, i) : span.load(r, begin, i), f);
 #pragma unroll
-          for (int e = 0; e < VEC; ++e) h[i][e] += f[e];
+          for (int e = 0; e < HALF; ++e) h[i][e] = __fadd2_rn(h[i][e], f[e]);
         }
-        if (!span.whole(i)) {
-#pragma unroll
-          for (int e = 0; e < VEC; ++e)
-            if (!span.owns(i, e)) h[i][e] = 0.0f;
-        }
+        span.mask(i, h[i]);
       }
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) sum += h[i][e] * h[i][e];
+      for (int e = 0; e < HALF; ++e) sum2 = __ffma2_rn(h[i][e], h[i][e], sum2);
     }
     if constexpr (PIPE) {
       fetch(begin + stages * begin_step, stage);
       stage = stage + stage_slots == stages * stage_slots ? 0 : stage + stage_slots;
     }
-    const float s = rsqrtf(norm_row_sum(sum, a.tpr, red, half) * inv_width + a.eps);
+    const float s = rsqrtf(norm_row_sum(sum2.x + sum2.y, a.tpr, red, half) * inv_width + a.eps);
     if (a.rstd && live && lane == 0) a.rstd[row] = s;
-    uint32_t amax = 0;
+    float amax = 0.0f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       if (live && span.has(i)) {
         if (a.h) span.store(static_cast<T*>(a.h), begin, i, h[i]);
-        float f[VEC];
+        float2 f[HALF];
         w.get(i, f);
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-          h[i][e] = h[i][e] * s * f[e];
-          if (FP8) amax = max(amax, abs_bits(h[i][e]));
+        for (int e = 0; e < HALF; ++e) {
+          h[i][e] = __fmul2_rn(__fmul2_rn(h[i][e], make_float2(s, s)), f[e]);
+          if (FP8 && a.group == 0) amax = max_abs(amax, h[i][e].x, h[i][e].y);
         }
         if constexpr (!FP8) span.store(static_cast<T*>(a.y), begin, i, h[i]);
       }
     }
     if constexpr (FP8) {
-      auto store = [&](int i) {
+      // Vector i times what its elements' groups ask for; elements from `edge`
+      // on are of the next group.
+      auto store = [&](int i, float inv0, float inv1, int edge) {
         uint8_t* q = static_cast<uint8_t*>(a.y) + span.at(begin, i);
+        Raw<uint16_t, HALF> q8;
+#pragma unroll
+        for (int e = 0; e < HALF; ++e)
+          q8.v[e] = to_fp8x2(__fmul2_rn(h[i][e], make_float2(2 * e < edge ? inv0 : inv1, 2 * e + 1 < edge ? inv0 : inv1)));
         if (span.whole(i)) {
-          store_fp8<VEC>(q, h[i]);
+          *reinterpret_cast<Raw<uint16_t, HALF>*>(q) = q8;
           return;
         }
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-          const float f[1] = {h[i][e]};
-          if (span.owns(i, e)) store_fp8<1>(q + e, f);
-        }
+        for (int e = 0; e < VEC; ++e)
+          if (span.owns(i, e)) q[e] = static_cast<uint8_t>(q8.v[e / 2] >> (e % 2 * 8));
       };
       const int groups = (a.width + kNormGroup - 1) / kNormGroup;
       if (a.group == 0) {
         float inv;
-        const float scale = fp8_scale(norm_row_max(amax, a.tpr, red + 64, half), &inv);
+        const float scale = fp8_scale_fast(norm_row_max(amax, a.tpr, red + 64, half), &inv);
         if (live && lane == 0) a.scale[row] = scale;
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-          if (live && span.has(i)) {
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) h[i][e] *= inv;
-            store(i);
-          }
-        }
+        for (int i = 0; i < NV; ++i)
+          if (live && span.has(i)) store(i, inv, inv, VEC);
       } else if constexpr (!RAGGED) {
         // The 128 / VEC lanes of a group are neighbours: a power of two, and a
         // divisor of tpr unless the row is narrower than a group.
         const int gl = min(kNormGroup / VEC, a.tpr);
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-          uint32_t m = 0;
+          float m = 0.0f;
 #pragma unroll
-          for (int e = 0; e < VEC; ++e) m = max(m, abs_bits(h[i][e]));
-          for (int o = gl / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+          for (int e = 0; e < HALF; ++e) m = max_abs(m, h[i][e].x, h[i][e].y);
+          for (int o = gl / 2; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
           float inv;
-          const float scale = fp8_scale(m, &inv);
+          const float scale = fp8_scale_fast(m, &inv);
           if (live && span.has(i)) {
             const int v = i * a.tpr + lane;
             if (v % gl == 0) a.scale[row * groups + v / gl] = scale;
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) h[i][e] *= inv;
-            store(i);
+            store(i, inv, inv, VEC);
           }
         }
       } else {
         // A vector may reach into two groups, and groups do not begin at a
         // lane: the maxima meet in shared memory (they do not depend on the
-        // order).
+        // order; their bits are ordered as they are).
         uint32_t* gmax = reinterpret_cast<uint32_t*>(smem_raw + 512) + sub * groups;
         __syncthreads();
         for (int k = lane; k < groups; k += a.tpr) gmax[k] = 0;
@@ -327,34 +332,32 @@ __global__ void __launch_bounds__(MAXT) rms_norm_fwd_kernel(const NormArgs a, in
         for (int i = 0; i < NV; ++i) {
           if (live && span.has(i)) {
             const int lo = max(span.col(i), 0) / kNormGroup, hi = (min(span.col(i) + VEC, a.width) - 1) / kNormGroup;
-            const int edge = (lo + 1) * kNormGroup - span.col(i);  // elements from here on are of the next group
-            uint32_t m0 = 0, m1 = 0;  // what is not the row's is zero
+            const int edge = (lo + 1) * kNormGroup - span.col(i);
+            float m0 = 0.0f, m1 = 0.0f;  // what is not the row's is zero
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) {
-              if (e < edge) m0 = max(m0, abs_bits(h[i][e]));
-              else m1 = max(m1, abs_bits(h[i][e]));
+            for (int e = 0; e < HALF; ++e) {
+              const float2 v = h[i][e];
+              m0 = max_abs(m0, 2 * e < edge ? v.x : 0.0f, 2 * e + 1 < edge ? v.y : 0.0f);
+              m1 = max_abs(m1, 2 * e < edge ? 0.0f : v.x, 2 * e + 1 < edge ? 0.0f : v.y);
             }
-            atomicMax(gmax + lo, m0);
-            if (hi != lo) atomicMax(gmax + hi, m1);
+            atomicMax(gmax + lo, abs_bits(m0));
+            if (hi != lo) atomicMax(gmax + hi, abs_bits(m1));
           }
         }
         __syncthreads();
         if (live)
           for (int k = lane; k < groups; k += a.tpr) {
             float inv;
-            a.scale[row * groups + k] = fp8_scale(gmax[k], &inv);
+            a.scale[row * groups + k] = fp8_scale_fast(__uint_as_float(gmax[k]), &inv);
           }
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
           if (live && span.has(i)) {
             const int lo = max(span.col(i), 0) / kNormGroup, hi = (min(span.col(i) + VEC, a.width) - 1) / kNormGroup;
-            const int edge = (lo + 1) * kNormGroup - span.col(i);
             float inv0, inv1;
-            fp8_scale(gmax[lo], &inv0);
-            fp8_scale(gmax[hi], &inv1);
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) h[i][e] *= e < edge ? inv0 : inv1;
-            store(i);
+            fp8_scale_fast(__uint_as_float(gmax[lo]), &inv0);
+            fp8_scale_fast(__uint_as_float(gmax[hi]), &inv1);
+            store(i, inv0, inv1, (lo + 1) * kNormGroup - span.col(i));
           }
         }
       }
@@ -387,7 +390,7 @@ struct NormBwdArgs {
 template <class T, class W, int NV, bool RAGGED, bool PIPE, int MAXT>
 __global__ void __launch_bounds__(MAXT, MAXT == 256 ? 2 : 1) rms_norm_bwd_kernel(const NormBwdArgs a, int stages) {
   using Span = RowSpan<T, NV, RAGGED>;
-  constexpr int VEC = Span::VEC;
+  constexpr int VEC = Span::VEC, HALF = VEC / 2;
   constexpr bool KEEP = NV <= 2;
   extern __shared__ __align__(16) uint8_t smem_raw[];
   float* red = reinterpret_cast<float*>(smem_raw);
@@ -421,11 +424,11 @@ __global__ void __launch_bounds__(MAXT, MAXT == 256 ? 2 : 1) rms_norm_bwd_kernel
   int64_t begin = first * a.width;
   if constexpr (PIPE)
     for (int k = 0; k < stages; ++k) fetch(begin + k * begin_step, k * stage_slots);
-  float dw[NV][VEC];
+  float2 dw[NV][HALF];
 #pragma unroll
   for (int i = 0; i < NV; ++i)
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) dw[i][e] = 0.0f;
+    for (int e = 0; e < HALF; ++e) dw[i][e] = make_float2(0.0f, 0.0f);
   NormWeights<T, W, NV, KEEP> w;
   w.load(span, static_cast<const W*>(a.w));
   norm_row_init(red, 64, a.tpr);
@@ -440,52 +443,50 @@ __global__ void __launch_bounds__(MAXT, MAXT == 256 ? 2 : 1) rms_norm_bwd_kernel
     s_next = row + step < a.rows ? a.rstd[row + step] : 0.0f;
     if constexpr (PIPE) cp_async_wait_upto(stages - 1);
     // n and G w of vector i, and G
-    auto terms = [&](int i, float (&n)[VEC], float (&gw)[VEC], float (&g)[VEC]) {
-      unpack(PIPE ? *slot(stage, 0, i) : span.load(in[0], begin, i), n);
-      unpack(PIPE ? *slot(stage, 1, i) : span.load(in[1], begin, i), g);
+    auto terms = [&](int i, float2 (&n)[HALF], float2 (&gw)[HALF], float2 (&g)[HALF]) {
+      unpack2(PIPE ? *slot(stage, 0, i) : span.load(in[0], begin, i), n);
+      unpack2(PIPE ? *slot(stage, 1, i) : span.load(in[1], begin, i), g);
       if (in[2]) {
-        float f[VEC];
-        unpack(PIPE ? *slot(stage, 2, i) : span.load(in[2], begin, i), f);
+        float2 f[HALF];
+        unpack2(PIPE ? *slot(stage, 2, i) : span.load(in[2], begin, i), f);
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) n[e] += f[e];
+        for (int e = 0; e < HALF; ++e) n[e] = __fadd2_rn(n[e], f[e]);
       }
-      if (!span.whole(i)) {
-#pragma unroll
-        for (int e = 0; e < VEC; ++e)
-          if (!span.owns(i, e)) n[e] = g[e] = 0.0f;
-      }
-      float f[VEC];
+      span.mask(i, n);
+      span.mask(i, g);
+      float2 f[HALF];
       w.get(i, f);
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        n[e] *= s;
-        gw[e] = g[e] * f[e];
+      for (int e = 0; e < HALF; ++e) {
+        n[e] = __fmul2_rn(n[e], make_float2(s, s));
+        gw[e] = __fmul2_rn(g[e], f[e]);
       }
     };
-    float n[KEEP ? NV : 1][VEC], gw[KEEP ? NV : 1][VEC], g[VEC];
-    float sum = 0.0f;
+    float2 n[KEEP ? NV : 1][HALF], gw[KEEP ? NV : 1][HALF], g[HALF];
+    float2 sum2 = make_float2(0.0f, 0.0f);
 #pragma unroll
     for (int i = 0; i < NV; ++i)
       if (live && span.has(i)) {
         const int k = KEEP ? i : 0;
         terms(i, n[k], gw[k], g);
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-          dw[i][e] += g[e] * n[k][e];
-          sum += gw[k][e] * n[k][e];
+        for (int e = 0; e < HALF; ++e) {
+          dw[i][e] = __ffma2_rn(g[e], n[k][e], dw[i][e]);
+          sum2 = __ffma2_rn(gw[k][e], n[k][e], sum2);
         }
       }
-    const float c = norm_row_sum(sum, a.tpr, red, half) * inv_width;
+    const float c = -norm_row_sum(sum2.x + sum2.y, a.tpr, red, half) * inv_width;
 #pragma unroll
     for (int i = 0; i < NV; ++i)
       if (live && span.has(i)) {
         const int k = KEEP ? i : 0;
         if constexpr (!KEEP) terms(i, n[k], gw[k], g);
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) g[e] = 0.0f;
-        if (in[3]) unpack(PIPE ? *slot(stage, gh_slot, i) : span.load(in[3], begin, i), g);
+        for (int e = 0; e < HALF; ++e) g[e] = make_float2(0.0f, 0.0f);
+        if (in[3]) unpack2(PIPE ? *slot(stage, gh_slot, i) : span.load(in[3], begin, i), g);
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) g[e] += s * (gw[k][e] - n[k][e] * c);
+        for (int e = 0; e < HALF; ++e)
+          g[e] = __ffma2_rn(__ffma2_rn(n[k][e], make_float2(c, c), gw[k][e]), make_float2(s, s), g[e]);
         span.store(static_cast<T*>(a.dx), begin, i, g);
       }
     if constexpr (PIPE) {
@@ -500,11 +501,13 @@ __global__ void __launch_bounds__(MAXT, MAXT == 256 ? 2 : 1) rms_norm_bwd_kernel
     for (int i = 0; i < NV; ++i)
       if (span.has(i)) {
         if (!RAGGED) {
-          store_vec<float, VEC>(out + span.col(i), dw[i]);
+          store_vec2<float, VEC>(out + span.col(i), dw[i]);
         } else {
 #pragma unroll
-          for (int e = 0; e < VEC; ++e)
-            if (span.owns(i, e)) out[span.col(i) + e] = dw[i][e];
+          for (int e = 0; e < HALF; ++e) {
+            if (span.owns(i, 2 * e)) out[span.col(i) + 2 * e] = dw[i][e].x;
+            if (span.owns(i, 2 * e + 1)) out[span.col(i) + 2 * e + 1] = dw[i][e].y;
+          }
         }
       }
     return;
@@ -516,8 +519,10 @@ __global__ void __launch_bounds__(MAXT, MAXT == 256 ? 2 : 1) rms_norm_bwd_kernel
   for (int i = 0; i < NV; ++i)
     if (span.has(i)) {
 #pragma unroll
-      for (int e = 0; e < VEC; ++e)
-        if (span.owns(i, e)) acc[sub * a.width + span.col(i) + e] = dw[i][e];
+      for (int e = 0; e < HALF; ++e) {
+        if (span.owns(i, 2 * e)) acc[sub * a.width + span.col(i) + 2 * e] = dw[i][e].x;
+        if (span.owns(i, 2 * e + 1)) acc[sub * a.width + span.col(i) + 2 * e + 1] = dw[i][e].y;
+      }
     }
   __syncthreads();
   for (int j = threadIdx.x; j < a.width; j += blockDim.x) {

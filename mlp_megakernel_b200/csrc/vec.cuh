@@ -225,4 +225,12 @@ __device__ __forceinline__ float fp8_scale(uint32_t amax_bits, float* inv) {
   return scale;
 }
 
+// The same with a reciprocal to within a unit of its last place.
+__device__ __forceinline__ float fp8_scale_fast(float amax, float* inv) {
+  float scale = amax * (1.0f / kFp8Max);
+  if (scale < 1.17549435e-38f) scale = 0.0f;
+  *inv = scale > 0.0f ? fast_reciprocal(scale) : 0.0f;
+  return scale;
+}
+
 }  // namespace mlpk
