@@ -194,7 +194,8 @@ struct NormArgs {
 // Shared memory: 128 floats for the row sums, then with FP8, RAGGED and groups
 // a maximum per group and row group, then the slots [stage][x, r][i][thread].
 template <class T, class W, int NV, bool RAGGED, bool PIPE, int MAXT, bool FP8>
-__global__ void __launch_bounds__(MAXT) rms_norm_fwd_kernel(const NormArgs a, int stages, int slots_at) {
+__global__ void __launch_bounds__(MAXT, !FP8 ? 0 : MAXT == 256 ? 3 : MAXT == 512 && NV == 2 ? 2 : 1)
+    rms_norm_fwd_kernel(const NormArgs a, int stages, int slots_at) {
   using Span = RowSpan<T, NV, RAGGED>;
   constexpr int VEC = Span::VEC, HALF = VEC / 2;
   extern __shared__ __align__(16) uint8_t smem_raw[];
@@ -225,7 +226,7 @@ __global__ void __launch_bounds__(MAXT) rms_norm_fwd_kernel(const NormArgs a, in
   int64_t begin = first * a.width;
   if constexpr (PIPE)
     for (int k = 0; k < stages; ++k) fetch(begin + k * begin_step, k * stage_slots);
-  NormWeights<T, W, NV, (NV <= 2)> w;
+  NormWeights<T, W, NV, (NV <= 2 && !FP8)> w;
   w.load(span, static_cast<const W*>(a.w));
   norm_row_init(red, 128, a.tpr);
 

@@ -15,15 +15,14 @@ inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // Threads a row (tpr) and vectors a thread (nv).  A row of up to 128 vectors
 // belongs to a warp or a part of one: no barrier.  Wider ones take 2 vectors a
-// thread while that is at most 512 threads (256 in the backward, whose
-// registers hold more), then 4, and 9 where 4 do not reach
+// thread while that is at most 512 threads, then 4, and 9 where 4 do not reach
 // (fp32 rows above 16,384 and the widest ragged ones: 32,767 fp32 values lie in
 // up to 8,193 vectors).
 struct RowPlan {
   int tpr, nv, rows_per_block, threads;
   bool ragged;
 };
-inline RowPlan row_plan(int width, int vec, bool bwd) {
+inline RowPlan row_plan(int width, int vec) {
   RowPlan p;
   p.ragged = width % vec != 0;
   const int nvec = static_cast<int>(ceil_div(width + (p.ragged ? vec - 1 : 0), vec));  // wherever a row begins
@@ -35,7 +34,7 @@ inline RowPlan row_plan(int width, int vec, bool bwd) {
     p.tpr = 32;
     p.nv = nvec <= 64 ? 2 : 4;
   } else {
-    p.nv = nvec <= (bwd ? 512 : 1024) ? 2 : nvec <= 4096 ? 4 : 9;
+    p.nv = nvec <= 1024 ? 2 : nvec <= 4096 ? 4 : 9;
     p.tpr = static_cast<int>(ceil_div(ceil_div(nvec, p.nv), 32)) * 32;
   }
   p.rows_per_block = p.tpr <= 32 ? kNormThreads / p.tpr : 1;
@@ -61,12 +60,16 @@ inline int64_t loop_blocks(int64_t rows, const RowPlan& p, int vec, int64_t resi
   return p.ragged ? std::max<int64_t>(resident / vec, 1) * vec : resident;
 }
 
+// Blocks of the backward pass that an SM holds: 512 threads in all (their
+// registers allow no more).
+inline int bwd_per_sm(const RowPlan& p) { return std::max(1, 512 / p.threads); }
+
 // Blocks of the backward pass, each of which leaves one row of dw's partial
 // sums.  (The same for every count of inputs, so that the workspace's size
 // follows from rows, width and type.)
 inline int64_t bwd_blocks(int64_t rows, int width, int dtype, int sm_count) {
-  const RowPlan p = row_plan(width, vec_of(dtype), true);
-  return loop_blocks(rows, p, vec_of(dtype), static_cast<int64_t>(sm_count) * (p.threads <= 256 ? 2 : 1));
+  const RowPlan p = row_plan(width, vec_of(dtype));
+  return loop_blocks(rows, p, vec_of(dtype), static_cast<int64_t>(sm_count) * bwd_per_sm(p));
 }
 
 // f(NV, RAGGED, PIPE, MAXT) of this call.
@@ -75,14 +78,13 @@ using Bool = std::integral_constant<bool, V>;
 template <int V>
 using Int = std::integral_constant<int, V>;
 
-template <class T, bool BWD, bool RAGGED, class F>
+template <class T, bool RAGGED, class F>
 int with_counts(const RowPlan& p, bool pipe, F&& f) {
   switch (p.nv) {
     case 1: return f(Int<1>{}, Bool<RAGGED>{}, Bool<true>{}, Int<256>{});
     case 2:
       if (p.threads <= 256) return f(Int<2>{}, Bool<RAGGED>{}, Bool<true>{}, Int<256>{});
-      if constexpr (!BWD) return f(Int<2>{}, Bool<RAGGED>{}, Bool<true>{}, Int<512>{});
-      return MLPK_ERR_UNSUPPORTED;
+      return f(Int<2>{}, Bool<RAGGED>{}, Bool<true>{}, Int<512>{});
     case 4:
       if (p.threads <= 512) return f(Int<4>{}, Bool<RAGGED>{}, Bool<true>{}, Int<512>{});
       return pipe ? f(Int<4>{}, Bool<RAGGED>{}, Bool<true>{}, Int<1024>{})
@@ -92,9 +94,9 @@ int with_counts(const RowPlan& p, bool pipe, F&& f) {
       return MLPK_ERR_UNSUPPORTED;
   }
 }
-template <class T, bool BWD, class F>
+template <class T, class F>
 int with_raggedness(const RowPlan& p, bool pipe, F&& f) {
-  return p.ragged ? with_counts<T, BWD, true>(p, pipe, f) : with_counts<T, BWD, false>(p, pipe, f);
+  return p.ragged ? with_counts<T, true>(p, pipe, f) : with_counts<T, false>(p, pipe, f);
 }
 
 template <class T, class W, bool FP8>
@@ -103,15 +105,15 @@ int forward(NormArgs a, cudaStream_t st) {
   int dev;
   int rc = host::current_device_info(&di, &dev);
   if (rc) return rc;
-  const RowPlan p = row_plan(a.width, kVecOf<T>, false);
+  const RowPlan p = row_plan(a.width, kVecOf<T>);
   const int streams = a.r ? 2 : 1;
-  const int stages = stages_of(p, streams, 72 * 1024);
+  const int stages = stages_of(p, streams, 52 * 1024);
   a.tpr = p.tpr;
   size_t slots_at = 128 * sizeof(float);
   if (FP8 && p.ragged && a.group)
     slots_at += ceil_div(sizeof(float) * p.rows_per_block * ceil_div(a.width, kNormGroup), 16) * 16;
   const size_t smem = slots_at + static_cast<size_t>(stages) * p.nv * p.threads * streams * 16;
-  return with_raggedness<T, false>(p, stages > 0, [&](auto nv, auto ragged, auto pipe, auto maxt) {
+  return with_raggedness<T>(p, stages > 0, [&](auto nv, auto ragged, auto pipe, auto maxt) {
     const auto kern = rms_norm_fwd_kernel<T, W, decltype(nv)::value, decltype(ragged)::value, decltype(pipe)::value,
                                           decltype(maxt)::value, FP8>;
     const int per_sm = host::blocks_per_sm(reinterpret_cast<const void*>(kern), p.threads, smem, dev);
@@ -125,14 +127,14 @@ int forward(NormArgs a, cudaStream_t st) {
 // `blocks` rows of partial sums in a.part (unless it is null), then dw.
 template <class T, class W>
 int backward(NormBwdArgs a, int64_t blocks, W* dw, int dev, cudaStream_t st) {
-  const RowPlan p = row_plan(a.width, kVecOf<T>, true);
+  const RowPlan p = row_plan(a.width, kVecOf<T>);
   const int streams = 2 + (a.r != nullptr) + (a.gh != nullptr);
-  const int stages = stages_of(p, streams, 100 * 1024);
+  const int stages = stages_of(p, streams, 200 * 1024 / bwd_per_sm(p));
   a.tpr = p.tpr;
   size_t smem = static_cast<size_t>(stages) * p.nv * p.threads * streams * 16;
   if (p.rows_per_block > 1) smem = std::max(smem, sizeof(float) * p.rows_per_block * static_cast<size_t>(a.width));
   smem += 64 * sizeof(float);
-  const int rc = with_raggedness<T, true>(p, stages > 0, [&](auto nv, auto ragged, auto pipe, auto maxt) {
+  const int rc = with_raggedness<T>(p, stages > 0, [&](auto nv, auto ragged, auto pipe, auto maxt) {
     const auto kern = rms_norm_bwd_kernel<T, W, decltype(nv)::value, decltype(ragged)::value, decltype(pipe)::value,
                                           decltype(maxt)::value>;
     if (host::blocks_per_sm(reinterpret_cast<const void*>(kern), p.threads, smem, dev) == 0)
