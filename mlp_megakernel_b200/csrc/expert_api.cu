@@ -1,7 +1,7 @@
 // C-ABI entry points of the rows sorted by expert and back (declared in
 // include/mlpk.h).
 #include <algorithm>
-#include <mutex>
+#include <atomic>
 #include <type_traits>
 
 #include "expert_kernel.cuh"
@@ -59,13 +59,12 @@ int sort_slots(int64_t slots, int experts, const void* ids_, int* row_of, int* o
   const auto kern = expert_sort_kernel<I>;
   if (blocks_per_sm(reinterpret_cast<const void*>(kern), kSortThreads, smem, dev) == 0) return MLPK_ERR_CUDA;
   if (p.blocks > 8) {  // more than a cluster has unasked
-    static std::once_flag asked[64];  // by device
-    int rc = MLPK_OK;
-    if (dev < 64)
-      std::call_once(asked[dev], [&] {
-        rc = cuda_status(cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
-      });
-    if (rc) return rc;
+    static std::atomic<bool> asked[64];  // by device; asking twice does no harm
+    if (dev >= 64 || !asked[dev].load(std::memory_order_relaxed)) {
+      const int rc = cuda_status(cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+      if (rc) return rc;
+      if (dev < 64) asked[dev].store(true, std::memory_order_relaxed);
+    }
   }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(p.blocks);

@@ -417,7 +417,8 @@ __global__ void __launch_bounds__(kRowThreads, VEC < kVecOf<T> ? 4 : GROUP == 2 
   const int rows_kept = *kept;
   int half = 0;
   for (int k0 = 0; k0 < top; k0 += GROUP, half ^= 1) {
-    int row[GROUP];  // below 0: no such slot
+    int row[GROUP];  // rows_kept and above: not kept; below 0: no such slot
+    int64_t row_at[U > 1 ? GROUP : 1];  // found once where it is used often
     float wk[GROUP], dot[GROUP];
 #pragma unroll
     for (int k = 0; k < GROUP; ++k) {
@@ -425,16 +426,22 @@ __global__ void __launch_bounds__(kRowThreads, VEC < kVecOf<T> ? 4 : GROUP == 2 
       row[k] = slot ? row_of[t * top + k0 + k] : -1;
       wk[k] = slot && w ? to_float(w[t * top + k0 + k]) : 1.0f;
       dot[k] = 0.0f;
+      if constexpr (U > 1) row_at[k] = static_cast<int64_t>(row[k]) * width;
     }
+    auto on = [&](int k) { return row[k] >= 0 && row[k] < rows_kept; };  // else y is not read and the gradients are zero
+    auto at = [&](int k) -> int64_t {
+      if constexpr (U > 1) return row_at[k];
+      return static_cast<int64_t>(row[k]) * width;
+    };
     for (int v = live ? span.lane : nvec; v < nvec; v += tpr * U) {
       Raw<T, VEC> gr[U], yr[GROUP][U];
 #pragma unroll
       for (int i = 0; i < U; ++i) {
-        if (v + i * tpr < nvec) gr[i] = load_raw<T, VEC>(gout + t * width + (v + i * tpr) * VEC);
+        if (v + i * tpr >= nvec) break;
+        gr[i] = load_raw<T, VEC>(gout + t * width + (v + i * tpr) * VEC);
 #pragma unroll
         for (int k = 0; k < GROUP; ++k)
-          if (dw && row[k] >= 0 && row[k] < rows_kept && v + i * tpr < nvec)
-            yr[k][i] = load_raw<T, VEC>(y + static_cast<int64_t>(row[k]) * width + (v + i * tpr) * VEC);
+          if (dw && on(k)) yr[k][i] = load_raw<T, VEC>(y + at(k) + (v + i * tpr) * VEC);
       }
 #pragma unroll
       for (int i = 0; i < U; ++i) {
@@ -443,18 +450,16 @@ __global__ void __launch_bounds__(kRowThreads, VEC < kVecOf<T> ? 4 : GROUP == 2 
         unpack(gr[i], g);
 #pragma unroll
         for (int k = 0; k < GROUP; ++k) {
-          if (row[k] < 0) continue;
-          const bool on = row[k] < rows_kept;  // else its row of y is not read and its gradients are zero
           float f[VEC];
-          if (dw && on) {
+          if (dw && on(k)) {
             unpack(yr[k][i], f);
 #pragma unroll
             for (int e = 0; e < VEC; ++e) dot[k] += g[e] * f[e];
           }
-          if (dy) {
+          if (dy && row[k] >= 0) {
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) f[e] = on ? wk[k] * g[e] : 0.0f;
-            store_vec<T, VEC>(dy + static_cast<int64_t>(row[k]) * width + (v + i * tpr) * VEC, f);
+            for (int e = 0; e < VEC; ++e) f[e] = on(k) ? wk[k] * g[e] : 0.0f;
+            store_vec<T, VEC>(dy + at(k) + (v + i * tpr) * VEC, f);
           }
         }
       }
@@ -462,7 +467,9 @@ __global__ void __launch_bounds__(kRowThreads, VEC < kVecOf<T> ? 4 : GROUP == 2 
     if (!dw) continue;
 #pragma unroll
     for (int k = 0; k < GROUP; ++k)
-      for (int o = (tpr < 32 ? tpr : 32) / 2; o > 0; o >>= 1) dot[k] += __shfl_xor_sync(0xffffffffu, dot[k], o);
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1)
+        if (o < tpr) dot[k] += __shfl_xor_sync(0xffffffffu, dot[k], o);
     if (tpr > 32) {
       const int warp = threadIdx.x / 32;
       if (threadIdx.x % 32 == 0) {

@@ -87,7 +87,7 @@ int current_device_info(DevInfo* out, int* dev_out) {
   return d.major == 10 ? MLPK_OK : MLPK_ERR_ARCH;
 }
 
-int blocks_per_sm(const void* kern, int threads, size_t smem, int dev) {
+int blocks_per_sm(const void* kern, int threads, size_t smem, int dev) try {
   static std::mutex mu;
   static std::map<std::tuple<const void*, int, size_t, int>, int> known;
   static std::map<std::pair<const void*, int>, size_t> allowed;  // dynamic shared memory that the kernel may have
@@ -101,8 +101,12 @@ int blocks_per_sm(const void* kern, int threads, size_t smem, int dev) {
       most = smem;
     }
     if (cuda_status(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, threads, smem))) n = 0;
+    else if (n == 0) cuda_status(cudaErrorLaunchOutOfResources);
   }
   return n;
+} catch (...) {  // the maps' memory; no exception may leave a C entry point
+  cuda_status(cudaErrorMemoryAllocation);
+  return 0;
 }
 
 }  // namespace host

@@ -48,12 +48,10 @@ __device__ __forceinline__ void norm_row_init(float* red, int n, int tpr) {
   __syncthreads();
 }
 __device__ __forceinline__ float norm_row_sum(float v, int tpr, float* red, int half) {
-  if (tpr <= 32) {
-    for (int o = tpr / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    return v;
-  }
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  for (int o = 16; o > 0; o >>= 1)
+    if (o < tpr) v += __shfl_xor_sync(0xffffffffu, v, o);
+  if (tpr <= 32) return v;
   red += half * 32;
   if (threadIdx.x % 32 == 0) red[threadIdx.x / 32] = v;
   __syncthreads();
@@ -68,7 +66,9 @@ __device__ __forceinline__ float norm_row_sum(float v, int tpr, float* red, int 
 
 // The largest v (not below 0) of the row's threads; a NaN stays.
 __device__ __forceinline__ float norm_row_max(float v, int tpr, float* red, int half) {
-  for (int o = (tpr < 32 ? tpr : 32) / 2; o > 0; o >>= 1) v = max_nan(v, __shfl_xor_sync(0xffffffffu, v, o));
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)
+    if (o < tpr) v = max_nan(v, __shfl_xor_sync(0xffffffffu, v, o));
   if (tpr <= 32) return v;
   red += half * 32;
   if (threadIdx.x % 32 == 0) red[threadIdx.x / 32] = v;
@@ -86,17 +86,21 @@ template <class T, int NV, bool RAGGED>
 struct RowSpan {
   static constexpr int VEC = kVecOf<T>;
   int64_t total;  // elements of the tensor
-  int width, tpr, lane, shift, nvec;
+  int width, tpr, lane, shift, nvec, step;  // step: elements from a vector to the thread's next
 
   // first_row: any row of the row group
   __device__ RowSpan(int64_t rows, int width_, int tpr_, int lane_, int64_t first_row)
       : total(rows * width_), width(width_), tpr(tpr_), lane(lane_) {
     shift = RAGGED ? static_cast<int>((first_row % VEC) * (width % VEC) % VEC) : 0;
     nvec = (width + shift + VEC - 1) / VEC;
+    step = tpr * VEC;
   }
   __device__ bool has(int i) const { return i * tpr + lane < nvec; }
   __device__ int col(int i) const { return (i * tpr + lane) * VEC - shift; }  // of element 0; may be below 0
-  __device__ int64_t at(int64_t begin, int i) const { return begin + col(i); }  // begin = row * width; a multiple of VEC
+  // The thread's first element of a row, and element 0 of its vector i behind
+  // it: multiples of VEC.
+  __device__ int64_t begin(int64_t row) const { return row * width + col(0); }
+  __device__ int64_t at(int64_t begin, int i) const { return begin + i * step; }
   __device__ bool owns(int i, int e) const {
     return !RAGGED || static_cast<unsigned>(col(i) + e) < static_cast<unsigned>(width);
   }
@@ -223,7 +227,7 @@ __global__ void __launch_bounds__(MAXT, !FP8 ? 0 : MAXT == 256 ? 3 : MAXT == 512
     cp_async_commit();
   };
   const int64_t begin_step = step * a.width;
-  int64_t begin = first * a.width;
+  int64_t begin = span.begin(first);  // (a thread beyond the last row may have one below span.total: what it copies is not used)
   if constexpr (PIPE)
     for (int k = 0; k < stages; ++k) fetch(begin + k * begin_step, k * stage_slots);
   NormWeights<T, W, NV, (NV <= 2 && !FP8)> w;
@@ -304,20 +308,22 @@ __global__ void __launch_bounds__(MAXT, !FP8 ? 0 : MAXT == 256 ? 3 : MAXT == 512
         for (int i = 0; i < NV; ++i)
           if (live && span.has(i)) store(i, inv, inv, VEC);
       } else if constexpr (!RAGGED) {
-        // The 128 / VEC lanes of a group are neighbours: a power of two, and a
-        // divisor of tpr unless the row is narrower than a group.
-        const int gl = min(kNormGroup / VEC, a.tpr);
+        // The 128 / VEC lanes of a group are neighbours, or the row is narrower
+        // than a group.
+        constexpr int LANES = kNormGroup / VEC;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
           float m = 0.0f;
 #pragma unroll
           for (int e = 0; e < HALF; ++e) m = max_abs(m, h[i][e].x, h[i][e].y);
-          for (int o = gl / 2; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+#pragma unroll
+          for (int o = LANES / 2; o > 0; o >>= 1)
+            if (o < a.tpr) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
           float inv;
           const float scale = fp8_scale_fast(m, &inv);
           if (live && span.has(i)) {
             const int v = i * a.tpr + lane;
-            if (v % gl == 0) a.scale[row * groups + v / gl] = scale;
+            if (v % LANES == 0) a.scale[row * groups + v / LANES] = scale;
             store(i, inv, inv, VEC);
           }
         }
@@ -422,7 +428,7 @@ __global__ void __launch_bounds__(MAXT, MAXT == 256 ? 2 : 1) rms_norm_bwd_kernel
     cp_async_commit();
   };
   const int64_t begin_step = step * a.width;
-  int64_t begin = first * a.width;
+  int64_t begin = span.begin(first);  // (a thread beyond the last row may have one below span.total: what it copies is not used)
   if constexpr (PIPE)
     for (int k = 0; k < stages; ++k) fetch(begin + k * begin_step, k * stage_slots);
   float2 dw[NV][HALF];

@@ -94,8 +94,8 @@ class FusedAdamW(torch.optim.Optimizer):
     gradient that is not finite makes its whole block's state NaN: use GradScaler
     or clip.)  ``master_weights=True`` keeps an fp32 copy of each 16-bit
     parameter, made when its state is, which is stepped and rounded into the
-    parameter; without it a 16-bit parameter is stepped in fp32 and rounded to
-    itself, as in torch.  ``lr`` is a number or a CUDA tensor of one element.
+    parameter (what else is written into the parameter later is lost); without it
+    a 16-bit parameter is stepped in fp32 and rounded to itself, as in torch.  ``lr`` is a number or a CUDA tensor of one element.
 
     A parameter whose ``grad`` is None is left as it is.  Gradients are in the
     parameter's dtype or fp32.  The step count is on the device, so ``step()``
@@ -131,8 +131,8 @@ class FusedAdamW(torch.optim.Optimizer):
                 raise ValueError("a tensor lr must be one float32 value on the GPU")
         elif not lr >= 0.0:
             raise ValueError(f"lr must not be negative, got {lr}")
-        if not (0.0 < b1 < 1.0 and 0.0 < b2 < 1.0):
-            raise ValueError(f"betas must lie between 0 and 1, got {(b1, b2)}")
+        if not (0.0 <= b1 < 1.0 and 0.0 <= b2 < 1.0):
+            raise ValueError(f"betas must be at least 0 and below 1, got {(b1, b2)}")
         if not group["eps"] >= 0.0 or not group["weight_decay"] >= 0.0:
             raise ValueError("eps and weight_decay must not be negative")
         for p in group["params"]:
@@ -156,7 +156,6 @@ class FusedAdamW(torch.optim.Optimizer):
             for i, p in enumerate(ps):
                 self.state[p] = {name: b.view(i, name) for name in b.flat}
 
-    @torch.no_grad()
     def step(self, closure=None, *, grad_scale=None, found_inf=None):
         """One step.  ``grad_scale`` and ``found_inf`` (fp32 values on the GPU, as
         GradScaler passes them): the gradients are divided by the one; a

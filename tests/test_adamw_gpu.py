@@ -227,6 +227,16 @@ def test_against_torch():
         assert (x.double() - y).abs().max().item() <= 10 * W * (3 * y.abs().max().item() + 100 * 1e-2)
 
 
+@pytest.mark.parametrize("bits", [8, 32])
+def test_betas_of_zero(bits):
+    """m = g and r = |g|: the step is lr * sign(g), as far as |g| is above eps."""
+    p = torch.nn.Parameter(torch.zeros(300, device="cuda"))
+    p.grad = randn(300, 1).clamp(min=0.1) * torch.where(randn(300, 2) > 0, 1.0, -1.0)
+    opt = FusedAdamW([p], lr=0.5, betas=(0.0, 0.0), eps=1e-12, weight_decay=0.0, state_bits=bits)
+    opt.step()
+    assert ((p.detach() + 0.5 * p.grad.sign()).abs() <= 0.5 * 20 * W).all()
+
+
 def test_strides_and_orders():
     """A transposed parameter, a gradient of another order, and one that is a
     slice: elements meet their own gradient."""

@@ -77,7 +77,7 @@ def test_adamw_refusals(fake):
                       (lambda: m.FusedAdamW([p], lr=-1.0), ValueError),
                       (lambda: m.FusedAdamW([p], lr=torch.tensor(1.0, device="cpu")), ValueError),
                       (lambda: m.FusedAdamW([p], betas=(1.0, 0.9)), ValueError),
-                      (lambda: m.FusedAdamW([p], betas=(0.9, 0.0)), ValueError),
+                      (lambda: m.FusedAdamW([p], betas=(0.9, -0.1)), ValueError),
                       (lambda: m.FusedAdamW([p], eps=-1e-8), ValueError),
                       (lambda: m.FusedAdamW([p], weight_decay=-0.1), ValueError),
                       (lambda: m.FusedAdamW([param(8, dtype=torch.float64)]), TypeError),
