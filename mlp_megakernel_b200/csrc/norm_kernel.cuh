@@ -8,11 +8,14 @@
 // or over each 128 columns.  Backward, from x, r and s (G = dL/dy):
 //   n_j = h_j s;   c = mean_j G_j w_j n_j
 //   dx_j = dr_j = s (G_j w_j - n_j c) + dL/dh_j;   dw_j = sum_rows G_j n_j
-// It adds x and r again: from the rounded h, dw would be half as exact again
-// (its own rounding and h's are of the same size), and h costs 2 bytes less of
-// 20 an element.
+// It adds x and r again.  From the rounded h, dw's error would be half as large
+// again (its own rounding and h's are of the same size); that would read 2 bytes
+// less of the 18 that both passes move an element in 16 bits.
 //
-// What bounds it: memory; every value is read once and written once.
+// What bounds it: memory; every value is read once and written once.  16,384
+// rows of 4096 bf16 values with a residual: forward 97 us, 5.5 TB/s (what is
+// left: half of it is writes); backward 105 us, 6.4 TB/s, with dw's sum; 8,192
+// rows of 5120 to 8 bits in groups of 128: 51 us, 5.8 TB/s.
 //
 // Layout: TPR threads share a row, NV 16-byte vectors each (vector i of lane l
 // is the row's vector i * TPR + l).  Up to 32 threads a row's sum is a warp
@@ -21,13 +24,16 @@
 // vectors of the next rows to its own slots of shared memory (cp.async) and
 // reads them back itself: enough bytes are in flight whatever the registers
 // hold, and no barrier guards the slots.  Rows whose slots do not fit (PIPE
-// false) are read directly.
+// false) are read directly.  (One block a row with its loads in registers: 246
+// us forward, 414 backward.)  The next row's s is loaded a row ahead (158 us
+// without), and arithmetic is on pairs of values (132 us one at a time).
 //
 // A width that no vector divides (RAGGED): a row begins `shift` elements into
 // an aligned vector of the tensor, its first and last vectors are shared with
 // its neighbours, and a thread leaves out the elements that are not its row's.
 // Blocks step by a multiple of VEC rows, so that `shift`, and with it each
-// thread's columns, are the same in all rows of a block's row group.
+// thread's columns, are the same in all rows of a block's row group.  (8,192
+// rows of 2049 bf16 values: forward 26 us, 0.78 of the copy rate.)
 #pragma once
 #include "pdl.cuh"
 #include "vec.cuh"
