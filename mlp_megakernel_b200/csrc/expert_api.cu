@@ -85,19 +85,18 @@ int sort_slots(int64_t slots, int experts, const void* ids_, int* row_of, int* o
 // Threads of a token's row of `items` words or vectors, `each` a thread, and the
 // blocks for the tokens, `tokens_each` a thread.
 struct RowGrid {
-  int tpr, threads;
-  dim3 grid;
+  dim3 grid, block;
 };
 RowGrid row_grid(int64_t tokens, int tokens_each, int64_t items, int each, bool parts) {
   RowGrid g;
   // Parts of a row of equal size, each at most what 256 threads take.
   const int64_t n = parts ? ceil_div(items, static_cast<int64_t>(kRowThreads) * each) : 1;
   const int64_t want = std::min<int64_t>(ceil_div(ceil_div(items, n), each), kRowThreads);
-  g.tpr = 1;
-  while (g.tpr < want && g.tpr < 32) g.tpr *= 2;
-  if (want > 32) g.tpr = static_cast<int>(ceil_div(want, 32)) * 32;
-  const int subs = kRowThreads / g.tpr;
-  g.threads = subs * g.tpr;
+  int tpr = 1;
+  while (tpr < want && tpr < 32) tpr *= 2;
+  if (want > 32) tpr = static_cast<int>(ceil_div(want, 32)) * 32;
+  const int subs = kRowThreads / tpr;
+  g.block = dim3(tpr, subs);
   g.grid = dim3(static_cast<unsigned>(ceil_div(tokens, static_cast<int64_t>(subs) * tokens_each)),
                 static_cast<unsigned>(n));
   return g;
@@ -108,8 +107,8 @@ int dispatch_words(int64_t tokens, int top, int64_t words, const void* x, const 
                    cudaStream_t st) {
   constexpr int NW = sizeof(U) == 16 ? 1 : sizeof(U) == 8 ? 2 : 4, NT = 2;
   const RowGrid g = row_grid(tokens, NT, words, NW, true);
-  return launch_kernel_early(expert_dispatch_kernel<U, NT, NW>, g.grid, g.threads, 0, st, static_cast<const U*>(x),
-                             tokens, top, static_cast<int>(words), g.tpr, row_of, kept, static_cast<U*>(xs));
+  return launch_kernel_early(expert_dispatch_kernel<U, NT, NW>, g.grid, g.block, 0, st, static_cast<const U*>(x),
+                             tokens, top, static_cast<int>(words), row_of, kept, static_cast<U*>(xs));
 }
 
 // f(T, W, VEC): 16-byte vectors where the width allows them, else pairs of
@@ -205,9 +204,9 @@ int mlpk_expert_combine(int64_t tokens, int top, int width, int dtype, const voi
     return with_group(top, [&](auto group) {
       constexpr int GROUP = decltype(group)::value;
       const RowGrid g = row_grid(tokens, 1, width / V, NW, true);
-      return launch_kernel_early(expert_combine_kernel<T, W, V, NW, GROUP>, g.grid, g.threads, 0,
+      return launch_kernel_early(expert_combine_kernel<T, W, V, NW, GROUP>, g.grid, g.block, 0,
                                  static_cast<cudaStream_t>(stream), static_cast<const T*>(y),
-                                 static_cast<const W*>(weights), tokens, top, width, g.tpr, row_of, kept,
+                                 static_cast<const W*>(weights), tokens, top, width, row_of, kept,
                                  static_cast<T*>(out));
     });
   });
@@ -231,9 +230,9 @@ int mlpk_expert_combine_bwd(int64_t tokens, int top, int width, int dtype, const
     return with_group(top, [&](auto group) {
       constexpr int GROUP = decltype(group)::value;
       const RowGrid g = row_grid(tokens, 1, width / V, V == kVecOf<T> ? 2 : 8, false);
-      return launch_kernel_early(expert_combine_bwd_kernel<T, W, V, GROUP>, g.grid, g.threads, 0,
+      return launch_kernel_early(expert_combine_bwd_kernel<T, W, V, GROUP>, g.grid, g.block, 0,
                                  static_cast<cudaStream_t>(stream), static_cast<const T*>(grad_out),
-                                 static_cast<const T*>(y), static_cast<const W*>(weights), tokens, top, width, g.tpr,
+                                 static_cast<const T*>(y), static_cast<const W*>(weights), tokens, top, width,
                                  row_of, kept, static_cast<T*>(dy), static_cast<W*>(dw));
     });
   });

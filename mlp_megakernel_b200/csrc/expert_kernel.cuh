@@ -305,24 +305,27 @@ __global__ void __launch_bounds__(kSortThreads)
 constexpr int kRowThreads = 256;
 constexpr int kRowWidthMax = 1 << 24;  // columns; 65,535 parts of a row are the grid's limit
 
-// Tokens of a thread: `tokens_each` of them, a block's tokens apart.
+// A block has blockDim.x (tpr) threads a token and blockDim.y tokens at a time
+// (two dimensions: a division by tpr is 20 instructions, of 180 for a short
+// row), and NT times as many in all.
+template <int NT>
 struct TokenSpan {
-  int lane, sub, subs;
+  int lane;
   int64_t first;
-  __device__ TokenSpan(int tpr, int tokens_each)
-      : lane(threadIdx.x % tpr), sub(threadIdx.x / tpr), subs(blockDim.x / tpr),
-        first(static_cast<int64_t>(blockIdx.x) * subs * tokens_each + sub) {}
-  __device__ int64_t token(int n) const { return first + static_cast<int64_t>(n) * subs; }
+  __device__ TokenSpan()
+      : lane(threadIdx.x), first(static_cast<int64_t>(blockIdx.x) * blockDim.y * NT + threadIdx.y) {}
+  __device__ int64_t token(int n) const { return first + static_cast<int64_t>(n) * blockDim.y; }
 };
 
 // Rows are moved as words of U (16, 8, 4 or 2 bytes: the widest that divides
 // a row), NW a thread and token.
 template <class U, int NT, int NW>
 __global__ void __launch_bounds__(kRowThreads)
-    expert_dispatch_kernel(const U* __restrict__ x, int64_t tokens, int top, int words, int tpr,
+    expert_dispatch_kernel(const U* __restrict__ x, int64_t tokens, int top, int words,
                            const int* __restrict__ row_of, const int* __restrict__ kept, U* __restrict__ xs) {
   pdl_enter();
-  const TokenSpan span(tpr, NT);
+  const TokenSpan<NT> span;
+  const int tpr = blockDim.x;
   const int c0 = blockIdx.y * tpr * NW + span.lane;
   U v[NT][NW];
 #pragma unroll
@@ -352,10 +355,11 @@ __global__ void __launch_bounds__(kRowThreads)
 // GROUP choices at a time.
 template <class T, class W, int VEC, int NW, int GROUP>
 __global__ void __launch_bounds__(kRowThreads, VEC < kVecOf<T> ? 4 : GROUP == 2 ? 8 : 5)
-    expert_combine_kernel(const T* __restrict__ y, const W* __restrict__ w, int64_t tokens, int top, int width, int tpr,
+    expert_combine_kernel(const T* __restrict__ y, const W* __restrict__ w, int64_t tokens, int top, int width,
                           const int* __restrict__ row_of, const int* __restrict__ kept, T* __restrict__ out) {
   pdl_enter();
-  const TokenSpan span(tpr, 1);
+  const TokenSpan<1> span;
+  const int tpr = blockDim.x;
   const int64_t t = span.first;
   if (t >= tokens) return;
   const int nvec = width / VEC;
@@ -405,12 +409,13 @@ __global__ void __launch_bounds__(kRowThreads, VEC < kVecOf<T> ? 4 : GROUP == 2 
 template <class T, class W, int VEC, int GROUP>
 __global__ void __launch_bounds__(kRowThreads, VEC < kVecOf<T> ? 4 : GROUP == 2 ? 6 : 4)
     expert_combine_bwd_kernel(const T* __restrict__ gout, const T* __restrict__ y, const W* __restrict__ w,
-                              int64_t tokens, int top, int width, int tpr, const int* __restrict__ row_of,
+                              int64_t tokens, int top, int width, const int* __restrict__ row_of,
                               const int* __restrict__ kept, T* __restrict__ dy, W* __restrict__ dw) {
   constexpr int U = VEC == kVecOf<T> ? 1 : 4;
   __shared__ float red[2][kRowThreads / 32][GROUP];
   pdl_enter();
-  const TokenSpan span(tpr, 1);
+  const TokenSpan<1> span;
+  const int tpr = blockDim.x;
   const int64_t t = span.first;
   const bool live = t < tokens;  // the others take part in the shuffles and barriers
   const int nvec = width / VEC;
@@ -471,8 +476,8 @@ __global__ void __launch_bounds__(kRowThreads, VEC < kVecOf<T> ? 4 : GROUP == 2 
       for (int o = 16; o > 0; o >>= 1)
         if (o < tpr) dot[k] += __shfl_xor_sync(0xffffffffu, dot[k], o);
     if (tpr > 32) {
-      const int warp = threadIdx.x / 32;
-      if (threadIdx.x % 32 == 0) {
+      const int warp = threadIdx.y * (tpr / 32) + span.lane / 32;
+      if (span.lane % 32 == 0) {
 #pragma unroll
         for (int k = 0; k < GROUP; ++k) red[half][warp][k] = dot[k];
       }

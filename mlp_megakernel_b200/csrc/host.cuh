@@ -45,11 +45,11 @@ inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 
 // training kernels do not (the config-3 step measured 40.8 us at 16,384 rows
 // without it, 42.4 with it).
 template <typename... KArgs, typename... Args>
-int launch_kernel_cfg(bool early, void (*kern)(KArgs...), dim3 grid, unsigned block, size_t smem,
+int launch_kernel_cfg(bool early, void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem,
                       cudaStream_t st, Args&&... args) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
-  cfg.blockDim = dim3(block, 1, 1);
+  cfg.blockDim = block;
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
@@ -60,12 +60,12 @@ int launch_kernel_cfg(bool early, void (*kern)(KArgs...), dim3 grid, unsigned bl
   return cuda_status(cudaLaunchKernelEx(&cfg, kern, std::forward<Args>(args)...));
 }
 template <typename... KArgs, typename... Args>
-int launch_kernel(void (*kern)(KArgs...), dim3 grid, unsigned block, size_t smem, cudaStream_t st,
+int launch_kernel(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st,
                   Args&&... args) {
   return launch_kernel_cfg(false, kern, grid, block, smem, st, std::forward<Args>(args)...);
 }
 template <typename... KArgs, typename... Args>
-int launch_kernel_early(void (*kern)(KArgs...), dim3 grid, unsigned block, size_t smem, cudaStream_t st,
+int launch_kernel_early(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st,
                         Args&&... args) {
   return launch_kernel_cfg(true, kern, grid, block, smem, st, std::forward<Args>(args)...);
 }
