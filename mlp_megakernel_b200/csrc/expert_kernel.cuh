@@ -306,8 +306,7 @@ constexpr int kRowThreads = 256;
 constexpr int kRowWidthMax = 1 << 24;  // columns; 65,535 parts of a row are the grid's limit
 
 // A block has blockDim.x (tpr) threads a token and blockDim.y tokens at a time
-// (two dimensions: a division by tpr is 20 instructions, of 180 for a short
-// row), and NT times as many in all.
+// (two dimensions spare the divisions by tpr), NT times as many in all.
 template <int NT>
 struct TokenSpan {
   int lane;
