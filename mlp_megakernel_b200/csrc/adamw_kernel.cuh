@@ -121,6 +121,7 @@ __device__ __forceinline__ unsigned long long adam_ticks(const AdamArgs& a, cons
 // The step's factors, twice each.
 struct AdamFactors {
   float2 minus_step, rcorr, keep, gs;
+  bool scaled;  // gs is not 1
 };
 // Thread 0 finds the factors, counts the step, and says whether to skip it.
 __device__ __forceinline__ bool adam_factors(const AdamArgs& a, const AdamTensor& t, const AdamPart& part,
@@ -148,13 +149,14 @@ __device__ __forceinline__ bool adam_factors(const AdamArgs& a, const AdamTensor
   f.rcorr = make_float2(scalars[1], scalars[1]);
   f.keep = make_float2(scalars[2], scalars[2]);
   f.gs = make_float2(scalars[3], scalars[3]);
+  f.scaled = scalars[3] != 1.0f;
   return skip;
 }
 
 // Two elements.
 __device__ __forceinline__ void adam_update(const AdamArgs& a, const AdamFactors& f, float2& p, float2 g, float2& m,
                                             float2& v, float2& r) {
-  const float2 x = mul2(g, f.gs);
+  const float2 x = f.scaled ? mul2(g, f.gs) : g;
   m = add2(mul2(m, a.b1), mul2(x, a.b1c));
   v = add2(mul2(v, a.b2), mul2(mul2(x, x), a.b2c));
   r = make_float2(__fsqrt_rn(v.x), __fsqrt_rn(v.y));
@@ -261,40 +263,41 @@ __global__ void __launch_bounds__(kAdamThreads, 3)
   if constexpr (MASTER) pr = master;
   else pr = p;
 
-  auto piece = [&](int stage, int k) { return slots + stage * S::STAGE + (k * kAdamThreads + threadIdx.x) * 16; };
-  auto scale_slot = [&](int stage) {
-    return reinterpret_cast<float*>(slots + stage * S::STAGE + S::PIECES * kAdamThreads * 16) + threadIdx.x;
-  };
+  // A stage's slots: the thread's 16-byte pieces, 16 * kAdamThreads apart, and
+  // its scale.  `stage` is the stage's offset in bytes.
+  constexpr int SCALES = S::PIECES * kAdamThreads * 16;
+  const uint32_t piece0 = smem_address(slots) + threadIdx.x * 16, scale0 = smem_address(slots) + SCALES + threadIdx.x * 4;
   // Copies chunk c to its slots.  A thread at the tensor's end, or of an
   // unaligned tensor, leaves out what it will read element by element.
   auto fetch = [&](int c, int stage) {
     const int ahead = c * kAdamChunk, here = part.left - ahead;
     if (c < part.mine && here + lane * 8 > 0) {  // the whole warp
       const bool whole = part.aligned && here >= 8;
+      const uint32_t to = piece0 + stage;
       if (MASTER || whole) {
 #pragma unroll
         for (int k = 0; k < S::P16; ++k)
-          cp_async16(piece(stage, k), reinterpret_cast<const uint4*>(pr + ahead) + k, 16);
+          cp_async16(to + k * kAdamThreads * 16, reinterpret_cast<const uint4*>(pr + ahead) + k);
       }
       if (whole) {
 #pragma unroll
         for (int k = 0; k < S::G16; ++k)
-          cp_async16(piece(stage, S::P16 + k), reinterpret_cast<const uint4*>(g + ahead) + k, 16);
+          cp_async16(to + (S::P16 + k) * kAdamThreads * 16, reinterpret_cast<const uint4*>(g + ahead) + k);
       }
-      uint8_t* st = piece(stage, S::P16 + S::G16);
-      cp_async_small<8>(st, sm + ahead);
-      cp_async_small<8>(st + 8, sr + ahead);
-      cp_async_small<4>(scale_slot(stage), scales + ahead / kAdamBlock);
+      cp_async_small<8>(to + (S::P16 + S::G16) * kAdamThreads * 16, sm + ahead);
+      cp_async_small<8>(to + (S::P16 + S::G16) * kAdamThreads * 16 + 8, sr + ahead);
+      cp_async_small<4>(scale0 + stage, scales + ahead / kAdamBlock);
     }
     cp_async_commit();
   };
   auto read16 = [&](auto& raw, int stage, int first) {
 #pragma unroll
     for (int k = 0; k < static_cast<int>(sizeof(raw) / 16); ++k)
-      reinterpret_cast<uint4*>(&raw)[k] = *reinterpret_cast<const uint4*>(piece(stage, first + k));
+      reinterpret_cast<uint4*>(&raw)[k] =
+          *reinterpret_cast<const uint4*>(slots + stage + ((first + k) * kAdamThreads + threadIdx.x) * 16);
   };
 #pragma unroll
-  for (int k = 0; k < kAdamStages8; ++k) fetch(k, k);
+  for (int k = 0; k < kAdamStages8; ++k) fetch(k, k * S::STAGE);
   AdamFactors f;
   if (adam_factors(a, t, part, ticks, f)) {
     cp_async_wait<0>();
@@ -316,7 +319,7 @@ __global__ void __launch_bounds__(kAdamThreads, 3)
     if (whole) read16(g8, stage, S::P16);
     else g8 = adam_load(g + ahead, false, here);
     read16(mr, stage, S::P16 + S::G16);
-    float scale = *scale_slot(stage);
+    float scale = *reinterpret_cast<const float*>(slots + stage + SCALES + threadIdx.x * 4);
     const float ms = __shfl_sync(0xffffffffu, scale, 0), rs = __shfl_sync(0xffffffffu, scale, 16);
     unpack2(p8, pf);
     unpack2(g8, gf);
@@ -329,7 +332,7 @@ __global__ void __launch_bounds__(kAdamThreads, 3)
       v[e] = mul2(v[e], v[e]);
     }
     fetch(c + kAdamStages8, stage);
-    stage = stage + 1 == kAdamStages8 ? 0 : stage + 1;
+    stage = stage + S::STAGE == S::BYTES ? 0 : stage + S::STAGE;
     float mmax = 0.0f, rmax = 0.0f;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
@@ -349,16 +352,26 @@ __global__ void __launch_bounds__(kAdamThreads, 3)
     float inv;
     scale = fp8_scale(abs_bits(top), &inv);
     const float mi = __shfl_sync(0xffffffffu, inv, 0), ri = __shfl_sync(0xffffffffu, inv, 16);
-    const float least = ri > 0.0f ? kFp8Tiny : 0.0f;
     Raw<uint16_t, 4> mq, rq;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       mq.v[e] = to_fp8x2(mul2(m[e], make_float2(mi, mi)));
-      // `least` for an r above 0 (the root of a number above 2^-150), 0 for 0.
-      const float2 q = mul2(r[e], make_float2(ri, ri));
-      const float2 z = mul2(make_float2(__saturatef(r[e].x * 1.0e30f), __saturatef(r[e].y * 1.0e30f)),
-                            make_float2(least, least));
-      rq.v[e] = to_fp8x2(make_float2(max_nan(q.x, z.x), max_nan(q.y, z.y)));
+      rq.v[e] = to_fp8x2(mul2(r[e], make_float2(ri, ri)));
+    }
+    // The smallest code for an r above 0 that was rounded to 0 (unless the
+    // whole block is): only if one of the 8 codes, all below 128, is 0.
+    uint32_t zero = 0;
+#pragma unroll
+    for (int e = 0; e < 4; e += 2) {
+      const uint32_t four = rq.v[e] | static_cast<uint32_t>(rq.v[e + 1]) << 16;
+      zero |= (four - 0x01010101u) & ~four & 0x80808080u;
+    }
+    if (zero && ri > 0.0f) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if ((rq.v[e] & 0xffu) == 0 && r[e].x > 0.0f) rq.v[e] |= 1u;
+        if ((rq.v[e] >> 8) == 0 && r[e].y > 0.0f) rq.v[e] |= 0x100u;
+      }
     }
     *reinterpret_cast<Raw<uint16_t, 4>*>(sm + ahead) = mq;
     *reinterpret_cast<Raw<uint16_t, 4>*>(sr + ahead) = rq;

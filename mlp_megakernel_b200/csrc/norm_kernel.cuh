@@ -87,9 +87,13 @@ __device__ __forceinline__ float norm_row_max(float v, int tpr, float* red, int 
   return v;
 }
 
-// A thread's vectors of the rows of its block's row group.
-template <class T, int NV, bool RAGGED>
+// A thread's vectors of the rows of its block's row group.  KIND: kRagged; kFull
+// where a block has one row and every thread all its NV vectors (nothing to ask
+// for each vector: a fifth of the instructions); else kPart.
+enum RowKind { kPart, kFull, kRagged };
+template <class T, int NV, int KIND>
 struct RowSpan {
+  static constexpr bool RAGGED = KIND == kRagged;
   static constexpr int VEC = kVecOf<T>;
   int64_t total;  // elements of the tensor
   int width, tpr, lane, shift, nvec, step;  // step: elements from a vector to the thread's next
@@ -101,7 +105,7 @@ struct RowSpan {
     nvec = (width + shift + VEC - 1) / VEC;
     step = tpr * VEC;
   }
-  __device__ bool has(int i) const { return i * tpr + lane < nvec; }
+  __device__ bool has(int i) const { return KIND == kFull || i * tpr + lane < nvec; }
   __device__ int col(int i) const { return (i * tpr + lane) * VEC - shift; }  // of element 0; may be below 0
   // The thread's first element of a row, and element 0 of its vector i behind
   // it: multiples of VEC.
@@ -203,10 +207,11 @@ struct NormArgs {
 
 // Shared memory: 128 floats for the row sums, then with FP8, RAGGED and groups
 // a maximum per group and row group, then the slots [stage][x, r][i][thread].
-template <class T, class W, int NV, bool RAGGED, bool PIPE, int MAXT, bool FP8>
-__global__ void __launch_bounds__(MAXT, !FP8 ? 0 : MAXT == 256 ? 3 : MAXT == 512 && NV == 2 ? 2 : 1)
+template <class T, class W, int NV, int KIND, bool PIPE, int MAXT, bool FP8>
+__global__ void __launch_bounds__(MAXT, !FP8 ? 0 : MAXT == 256 ? (KIND == kRagged ? 3 : 4) : MAXT == 512 && NV == 2 ? 2 : 1)
     rms_norm_fwd_kernel(const NormArgs a, int stages, int slots_at) {
-  using Span = RowSpan<T, NV, RAGGED>;
+  using Span = RowSpan<T, NV, KIND>;
+  constexpr bool RAGGED = Span::RAGGED;
   constexpr int VEC = Span::VEC, HALF = VEC / 2;
   extern __shared__ __align__(16) uint8_t smem_raw[];
   float* red = reinterpret_cast<float*>(smem_raw);
@@ -226,8 +231,8 @@ __global__ void __launch_bounds__(MAXT, !FP8 ? 0 : MAXT == 256 ? 3 : MAXT == 512
 #pragma unroll
       for (int i = 0; i < NV; ++i)
         if (span.has(i)) {
-          cp_async16(slot(stage, 0, i), x + span.at(begin, i), span.bytes(begin, i));
-          if (r) cp_async16(slot(stage, 1, i), r + span.at(begin, i), span.bytes(begin, i));
+          cp_async16(smem_address(slot(stage, 0, i)), x + span.at(begin, i), span.bytes(begin, i));
+          if (r) cp_async16(smem_address(slot(stage, 1, i)), r + span.at(begin, i), span.bytes(begin, i));
         }
     }
     cp_async_commit();
@@ -246,7 +251,7 @@ __global__ void __launch_bounds__(MAXT, !FP8 ? 0 : MAXT == 256 ? 3 : MAXT == 512
   // shuffles and barriers.
   int64_t row = first;
   for (int64_t row0 = first - sub; row0 < a.rows; row0 += step, row += step, begin += begin_step, half ^= 1) {
-    const bool live = row < a.rows;
+    const bool live = KIND == kFull || row < a.rows;
     if constexpr (PIPE) cp_async_wait_upto(stages - 1);
     float2 h[NV][HALF];
     float2 sum2 = make_float2(0.0f, 0.0f);
@@ -400,9 +405,10 @@ struct NormBwdArgs {
 // second time from L2.
 // Shared memory: 64 floats, then the slots [stage][x, gy, r, gh][i][thread], which
 // the sum over the row groups takes over at the end.
-template <class T, class W, int NV, bool RAGGED, bool PIPE, int MAXT>
+template <class T, class W, int NV, int KIND, bool PIPE, int MAXT>
 __global__ void __launch_bounds__(MAXT, MAXT == 256 ? 2 : 1) rms_norm_bwd_kernel(const NormBwdArgs a, int stages) {
-  using Span = RowSpan<T, NV, RAGGED>;
+  using Span = RowSpan<T, NV, KIND>;
+  constexpr bool RAGGED = Span::RAGGED;
   constexpr int VEC = Span::VEC, HALF = VEC / 2;
   constexpr bool KEEP = NV <= 2;
   extern __shared__ __align__(16) uint8_t smem_raw[];
@@ -425,10 +431,10 @@ __global__ void __launch_bounds__(MAXT, MAXT == 256 ? 2 : 1) rms_norm_bwd_kernel
       for (int i = 0; i < NV; ++i)
         if (span.has(i)) {
           const int n = span.bytes(begin, i);
-          cp_async16(slot(stage, 0, i), in[0] + span.at(begin, i), n);
-          cp_async16(slot(stage, 1, i), in[1] + span.at(begin, i), n);
-          if (in[2]) cp_async16(slot(stage, 2, i), in[2] + span.at(begin, i), n);
-          if (in[3]) cp_async16(slot(stage, gh_slot, i), in[3] + span.at(begin, i), n);
+          cp_async16(smem_address(slot(stage, 0, i)), in[0] + span.at(begin, i), n);
+          cp_async16(smem_address(slot(stage, 1, i)), in[1] + span.at(begin, i), n);
+          if (in[2]) cp_async16(smem_address(slot(stage, 2, i)), in[2] + span.at(begin, i), n);
+          if (in[3]) cp_async16(smem_address(slot(stage, gh_slot, i)), in[3] + span.at(begin, i), n);
         }
     }
     cp_async_commit();
@@ -451,7 +457,7 @@ __global__ void __launch_bounds__(MAXT, MAXT == 256 ? 2 : 1) rms_norm_bwd_kernel
   const float inv_width = 1.0f / static_cast<float>(a.width);
   float s_next = row < a.rows ? a.rstd[row] : 0.0f;
   for (int64_t row0 = first - sub; row0 < a.rows; row0 += step, row += step, begin += begin_step, half ^= 1) {
-    const bool live = row < a.rows;
+    const bool live = KIND == kFull || row < a.rows;
     const float s = s_next;  // the next row's is on its way while this one is worked on
     s_next = row + step < a.rows ? a.rstd[row + step] : 0.0f;
     if constexpr (PIPE) cp_async_wait_upto(stages - 1);

@@ -20,7 +20,7 @@ inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 // up to 8,193 vectors).
 struct RowPlan {
   int tpr, nv, rows_per_block, threads;
-  bool ragged;
+  bool ragged, full;  // full: one row a block, every thread with all its vectors
 };
 inline RowPlan row_plan(int width, int vec) {
   RowPlan p;
@@ -39,6 +39,7 @@ inline RowPlan row_plan(int width, int vec) {
   }
   p.rows_per_block = p.tpr <= 32 ? kNormThreads / p.tpr : 1;
   p.threads = p.rows_per_block * p.tpr;
+  p.full = !p.ragged && p.tpr > 32 && nvec == p.tpr * p.nv;
   return p;
 }
 inline int vec_of(int dtype) { return dtype == MLPK_DT_F32 ? 4 : 8; }
@@ -72,31 +73,34 @@ inline int64_t bwd_blocks(int64_t rows, int width, int dtype, int sm_count) {
   return loop_blocks(rows, p, vec_of(dtype), static_cast<int64_t>(sm_count) * bwd_per_sm(p));
 }
 
-// f(NV, RAGGED, PIPE, MAXT) of this call.
+// f(NV, KIND, PIPE, MAXT) of this call.
 template <bool V>
 using Bool = std::integral_constant<bool, V>;
 template <int V>
 using Int = std::integral_constant<int, V>;
 
-template <class T, bool RAGGED, class F>
+template <class T, int KIND, class F>
 int with_counts(const RowPlan& p, bool pipe, F&& f) {
+  using Kind = Int<KIND>;
   switch (p.nv) {
-    case 1: return f(Int<1>{}, Bool<RAGGED>{}, Bool<true>{}, Int<256>{});
+    case 1:
+      if constexpr (KIND != kFull) return f(Int<1>{}, Kind{}, Bool<true>{}, Int<256>{});
+      return MLPK_ERR_UNSUPPORTED;
     case 2:
-      if (p.threads <= 256) return f(Int<2>{}, Bool<RAGGED>{}, Bool<true>{}, Int<256>{});
-      return f(Int<2>{}, Bool<RAGGED>{}, Bool<true>{}, Int<512>{});
+      return p.threads <= 256 ? f(Int<2>{}, Kind{}, Bool<true>{}, Int<256>{})
+                              : f(Int<2>{}, Kind{}, Bool<true>{}, Int<512>{});
     case 4:
-      if (p.threads <= 512) return f(Int<4>{}, Bool<RAGGED>{}, Bool<true>{}, Int<512>{});
-      return pipe ? f(Int<4>{}, Bool<RAGGED>{}, Bool<true>{}, Int<1024>{})
-                  : f(Int<4>{}, Bool<RAGGED>{}, Bool<false>{}, Int<1024>{});
+      if (p.threads <= 512) return f(Int<4>{}, Kind{}, Bool<true>{}, Int<512>{});
+      return pipe ? f(Int<4>{}, Kind{}, Bool<true>{}, Int<1024>{}) : f(Int<4>{}, Kind{}, Bool<false>{}, Int<1024>{});
     default:
-      if constexpr (sizeof(T) == 4 || RAGGED) return f(Int<9>{}, Bool<RAGGED>{}, Bool<false>{}, Int<1024>{});
+      if constexpr (sizeof(T) == 4 || KIND == kRagged) return f(Int<9>{}, Kind{}, Bool<false>{}, Int<1024>{});
       return MLPK_ERR_UNSUPPORTED;
   }
 }
 template <class T, class F>
-int with_raggedness(const RowPlan& p, bool pipe, F&& f) {
-  return p.ragged ? with_counts<T, true>(p, pipe, f) : with_counts<T, false>(p, pipe, f);
+int with_kind(const RowPlan& p, bool pipe, F&& f) {
+  if (p.ragged) return with_counts<T, kRagged>(p, pipe, f);
+  return p.full ? with_counts<T, kFull>(p, pipe, f) : with_counts<T, kPart>(p, pipe, f);
 }
 
 template <class T, class W, bool FP8>
@@ -113,8 +117,8 @@ int forward(NormArgs a, cudaStream_t st) {
   if (FP8 && p.ragged && a.group)
     slots_at += ceil_div(sizeof(float) * p.rows_per_block * ceil_div(a.width, kNormGroup), 16) * 16;
   const size_t smem = slots_at + static_cast<size_t>(stages) * p.nv * p.threads * streams * 16;
-  return with_raggedness<T>(p, stages > 0, [&](auto nv, auto ragged, auto pipe, auto maxt) {
-    const auto kern = rms_norm_fwd_kernel<T, W, decltype(nv)::value, decltype(ragged)::value, decltype(pipe)::value,
+  return with_kind<T>(p, stages > 0, [&](auto nv, auto kind, auto pipe, auto maxt) {
+    const auto kern = rms_norm_fwd_kernel<T, W, decltype(nv)::value, decltype(kind)::value, decltype(pipe)::value,
                                           decltype(maxt)::value, FP8>;
     const int per_sm = host::blocks_per_sm(reinterpret_cast<const void*>(kern), p.threads, smem, dev);
     if (per_sm == 0) return static_cast<int>(MLPK_ERR_CUDA);
@@ -134,8 +138,8 @@ int backward(NormBwdArgs a, int64_t blocks, W* dw, int dev, cudaStream_t st) {
   size_t smem = static_cast<size_t>(stages) * p.nv * p.threads * streams * 16;
   if (p.rows_per_block > 1) smem = std::max(smem, sizeof(float) * p.rows_per_block * static_cast<size_t>(a.width));
   smem += 64 * sizeof(float);
-  const int rc = with_raggedness<T>(p, stages > 0, [&](auto nv, auto ragged, auto pipe, auto maxt) {
-    const auto kern = rms_norm_bwd_kernel<T, W, decltype(nv)::value, decltype(ragged)::value, decltype(pipe)::value,
+  const int rc = with_kind<T>(p, stages > 0, [&](auto nv, auto kind, auto pipe, auto maxt) {
+    const auto kern = rms_norm_bwd_kernel<T, W, decltype(nv)::value, decltype(kind)::value, decltype(pipe)::value,
                                           decltype(maxt)::value>;
     if (host::blocks_per_sm(reinterpret_cast<const void*>(kern), p.threads, smem, dev) == 0)
       return static_cast<int>(MLPK_ERR_CUDA);

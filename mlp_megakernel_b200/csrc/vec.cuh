@@ -106,18 +106,18 @@ __device__ __forceinline__ void store_32b(float* p, const float2 (&f)[4]) {
 // A 16-byte copy from global to shared memory that the thread waits for later;
 // `bytes` of it are read, the rest are zeros.  A thread that reads back only
 // what it copied itself needs no barrier, just cp_async_wait.
-__device__ __forceinline__ void cp_async16(void* smem, const void* global, int bytes) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
-                   static_cast<uint32_t>(__cvta_generic_to_shared(smem))),
-               "l"(global), "r"(bytes)
-               : "memory");
+__device__ __forceinline__ uint32_t smem_address(const void* p) {
+  return static_cast<uint32_t>(__cvta_generic_to_shared(p));
+}
+__device__ __forceinline__ void cp_async16(uint32_t smem, const void* global, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem), "l"(global), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_async16(uint32_t smem, const void* global) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem), "l"(global) : "memory");
 }
 template <int BYTES>  // 4 or 8
-__device__ __forceinline__ void cp_async_small(void* smem, const void* global) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(
-                   static_cast<uint32_t>(__cvta_generic_to_shared(smem))),
-               "l"(global), "n"(BYTES)
-               : "memory");
+__device__ __forceinline__ void cp_async_small(uint32_t smem, const void* global) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(smem), "l"(global), "n"(BYTES) : "memory");
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 // Until all but the N youngest groups of this thread have arrived.
