@@ -27,14 +27,16 @@
 // 6.65 TB/s.  Measured against it: all loads of both chunks first, 3 thread
 // blocks an SM, 536 us; 16-byte accesses 506; 5 thread blocks 503; 8 chunks 493.
 //
-// 8-bit state: 10 bytes an element and 54 instructions (a root, a quotient,
-// four conversions), so memory bounds it only while the warps hardly wait.  A
-// thread block has up to 16 chunks, one after the other, and each thread copies
-// its part of the next ones to its own slots of shared memory (cp.async): 3
-// under way.  233 million bf16 parameters: 438 us, 5.4 TB/s.  Measured against
-// it: all loads of two chunks first 516 us; one chunk ahead in registers 760 (the
-// loads were put off behind the work they were to overlap); 4 thread blocks an
-// SM with their registers spilling 516, 3 without 438; 4 copies under way 442.
+// 8-bit state: 10 bytes an element and some 49 instructions (a root, a
+// quotient, four conversions), so memory bounds it only while the warps hardly
+// wait.  A thread block has up to 16 chunks, one after the other, and each
+// thread copies its part of the next ones to its own slots of shared memory
+// (cp.async): 3 under way.  233 million bf16 parameters: 419 us, 5.6 TB/s; 480
+// us back to back for seconds, when the power cap takes the clock from 1.97 to
+// 1.7 GHz.  Measured against it (438 us then): all loads of two chunks first 516
+// us; one chunk ahead in registers 760 (the loads were put off behind the work
+// they were to overlap); 4 thread blocks an SM with their registers spilling
+// 516, 3 without 438; 4 copies under way 442.
 #pragma once
 #include <type_traits>
 

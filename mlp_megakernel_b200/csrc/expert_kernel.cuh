@@ -298,7 +298,7 @@ __global__ void __launch_bounds__(kSortThreads)
 // allows.  A row waits for its place and then for its values, so what counts is
 // how many rows an SM has under way: a thread has few (2 or 4 choices of one
 // token) and few registers, and the SM as many threads as it can hold.  Of
-// 32,768 tokens' 8 rows of 2048 bf16 values the combine takes 191 us (6.3 TB/s)
+// 32,768 tokens' 8 rows of 2048 bf16 values the combine takes 187 us (6.5 TB/s)
 // with 48 registers a thread, 231 with 80 to 100 and twice the rows; of 131,072
 // tokens' 2 rows of 256 fp16 values 36.7 with 32 registers, 45 with 100.
 

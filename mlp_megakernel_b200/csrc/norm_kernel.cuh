@@ -13,9 +13,9 @@
 // less of the 18 that both passes move an element in 16 bits.
 //
 // What bounds it: memory; every value is read once and written once.  16,384
-// rows of 4096 bf16 values with a residual: forward 97 us, 5.5 TB/s (what is
-// left: half of it is writes); backward 105 us, 6.4 TB/s, with dw's sum; 8,192
-// rows of 5120 to 8 bits in groups of 128: 51 us, 5.8 TB/s.
+// rows of 4096 bf16 values with a residual: forward 95 us, 5.7 TB/s; backward
+// 104 us, 6.5 TB/s, with dw's sum; 8,192 rows of 5120 to 8 bits in groups of 128:
+// 50 us, 5.9 TB/s.
 //
 // Layout: TPR threads share a row, NV 16-byte vectors each (vector i of lane l
 // is the row's vector i * TPR + l).  Up to 32 threads a row's sum is a warp
