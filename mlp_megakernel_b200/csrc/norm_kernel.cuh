@@ -96,6 +96,7 @@ struct RowSpan {
   static constexpr bool RAGGED = KIND == kRagged;
   static constexpr int VEC = kVecOf<T>;
   int64_t total;  // elements of the tensor
+  int64_t end;    // what begin() is below in the rows there are
   int width, tpr, lane, shift, nvec, step;  // step: elements from a vector to the thread's next
 
   // first_row: any row of the row group
@@ -104,6 +105,7 @@ struct RowSpan {
     shift = RAGGED ? static_cast<int>((first_row % VEC) * (width % VEC) % VEC) : 0;
     nvec = (width + shift + VEC - 1) / VEC;
     step = tpr * VEC;
+    end = total + col(0);
   }
   __device__ bool has(int i) const { return KIND == kFull || i * tpr + lane < nvec; }
   __device__ int col(int i) const { return (i * tpr + lane) * VEC - shift; }  // of element 0; may be below 0
@@ -227,7 +229,7 @@ __global__ void __launch_bounds__(MAXT, !FP8 ? 0 : MAXT == 256 ? (KIND == kRagge
   const int stage_slots = streams * NV * blockDim.x;  // `stage` counts them
   auto slot = [&](int stage, int stream, int i) { return slots + (stage + (stream * NV + i) * blockDim.x); };
   auto fetch = [&](int64_t begin, int stage) {
-    if (begin < span.total) {
+    if (begin < span.end) {
 #pragma unroll
       for (int i = 0; i < NV; ++i)
         if (span.has(i)) {
@@ -238,7 +240,7 @@ __global__ void __launch_bounds__(MAXT, !FP8 ? 0 : MAXT == 256 ? (KIND == kRagge
     cp_async_commit();
   };
   const int64_t begin_step = step * a.width;
-  int64_t begin = span.begin(first);  // (a thread beyond the last row may have one below span.total: what it copies is not used)
+  int64_t begin = span.begin(first);
   if constexpr (PIPE)
     for (int k = 0; k < stages; ++k) fetch(begin + k * begin_step, k * stage_slots);
   NormWeights<T, W, NV, (NV <= 2 && !FP8)> w;
@@ -426,7 +428,7 @@ __global__ void __launch_bounds__(MAXT, MAXT == 256 ? 2 : 1) rms_norm_bwd_kernel
   const int stage_slots = streams * NV * blockDim.x;  // `stage` counts them
   auto slot = [&](int stage, int stream, int i) { return slots + (stage + (stream * NV + i) * blockDim.x); };
   auto fetch = [&](int64_t begin, int stage) {
-    if (begin < span.total) {
+    if (begin < span.end) {
 #pragma unroll
       for (int i = 0; i < NV; ++i)
         if (span.has(i)) {
@@ -440,7 +442,7 @@ __global__ void __launch_bounds__(MAXT, MAXT == 256 ? 2 : 1) rms_norm_bwd_kernel
     cp_async_commit();
   };
   const int64_t begin_step = step * a.width;
-  int64_t begin = span.begin(first);  // (a thread beyond the last row may have one below span.total: what it copies is not used)
+  int64_t begin = span.begin(first);
   if constexpr (PIPE)
     for (int k = 0; k < stages; ++k) fetch(begin + k * begin_step, k * stage_slots);
   float2 dw[NV][HALF];

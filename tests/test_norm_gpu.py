@@ -163,6 +163,37 @@ def test_many_rows_and_repeatable():
     assert ((first[1].double() - gn.sum(0)).abs() - room).max().item() <= 0
 
 
+@pytest.mark.parametrize("rows,width,dtype", [(1, 1999, torch.float16), (7, 2049, torch.bfloat16), (296, 517, torch.float32),
+                                              (592, 2049, torch.bfloat16), (1776, 300, torch.float16),
+                                              (148, 8190, torch.float16)])
+def test_last_rows_of_ragged_widths(rows, width, dtype):
+    """Rows whose next one would begin at the tensor's end: what lies behind the
+    tensor (NaN here) is neither read nor used, and nothing is written there."""
+    def edged(seed):
+        big = torch.full((rows * width + 4096,), math.nan, device="cuda", dtype=dtype)
+        big[:rows * width] = make(1, rows * width, dtype, seed)[0]
+        return big, big[:rows * width].view(rows, width)
+
+    (_, x), (_, r), (_, gy), (_, gh) = (edged(k) for k in range(4))
+    w = torch.ones(width, device="cuda", dtype=dtype, requires_grad=True)
+    xl, rl = x.detach().requires_grad_(), r.detach().requires_grad_()
+    y, h = fused_rms_norm(xl, w, residual=rl, eps=EPS)
+    ref_h, s, ref = reference(x, None, r)
+    close(y, ref, U[dtype] + 60 * W)
+    dx, dw = torch.autograd.grad((y, h), (xl, w), (gy, gh))
+    n, g = ref_h * s, gy.double()
+    want = s * (g - n * (g * n).mean(-1, keepdim=True))
+    room = 110 * W * s * (g.abs() + n.abs() * (g * n).abs().mean(-1, keepdim=True)) + W * gh.double().abs()
+    want = want + gh.double()
+    assert ((dx.double() - want).abs() - U[dtype] * want.abs() - room - 2.0 ** -25).max().item() <= 0
+    gn = g * n
+    assert ((dw.double() - gn.sum(0)).abs() - U[dtype] * gn.sum(0).abs() - (rows + 110) * W * gn.abs().sum(0)
+            - 2.0 ** -25).max().item() <= 0
+    with torch.no_grad():
+        q, scale = fused_rms_norm_fp8(x, group=128)
+    assert q.float().isfinite().all() and scale.isfinite().all()
+
+
 def test_rows_without_values():
     for shape in ((0, 64), (3, 0, 128), (0, 7)):
         x = torch.empty(shape, device="cuda", requires_grad=True)
