@@ -352,7 +352,7 @@ __global__ void __launch_bounds__(kAdamThreads, 3)
 #pragma unroll
     for (int o = 8; o > 0; o >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
     float inv;
-    scale = fp8_scale(abs_bits(top), &inv);
+    scale = fp8_scale(top, &inv);
     const float mi = __shfl_sync(0xffffffffu, inv, 0), ri = __shfl_sync(0xffffffffu, inv, 16);
     Raw<uint16_t, 4> mq, rq;
 #pragma unroll

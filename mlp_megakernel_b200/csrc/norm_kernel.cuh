@@ -15,7 +15,8 @@
 // What bounds it: memory; every value is read once and written once.  16,384
 // rows of 4096 bf16 values with a residual: forward 95 us, 5.7 TB/s; backward
 // 104 us, 6.5 TB/s, with dw's sum; 8,192 rows of 5120 to 8 bits in groups of 128:
-// 50 us, 5.9 TB/s.
+// 56 us, 5.3 TB/s (53 with a reciprocal of the scale that is off by a unit of its
+// last place in an eighth of the cases, which moves values next to a tie).
 //
 // Layout: TPR threads share a row, NV 16-byte vectors each (vector i of lane l
 // is the row's vector i * TPR + l).  Up to 32 threads a row's sum is a warp
@@ -248,7 +249,7 @@ __global__ void __launch_bounds__(MAXT, !FP8 ? 0 : MAXT == 256 ? (KIND == kRagge
   norm_row_init(red, 128, a.tpr);
 
   int stage = 0, half = 0;
-  const float inv_width = 1.0f / static_cast<float>(a.width);
+  const float width = static_cast<float>(a.width), inv_width = 1.0f / width;
   // Whole blocks loop together: the last rows' missing ones take part in the
   // shuffles and barriers.
   int64_t row = first;
@@ -278,7 +279,9 @@ __global__ void __launch_bounds__(MAXT, !FP8 ? 0 : MAXT == 256 ? (KIND == kRagge
       fetch(begin + stages * begin_step, stage);
       stage = stage + stage_slots == stages * stage_slots ? 0 : stage + stage_slots;
     }
-    const float s = rsqrtf(norm_row_sum(sum2.x + sum2.y, a.tpr, red, half) * inv_width + a.eps);
+    // The mean is a quotient: as a product with a rounded 1 / width it is off by
+    // a unit of its last place now and then.
+    const float s = rsqrtf(quotient(norm_row_sum(sum2.x + sum2.y, a.tpr, red, half), width, inv_width) + a.eps);
     if (a.rstd && live && lane == 0) a.rstd[row] = s;
     float amax = 0.0f;
 #pragma unroll
@@ -315,7 +318,7 @@ __global__ void __launch_bounds__(MAXT, !FP8 ? 0 : MAXT == 256 ? (KIND == kRagge
       const int groups = (a.width + kNormGroup - 1) / kNormGroup;
       if (a.group == 0) {
         float inv;
-        const float scale = fp8_scale_fast(norm_row_max(amax, a.tpr, red + 64, half), &inv);
+        const float scale = fp8_scale(norm_row_max(amax, a.tpr, red + 64, half), &inv);
         if (live && lane == 0) a.scale[row] = scale;
 #pragma unroll
         for (int i = 0; i < NV; ++i)
@@ -333,7 +336,7 @@ __global__ void __launch_bounds__(MAXT, !FP8 ? 0 : MAXT == 256 ? (KIND == kRagge
           for (int o = LANES / 2; o > 0; o >>= 1)
             if (o < a.tpr) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
           float inv;
-          const float scale = fp8_scale_fast(m, &inv);
+          const float scale = fp8_scale(m, &inv);
           if (live && span.has(i)) {
             const int v = i * a.tpr + lane;
             if (v % LANES == 0) a.scale[row * groups + v / LANES] = scale;
@@ -368,15 +371,15 @@ __global__ void __launch_bounds__(MAXT, !FP8 ? 0 : MAXT == 256 ? (KIND == kRagge
         if (live)
           for (int k = lane; k < groups; k += a.tpr) {
             float inv;
-            a.scale[row * groups + k] = fp8_scale_fast(__uint_as_float(gmax[k]), &inv);
+            a.scale[row * groups + k] = fp8_scale(__uint_as_float(gmax[k]), &inv);
           }
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
           if (live && span.has(i)) {
             const int lo = max(span.col(i), 0) / kNormGroup, hi = (min(span.col(i) + VEC, a.width) - 1) / kNormGroup;
             float inv0, inv1;
-            fp8_scale_fast(__uint_as_float(gmax[lo]), &inv0);
-            fp8_scale_fast(__uint_as_float(gmax[hi]), &inv1);
+            fp8_scale(__uint_as_float(gmax[lo]), &inv0);
+            fp8_scale(__uint_as_float(gmax[hi]), &inv1);
             store(i, inv0, inv1, (lo + 1) * kNormGroup - span.col(i));
           }
         }

@@ -210,26 +210,34 @@ __device__ __forceinline__ float fast_reciprocal(float v) {
   return r;
 }
 
+// Both correctly rounded by one step with a fused remainder (P. Markstein,
+// "Computation of elementary functions on the IBM RISC System/6000 processor",
+// 1990), in less than the compiler's division, which has to take any operands.
+// 1 / v; v and 1 / v are normal numbers.
+__device__ __forceinline__ float reciprocal(float v) {
+  const float r = fast_reciprocal(v);
+  return fmaf(r, fmaf(-v, r, 1.0f), r);
+}
+// a / b for a whole number b and its correctly rounded reciprocal; a may be
+// infinite or NaN (the remainder is NaN then).
+__device__ __forceinline__ float quotient(float a, float b, float reciprocal_b) {
+  const float q = a * reciprocal_b, rest = fmaf(-q, b, a);
+  return rest == rest ? fmaf(rest, reciprocal_b, q) : q;
+}
+
 // |v| as an unsigned whole number: ordered like |v|, with a NaN above
 // infinity, so a maximum over it keeps a NaN.
 __device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
 
-// The scale of a group of 8-bit values whose largest magnitude has these
-// bits, and what to multiply by before the rounding.  A scale below the
-// smallest normal number has no finite reciprocal (and zero times infinity
+// The scale of a group of 8-bit values whose largest magnitude is `amax` (the
+// product with 1 / 448 as fp32 holds it), and what to multiply by before the
+// rounding: the scale's reciprocal, rounded once.  A scale below
+// the smallest normal number has no finite reciprocal (and zero times infinity
 // would put NaN into the group's zeros): such a group is all zeros.
-__device__ __forceinline__ float fp8_scale(uint32_t amax_bits, float* inv) {
-  float scale = __uint_as_float(amax_bits) * (1.0f / kFp8Max);
-  if (scale < 1.17549435e-38f) scale = 0.0f;
-  *inv = scale > 0.0f ? 1.0f / scale : 0.0f;
-  return scale;
-}
-
-// The same with a reciprocal to within a unit of its last place.
-__device__ __forceinline__ float fp8_scale_fast(float amax, float* inv) {
+__device__ __forceinline__ float fp8_scale(float amax, float* inv) {
   float scale = amax * (1.0f / kFp8Max);
   if (scale < 1.17549435e-38f) scale = 0.0f;
-  *inv = scale > 0.0f ? fast_reciprocal(scale) : 0.0f;
+  *inv = scale > 0.0f && scale <= 3.402823466e+38f ? reciprocal(scale) : 0.0f;
   return scale;
 }
 
