@@ -6,6 +6,11 @@
 // interpreter's lock); many of these calls are of small kernels, so the binding
 // is native.  It has no kernels and no checks' messages: where the arguments are
 // not what an operator takes, a call returns None and the Python layer says why.
+// It does so too where torch's dispatcher would not go straight to a CUDA kernel
+// (a mode, a tracer, a transform, a tensor subclass): the Python layer then calls
+// the operators torch.ops.mlpk.*, which those see.
+#include <ATen/core/dispatch/Dispatcher.h>
+#include <c10/core/impl/LocalDispatchKeySet.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -67,6 +72,29 @@ bool needs_grad(std::initializer_list<const Tensor*> ts) {
   for (const Tensor* t : ts)
     if (t->defined() && t->requires_grad()) return true;
   return false;
+}
+
+// Whether the dispatcher would take these tensors to a CUDA kernel with nothing
+// but autograd before it: no dispatch mode, tracer, functionalization or
+// function transform is active, and none is a subclass or a lazy view.
+bool direct(std::initializer_list<const Tensor*> ts) {
+  static const c10::DispatchKeySet ordinary =
+      c10::DispatchKeySet({c10::DispatchKey::CUDA, c10::DispatchKey::AutogradCUDA, c10::DispatchKey::ADInplaceOrView,
+                           c10::DispatchKey::BackendSelect}) |
+      c10::autocast_dispatch_keyset;
+  const auto local = c10::impl::tls_local_dispatch_key_set();
+  c10::DispatchKeySet keys = local.included_;
+  for (const Tensor* t : ts)
+    if (t->defined()) keys = keys | t->key_set();
+  return ((keys - local.excluded_ - ordinary).raw_repr() >> c10::num_backends) == 0;
+}
+// The operator torch.ops.mlpk.<name>.
+template <class... Args>
+c10::IValue operate(const char* name, Args&&... args) {
+  torch::jit::Stack stack;
+  torch::jit::push(stack, std::forward<Args>(args)...);
+  c10::Dispatcher::singleton().findSchemaOrThrow(name, "").callBoxed(&stack);
+  return std::move(stack.at(0));
 }
 
 // The gradients of a backward that is itself differentiated (create_graph)
@@ -139,8 +167,16 @@ struct NormNode : torch::autograd::Function<NormNode> {
     const size_t r_at = w.defined() ? 2 : 1;  // the residual's place among the inputs there are
     {
       const at::NoGradGuard no_grad;
-      std::tie(dx, dw) = norm_backward(saved[0], w, r, saved[3], grads[0], grads.size() > 1 ? grads[1] : Tensor(),
-                                       w.defined() && ctx->needs_input_grad(1));
+      const Tensor &gy = grads[0], gh = grads.size() > 1 ? grads[1] : Tensor();
+      const bool want_dw = w.defined() && ctx->needs_input_grad(1);
+      if (!gy.defined() || direct({&gy, &gh, &saved[0], &w, &r})) {
+        std::tie(dx, dw) = norm_backward(saved[0], w, r, saved[3], gy, gh, want_dw);
+      } else {
+        const std::vector<Tensor> got =
+            operate("mlpk::rms_norm_bwd", saved[0], maybe(r), maybe(w), saved[3], gy, maybe(gh), want_dw).toTensorVector();
+        dx = got[0];
+        if (want_dw) dw = got[1];
+      }
     }
     return once({ctx->needs_input_grad(0) ? dx : Tensor(), dw,
                  r.defined() && ctx->needs_input_grad(r_at) ? dx : Tensor(), Tensor()},
@@ -160,7 +196,7 @@ bool norm_takes(const Tensor& x, const Tensor& w, const Tensor& r, double eps) {
 py::object rms_norm(const Tensor& x, const std::optional<Tensor>& weight, const std::optional<Tensor>& residual,
                     double eps) {
   const Tensor w = weight.value_or(Tensor()), r = residual.value_or(Tensor());
-  if (!norm_takes(x, w, r, eps)) return py::none();
+  if (!norm_takes(x, w, r, eps) || !direct({&x, &w, &r})) return py::none();
   variable_list out;
   {
     py::gil_scoped_release no_gil;
@@ -175,17 +211,13 @@ py::object rms_norm(const Tensor& x, const std::optional<Tensor>& weight, const 
   return r.defined() ? py::object(py::make_tuple(out[0], out[1])) : py::cast(out[0]);
 }
 
-// None also where a gradient would be needed.
-py::object rms_norm_fp8(const Tensor& x_in, const std::optional<Tensor>& weight, const std::optional<Tensor>& residual,
-                        double eps, int64_t group) {
-  const Tensor w_in = weight.value_or(Tensor()), r_in = residual.value_or(Tensor());
-  if (!norm_takes(x_in, w_in, r_in, eps) || (group != 0 && group != 128) || needs_grad({&x_in, &w_in, &r_in}))
-    return py::none();
+py::object norm_fp8(const Tensor& x_in, const std::optional<Tensor>& weight, const std::optional<Tensor>& residual,
+                    double eps, int64_t group) {
   Tensor q, scale, h;
   {
     py::gil_scoped_release no_gil;
     const c10::cuda::CUDAGuard guard(x_in.device());
-    const Tensor x = aligned(x_in), w = aligned(w_in), r = aligned(r_in);
+    const Tensor x = aligned(x_in), w = aligned(weight.value_or(Tensor())), r = aligned(residual.value_or(Tensor()));
     const int64_t width = x.size(-1), rows = x.numel() / width;
     q = at::empty(x.sizes(), x.options().dtype(at::kFloat8_e4m3fn));
     std::vector<int64_t> shape(x.sizes().begin(), x.sizes().end());
@@ -199,13 +231,18 @@ py::object rms_norm_fp8(const Tensor& x_in, const std::optional<Tensor>& weight,
   }
   return h.defined() ? py::make_tuple(q, scale, h) : py::make_tuple(q, scale);
 }
+// None also where a gradient would be needed.
+py::object rms_norm_fp8(const Tensor& x, const std::optional<Tensor>& weight, const std::optional<Tensor>& residual,
+                        double eps, int64_t group) {
+  const Tensor w = weight.value_or(Tensor()), r = residual.value_or(Tensor());
+  if (!norm_takes(x, w, r, eps) || (group != 0 && group != 128) || needs_grad({&x, &w, &r}) || !direct({&x, &w, &r}))
+    return py::none();
+  return norm_fp8(x, weight, residual, eps, group);
+}
 
 // ------------------------------------------------------------------ experts
-py::object expert_sort(const Tensor& ids_in, int64_t experts) {
+py::object sort_ids(const Tensor& ids_in, int64_t experts) {
   const bool wide = ids_in.scalar_type() == at::kLong;
-  if (!ids_in.is_cuda() || ids_in.dim() != 2 || !(wide || ids_in.scalar_type() == at::kInt) || experts < 1 ||
-      experts > kExpertMax || ids_in.size(1) < 1 || ids_in.numel() > 0x7fffffff)
-    return py::none();
   Tensor row_of, offsets;
   {
     py::gil_scoped_release no_gil;
@@ -221,6 +258,13 @@ py::object expert_sort(const Tensor& ids_in, int64_t experts) {
                            stream_of(ids)));
   }
   return py::make_tuple(row_of, offsets);
+}
+
+py::object expert_sort(const Tensor& ids, int64_t experts) {
+  if (!ids.is_cuda() || ids.dim() != 2 || !(ids.scalar_type() == at::kLong || ids.scalar_type() == at::kInt) ||
+      experts < 1 || experts > kExpertMax || ids.size(1) < 1 || ids.numel() > 0x7fffffff || !direct({&ids}))
+    return py::none();
+  return sort_ids(ids, experts);
 }
 
 const int32_t* kept(const Tensor& offsets) { return offsets.data_ptr<int32_t>() + offsets.size(0) - 1; }
@@ -271,7 +315,9 @@ struct DispatchNode : torch::autograd::Function<DispatchNode> {
     {
       const at::NoGradGuard no_grad;
       const variable_list saved = ctx->get_saved_variables();
-      dx = combine_rows(grads[0], Tensor(), saved[0], saved[1]);
+      dx = direct({&grads[0], &saved[0], &saved[1]})
+               ? combine_rows(grads[0], Tensor(), saved[0], saved[1])
+               : operate("mlpk::expert_combine", grads[0], std::optional<Tensor>(), saved[0], saved[1]).toTensor();
     }
     return once({dx, Tensor(), Tensor()}, grads);
   }
@@ -290,8 +336,16 @@ struct CombineNode : torch::autograd::Function<CombineNode> {
     {
       const at::NoGradGuard no_grad;
       const variable_list saved = ctx->get_saved_variables();
-      std::tie(dy, dw) = combine_backward(grads[0], saved[0], saved[1], saved[2], saved[3], ctx->needs_input_grad(0),
-                                          saved[1].defined() && ctx->needs_input_grad(1));
+      const bool want_dy = ctx->needs_input_grad(0), want_dw = saved[1].defined() && ctx->needs_input_grad(1);
+      if (direct({&grads[0], &saved[0], &saved[1], &saved[2], &saved[3]})) {
+        std::tie(dy, dw) = combine_backward(grads[0], saved[0], saved[1], saved[2], saved[3], want_dy, want_dw);
+      } else {
+        const std::vector<Tensor> got = operate("mlpk::expert_combine_bwd", grads[0], saved[0], maybe(saved[1]), saved[2],
+                                                saved[3], want_dy, want_dw)
+                                            .toTensorVector();
+        if (want_dy) dy = got.front();
+        if (want_dw) dw = got.back();
+      }
     }
     return once({dy, dw, Tensor(), Tensor()}, grads);
   }
@@ -301,7 +355,7 @@ bool rows_take(const Tensor& t, int64_t rows, const Tensor& row_of, const Tensor
   return t.is_cuda() && code(t) >= 0 && t.dim() == 2 && t.size(0) == rows && t.size(1) >= 1 && row_of.dim() == 2 &&
          row_of.scalar_type() == at::kInt && offsets.scalar_type() == at::kInt && offsets.dim() == 1 &&
          offsets.size(0) > 1 && offsets.is_contiguous() && t.device() == row_of.device() &&
-         t.device() == offsets.device();
+         t.device() == offsets.device() && direct({&t, &row_of, &offsets});
 }
 
 py::object expert_dispatch(const Tensor& x, const Tensor& row_of, const Tensor& offsets) {
@@ -318,7 +372,7 @@ py::object expert_combine(const Tensor& y, const std::optional<Tensor>& weights,
                           const Tensor& offsets) {
   const Tensor w = weights.value_or(Tensor());
   if (!rows_take(y, row_of.numel(), row_of, offsets)) return py::none();
-  if (w.defined() && (w.sizes() != row_of.sizes() || w.device() != y.device() || !weight_type(w, y)))
+  if (w.defined() && (w.sizes() != row_of.sizes() || w.device() != y.device() || !weight_type(w, y) || !direct({&w})))
     return py::none();
   Tensor out;
   {
@@ -454,6 +508,8 @@ PYBIND11_MODULE(mlpk_torch, m) {
                             const Tensor& rstd, const Tensor& gy, const std::optional<Tensor>& gh, bool want_dw) {
     return norm_backward(x, w.value_or(Tensor()), r.value_or(Tensor()), rstd, gy, gh.value_or(Tensor()), want_dw);
   });
+  m.def("norm_fp8", &norm_fp8);
+  m.def("sort_ids", &sort_ids);
   m.def("dispatch_rows", &dispatch_rows);
   m.def("combine_rows", [](const Tensor& y, const std::optional<Tensor>& w, const Tensor& row_of,
                            const Tensor& offsets) { return combine_rows(y, w.value_or(Tensor()), row_of, offsets); });

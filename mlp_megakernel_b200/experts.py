@@ -12,8 +12,8 @@ MLP experts (no counterpart in the reference, which has one MLP).
 Rows are fp16, bf16 or fp32 of any width; sums are fp32 in a fixed order, so
 results are the same from run to run.  Everything runs on the current CUDA
 stream without a wait of the host; there is no CPU path.  Eager calls go through
-the native binding (_native.py); under torch.compile and on fake tensors the
-calls are the operators ``torch.ops.mlpk.expert_*``.
+the native binding (_native.py); under torch.compile, tracers and dispatch modes
+and on fake tensors the calls are the operators ``torch.ops.mlpk.expert_*``.
 """
 from __future__ import annotations
 
@@ -59,7 +59,7 @@ def _require_cuda(*ts):
 @torch.library.custom_op("mlpk::expert_sort", mutates_args=())
 def _sort_op(ids: Tensor, num_experts: int) -> list[Tensor]:
     _require_cuda(ids)
-    return list(native().expert_sort(ids, num_experts))
+    return list(native().sort_ids(ids, num_experts))
 
 
 @_sort_op.register_fake

@@ -10,9 +10,9 @@ reference, whose MLP takes its rows as they come).
 x is fp16, bf16 or fp32 of shape ``[..., width]`` with width up to 32768; all
 arithmetic is fp32.  The kernels run on the current CUDA stream; there is no
 CPU path.  Eager calls go through the native binding (_native.py), whose
-autograd nodes are native too; under torch.compile and on fake tensors the
-calls are the operators ``torch.ops.mlpk.rms_norm`` / ``rms_norm_bwd`` /
-``rms_norm_fp8``.
+autograd nodes are native too; under torch.compile, tracers and dispatch modes and
+on fake tensors the calls are the operators ``torch.ops.mlpk.rms_norm`` /
+``rms_norm_bwd`` / ``rms_norm_fp8``.
 """
 from __future__ import annotations
 
@@ -29,8 +29,8 @@ DTYPES = {torch.float16: _lib.DT_F16, torch.float32: _lib.DT_F32, torch.bfloat16
 
 
 def _eager(x) -> bool:
-    """Whether x is an ordinary tensor outside of tracing: the native calls take
-    it."""
+    """Whether the native calls may take x.  (They in turn leave it to the
+    operators where a dispatch mode, a tracer or a transform is to see them.)"""
     return (type(x) is Tensor or type(x) is nn.Parameter) and not torch.compiler.is_compiling()
 
 
@@ -86,8 +86,7 @@ def rms_norm_fp8(x: Tensor, weight: Optional[Tensor], residual: Optional[Tensor]
                  group: int) -> list[Tensor]:
     """[q, scale], and h with a residual."""
     _check(x, weight, residual, eps)
-    with torch.no_grad():
-        return list(native().rms_norm_fp8(x, weight, residual, eps, group))
+    return list(native().norm_fp8(x, weight, residual, eps, group))
 
 
 @rms_norm_fp8.register_fake
