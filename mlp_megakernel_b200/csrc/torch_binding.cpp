@@ -8,7 +8,7 @@
 // not what an operator takes, a call returns None and the Python layer says why.
 // It does so too where torch's dispatcher would not go straight to a CUDA kernel
 // (a mode, a tracer, a transform, a tensor subclass): the Python layer then calls
-// the operators torch.ops.mlpk.*, which those see.
+// the operators torch.ops.mlpk.*, which those see, or says that there is no rule.
 #include <ATen/core/dispatch/Dispatcher.h>
 #include <c10/core/impl/LocalDispatchKeySet.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -75,8 +75,9 @@ bool needs_grad(std::initializer_list<const Tensor*> ts) {
 }
 
 // Whether the dispatcher would take these tensors to a CUDA kernel with nothing
-// but autograd before it: no dispatch mode, tracer, functionalization or
-// function transform is active, and none is a subclass or a lazy view.
+// but backward-mode autograd before it: no dispatch mode, tracer,
+// functionalization or function transform is active, none is a subclass or a
+// lazy view, and none has a tangent.
 bool direct(std::initializer_list<const Tensor*> ts) {
   static const c10::DispatchKeySet ordinary =
       c10::DispatchKeySet({c10::DispatchKey::CUDA, c10::DispatchKey::AutogradCUDA, c10::DispatchKey::ADInplaceOrView,
@@ -84,9 +85,18 @@ bool direct(std::initializer_list<const Tensor*> ts) {
       c10::autocast_dispatch_keyset;
   const auto local = c10::impl::tls_local_dispatch_key_set();
   c10::DispatchKeySet keys = local.included_;
-  for (const Tensor* t : ts)
-    if (t->defined()) keys = keys | t->key_set();
+  for (const Tensor* t : ts) {
+    if (!t->defined()) continue;
+    if (t->_fw_grad(/*level=*/0).defined()) return false;
+    keys = keys | t->key_set();
+  }
   return ((keys - local.excluded_ - ordinary).raw_repr() >> c10::num_backends) == 0;
+}
+// What a backward says where an operator's gradient would drop a tangent.
+void refuse_tangents(std::initializer_list<const Tensor*> ts) {
+  for (const Tensor* t : ts)
+    TORCH_CHECK(!t->defined() || !t->_fw_grad(/*level=*/0).defined(),
+                "the gradient of this operator has no forward-mode derivative");
 }
 // The operator torch.ops.mlpk.<name>.
 template <class... Args>
@@ -172,6 +182,7 @@ struct NormNode : torch::autograd::Function<NormNode> {
       if (!gy.defined() || direct({&gy, &gh, &saved[0], &w, &r})) {
         std::tie(dx, dw) = norm_backward(saved[0], w, r, saved[3], gy, gh, want_dw);
       } else {
+        refuse_tangents({&gy, &gh, &saved[0], &w, &r});
         const std::vector<Tensor> got =
             operate("mlpk::rms_norm_bwd", saved[0], maybe(r), maybe(w), saved[3], gy, maybe(gh), want_dw).toTensorVector();
         dx = got[0];
@@ -315,9 +326,12 @@ struct DispatchNode : torch::autograd::Function<DispatchNode> {
     {
       const at::NoGradGuard no_grad;
       const variable_list saved = ctx->get_saved_variables();
-      dx = direct({&grads[0], &saved[0], &saved[1]})
-               ? combine_rows(grads[0], Tensor(), saved[0], saved[1])
-               : operate("mlpk::expert_combine", grads[0], std::optional<Tensor>(), saved[0], saved[1]).toTensor();
+      if (direct({&grads[0], &saved[0], &saved[1]})) {
+        dx = combine_rows(grads[0], Tensor(), saved[0], saved[1]);
+      } else {
+        refuse_tangents({&grads[0]});
+        dx = operate("mlpk::expert_combine", grads[0], std::optional<Tensor>(), saved[0], saved[1]).toTensor();
+      }
     }
     return once({dx, Tensor(), Tensor()}, grads);
   }
@@ -340,6 +354,7 @@ struct CombineNode : torch::autograd::Function<CombineNode> {
       if (direct({&grads[0], &saved[0], &saved[1], &saved[2], &saved[3]})) {
         std::tie(dy, dw) = combine_backward(grads[0], saved[0], saved[1], saved[2], saved[3], want_dy, want_dw);
       } else {
+        refuse_tangents({&grads[0], &saved[0], &saved[1]});
         const std::vector<Tensor> got = operate("mlpk::expert_combine_bwd", grads[0], saved[0], maybe(saved[1]), saved[2],
                                                 saved[3], want_dy, want_dw)
                                             .toTensorVector();

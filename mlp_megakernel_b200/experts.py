@@ -27,7 +27,7 @@ from torch import Tensor
 from . import _lib
 from ._native import native
 from .modules import FusedMLPSoftplus
-from .norm import DTYPES, FusedRMSNorm, _eager, _needs_grad
+from .norm import DTYPES, FusedRMSNorm, _eager, _needs_grad, _refuse_transforms
 
 
 class ExpertPlan(NamedTuple):
@@ -115,6 +115,7 @@ class _DispatchFn(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
+        _refuse_transforms("the gradient of expert_dispatch", grad)
         return torch.ops.mlpk.expert_combine(grad, None, *ctx.saved_tensors), None, None
 
 
@@ -128,6 +129,7 @@ class _CombineFn(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
         y, weights, row_of, offsets = ctx.saved_tensors
+        _refuse_transforms("the gradient of expert_combine", grad, y, weights)
         want_dy, want_dw = ctx.needs_input_grad[0], weights is not None and ctx.needs_input_grad[1]
         got = torch.ops.mlpk.expert_combine_bwd(grad, y, weights, row_of, offsets, want_dy, want_dw)
         return got[0] if want_dy else None, got[-1] if want_dw else None, None, None
@@ -147,6 +149,7 @@ def expert_sort(ids: Tensor, num_experts: int) -> ExpertPlan:
         got = native().expert_sort(ids, num_experts)
         if got is not None:
             return ExpertPlan(*got)
+    _refuse_transforms("expert_sort", ids)
     if not isinstance(ids, Tensor) or ids.dim() != 2:
         raise ValueError("ids must be a 2-D tensor [tokens, choices]")
     _require_cuda(ids)
@@ -178,6 +181,7 @@ def expert_dispatch(x: Tensor, plan: ExpertPlan) -> Tensor:
         got = native().expert_dispatch(x, *plan)
         if got is not None:
             return got
+    _refuse_transforms("expert_dispatch", x, *plan)
     _check_rows("x", x, plan.row_of.shape[0], plan)
     if _needs_grad(x):
         return _DispatchFn.apply(x, *plan)
@@ -193,6 +197,7 @@ def expert_combine(y: Tensor, weights: Optional[Tensor], plan: ExpertPlan) -> Te
         got = native().expert_combine(y, weights, *plan)
         if got is not None:
             return got
+    _refuse_transforms("expert_combine", y, weights, *plan)
     _check_rows("y", y, plan.row_of.numel(), plan)
     if weights is not None and (weights.shape != plan.row_of.shape or weights.device != y.device
                                 or (weights.dtype != y.dtype and weights.dtype != torch.float32)):

@@ -19,6 +19,7 @@ from __future__ import annotations
 from typing import Optional
 
 import torch
+import torch.autograd.forward_ad as forward_ad
 import torch.nn as nn
 from torch import Tensor
 
@@ -32,6 +33,19 @@ def _eager(x) -> bool:
     """Whether the native calls may take x.  (They in turn leave it to the
     operators where a dispatch mode, a tracer or a transform is to see them.)"""
     return (type(x) is Tensor or type(x) is nn.Parameter) and not torch.compiler.is_compiling()
+
+
+def _refuse_transforms(name: str, *ts) -> None:
+    """Raises where a tangent, or a transform of torch.func, would be lost."""
+    if torch.compiler.is_compiling():
+        return
+    for t in ts:
+        if not isinstance(t, Tensor):
+            continue
+        if torch._C._functorch.is_functorch_wrapped_tensor(t):
+            raise RuntimeError(f"{name} has no rule for torch.func's transforms (vmap, grad, jvp and the like)")
+        if forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError(f"{name} has no forward-mode derivative")
 
 
 def _check(x, weight, residual, eps):
@@ -112,6 +126,7 @@ class _RMSNormFn(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad_y, grad_h=None):
         x, residual, weight, rstd = ctx.saved_tensors
+        _refuse_transforms("the gradient of fused_rms_norm", grad_y, grad_h, x, residual, weight)
         want_dw = weight is not None and ctx.needs_input_grad[1]
         if grad_y is None:  # y was not used: the norm adds nothing
             dx, dw = grad_h, torch.zeros_like(weight) if want_dw and grad_h is not None else None
@@ -141,6 +156,7 @@ def fused_rms_norm(x: Tensor, weight: Optional[Tensor] = None, *, residual: Opti
         got = native().rms_norm(x, weight, residual, eps)
         if got is not None:
             return got
+    _refuse_transforms("fused_rms_norm", x, weight, residual)
     _check(x, weight, residual, eps)
     if _needs_grad(x, weight, residual):
         return _RMSNormFn.apply(x, weight, residual, eps)
@@ -162,6 +178,7 @@ def fused_rms_norm_fp8(x: Tensor, weight: Optional[Tensor] = None, *, residual: 
         got = native().rms_norm_fp8(x, weight, residual, eps, group)
         if got is not None:
             return got
+    _refuse_transforms("fused_rms_norm_fp8", x, weight, residual)
     _check(x, weight, residual, eps)
     if group not in (0, _lib.NORM_GROUP):
         raise ValueError(f"group must be 0 (the row) or {_lib.NORM_GROUP}, got {group}")
