@@ -107,18 +107,14 @@ c10::IValue operate(const char* name, Args&&... args) {
   return std::move(stack.at(0));
 }
 
-// The gradients of a backward that is itself differentiated (create_graph)
-// raise if their derivative is asked for: the operators have none.
-variable_list once(variable_list out, const variable_list& grads) {
-  bool again = false;
-  if (at::GradMode::is_enabled())
-    for (const Tensor& g : grads) again = again || (g.defined() && g.requires_grad());
-  if (!again) return out;
-  variable_list fake;
-  for (const Tensor& t : out) fake.push_back(t.defined() ? t.detach().requires_grad_(true) : t);
-  auto node = std::make_shared<torch::autograd::DelayedError>(
-      "the gradient of this operator cannot be differentiated again", static_cast<int64_t>(fake.size()));
-  return (*node)(std::move(fake));
+// A gradient in a backward that is itself recorded (create_graph).  The
+// operators have no second derivatives: if the gradient depends on a tensor that
+// needs one, asking for its derivative raises.
+Tensor once(const Tensor& grad, std::initializer_list<const Tensor*> depends_on) {
+  if (!grad.defined() || !needs_grad(depends_on)) return grad;
+  auto node =
+      std::make_shared<torch::autograd::DelayedError>("the gradient of this operator cannot be differentiated again", 1);
+  return (*node)({grad.detach().requires_grad_(true)})[0];
 }
 
 // ------------------------------------------------------------------ norm
@@ -173,25 +169,28 @@ struct NormNode : torch::autograd::Function<NormNode> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     Tensor dx, dw;
     const variable_list saved = ctx->get_saved_variables();
-    const Tensor &w = saved[1], &r = saved[2];
+    const Tensor &x = saved[0], &w = saved[1], &r = saved[2], &gy = grads[0];
+    const Tensor gh = grads.size() > 1 ? grads[1] : Tensor();
     const size_t r_at = w.defined() ? 2 : 1;  // the residual's place among the inputs there are
     {
       const at::NoGradGuard no_grad;
-      const Tensor &gy = grads[0], gh = grads.size() > 1 ? grads[1] : Tensor();
       const bool want_dw = w.defined() && ctx->needs_input_grad(1);
-      if (!gy.defined() || direct({&gy, &gh, &saved[0], &w, &r})) {
-        std::tie(dx, dw) = norm_backward(saved[0], w, r, saved[3], gy, gh, want_dw);
+      if (!gy.defined() || direct({&gy, &gh, &x, &w, &r})) {
+        std::tie(dx, dw) = norm_backward(x, w, r, saved[3], gy, gh, want_dw);
       } else {
-        refuse_tangents({&gy, &gh, &saved[0], &w, &r});
+        refuse_tangents({&gy, &gh, &x, &w, &r});
         const std::vector<Tensor> got =
-            operate("mlpk::rms_norm_bwd", saved[0], maybe(r), maybe(w), saved[3], gy, maybe(gh), want_dw).toTensorVector();
+            operate("mlpk::rms_norm_bwd", x, maybe(r), maybe(w), saved[3], gy, maybe(gh), want_dw).toTensorVector();
         dx = got[0];
         if (want_dw) dw = got[1];
       }
     }
-    return once({ctx->needs_input_grad(0) ? dx : Tensor(), dw,
-                 r.defined() && ctx->needs_input_grad(r_at) ? dx : Tensor(), Tensor()},
-                grads);
+    if (gy.defined()) {  // else dx is gh itself
+      dx = once(dx, {&gy, &gh, &x, &w, &r});
+      dw = once(dw, {&gy, &x, &r});
+    }
+    return {ctx->needs_input_grad(0) ? dx : Tensor(), dw, r.defined() && ctx->needs_input_grad(r_at) ? dx : Tensor(),
+            Tensor()};
   }
 };
 
@@ -333,7 +332,7 @@ struct DispatchNode : torch::autograd::Function<DispatchNode> {
         dx = operate("mlpk::expert_combine", grads[0], std::optional<Tensor>(), saved[0], saved[1]).toTensor();
       }
     }
-    return once({dx, Tensor(), Tensor()}, grads);
+    return {once(dx, {&grads[0]}), Tensor(), Tensor()};
   }
 };
 
@@ -347,9 +346,9 @@ struct CombineNode : torch::autograd::Function<CombineNode> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     Tensor dy, dw;
+    const variable_list saved = ctx->get_saved_variables();
     {
       const at::NoGradGuard no_grad;
-      const variable_list saved = ctx->get_saved_variables();
       const bool want_dy = ctx->needs_input_grad(0), want_dw = saved[1].defined() && ctx->needs_input_grad(1);
       if (direct({&grads[0], &saved[0], &saved[1], &saved[2], &saved[3]})) {
         std::tie(dy, dw) = combine_backward(grads[0], saved[0], saved[1], saved[2], saved[3], want_dy, want_dw);
@@ -362,7 +361,7 @@ struct CombineNode : torch::autograd::Function<CombineNode> {
         if (want_dw) dw = got.back();
       }
     }
-    return once({dy, dw, Tensor(), Tensor()}, grads);
+    return {once(dy, {&grads[0], &saved[1]}), once(dw, {&grads[0], &saved[0]}), Tensor(), Tensor()};
   }
 };
 

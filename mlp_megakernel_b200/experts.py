@@ -105,7 +105,8 @@ def _combine_bwd_fake(grad_out, y, weights, row_of, offsets, want_dy, want_dw):
 
 # ------------------------------------------------------------ autograd
 class _DispatchFn(torch.autograd.Function):
-    """The node that torch.compile traces (as _CombineFn)."""
+    """The node that tracers and modes see (as _CombineFn).  Its gradient is an
+    operator without a derivative: asking for one raises."""
 
     @staticmethod
     def forward(ctx, x, row_of, offsets):
@@ -113,7 +114,6 @@ class _DispatchFn(torch.autograd.Function):
         return torch.ops.mlpk.expert_dispatch(x, row_of, offsets)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
         _refuse_transforms("the gradient of expert_dispatch", grad)
         return torch.ops.mlpk.expert_combine(grad, None, *ctx.saved_tensors), None, None
@@ -126,11 +126,14 @@ class _CombineFn(torch.autograd.Function):
         return torch.ops.mlpk.expert_combine(y, weights, row_of, offsets)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
         y, weights, row_of, offsets = ctx.saved_tensors
         _refuse_transforms("the gradient of expert_combine", grad, y, weights)
         want_dy, want_dw = ctx.needs_input_grad[0], weights is not None and ctx.needs_input_grad[1]
+        if not want_dw:  # dy does not depend on y, nor dw on the weights
+            y = y.detach()
+        if not want_dy:
+            weights = weights.detach()
         got = torch.ops.mlpk.expert_combine_bwd(grad, y, weights, row_of, offsets, want_dy, want_dw)
         return got[0] if want_dy else None, got[-1] if want_dw else None, None, None
 

@@ -113,7 +113,8 @@ def _rms_norm_fp8_fake(x, weight, residual, eps, group):
 
 # ------------------------------------------------------------ autograd
 class _RMSNormFn(torch.autograd.Function):
-    """The node that torch.compile traces."""
+    """The node that tracers and modes see.  Its gradients are operators without a
+    derivative: asking for one raises."""
 
     @staticmethod
     def forward(ctx, x, weight, residual, eps):
@@ -123,7 +124,6 @@ class _RMSNormFn(torch.autograd.Function):
         return (y, h[0]) if h else y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, grad_y, grad_h=None):
         x, residual, weight, rstd = ctx.saved_tensors
         _refuse_transforms("the gradient of fused_rms_norm", grad_y, grad_h, x, residual, weight)
@@ -131,6 +131,8 @@ class _RMSNormFn(torch.autograd.Function):
         if grad_y is None:  # y was not used: the norm adds nothing
             dx, dw = grad_h, torch.zeros_like(weight) if want_dw and grad_h is not None else None
         else:
+            if not (ctx.needs_input_grad[0] or ctx.needs_input_grad[2]):
+                weight = weight.detach()  # dw alone, which does not depend on it
             dx, *dws = torch.ops.mlpk.rms_norm_bwd(x, residual, weight, rstd, grad_y, grad_h, want_dw)
             dw = dws[0] if dws else None
         return (dx if ctx.needs_input_grad[0] else None, dw,
