@@ -210,12 +210,13 @@ class FusedAdamW(torch.optim.Optimizer):
     @torch.no_grad()
     def load_state_dict(self, state_dict) -> None:
         """Takes what ``state_dict`` gave, of the same ``state_bits`` and
-        ``master_weights``; the values are copied."""
+        ``master_weights``; the values are copied, from any device.  A load that is
+        refused changes nothing."""
         groups, state = state_dict["param_groups"], state_dict["state"]
         if len(groups) != len(self.param_groups) or \
                 any(len(a["params"]) != len(b["params"]) for a, b in zip(groups, self.param_groups)):
             raise ValueError("the state is of other parameter groups")
-        plans = []
+        loads = []
         for g, (saved, group) in enumerate(zip(groups, self.param_groups)):
             found = [(p, state[i]) for i, p in zip(saved["params"], group["params"]) if i in state]
             for p, s in found:
@@ -224,19 +225,24 @@ class FusedAdamW(torch.optim.Optimizer):
                 names |= {"master_param"} if self._master and p.dtype != torch.float32 else set()
                 if set(s) != names | {"step"}:
                     raise ValueError(f"the state of a parameter holds {sorted(s)}, expected {sorted(names | {'step'})}")
+                if int(s["step"]) < 0:
+                    raise ValueError(f"a step count must not be negative, got {s['step']}")
                 for name in names:
                     n = _blocks(p.numel()) if name.endswith("_scale") else p.numel()
                     kind = torch.float8_e4m3fn if self._state_bits == 8 and name in ("exp_avg", "exp_avg_rms") else \
                         torch.float32
                     if s[name].numel() != n or s[name].dtype != kind:
                         raise ValueError(f"{name} must hold {n} values of {kind}")
-            plans.append(found)
+            options = {k: v.clone() if isinstance(v, Tensor) else v for k, v in saved.items() if k != "params"}
+            if isinstance(options.get("lr"), Tensor) and group["params"]:  # a checkpoint read to the host
+                options["lr"] = options["lr"].to(group["params"][0].device)
+            self._check_group({**group, **options})
+            loads.append((found, options))
+        # Nothing has changed so far, and nothing is refused from here on.
         self.state.clear()
         self._buckets = [[] for _ in self.param_groups]
-        for g, found in enumerate(plans):
-            self.param_groups[g].update({k: v.clone() if isinstance(v, Tensor) else v
-                                         for k, v in groups[g].items() if k != "params"})
-            self._check_group(self.param_groups[g])
+        for g, (found, options) in enumerate(loads):
+            self.param_groups[g].update(options)
             self._bucket(g, [p for p, _ in found])
             saved = dict(found)
             for b in self._buckets[g]:

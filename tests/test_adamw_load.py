@@ -1,0 +1,23 @@
+"""What FusedAdamW's load_state_dict and hooks do before there is any state (no
+GPU needed)."""
+import pytest
+import torch
+from torch._subclasses.fake_tensor import FakeTensorMode
+
+import mlp_megakernel_b200 as m
+
+
+@pytest.fixture
+def opt():
+    with FakeTensorMode():
+        yield m.FusedAdamW([torch.nn.Parameter(torch.empty(8, device="cuda"))], lr=1e-3)
+
+
+@pytest.mark.parametrize("change", [dict(lr=-1.0), dict(lr=float("nan")), dict(betas=(0.9, 1.0)), dict(eps=-1.0)])
+def test_a_refused_load_keeps_the_options(opt, change):
+    saved = opt.state_dict()
+    saved["param_groups"][0].update(change)
+    with pytest.raises(ValueError):
+        opt.load_state_dict(saved)
+    assert opt.param_groups[0]["lr"] == 1e-3 and opt.param_groups[0]["betas"] == (0.9, 0.999)
+    assert opt.param_groups[0]["eps"] == 1e-8
