@@ -2,7 +2,9 @@
 (no counterpart in the reference, which leaves the step to its caller).
 
 ``FusedAdamW`` is a ``torch.optim.Optimizer``: learning-rate schedulers,
-parameter groups, ``state_dict`` and GradScaler work as with torch's AdamW.
+parameter groups, ``state_dict``, its hooks and GradScaler work as with torch's
+AdamW.  (What differs: ``state[p]`` holds parts of flat buffers, to be read and
+written in place, and has no ``step``, which is in ``state_dict`` alone.)
 All tensors of a parameter group that share their types are stepped by one
 kernel launch on the current CUDA stream (768 tensors at most each); there is
 no CPU path.
@@ -193,8 +195,10 @@ class FusedAdamW(torch.optim.Optimizer):
         return [b.flat for buckets in self._buckets for b in buckets]
 
     def state_dict(self) -> dict:
-        """As torch's: ``state[i]`` has ``step`` (a number; the host waits for the
-        GPU) and the tensors of parameter i, ``param_groups`` the rest."""
+        """As torch's, hooks included: ``state[i]`` has ``step`` (a number; the host
+        waits for the GPU) and the tensors of parameter i, ``param_groups`` the rest."""
+        for hook in list(self._optimizer_state_dict_pre_hooks.values()):
+            hook(self)
         place, groups = {}, []
         for group in self.param_groups:
             packed = {k: v for k, v in group.items() if k != "params"}
@@ -205,13 +209,21 @@ class FusedAdamW(torch.optim.Optimizer):
             for b in buckets:
                 for i, (p, step) in enumerate(zip(b.params, b.steps())):
                     state[place[p]] = {"step": step, **{name: b.view(i, name) for name in b.flat}}
-        return {"state": state, "param_groups": groups}
+        found = {"state": state, "param_groups": groups}
+        for hook in list(self._optimizer_state_dict_post_hooks.values()):
+            got = hook(self, found)
+            found = found if got is None else got
+        return found
 
     @torch.no_grad()
     def load_state_dict(self, state_dict) -> None:
         """Takes what ``state_dict`` gave, of the same ``state_bits`` and
         ``master_weights``; the values are copied, from any device.  A load that is
-        refused changes nothing."""
+        refused changes nothing.  Hooks are called as torch's optimizers call them."""
+        state_dict = state_dict.copy()
+        for hook in list(self._optimizer_load_state_dict_pre_hooks.values()):
+            got = hook(self, state_dict)
+            state_dict = state_dict if got is None else got
         groups, state = state_dict["param_groups"], state_dict["state"]
         if len(groups) != len(self.param_groups) or \
                 any(len(a["params"]) != len(b["params"]) for a, b in zip(groups, self.param_groups)):
@@ -251,3 +263,5 @@ class FusedAdamW(torch.optim.Optimizer):
                         v = b.view(i, name)
                         v.copy_(saved[p][name].reshape(v.shape))
                 b.ticks.copy_(torch.tensor([int(saved[p]["step"]) * c for p, c in zip(b.params, b.chunks)]))
+        for hook in list(self._optimizer_load_state_dict_post_hooks.values()):
+            hook(self)

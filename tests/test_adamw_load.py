@@ -21,3 +21,17 @@ def test_a_refused_load_keeps_the_options(opt, change):
         opt.load_state_dict(saved)
     assert opt.param_groups[0]["lr"] == 1e-3 and opt.param_groups[0]["betas"] == (0.9, 0.999)
     assert opt.param_groups[0]["eps"] == 1e-8
+
+
+def test_hooks_are_called(opt):
+    said = []
+    opt.register_state_dict_pre_hook(lambda o: said.append("pre"))
+    opt.register_state_dict_post_hook(lambda o, d: said.append("post") or {**d, "more": 1})
+    opt.register_load_state_dict_pre_hook(lambda o, d: said.append("load") or
+                                          {**d, "param_groups": [{**g, "lr": 0.5} for g in d["param_groups"]]})
+    opt.register_load_state_dict_post_hook(lambda o: said.append("loaded"))
+    saved = opt.state_dict()
+    assert saved["more"] == 1
+    opt.load_state_dict(saved)
+    assert said == ["pre", "post", "load", "loaded"] and opt.param_groups[0]["lr"] == 0.5
+    assert saved["param_groups"][0]["lr"] == 1e-3  # the caller's dict is not changed

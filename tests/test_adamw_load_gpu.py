@@ -93,3 +93,25 @@ def test_its_own_state_loaded_again(bits):
     for opt in (a, b):
         opt.step()
     assert all(torch.equal(x, y) for x, y in zip(p, q))
+
+
+def test_hooks_of_state_dict_and_load():
+    """Called as torch's optimizers call them; a result replaces the dict."""
+    p = make([40])
+    opt = FusedAdamW(p, **HYPER)
+    opt.step()
+    said = []
+    opt.register_state_dict_pre_hook(lambda o: said.append(("pre", o is opt)))
+    opt.register_state_dict_post_hook(lambda o, d: {**d, "more": len(d["state"])})
+    opt.register_load_state_dict_pre_hook(lambda o, d: said.append(("load", "more" in d)) or
+                                          {k: v for k, v in d.items() if k != "more"})
+    opt.register_load_state_dict_post_hook(lambda o: said.append(("loaded", o.state_dict()["state"][0]["step"])))
+    saved = opt.state_dict()
+    assert saved["more"] == 1 and saved["state"][0]["step"] == 1
+    opt.step()
+    opt.load_state_dict(saved)
+    assert said == [("pre", True), ("load", True), ("pre", True), ("loaded", 1)]
+    opt.register_load_state_dict_pre_hook(lambda o, d: d["param_groups"][0].update(lr=-1.0))
+    with pytest.raises(ValueError):
+        opt.load_state_dict(saved)
+    assert opt.param_groups[0]["lr"] == HYPER["lr"]
