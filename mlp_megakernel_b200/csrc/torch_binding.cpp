@@ -397,13 +397,14 @@ py::object expert_combine(const Tensor& y, const std::optional<Tensor>& weights,
 }
 
 // ------------------------------------------------------------------ AdamW
-// Some tensors of one type and device with their places in the flat state.
+// Some tensors of one type and device with their places in the flat state and
+// in its step counts.
 class AdamwBucket {
  public:
-  AdamwBucket(std::vector<Tensor> params, std::vector<int64_t> off, int bits, const Tensor& exp_avg,
-              const Tensor& exp_avg_sq, const std::optional<Tensor>& avg_scale, const std::optional<Tensor>& sq_scale,
-              const std::optional<Tensor>& master, const Tensor& ticks)
-      : params_(std::move(params)), off_(std::move(off)), device_(params_[0].device()),
+  AdamwBucket(std::vector<Tensor> params, std::vector<int64_t> off, std::vector<int32_t> tick, int bits,
+              const Tensor& exp_avg, const Tensor& exp_avg_sq, const std::optional<Tensor>& avg_scale,
+              const std::optional<Tensor>& sq_scale, const std::optional<Tensor>& master, const Tensor& ticks)
+      : params_(std::move(params)), off_(std::move(off)), tick_(std::move(tick)), device_(params_[0].device()),
         type_(params_[0].scalar_type()),
         keep_{exp_avg, exp_avg_sq, avg_scale.value_or(Tensor()), sq_scale.value_or(Tensor()),
               master.value_or(Tensor()), ticks} {
@@ -455,7 +456,7 @@ class AdamwBucket {
       }
       part.numel.push_back(numel_[i]);
       part.off.push_back(off_[i]);
-      part.tick.push_back(static_cast<int32_t>(i));
+      part.tick.push_back(tick_[i]);
       part.p.push_back(p.data_ptr());
       part.g.push_back(gp);
       p.unsafeGetTensorImpl()->bump_version();
@@ -487,6 +488,7 @@ class AdamwBucket {
 
   std::vector<Tensor> params_;
   std::vector<int64_t> off_, numel_;
+  std::vector<int32_t> tick_;
   std::vector<std::vector<int64_t>> strides_;
   at::Device device_;
   at::ScalarType type_;
@@ -531,8 +533,16 @@ PYBIND11_MODULE(mlpk_torch, m) {
                                const Tensor& offsets, bool want_dy, bool want_dw) {
     return combine_backward(g, y, w.value_or(Tensor()), row_of, offsets, want_dy, want_dw);
   });
+  // Whether two lists hold the same objects in the same order.
+  m.def("same_items", [](const py::list& a, const py::list& b) {
+    const Py_ssize_t n = PyList_GET_SIZE(a.ptr());
+    if (n != PyList_GET_SIZE(b.ptr())) return false;
+    for (Py_ssize_t i = 0; i < n; ++i)
+      if (PyList_GET_ITEM(a.ptr(), i) != PyList_GET_ITEM(b.ptr(), i)) return false;
+    return true;
+  });
   py::class_<AdamwBucket>(m, "AdamwBucket")
-      .def(py::init<std::vector<Tensor>, std::vector<int64_t>, int, const Tensor&, const Tensor&,
+      .def(py::init<std::vector<Tensor>, std::vector<int64_t>, std::vector<int32_t>, int, const Tensor&, const Tensor&,
                     const std::optional<Tensor>&, const std::optional<Tensor>&, const std::optional<Tensor>&,
                     const Tensor&>())
       .def("step", &AdamwBucket::step, py::call_guard<py::gil_scoped_release>());

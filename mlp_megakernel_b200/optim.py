@@ -11,6 +11,8 @@ no CPU path.
 """
 from __future__ import annotations
 
+import bisect
+
 import torch
 from torch import Tensor
 
@@ -39,11 +41,12 @@ def _dense(t: Tensor) -> bool:
 
 
 class _Bucket:
-    """The flat state of some tensors of one parameter group: each begins at a
-    multiple of BLOCK elements, and what pads it is zero."""
+    """The flat state of some tensors that got it together: each begins at a
+    multiple of BLOCK elements, and what pads it is zero.  `group` is the place of
+    the parameter group that they were in."""
 
-    def __init__(self, params, bits: int, master: bool):
-        self.params, self.bits = list(params), bits
+    def __init__(self, params, group: int, bits: int, master: bool):
+        self.params, self.group, self.bits = list(params), group, bits
         self.numel = [p.numel() for p in self.params]
         self.off, total = [], 0
         for n in self.numel:
@@ -68,10 +71,14 @@ class _Bucket:
         if master:
             for i, p in enumerate(self.params):
                 self.view(i, "master_param").copy_(p.detach())
-        sq = self.flat["exp_avg_rms" if bits == 8 else "exp_avg_sq"]
-        self.native = native().AdamwBucket(
-            self.params, self.off, bits, self.flat["exp_avg"], sq, self.flat.get("exp_avg_scale"),
-            self.flat.get("exp_avg_rms_scale"), self.flat.get("master_param"), self.ticks)
+
+    def launch(self, members):
+        """What steps the members (their places in this bucket) in one go."""
+        sq = self.flat["exp_avg_rms" if self.bits == 8 else "exp_avg_sq"]
+        return native().AdamwBucket(
+            [self.params[i] for i in members], [self.off[i] for i in members], list(members), self.bits,
+            self.flat["exp_avg"], sq, self.flat.get("exp_avg_scale"), self.flat.get("exp_avg_rms_scale"),
+            self.flat.get("master_param"), self.ticks)
 
     def view(self, i: int, name: str) -> Tensor:
         """Tensor i's part of a flat buffer: of its own shape and strides, or
@@ -87,6 +94,14 @@ class _Bucket:
         return [int(t) // c for t, c in zip(self.ticks.tolist(), self.chunks)]
 
 
+class _Plan:
+    """What a step of one parameter group does, as long as the group holds the same
+    parameters: the launches, and the parameters that have no state yet."""
+
+    def __init__(self, group, params, launches, waiting):
+        self.group, self.params, self.launches, self.waiting = group, params, launches, waiting
+
+
 class FusedAdamW(torch.optim.Optimizer):
     """AdamW (decoupled weight decay) for CUDA parameters in fp32, fp16 or bf16.
 
@@ -99,10 +114,12 @@ class FusedAdamW(torch.optim.Optimizer):
     parameter (what else is written into the parameter later is lost); without it
     a 16-bit parameter is stepped in fp32 and rounded to itself, as in torch.  ``lr`` is a number or a CUDA tensor of one element.
 
-    A parameter whose ``grad`` is None is left as it is.  Gradients are in the
-    parameter's dtype or fp32.  The step count is on the device, so ``step()``
-    can be captured in a CUDA graph after one ordinary step, and a step that
-    GradScaler's ``found_inf`` skips does not count.
+    A step is over what the parameter groups hold then: a parameter that moves to
+    another group keeps its state, one taken out is left as it is, and one whose
+    entry of ``state`` is deleted begins anew.  A parameter whose ``grad`` is None is
+    left as it is.  Gradients are in the parameter's dtype or fp32.  The step count
+    is on the device, so ``step()`` can be captured in a CUDA graph after one
+    ordinary step, and a step that GradScaler's ``found_inf`` skips does not count.
     """
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 1e-2, *,
@@ -111,7 +128,10 @@ class FusedAdamW(torch.optim.Optimizer):
             raise ValueError(f"state_bits must be 8 or 32, got {state_bits}")
         defaults = dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay, maximize=maximize)
         self._state_bits, self._master = state_bits, master_weights
-        self._buckets: list = []  # lists of buckets, a list for each parameter group
+        self._buckets: list = []  # in the order of their groups
+        self._place: dict = {}    # parameter: (bucket, its place there, its dict in self.state)
+        self._plans: dict = {}    # id of a parameter group: _Plan
+        self._known = 0           # entries of self.state when it was looked through
         self._step_supports_amp_scaling = True
         super().__init__(params, defaults)
 
@@ -123,7 +143,6 @@ class FusedAdamW(torch.optim.Optimizer):
         except Exception:
             self.param_groups.pop()
             raise
-        self._buckets.append([])
 
     @staticmethod
     def _check_group(group) -> None:
@@ -137,7 +156,11 @@ class FusedAdamW(torch.optim.Optimizer):
             raise ValueError(f"betas must be at least 0 and below 1, got {(b1, b2)}")
         if not group["eps"] >= 0.0 or not group["weight_decay"] >= 0.0:
             raise ValueError("eps and weight_decay must not be negative")
-        for p in group["params"]:
+        FusedAdamW._check_params(group["params"])
+
+    @staticmethod
+    def _check_params(params) -> None:
+        for p in params:
             if not p.is_cuda:
                 raise RuntimeError("FusedAdamW runs on CUDA (sm_100) only; got a CPU parameter")
             if p.dtype not in DTYPES:
@@ -145,7 +168,7 @@ class FusedAdamW(torch.optim.Optimizer):
             if not _dense(p):
                 raise ValueError(f"a parameter of shape {tuple(p.shape)} and strides {p.stride()} does not fill its memory")
 
-    def _bucket(self, g: int, params) -> None:
+    def _add_state(self, g: int, params) -> None:
         """State for parameters of group g that have none, a bucket for each type
         and device."""
         kinds: dict = {}
@@ -153,10 +176,42 @@ class FusedAdamW(torch.optim.Optimizer):
             kinds.setdefault((p.dtype, p.device), []).append(p)
         for (dtype, dev), ps in kinds.items():
             with torch.cuda.device(dev):
-                b = _Bucket(ps, self._state_bits, self._master and dtype != torch.float32)
-            self._buckets[g].append(b)
+                b = _Bucket(ps, g, self._state_bits, self._master and dtype != torch.float32)
+            bisect.insort(self._buckets, b, key=lambda b: b.group)
             for i, p in enumerate(ps):
                 self.state[p] = {name: b.view(i, name) for name in b.flat}
+                self._place[p] = (b, i, self.state[p])
+        self._known = len(self.state)
+
+    def _look_through_state(self) -> None:
+        """Parameters whose state was taken out of self.state have none."""
+        self._place = {p: place for p, place in self._place.items() if self.state.get(p) is place[2]}
+        left = {id(b) for b, *_ in self._place.values()}
+        self._buckets = [b for b in self._buckets if id(b) in left]
+        self._plans.clear()
+        self._known = len(self.state)
+
+    def _plan(self, g: int, group) -> _Plan:
+        """The plan of group g: made anew when its list of parameters has changed, or
+        when one without state has got its first gradient."""
+        plan, params = self._plans.get(id(group)), group["params"]
+        if plan is not None and native().same_items(plan.params, params) and \
+                all(p.grad is None for p in plan.waiting):
+            return plan
+        new = [p for p in params if p not in self._place and p.grad is not None]
+        self._check_params(new)
+        self._add_state(g, new)
+        members: dict = {}  # of each bucket
+        for p in params:
+            if p in self._place:
+                b, i, _ = self._place[p]
+                members.setdefault(id(b), (b, []))[1].append(i)
+        plan = _Plan(group, list(params), [b.launch(m) for b, m in members.values()],
+                     [p for p in params if p not in self._place])
+        groups = {id(other) for other in self.param_groups}
+        self._plans = {k: v for k, v in self._plans.items() if k in groups}
+        self._plans[id(group)] = plan
+        return plan
 
     def step(self, closure=None, *, grad_scale=None, found_inf=None):
         """One step.  ``grad_scale`` and ``found_inf`` (fp32 values on the GPU, as
@@ -169,17 +224,15 @@ class FusedAdamW(torch.optim.Optimizer):
                 loss = closure()
         grad_scale = getattr(self, "grad_scale", None) if grad_scale is None else grad_scale
         found_inf = getattr(self, "found_inf", None) if found_inf is None else found_inf
+        if len(self.state) != self._known:
+            self._look_through_state()
         for g, group in enumerate(self.param_groups):
-            buckets = self._buckets[g]
-            if sum(len(b.params) for b in buckets) < len(group["params"]):
-                new = [p for p in group["params"] if p.grad is not None and p not in self.state]
-                if new:
-                    self._bucket(g, new)
+            launches = self._plan(g, group).launches
             lr, (b1, b2) = group["lr"], group["betas"]
             lr, lr_tensor = (0.0, lr) if isinstance(lr, Tensor) else (lr, None)
-            for b in buckets:
-                b.native.step(lr, lr_tensor, b1, b2, group["eps"], group["weight_decay"], group["maximize"], grad_scale,
-                              found_inf)
+            for launch in launches:
+                launch.step(lr, lr_tensor, b1, b2, group["eps"], group["weight_decay"], group["maximize"], grad_scale,
+                            found_inf)
         return loss
 
     def __reduce__(self):
@@ -188,27 +241,30 @@ class FusedAdamW(torch.optim.Optimizer):
     # ------------------------------------------------------------ state
     def flat_state(self) -> list:
         """The state's own buffers, a dict for each group and type of tensors in
-        the order they got their state: ``exp_avg`` and ``exp_avg_sq`` (32 bits), or
+        the order they got their state (each in the group that it had then): ``exp_avg`` and ``exp_avg_sq`` (32 bits), or
         ``exp_avg``, ``exp_avg_scale``, ``exp_avg_rms`` and ``exp_avg_rms_scale``
         (8 bits), and ``master_param``.  A tensor's part begins at a multiple of
         256 elements; what pads it is zero."""
-        return [b.flat for buckets in self._buckets for b in buckets]
+        return [b.flat for b in self._buckets]
 
     def state_dict(self) -> dict:
         """As torch's, hooks included: ``state[i]`` has ``step`` (a number; the host
         waits for the GPU) and the tensors of parameter i, ``param_groups`` the rest."""
         for hook in list(self._optimizer_state_dict_pre_hooks.values()):
             hook(self)
-        place, groups = {}, []
+        if len(self.state) != self._known:
+            self._look_through_state()
+        number, groups = {}, []
         for group in self.param_groups:
             packed = {k: v for k, v in group.items() if k != "params"}
-            packed["params"] = [place.setdefault(p, len(place)) for p in group["params"]]
+            packed["params"] = [number.setdefault(p, len(number)) for p in group["params"]]
             groups.append(packed)
+        steps = {id(b): b.steps() for b in self._buckets}
         state = {}
-        for buckets in self._buckets:
-            for b in buckets:
-                for i, (p, step) in enumerate(zip(b.params, b.steps())):
-                    state[place[p]] = {"step": step, **{name: b.view(i, name) for name in b.flat}}
+        for p, n in number.items():
+            if p in self._place:
+                b, i, _ = self._place[p]
+                state[n] = {"step": steps[id(b)][i], **{name: b.view(i, name) for name in b.flat}}
         found = {"state": state, "param_groups": groups}
         for hook in list(self._optimizer_state_dict_post_hooks.values()):
             got = hook(self, found)
@@ -252,16 +308,16 @@ class FusedAdamW(torch.optim.Optimizer):
             loads.append((found, options))
         # Nothing has changed so far, and nothing is refused from here on.
         self.state.clear()
-        self._buckets = [[] for _ in self.param_groups]
+        self._buckets, self._place, self._plans = [], {}, {}
         for g, (found, options) in enumerate(loads):
             self.param_groups[g].update(options)
-            self._bucket(g, [p for p, _ in found])
-            saved = dict(found)
-            for b in self._buckets[g]:
-                for i, p in enumerate(b.params):
-                    for name in b.flat:
-                        v = b.view(i, name)
-                        v.copy_(saved[p][name].reshape(v.shape))
-                b.ticks.copy_(torch.tensor([int(saved[p]["step"]) * c for p, c in zip(b.params, b.chunks)]))
+            self._add_state(g, [p for p, _ in found])
+        saved = dict(pair for found, _ in loads for pair in found)
+        for b in self._buckets:
+            for i, p in enumerate(b.params):
+                for name in b.flat:
+                    v = b.view(i, name)
+                    v.copy_(saved[p][name].reshape(v.shape))
+            b.ticks.copy_(torch.tensor([int(saved[p]["step"]) * c for p, c in zip(b.params, b.chunks)]))
         for hook in list(self._optimizer_load_state_dict_post_hooks.values()):
             hook(self)
