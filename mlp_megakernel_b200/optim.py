@@ -160,6 +160,8 @@ class FusedAdamW(torch.optim.Optimizer):
 
     @staticmethod
     def _check_params(params) -> None:
+        if len({id(p) for p in params}) != len(params):  # its steps would be one launch's, over the same values
+            raise ValueError("a parameter group holds a parameter twice")
         for p in params:
             if not p.is_cuda:
                 raise RuntimeError("FusedAdamW runs on CUDA (sm_100) only; got a CPU parameter")
@@ -196,11 +198,10 @@ class FusedAdamW(torch.optim.Optimizer):
         when one without state has got its first gradient."""
         plan, params = self._plans.get(id(group)), group["params"]
         if plan is not None and native().same_items(plan.params, params) and \
-                all(p.grad is None for p in plan.waiting):
+                not (plan.waiting and any(p.grad is not None for p in plan.waiting)):
             return plan
-        new = [p for p in params if p not in self._place and p.grad is not None]
-        self._check_params(new)
-        self._add_state(g, new)
+        self._check_params(params)
+        self._add_state(g, [p for p in params if p not in self._place and p.grad is not None])
         members: dict = {}  # of each bucket
         for p in params:
             if p in self._place:

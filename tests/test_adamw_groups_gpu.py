@@ -146,3 +146,19 @@ def test_a_parameter_that_it_does_not_take_is_refused_in_a_changed_group():
             opt.step()
         opt.param_groups[0]["params"].pop()
     assert torch.equal(p[0], kept)
+
+
+def test_a_parameter_given_twice_is_refused():
+    """Its two steps would be one launch's, over the same values."""
+    p, = make([300])
+    with pytest.raises(ValueError):
+        FusedAdamW([p, p])
+    opt = FusedAdamW([p])
+    with pytest.raises(ValueError):
+        opt.add_param_group({"params": [p]})
+    opt.step()
+    opt.param_groups[0]["params"].append(p)
+    kept = p.detach().clone()
+    with pytest.raises(ValueError):
+        opt.step()
+    assert torch.equal(p, kept)

@@ -1,5 +1,5 @@
-"""What FusedAdamW's load_state_dict and hooks do before there is any state (no
-GPU needed)."""
+"""What FusedAdamW refuses, loads and calls before there is any state (no GPU
+needed)."""
 import pytest
 import torch
 from torch._subclasses.fake_tensor import FakeTensorMode
@@ -35,3 +35,9 @@ def test_hooks_are_called(opt):
     opt.load_state_dict(saved)
     assert said == ["pre", "post", "load", "loaded"] and opt.param_groups[0]["lr"] == 0.5
     assert saved["param_groups"][0]["lr"] == 1e-3  # the caller's dict is not changed
+
+
+def test_duplicates_are_refused(opt):
+    p = opt.param_groups[0]["params"][0]
+    with pytest.raises(ValueError):
+        m.FusedAdamW([p, p])
