@@ -52,40 +52,86 @@ class ExpertPlan(NamedTuple):
 # ------------------------------------------------------------ torch.ops.mlpk
 def _require_cuda(*ts):
     for t in ts:
-        if t is not None and not t.is_cuda:
+        if isinstance(t, Tensor) and not t.is_cuda:
             raise RuntimeError("the expert operators run on CUDA (sm_100) only; got a CPU tensor")
+
+
+def _check_ids(ids, num_experts) -> None:
+    if not isinstance(ids, Tensor) or ids.dim() != 2:
+        raise ValueError("ids must be a 2-D tensor [tokens, choices]")
+    if ids.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"ids must be int32 or int64, got {ids.dtype}")
+    if not 1 <= num_experts <= _lib.EXPERT_MAX:
+        raise ValueError(f"num_experts must be 1 to {_lib.EXPERT_MAX}, got {num_experts}")
+    if ids.shape[1] < 1 or ids.numel() > 2 ** 31 - 1:
+        raise ValueError(f"ids must have at least one choice a token and at most 2^31 - 1 slots, got {tuple(ids.shape)}")
+
+
+def _check_rows(what: str, t, of_slots: bool, row_of, offsets) -> None:
+    """A tensor with a row for each slot, or each token, of a plan."""
+    if row_of.dim() != 2 or row_of.dtype != torch.int32 or row_of.shape[1] < 1 or offsets.dim() != 1 or \
+            offsets.dtype != torch.int32 or offsets.shape[0] < 2 or not offsets.is_contiguous():
+        raise ValueError("plan must be what expert_sort returned")
+    rows = row_of.numel() if of_slots else row_of.shape[0]
+    if not isinstance(t, Tensor) or t.dim() != 2 or t.shape[0] != rows or t.shape[1] < 1:
+        raise ValueError(f"{what} must be a 2-D tensor of {rows} rows")
+    if t.dtype not in DTYPES:
+        raise TypeError(f"{what} must be fp16, bf16 or fp32, got {t.dtype}")
+    if t.device != row_of.device or t.device != offsets.device:
+        raise ValueError(f"{what} is on {t.device}, the plan on {row_of.device} and {offsets.device}")
+
+
+def _check_combine(y, weights, row_of, offsets) -> None:
+    _check_rows("y", y, True, row_of, offsets)
+    if weights is not None and (weights.shape != row_of.shape or weights.device != y.device
+                                or (weights.dtype != y.dtype and weights.dtype != torch.float32)):
+        raise ValueError(f"weights must be a {tuple(row_of.shape)} tensor of {y.dtype} or float32 on {y.device}")
+
+
+def _check_combine_bwd(grad_out, y, weights, row_of, offsets, want_dw) -> None:
+    _check_combine(y, weights, row_of, offsets)
+    if grad_out.shape != (row_of.shape[0], y.shape[1]) or grad_out.dtype != y.dtype or grad_out.device != y.device:
+        raise ValueError(f"grad_out must be a {(row_of.shape[0], y.shape[1])} {y.dtype} tensor on {y.device}")
+    if want_dw and weights is None:
+        raise ValueError("there are no weights to have a gradient")
 
 
 @torch.library.custom_op("mlpk::expert_sort", mutates_args=())
 def _sort_op(ids: Tensor, num_experts: int) -> list[Tensor]:
     _require_cuda(ids)
+    _check_ids(ids, num_experts)
     return list(native().sort_ids(ids, num_experts))
 
 
 @_sort_op.register_fake
 def _sort_fake(ids, num_experts):
+    _check_ids(ids, num_experts)
     return [ids.new_empty(ids.shape, dtype=torch.int32), ids.new_empty((num_experts + 1,), dtype=torch.int32)]
 
 
 @torch.library.custom_op("mlpk::expert_dispatch", mutates_args=())
 def _dispatch_op(x: Tensor, row_of: Tensor, offsets: Tensor) -> Tensor:
     _require_cuda(x, row_of, offsets)
+    _check_rows("x", x, False, row_of, offsets)
     return native().dispatch_rows(x, row_of, offsets)
 
 
 @_dispatch_op.register_fake
 def _dispatch_fake(x, row_of, offsets):
+    _check_rows("x", x, False, row_of, offsets)
     return x.new_empty((row_of.shape[0] * row_of.shape[1], x.shape[1]))
 
 
 @torch.library.custom_op("mlpk::expert_combine", mutates_args=())
 def _combine_op(y: Tensor, weights: Optional[Tensor], row_of: Tensor, offsets: Tensor) -> Tensor:
     _require_cuda(y, weights, row_of, offsets)
+    _check_combine(y, weights, row_of, offsets)
     return native().combine_rows(y, weights, row_of, offsets)
 
 
 @_combine_op.register_fake
 def _combine_fake(y, weights, row_of, offsets):
+    _check_combine(y, weights, row_of, offsets)
     return y.new_empty((row_of.shape[0], y.shape[1]))
 
 
@@ -94,12 +140,14 @@ def _combine_bwd_op(grad_out: Tensor, y: Tensor, weights: Optional[Tensor], row_
                     want_dy: bool, want_dw: bool) -> list[Tensor]:
     """[dy] and / or [dw], as wanted."""
     _require_cuda(grad_out, y, weights, row_of, offsets)
+    _check_combine_bwd(grad_out, y, weights, row_of, offsets, want_dw)
     dy, dw = native().combine_backward(grad_out, y, weights, row_of, offsets, want_dy, want_dw)
     return ([dy] if want_dy else []) + ([dw] if want_dw else [])
 
 
 @_combine_bwd_op.register_fake
 def _combine_bwd_fake(grad_out, y, weights, row_of, offsets, want_dy, want_dw):
+    _check_combine_bwd(grad_out, y, weights, row_of, offsets, want_dw)
     return ([y.new_empty(y.shape)] if want_dy else []) + ([weights.new_empty(weights.shape)] if want_dw else [])
 
 
@@ -153,28 +201,9 @@ def expert_sort(ids: Tensor, num_experts: int) -> ExpertPlan:
         if got is not None:
             return ExpertPlan(*got)
     _refuse_transforms("expert_sort", ids)
-    if not isinstance(ids, Tensor) or ids.dim() != 2:
-        raise ValueError("ids must be a 2-D tensor [tokens, choices]")
     _require_cuda(ids)
-    if ids.dtype not in (torch.int32, torch.int64):
-        raise TypeError(f"ids must be int32 or int64, got {ids.dtype}")
-    if not 1 <= num_experts <= _lib.EXPERT_MAX:
-        raise ValueError(f"num_experts must be 1 to {_lib.EXPERT_MAX}, got {num_experts}")
-    if ids.shape[1] < 1 or ids.numel() > 2 ** 31 - 1:
-        raise ValueError(f"ids must have at least one choice a token and at most 2^31 - 1 slots, got {tuple(ids.shape)}")
+    _check_ids(ids, num_experts)
     return ExpertPlan(*torch.ops.mlpk.expert_sort(ids, num_experts))
-
-
-def _check_rows(what: str, t: Tensor, rows: int, plan: ExpertPlan) -> None:
-    if plan.row_of.dtype != torch.int32 or plan.offsets.dtype != torch.int32 or not plan.offsets.is_contiguous():
-        raise ValueError("plan must be what expert_sort returned")
-    if not isinstance(t, Tensor) or t.dim() != 2 or t.shape[0] != rows or t.shape[1] < 1:
-        raise ValueError(f"{what} must be a 2-D tensor of {rows} rows")
-    _require_cuda(t)
-    if t.dtype not in DTYPES:
-        raise TypeError(f"{what} must be fp16, bf16 or fp32, got {t.dtype}")
-    if t.device != plan.row_of.device:
-        raise ValueError(f"{what} is on {t.device}, the plan on {plan.row_of.device}")
 
 
 def expert_dispatch(x: Tensor, plan: ExpertPlan) -> Tensor:
@@ -185,7 +214,8 @@ def expert_dispatch(x: Tensor, plan: ExpertPlan) -> Tensor:
         if got is not None:
             return got
     _refuse_transforms("expert_dispatch", x, *plan)
-    _check_rows("x", x, plan.row_of.shape[0], plan)
+    _require_cuda(x, *plan)
+    _check_rows("x", x, False, *plan)
     if _needs_grad(x):
         return _DispatchFn.apply(x, *plan)
     return torch.ops.mlpk.expert_dispatch(x, *plan)
@@ -201,10 +231,8 @@ def expert_combine(y: Tensor, weights: Optional[Tensor], plan: ExpertPlan) -> Te
         if got is not None:
             return got
     _refuse_transforms("expert_combine", y, weights, *plan)
-    _check_rows("y", y, plan.row_of.numel(), plan)
-    if weights is not None and (weights.shape != plan.row_of.shape or weights.device != y.device
-                                or (weights.dtype != y.dtype and weights.dtype != torch.float32)):
-        raise ValueError(f"weights must be a {tuple(plan.row_of.shape)} tensor of {y.dtype} or float32 on {y.device}")
+    _require_cuda(y, weights, *plan)
+    _check_combine(y, weights, *plan)
     if _needs_grad(y, weights):
         return _CombineFn.apply(y, weights, *plan)
     return torch.ops.mlpk.expert_combine(y, weights, *plan)

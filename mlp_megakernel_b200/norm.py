@@ -48,11 +48,10 @@ def _refuse_transforms(name: str, *ts) -> None:
             raise RuntimeError(f"{name} has no forward-mode derivative")
 
 
-def _check(x, weight, residual, eps):
+def _check_args(x, weight, residual, eps):
+    """Types and shapes; tensors of any device, the same for all."""
     if not isinstance(x, Tensor) or x.dim() < 1:
         raise ValueError("x must be a tensor [..., width]")
-    if not x.is_cuda:
-        raise RuntimeError("fused_rms_norm runs on CUDA (sm_100) only; got a CPU tensor")
     if x.dtype not in DTYPES:
         raise TypeError(f"fused_rms_norm takes fp16, bf16 or fp32; got {x.dtype}")
     width = x.shape[-1]
@@ -61,10 +60,40 @@ def _check(x, weight, residual, eps):
     if weight is not None and (weight.shape != (width,) or weight.device != x.device
                                or (weight.dtype != x.dtype and weight.dtype != torch.float32)):
         raise ValueError(f"weight must be a [{width}] tensor of {x.dtype} or float32 on {x.device}")
-    if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype or residual.device != x.device):
-        raise ValueError(f"residual must be a {tuple(x.shape)} {x.dtype} tensor on {x.device}")
+    _check_like("residual", residual, x)
     if not eps >= 0.0:
         raise ValueError(f"eps must not be negative, got {eps}")
+
+
+def _check_like(what, t, x):
+    if t is not None and (t.shape != x.shape or t.dtype != x.dtype or t.device != x.device):
+        raise ValueError(f"{what} must be a {tuple(x.shape)} {x.dtype} tensor on {x.device}")
+
+
+def _check_cuda(x):
+    if isinstance(x, Tensor) and not x.is_cuda:
+        raise RuntimeError("fused_rms_norm runs on CUDA (sm_100) only; got a CPU tensor")
+
+
+def _check(x, weight, residual, eps):
+    _check_cuda(x)
+    _check_args(x, weight, residual, eps)
+
+
+def _check_bwd(x, residual, weight, rstd, grad_y, grad_h, want_dw):
+    _check_args(x, weight, residual, 0.0)
+    _check_like("grad_y", grad_y, x)
+    _check_like("grad_h", grad_h, x)
+    rows = x.numel() // x.shape[-1]
+    if rstd.shape != (rows,) or rstd.dtype != torch.float32 or rstd.device != x.device or not rstd.is_contiguous():
+        raise ValueError(f"rstd must be a contiguous [{rows}] float32 tensor on {x.device}")
+    if want_dw and weight is None:
+        raise ValueError("there is no weight to have a gradient")
+
+
+def _check_group(group):
+    if group not in (0, _lib.NORM_GROUP):
+        raise ValueError(f"group must be 0 (the row) or {_lib.NORM_GROUP}, got {group}")
 
 
 # ------------------------------------------------------------ torch.ops.mlpk
@@ -78,6 +107,7 @@ def rms_norm(x: Tensor, weight: Optional[Tensor], residual: Optional[Tensor], ep
 
 @rms_norm.register_fake
 def _rms_norm_fake(x, weight, residual, eps):
+    _check_args(x, weight, residual, eps)
     rstd = x.new_empty((x.numel() // x.shape[-1],), dtype=torch.float32)
     return [x.new_empty(x.shape), rstd] + ([] if residual is None else [x.new_empty(x.shape)])
 
@@ -86,12 +116,15 @@ def _rms_norm_fake(x, weight, residual, eps):
 def rms_norm_bwd(x: Tensor, residual: Optional[Tensor], weight: Optional[Tensor], rstd: Tensor, grad_y: Tensor,
                  grad_h: Optional[Tensor], want_dw: bool) -> list[Tensor]:
     """[dx], and dw if wanted."""
+    _check_cuda(x)
+    _check_bwd(x, residual, weight, rstd, grad_y, grad_h, want_dw)
     dx, dw = native().norm_backward(x, residual, weight, rstd, grad_y, grad_h, want_dw)
     return [dx, dw] if want_dw else [dx]
 
 
 @rms_norm_bwd.register_fake
 def _rms_norm_bwd_fake(x, residual, weight, rstd, grad_y, grad_h, want_dw):
+    _check_bwd(x, residual, weight, rstd, grad_y, grad_h, want_dw)
     return [x.new_empty(x.shape)] + ([weight.new_empty(weight.shape)] if want_dw else [])
 
 
@@ -100,11 +133,14 @@ def rms_norm_fp8(x: Tensor, weight: Optional[Tensor], residual: Optional[Tensor]
                  group: int) -> list[Tensor]:
     """[q, scale], and h with a residual."""
     _check(x, weight, residual, eps)
+    _check_group(group)
     return list(native().norm_fp8(x, weight, residual, eps, group))
 
 
 @rms_norm_fp8.register_fake
 def _rms_norm_fp8_fake(x, weight, residual, eps, group):
+    _check_args(x, weight, residual, eps)
+    _check_group(group)
     groups = -(-x.shape[-1] // group) if group else 1
     return [x.new_empty(x.shape, dtype=torch.float8_e4m3fn),
             x.new_empty((*x.shape[:-1], groups), dtype=torch.float32)] + \
@@ -182,8 +218,7 @@ def fused_rms_norm_fp8(x: Tensor, weight: Optional[Tensor] = None, *, residual: 
             return got
     _refuse_transforms("fused_rms_norm_fp8", x, weight, residual)
     _check(x, weight, residual, eps)
-    if group not in (0, _lib.NORM_GROUP):
-        raise ValueError(f"group must be 0 (the row) or {_lib.NORM_GROUP}, got {group}")
+    _check_group(group)
     if _needs_grad(x, weight, residual):
         raise RuntimeError("fused_rms_norm_fp8 has no gradient: call it under torch.no_grad()")
     return tuple(torch.ops.mlpk.rms_norm_fp8(x, weight, residual, eps, group))
