@@ -282,7 +282,9 @@ int64_t mlpk_expert_sort_workspace_size(int64_t slots, int experts);
 int mlpk_expert_sort(int64_t slots, int experts, const void* ids, int id_bytes, int32_t* row_of, int32_t* offsets,
                      void* workspace, int64_t workspace_bytes, mlpk_stream_t stream);
 /* Slot t * top + k is token t's k-th choice; kept points to offsets[experts]
- * (device memory).  xs[row_of[t, k]] = x[t]; rows of dropped slots are zero.
+ * (device memory).  xs[row_of[t, k]] = x[t]; rows of dropped slots are zero.  (In
+ * all three calls a place outside [0, tokens * top), which no sort gives, is no
+ * row: nothing is read or written there.)
  * x: [tokens][width], xs: [tokens * top][width] of dtype. */
 int mlpk_expert_dispatch(int64_t tokens, int top, int width, int dtype, const void* x, const int32_t* row_of,
                          const int32_t* kept, void* xs, mlpk_stream_t stream);

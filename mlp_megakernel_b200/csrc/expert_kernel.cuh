@@ -10,7 +10,8 @@
 //     dy[row_of[t,k]] = w[t,k] G[t] (zeros in the dropped slots' rows)
 //     dw[t,k] = sum_j G[t,j] y[row_of[t,k],j]
 //   backward of the dispatch: the combine of dL/dxs with weights of 1.
-// Sums over k and over columns are fp32 in a fixed order.
+// Sums over k and over columns are fp32 in a fixed order.  A place outside the
+// T K rows, which no sort gives, is no row: nothing is read or written there.
 #pragma once
 #include <cooperative_groups.h>
 
@@ -316,6 +317,11 @@ struct TokenSpan {
   __device__ int64_t token(int n) const { return first + static_cast<int64_t>(n) * blockDim.y; }
 };
 
+// The rows kept of `slots`.
+__device__ __forceinline__ unsigned rows_kept_of(const int* kept, unsigned slots) {
+  return min(static_cast<unsigned>(max(*kept, 0)), slots);
+}
+
 // Rows are moved as words of U (16, 8, 4 or 2 bytes: the widest that divides
 // a row), NW a thread and token.
 template <class U, int NT, int NW>
@@ -334,14 +340,14 @@ __global__ void __launch_bounds__(kRowThreads)
     for (int i = 0; i < NW; ++i)
       if (t < tokens && c0 + i * tpr < words) v[n][i] = x[t * words + c0 + i * tpr];
   }
-  const int rows_kept = *kept;
+  const unsigned slots = static_cast<unsigned>(tokens) * top, rows_kept = rows_kept_of(kept, slots);
   for (int k = 0; k < top; ++k) {
-    int row[NT];
+    unsigned row[NT];
 #pragma unroll
-    for (int n = 0; n < NT; ++n) row[n] = span.token(n) < tokens ? row_of[span.token(n) * top + k] : -1;
+    for (int n = 0; n < NT; ++n) row[n] = span.token(n) < tokens ? row_of[span.token(n) * top + k] : slots;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      if (row[n] < 0) continue;
+      if (row[n] >= slots) continue;
       U* to = xs + static_cast<int64_t>(row[n]) * words + c0;
 #pragma unroll
       for (int i = 0; i < NW; ++i)
@@ -363,15 +369,15 @@ __global__ void __launch_bounds__(kRowThreads, VEC < kVecOf<T> ? 4 : GROUP == 2 
   if (t >= tokens) return;
   const int nvec = width / VEC;
   const int c0 = blockIdx.y * tpr * NW + span.lane;
-  const int rows_kept = *kept;
+  const unsigned rows_kept = rows_kept_of(kept, static_cast<unsigned>(tokens) * top);
   float acc[NW][VEC];
 #pragma unroll
   for (int i = 0; i < NW; ++i)
 #pragma unroll
     for (int e = 0; e < VEC; ++e) acc[i][e] = 0.0f;
   for (int k0 = 0; k0 < top; k0 += GROUP) {
-    // A dropped slot's row is not read (it may hold anything), nor its weight.
-    int row[GROUP];
+    // A dropped slot's row is not read (it may hold anything), its weight not used.
+    unsigned row[GROUP];
     float wk[GROUP];
     Raw<T, VEC> v[GROUP][NW];
 #pragma unroll
@@ -418,21 +424,21 @@ __global__ void __launch_bounds__(kRowThreads, VEC < kVecOf<T> ? 4 : GROUP == 2 
   const int64_t t = span.first;
   const bool live = t < tokens;  // the others take part in the shuffles and barriers
   const int nvec = width / VEC;
-  const int rows_kept = *kept;
+  const unsigned slots = static_cast<unsigned>(tokens) * top, rows_kept = rows_kept_of(kept, slots);
   int half = 0;
   for (int k0 = 0; k0 < top; k0 += GROUP, half ^= 1) {
-    int row[GROUP];  // rows_kept and above: not kept; below 0: no such slot
+    unsigned row[GROUP];  // rows_kept and above: not kept; slots and above: no such slot
     int64_t row_at[U > 1 ? GROUP : 1];  // found once where it is used often
     float wk[GROUP], dot[GROUP];
 #pragma unroll
     for (int k = 0; k < GROUP; ++k) {
       const bool slot = live && k0 + k < top;
-      row[k] = slot ? row_of[t * top + k0 + k] : -1;
+      row[k] = slot ? row_of[t * top + k0 + k] : slots;
       wk[k] = slot && w ? to_float(w[t * top + k0 + k]) : 1.0f;
       dot[k] = 0.0f;
       if constexpr (U > 1) row_at[k] = static_cast<int64_t>(row[k]) * width;
     }
-    auto on = [&](int k) { return row[k] >= 0 && row[k] < rows_kept; };  // else y is not read and the gradients are zero
+    auto on = [&](int k) { return row[k] < rows_kept; };  // else y is not read and the gradients are zero
     auto at = [&](int k) -> int64_t {
       if constexpr (U > 1) return row_at[k];
       return static_cast<int64_t>(row[k]) * width;
@@ -460,7 +466,7 @@ __global__ void __launch_bounds__(kRowThreads, VEC < kVecOf<T> ? 4 : GROUP == 2 
 #pragma unroll
             for (int e = 0; e < VEC; ++e) dot[k] += g[e] * f[e];
           }
-          if (dy && row[k] >= 0) {
+          if (dy && row[k] < slots) {
 #pragma unroll
             for (int e = 0; e < VEC; ++e) f[e] = on(k) ? wk[k] * g[e] : 0.0f;
             store_vec<T, VEC>(dy + at(k) + (v + i * tpr) * VEC, f);
