@@ -27,7 +27,7 @@ SOURCES = {
                     "wn_kernel.cuh", "stream_kernel.cuh", "wgrad_kernel.cuh", "peer_kernel.cuh", "cast_kernel.cuh"],
     **{f"norm_{part}.cu": ["host.cuh", "pdl.cuh", "vec.cuh", "norm_kernel.cuh", "norm_launch.cuh"]
        for part in ("api", "f16", "bf16", "f32")},
-    "expert_api.cu": ["host.cuh", "pdl.cuh", "vec.cuh", "expert_kernel.cuh"],
+    "expert_api.cu": ["host.cuh", "pdl.cuh", "vec.cuh", "expert_plan.cuh", "expert_kernel.cuh"],
     "adamw_api.cu": ["host.cuh", "pdl.cuh", "vec.cuh", "adamw_kernel.cuh"],
 }
 

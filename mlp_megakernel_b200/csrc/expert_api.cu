@@ -5,14 +5,13 @@
 #include <type_traits>
 
 #include "expert_kernel.cuh"
+#include "expert_plan.cuh"
 #include "host.cuh"
 
 namespace {
 
 using namespace mlpk;
 using namespace mlpk::host;
-
-int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 int check_rows(int64_t tokens, int top, int width, int dtype) {
   if (tokens < 0 || top < 1 || width < 1 || tokens > 0x7fffffff / top) return MLPK_ERR_SHAPE;
@@ -21,32 +20,12 @@ int check_rows(int64_t tokens, int top, int width, int dtype) {
   return MLPK_OK;
 }
 
-// Thread blocks of a sort and slots of a warp: a cluster's blocks up to 16,
-// above that (two launches) at most one an SM.
-struct SortPlan {
-  int blocks;
-  int64_t part;
-  bool cluster() const { return blocks <= 16; }
-};
-SortPlan sort_plan(int64_t slots, int sm_count) {
-  SortPlan p;
-  const int64_t want = ceil_div(slots, kSortBlockSlots);
-  if (want <= 16) {
-    p.blocks = 1;
-    while (p.blocks < want) p.blocks *= 2;
-  } else {
-    p.blocks = static_cast<int>(std::min<int64_t>(want, sm_count));
-  }
-  p.part = std::max<int64_t>(ceil_div(ceil_div(slots, static_cast<int64_t>(p.blocks) * kSortWarps), 32), 1) * 32;
-  return p;
-}
-
 template <class I>
 int sort_slots(int64_t slots, int experts, const void* ids_, int* row_of, int* offsets, int* hist, int dev,
                const SortPlan& p, cudaStream_t st) {
   const I* ids = static_cast<const I*>(ids_);
   const size_t smem = sizeof(int) * (kSortWarps + static_cast<size_t>(kSortWarps + 1) * (experts + 1));
-  if (!p.cluster()) {
+  if (!p.cluster) {
     const auto rank = p.part <= 32 * kSortGroups ? expert_rank_kernel<I, true> : expert_rank_kernel<I, false>;
     if (blocks_per_sm(reinterpret_cast<const void*>(rank), kSortThreads, smem, dev) == 0) return MLPK_ERR_CUDA;
     const int rc =
@@ -142,10 +121,10 @@ extern "C" {
 
 int64_t mlpk_expert_sort_workspace_size(int64_t slots, int experts) {
   if (slots < 0 || slots > 0x7fffffff || experts < 1 || experts > kExpertMax) return -1;
-  if (slots <= 16 * kSortBlockSlots) return 0;
+  if (sort_plan(slots, 1).cluster) return 0;  // on every device
   DevInfo di;
   if (current_device_info(&di, nullptr)) return -1;
-  return sort_plan(slots, di.sm_count).blocks * (experts + 1) * static_cast<int64_t>(sizeof(int));
+  return sort_plan(slots, di.sm_count).workspace(experts);
 }
 
 int mlpk_expert_sort(int64_t slots, int experts, const void* ids, int id_bytes, int32_t* row_of, int32_t* offsets,
@@ -159,9 +138,9 @@ int mlpk_expert_sort(int64_t slots, int experts, const void* ids, int id_bytes, 
   int rc = current_device_info(&di, &dev);
   if (rc) return rc;
   const SortPlan p = sort_plan(slots, di.sm_count);
-  if (!p.cluster()) {
+  if (!p.cluster) {
     if (!workspace) return MLPK_ERR_NULL;
-    if (workspace_bytes < p.blocks * (experts + 1) * static_cast<int64_t>(sizeof(int))) return MLPK_ERR_SCRATCH;
+    if (workspace_bytes < p.workspace(experts)) return MLPK_ERR_SCRATCH;
   }
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   int* hist = static_cast<int*>(workspace);

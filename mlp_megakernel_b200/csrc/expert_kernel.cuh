@@ -15,6 +15,7 @@
 #pragma once
 #include <cooperative_groups.h>
 
+#include "expert_plan.cuh"
 #include "pdl.cuh"
 #include "vec.cuh"
 
@@ -37,11 +38,6 @@ namespace mlpk {
 // instructions for 32 slots.)  Up to 128 slots a warp, ids and ranks stay in
 // registers; 512 were held once, and the unrolled code made the smallest sorts
 // slower (16 slots: 4.6 us).
-constexpr int kSortThreads = 1024;
-constexpr int kSortWarps = kSortThreads / 32;
-constexpr int kExpertMax = 1024;
-constexpr int kSortGroups = 4;       // groups of 32 slots of a warp that registers hold
-constexpr int kSortBlockSlots = 4096;
 constexpr int kSortRounds = (kExpertMax + kSortThreads) / kSortThreads;  // of kSortThreads ids
 
 template <class I>
