@@ -90,7 +90,8 @@ __device__ __forceinline__ float norm_row_max(float v, int tpr, float* red, int 
 
 // A thread's vectors of the rows of its block's row group.  KIND: kRagged; kFull
 // where a block has one row and every thread all its NV vectors (nothing to ask
-// for each vector: a fifth of the instructions); else kPart.
+// for each vector: a fifth of the instructions); else kPart.  Where it lies is
+// arithmetic of no device, which tests/test_norm_copies.py goes over.
 enum RowKind { kPart, kFull, kRagged };
 template <class T, int NV, int KIND>
 struct RowSpan {
@@ -101,25 +102,28 @@ struct RowSpan {
   int width, tpr, lane, shift, nvec, step;  // step: elements from a vector to the thread's next
 
   // first_row: any row of the row group
-  __device__ RowSpan(int64_t rows, int width_, int tpr_, int lane_, int64_t first_row)
+  __host__ __device__ RowSpan(int64_t rows, int width_, int tpr_, int lane_, int64_t first_row)
       : total(rows * width_), width(width_), tpr(tpr_), lane(lane_) {
     shift = RAGGED ? static_cast<int>((first_row % VEC) * (width % VEC) % VEC) : 0;
     nvec = (width + shift + VEC - 1) / VEC;
     step = tpr * VEC;
     end = total + col(0);
   }
-  __device__ bool has(int i) const { return KIND == kFull || i * tpr + lane < nvec; }
-  __device__ int col(int i) const { return (i * tpr + lane) * VEC - shift; }  // of element 0; may be below 0
+  __host__ __device__ bool has(int i) const { return KIND == kFull || i * tpr + lane < nvec; }
+  __host__ __device__ int col(int i) const { return (i * tpr + lane) * VEC - shift; }  // of element 0; may be below 0
   // The thread's first element of a row, and element 0 of its vector i behind
   // it: multiples of VEC.
-  __device__ int64_t begin(int64_t row) const { return row * width + col(0); }
-  __device__ int64_t at(int64_t begin, int i) const { return begin + i * step; }
-  __device__ bool owns(int i, int e) const {
+  __host__ __device__ int64_t begin(int64_t row) const { return row * width + col(0); }
+  __host__ __device__ int64_t at(int64_t begin, int i) const { return begin + i * step; }
+  __host__ __device__ bool owns(int i, int e) const {
     return !RAGGED || static_cast<unsigned>(col(i) + e) < static_cast<unsigned>(width);
   }
-  __device__ bool whole(int i) const { return !RAGGED || (col(i) >= 0 && col(i) + VEC <= width); }
+  __host__ __device__ bool whole(int i) const { return !RAGGED || (col(i) >= 0 && col(i) + VEC <= width); }
+  // Whether there is such a row: only then do its vectors lie inside the tensor
+  // (a ragged row's first one alone says nothing about the others).
+  __host__ __device__ bool exists(int64_t begin) const { return begin < end; }
   // Bytes of the vector that lie inside the tensor.
-  __device__ int bytes(int64_t begin, int i) const {
+  __host__ __device__ int bytes(int64_t begin, int i) const {
     if (!RAGGED) return 16;
     const int64_t left = total - at(begin, i);
     return left >= VEC ? 16 : static_cast<int>(left) * static_cast<int>(sizeof(T));
@@ -230,7 +234,7 @@ __global__ void __launch_bounds__(MAXT, !FP8 ? 0 : MAXT == 256 ? (KIND == kRagge
   const int stage_slots = streams * NV * blockDim.x;  // `stage` counts them
   auto slot = [&](int stage, int stream, int i) { return slots + (stage + (stream * NV + i) * blockDim.x); };
   auto fetch = [&](int64_t begin, int stage) {
-    if (begin < span.end) {
+    if (span.exists(begin)) {
 #pragma unroll
       for (int i = 0; i < NV; ++i)
         if (span.has(i)) {
@@ -431,7 +435,7 @@ __global__ void __launch_bounds__(MAXT, MAXT == 256 ? 2 : 1) rms_norm_bwd_kernel
   const int stage_slots = streams * NV * blockDim.x;  // `stage` counts them
   auto slot = [&](int stage, int stream, int i) { return slots + (stage + (stream * NV + i) * blockDim.x); };
   auto fetch = [&](int64_t begin, int stage) {
-    if (begin < span.end) {
+    if (span.exists(begin)) {
 #pragma unroll
       for (int i = 0; i < NV; ++i)
         if (span.has(i)) {
