@@ -119,13 +119,29 @@ def _torch_flags() -> list:
                     "-Wl,-rpath,$ORIGIN"]
 
 
+def built_for() -> str:
+    """What the binding is compiled against: another torch or Python may have other
+    layouts under the same names."""
+    import torch
+
+    return f"mlpk_torch for torch {torch.__version__}, Python {sys.version_info[0]}.{sys.version_info[1]}"
+
+
+def _binding_stale() -> bool:
+    if _newer([os.path.join(CSRC, BINDING_SRC), os.path.join(ROOT, "include", "mlpk.h"), os.path.abspath(__file__)],
+              BINDING):
+        return True
+    with open(BINDING, "rb") as f:
+        return built_for().encode() + b"\0" not in f.read()
+
+
 def build_binding(force: bool = False, verbose: bool = False) -> str:
     """Compile the torch binding of the block operators (host code only) if it is
-    missing or older than its source; return its path."""
-    source = os.path.join(CSRC, BINDING_SRC)
-    if force or _newer([source, os.path.join(ROOT, "include", "mlpk.h"), os.path.abspath(__file__)], BINDING):
-        _run([os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-o",
-              BINDING + ".tmp", source, *_torch_flags()], verbose)
+    missing, older than its source or of another torch; return its path."""
+    if force or _binding_stale():
+        _run([os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+              f'-DMLPK_BUILT_FOR="{built_for()}"', "-o", BINDING + ".tmp", os.path.join(CSRC, BINDING_SRC),
+              *_torch_flags()], verbose)
         os.replace(BINDING + ".tmp", BINDING)
     return BINDING
 

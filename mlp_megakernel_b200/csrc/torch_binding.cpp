@@ -498,7 +498,12 @@ class AdamwBucket {
 
 }  // namespace
 
+#ifndef MLPK_BUILT_FOR  // the versions of torch and Python, from build.py
+#define MLPK_BUILT_FOR "unknown"
+#endif
+
 PYBIND11_MODULE(mlpk_torch, m) {
+  m.attr("built_for") = MLPK_BUILT_FOR;
   py::register_exception_translator([](std::exception_ptr p) {
     try {
       if (p) std::rethrow_exception(p);
