@@ -73,6 +73,12 @@ except ImportError:  # no FakeTensor support: every tensor is real
         return False
 
 
+def _observed() -> bool:
+    """Whether a dispatch mode or a tracer is to see the operators (outside of
+    torch.compile)."""
+    return torch._C._len_torch_dispatch_stack() > 0 or torch._C._get_tracing_state() is not None
+
+
 def _eager_fwd(x: torch.Tensor, weights, out: torch.Tensor) -> None:
     """The fp16 forward straight through the C ABI (no operator dispatch):
     the per-call cost of an eager call is the host work here, so it is kept to
@@ -98,9 +104,9 @@ def fused_mlp_fwd(x: torch.Tensor, *weights: torch.Tensor, out: torch.Tensor = N
     (kernel.py:110, kernel.py:117).  Like the reference (kernel.py:136) the
     result is a new tensor unless ``out`` (contiguous, ``[M, out_features]``,
     x's dtype and device) is given, which lets a serving loop reuse one buffer.
-    Under torch.compile it is the custom operator ``torch.ops.mlpk.fwd``
-    (``fwd_out`` with ``out``), traced as one operator; eager fp16 calls go
-    straight to the C ABI.
+    Under torch.compile, tracers and dispatch modes it is the custom operator
+    ``torch.ops.mlpk.fwd`` (``fwd_out`` with ``out``), traced as one operator;
+    other eager fp16 calls go straight to the C ABI.
     """
     dims = _check_operands(x, weights)
     M = x.shape[0]
@@ -108,7 +114,7 @@ def fused_mlp_fwd(x: torch.Tensor, *weights: torch.Tensor, out: torch.Tensor = N
                             or not out.is_contiguous()):
         raise ValueError("out must be a contiguous, 16-byte aligned "
                          f"[{M}, {dims[-1]}] {x.dtype} tensor on {x.device}")
-    if torch.compiler.is_compiling() or x.dtype != torch.float16 or _is_fake(x):
+    if torch.compiler.is_compiling() or x.dtype != torch.float16 or _observed() or _is_fake(x):
         if out is None:
             return torch.ops.mlpk.fwd(x, list(weights))
         torch.ops.mlpk.fwd_out(x, list(weights), out)
