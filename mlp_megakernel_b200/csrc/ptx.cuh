@@ -21,7 +21,8 @@ namespace mlpk {
 
 // Device-global status word (0 = ok).  Set by bounded waits that expire.
 // mlpk_api.cu is the one translation unit that includes this header (the
-// kernels of block_api.cu have no waits), so this is the single definition.
+// kernels of the norm, the experts and AdamW have no such waits), so this is the
+// single definition.
 __device__ int g_device_status = 0;
 
 enum DeviceStatus : int {

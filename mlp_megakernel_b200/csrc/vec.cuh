@@ -1,6 +1,7 @@
 // Element types and vector access of the block kernels (norm, experts,
-// AdamW): fp16, bf16 and fp32 values are held as fp32 in registers; a vector
-// is 16 bytes where the row allows it, else one element.
+// AdamW): fp16, bf16 and fp32 values are held as fp32 in registers, and move in
+// vectors of 16 bytes (32 for AdamW's fp32 state) or, where a row of the experts
+// does not allow that, of 4 bytes or one element.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -168,21 +169,9 @@ __device__ __forceinline__ void store_vec2(T* p, const float2 (&f)[VEC / 2]) {
 // The 8-bit type: 4 exponent bits, 3 of mantissa (e4m3), largest value 448,
 // smallest positive one 2^-9.
 constexpr float kFp8Max = 448.0f;
-constexpr float kFp8Tiny = 0.001953125f;
 
 // Rounded to e4m3 (to nearest even, NaN kept, magnitudes above 448 clipped).
 __device__ __forceinline__ uint16_t to_fp8x2(float2 f) { return __nv_cvt_float2_to_fp8x2(f, __NV_SATFINITE, __NV_E4M3); }
-template <int VEC>
-__device__ __forceinline__ void store_fp8(uint8_t* p, const float (&f)[VEC]) {
-  if constexpr (VEC == 1) {
-    *p = __nv_cvt_float_to_fp8(f[0], __NV_SATFINITE, __NV_E4M3);
-  } else {
-    Raw<uint16_t, VEC / 2> r;
-#pragma unroll
-    for (int e = 0; e < VEC / 2; ++e) r.v[e] = to_fp8x2(make_float2(f[2 * e], f[2 * e + 1]));
-    *reinterpret_cast<Raw<uint16_t, VEC / 2>*>(p) = r;
-  }
-}
 
 // VEC values of the 8-bit type as fp32 (exact).
 template <int VEC>

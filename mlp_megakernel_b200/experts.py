@@ -11,7 +11,8 @@ MLP experts (no counterpart in the reference, which has one MLP).
 
 Rows are fp16, bf16 or fp32 of any width; sums are fp32 in a fixed order, so
 results are the same from run to run.  Everything runs on the current CUDA
-stream without a wait of the host; there is no CPU path.  Eager calls go through
+stream; the three calls never make the host wait, FusedMLPExperts does once a
+call.  There is no CPU path.  Eager calls go through
 the native binding (_native.py); under torch.compile, tracers and dispatch modes
 and on fake tensors the calls are the operators ``torch.ops.mlpk.expert_*``.
 """
