@@ -156,12 +156,16 @@ class FusedAdamW(torch.optim.Optimizer):
             raise ValueError(f"betas must be at least 0 and below 1, got {(b1, b2)}")
         if not group["eps"] >= 0.0 or not group["weight_decay"] >= 0.0:
             raise ValueError("eps and weight_decay must not be negative")
+        FusedAdamW._check_once(group["params"])
         FusedAdamW._check_params(group["params"])
 
     @staticmethod
-    def _check_params(params) -> None:
+    def _check_once(params) -> None:
         if len({id(p) for p in params}) != len(params):  # its steps would be one launch's, over the same values
             raise ValueError("a parameter group holds a parameter twice")
+
+    @staticmethod
+    def _check_params(params) -> None:
         for p in params:
             if not p.is_cuda:
                 raise RuntimeError("FusedAdamW runs on CUDA (sm_100) only; got a CPU parameter")
@@ -200,8 +204,14 @@ class FusedAdamW(torch.optim.Optimizer):
         if plan is not None and native().same_items(plan.params, params) and \
                 not (plan.waiting and any(p.grad is not None for p in plan.waiting)):
             return plan
-        self._check_params(params)
-        self._add_state(g, [p for p in params if p not in self._place and p.grad is not None])
+        self._check_once(params)
+        new = [p for p in params if p not in self._place and p.grad is not None]
+        self._check_params(new)
+        self._add_state(g, new)
+        return self._make_plan(group)
+
+    def _make_plan(self, group) -> _Plan:
+        params = group["params"]
         members: dict = {}  # of each bucket
         for p in params:
             if p in self._place:
@@ -320,5 +330,7 @@ class FusedAdamW(torch.optim.Optimizer):
                     v = b.view(i, name)
                     v.copy_(saved[p][name].reshape(v.shape))
             b.ticks.copy_(torch.tensor([int(saved[p]["step"]) * c for p, c in zip(b.params, b.chunks)]))
+        for group in self.param_groups:  # here and not in the first step
+            self._make_plan(group)
         for hook in list(self._optimizer_load_state_dict_post_hooks.values()):
             hook(self)
