@@ -13,7 +13,7 @@
 // less of the 18 that both passes move an element in 16 bits.
 //
 // What bounds it: memory; every value is read once and written once.  16,384
-// rows of 4096 bf16 values with a residual: forward 95 us, 5.7 TB/s; backward
+// rows of 4096 bf16 values with a residual: forward 96 us, 5.6 TB/s; backward
 // 104 us, 6.5 TB/s, with dw's sum; 8,192 rows of 5120 to 8 bits in groups of 128:
 // 56 us, 5.3 TB/s (53 with a reciprocal of the scale that is off by a unit of its
 // last place in an eighth of the cases, which moves values next to a tie).
@@ -34,7 +34,7 @@
 // its neighbours, and a thread leaves out the elements that are not its row's.
 // Blocks step by a multiple of VEC rows, so that `shift`, and with it each
 // thread's columns, are the same in all rows of a block's row group.  (8,192
-// rows of 2049 bf16 values: forward 26 us, 0.78 of the copy rate.)
+// rows of 2049 bf16 values with a residual: forward 28 us, 0.73 of the copy rate.)
 #pragma once
 #include "pdl.cuh"
 #include "vec.cuh"
