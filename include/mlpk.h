@@ -338,6 +338,73 @@ int mlpk_adamw_step(int count, const int64_t* numel, void* const* params, const 
                     const int64_t* state_off, const int32_t* tick, int p_dtype, int g_dtype,
                     const mlpk_adamw_state* state, const mlpk_adamw_args* args, mlpk_stream_t stream);
 
+/* ---- Feed-forward operators.  No counterpart in the reference, whose layers are
+ * at most 256 wide and have one activation.  Operands are MLPK_DT_F16 or
+ * MLPK_DT_BF16 (accumulators, bias, activation and residual are fp32), widths
+ * multiples of 8, rows below 2^31 - 256, tensors contiguous and 16-byte aligned.
+ * A weight [in][out] is stored so (MLPK_W_IN_OUT) or as its transpose
+ * (MLPK_W_OUT_IN); a bias is of dtype or fp32. */
+#define MLPK_W_IN_OUT 0
+#define MLPK_W_OUT_IN 1
+#define MLPK_ACT_NONE 0
+#define MLPK_ACT_RELU 1
+#define MLPK_ACT_SILU 2
+#define MLPK_ACT_GELU_TANH 3 /* 0.5 z (1 + tanh(sqrt(2 / pi) (z + 0.044715 z^3))) */
+#define MLPK_ACT_SOFTPLUS 4
+#define MLPK_ACT_SIGMOID 5
+/* What a forward call keeps for the backward: nothing, values of dtype
+ * [rows][width], or 8-bit values [rows][mlpk_fp8_pitch(width)] with fp32 scales
+ * [rows][ceil(width / 128)] (see mlpk_fp8_checkpoint). */
+#define MLPK_KEEP_NONE 0
+#define MLPK_KEEP_16 1
+#define MLPK_KEEP_FP8 2
+int64_t mlpk_fp8_pitch(int width); /* width rounded up to 128 */
+
+/* out = act(z) + residual, z = x w + bias.  x: [rows][d_in]; w: [d_in][d_out]
+ * in w_layout; bias: [d_out] or NULL; residual: [rows][d_out] or NULL; z (and
+ * z_scale) as `keep` says. */
+int mlpk_linear(int64_t rows, int d_in, int d_out, int dtype, const void* x, const void* w, int w_layout,
+                const void* bias, int bias_dtype, int act, const void* residual, void* out, int keep, void* z,
+                float* z_scale, mlpk_stream_t stream);
+/* dz = grad_out act'(z) (NULL: not wanted) and db, the sum of dz over the rows
+ * before its rounding, in a fixed order (of dtype or fp32; NULL: not wanted; it
+ * alone needs the workspace).  z as `keep` says; unused without an activation. */
+int64_t mlpk_linear_dz_workspace_size(int64_t rows, int width, int dtype);
+int mlpk_linear_dz(int64_t rows, int width, int dtype, int act, const void* grad_out, int keep, const void* z,
+                   const float* z_scale, void* dz, void* db, int db_dtype, void* workspace, int64_t workspace_bytes,
+                   mlpk_stream_t stream);
+/* dx = the sum over i < count (1 or 2) of dz[i] w[i]^T; dz[i]: [rows][d_out]. */
+int mlpk_linear_dx(int64_t rows, int d_in, int d_out, int dtype, int count, const void* const* dz,
+                   const void* const* w, int w_layout, void* dx, mlpk_stream_t stream);
+/* dw[i] = x^T dz[i] for i < count (1 or 2), summed over the rows in fp32 in a
+ * fixed order, stored in w_layout. */
+int64_t mlpk_linear_dw_workspace_size(int64_t rows, int d_in, int d_out, int dtype, int count);
+int mlpk_linear_dw(int64_t rows, int d_in, int d_out, int dtype, int count, const void* x, const void* const* dz,
+                   void* const* dw, int w_layout, void* workspace, int64_t workspace_bytes, mlpk_stream_t stream);
+
+/* h = act(g) u with g = x w_gate, u = x w_up, in one kernel; g and u as `keep`
+ * says. */
+int mlpk_gated(int64_t rows, int d_in, int hidden, int dtype, int act, const void* x, const void* w_gate,
+               const void* w_up, int w_layout, void* h, int keep, void* g, float* g_scale, void* u, float* u_scale,
+               mlpk_stream_t stream);
+/* Its backward behind out = h w_down: dh = grad_out w_down^T, dg = dh u act'(g),
+ * du = dh act(g), and h = act(g) u again (for w_down's gradient), in one kernel.
+ * w_down: [hidden][d_out] in w_layout. */
+int mlpk_gated_bwd(int64_t rows, int hidden, int d_out, int dtype, int act, const void* grad_out, const void* w_down,
+                   int w_layout, int keep, const void* g, const float* g_scale, const void* u, const float* u_scale,
+                   void* dg, void* du, void* h, mlpk_stream_t stream);
+
+/* Activations kept in 8 bits: q = e4m3(x / scale), scale the smallest power of
+ * two (2^-126 at least) with max|x| / scale <= 448 over a row's 128 columns (the
+ * last group may be shorter), NaN where a value is not finite; and back, x = q
+ * scale (exact in fp32 and bf16; clipped to dtype's largest finite value, which
+ * rounding up may pass).  x: fp16, bf16 or fp32 [rows][width], any width; q:
+ * [rows][width]; scale: [rows][ceil(width / 128)]. */
+int mlpk_fp8_checkpoint(int64_t rows, int width, int dtype, const void* x, void* q, float* scale,
+                        mlpk_stream_t stream);
+int mlpk_fp8_restore(int64_t rows, int width, int dtype, const void* q, const float* scale, void* x,
+                     mlpk_stream_t stream);
+
 /* Text of the CUDA runtime / driver failure behind the calling thread's most
  * recent MLPK_ERR_CUDA ("no error" if none).  The reference reports failures as
  * Python exceptions carrying the CUDA message (cutile_mlp.py:388); this is the

@@ -93,6 +93,18 @@ SIGNATURES = {
     "mlpk_expert_dispatch": (_i32, [_i64, _i32, _i32, _i32, _vp, _vp, _vp, _vp, _vp]),
     "mlpk_expert_combine": (_i32, [_i64, _i32, _i32, _i32, _vp, _vp, _i32, _vp, _vp, _vp, _vp]),
     "mlpk_expert_combine_bwd": (_i32, [_i64, _i32, _i32, _i32, _vp, _vp, _vp, _i32, _vp, _vp, _vp, _vp, _vp]),
+    "mlpk_fp8_pitch": (_i64, [_i32]),
+    "mlpk_linear": (_i32, [_i64, _i32, _i32, _i32, _vp, _vp, _i32, _vp, _i32, _i32, _vp, _vp, _i32, _vp, _vp, _vp]),
+    "mlpk_linear_dz_workspace_size": (_i64, [_i64, _i32, _i32]),
+    "mlpk_linear_dz": (_i32, [_i64, _i32, _i32, _i32, _vp, _i32, _vp, _vp, _vp, _vp, _i32, _vp, _i64, _vp]),
+    "mlpk_linear_dx": (_i32, [_i64, _i32, _i32, _i32, _i32, _VPP, _VPP, _i32, _vp, _vp]),
+    "mlpk_linear_dw_workspace_size": (_i64, [_i64, _i32, _i32, _i32, _i32]),
+    "mlpk_linear_dw": (_i32, [_i64, _i32, _i32, _i32, _i32, _vp, _VPP, _VPP, _i32, _vp, _i64, _vp]),
+    "mlpk_gated": (_i32, [_i64, _i32, _i32, _i32, _i32, _vp, _vp, _vp, _i32, _vp, _i32, _vp, _vp, _vp, _vp, _vp]),
+    "mlpk_gated_bwd": (_i32, [_i64, _i32, _i32, _i32, _i32, _vp, _vp, _i32, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
+                              _vp]),
+    "mlpk_fp8_checkpoint": (_i32, [_i64, _i32, _i32, _vp, _vp, _vp, _vp]),
+    "mlpk_fp8_restore": (_i32, [_i64, _i32, _i32, _vp, _vp, _vp, _vp]),
     "mlpk_adamw_step": (_i32, [_i32, _vp, _vp, _vp, _vp, _vp, _i32, _i32, ctypes.POINTER(MlpkAdamwState),
                                ctypes.POINTER(MlpkAdamwArgs), _vp]),
 }
@@ -105,6 +117,8 @@ DT_BF16 = 2  # MLPK_DT_BF16: bf16 values (the block operators)
 ADAMW_BLOCK = 256  # MLPK_ADAMW_BLOCK: elements that share a scale of the 8-bit state
 ADAMW_CHUNK = 2048  # MLPK_ADAMW_CHUNK: the unit of the step counts, in elements
 EXPERT_MAX = 1024
+FF_MAX_ROWS = 2 ** 31 - 1 - 256
+FF_MAX_WIDTH = 2 ** 20
 NORM_MAX_WIDTH = 32768
 NORM_GROUP = 128  # columns that share a scale of the 8-bit norm
 PEER_HANDLE_BYTES = 64

@@ -28,6 +28,11 @@ SOURCES = {
     **{f"norm_{part}.cu": ["host.cuh", "pdl.cuh", "vec.cuh", "norm_kernel.cuh", "norm_launch.cuh"]
        for part in ("api", "f16", "bf16", "f32")},
     "expert_api.cu": ["host.cuh", "pdl.cuh", "vec.cuh", "expert_plan.cuh", "expert_kernel.cuh"],
+    **{f"product_{part}.cu": ["host.cuh", "pdl.cuh", "ptx.cuh", "pair.cuh", "layout.cuh", "softplus.cuh", "vec.cuh",
+                              "act.cuh", "product_epi.cuh", "product_kernel.cuh", "product_launch.cuh",
+                              "product_type.cuh"] for part in ("f16", "bf16")},
+    "ff_api.cu": ["host.cuh", "pdl.cuh", "ptx.cuh", "softplus.cuh", "vec.cuh", "act.cuh", "product_epi.cuh",
+                  "product_launch.cuh", "ff_kernel.cuh"],
     "adamw_api.cu": ["host.cuh", "pdl.cuh", "vec.cuh", "adamw_kernel.cuh"],
 }
 

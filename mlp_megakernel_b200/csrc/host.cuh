@@ -3,6 +3,7 @@
 // thread's last CUDA failure.  The functions are defined in mlpk_api.cu and
 // are not exported.
 #pragma once
+#include <cuda.h>
 #include <cuda_runtime.h>
 
 #include <cstdint>
@@ -32,6 +33,18 @@ constexpr int kMaxBlockSmem = 227 * 1024;  // dynamic shared memory of a block
 // lets the kernel have that much dynamic shared memory); 0 on a failure, whose
 // status is kept for mlpk_last_cuda_error.
 __attribute__((visibility("hidden"))) int blocks_per_sm(const void* kern, int threads, size_t smem, int dev);
+
+// The tensor map of a 2-D tensor [outer][inner] (inner contiguous) of 16-bit
+// elements (elem_bytes 2) or fp32 (4), box {box_inner, box_outer}, swizzled in the
+// box's row pitch (128, 64 or 32 bytes).  atom32: 128-byte rows swizzled in
+// 32-byte granules (the MN-major tf32 operand layout, layout.cuh).
+__attribute__((visibility("hidden"))) int make_map_2d(CUtensorMap* map, const void* ptr, uint64_t inner,
+                                                      uint64_t outer, uint32_t box_inner, uint32_t box_outer,
+                                                      uint32_t elem_bytes = 2, bool atom32 = false);
+
+// The current device's status word, for kernels outside mlpk_api.cu; NULL on a
+// failure, whose status is kept for mlpk_last_cuda_error.
+__attribute__((visibility("hidden"))) int* device_status_word(int dev);
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 

@@ -7,6 +7,7 @@
 #include <cuda_runtime.h>
 #include <cudaTypedefs.h>
 
+#include <atomic>
 #include <cstdint>
 #include <cstdio>
 #include <cstring>
@@ -37,6 +38,7 @@ using mlpk::host::DevInfo;
 using mlpk::host::launch_kernel;
 using mlpk::host::launch_kernel_cfg;
 using mlpk::host::launch_kernel_early;
+using mlpk::host::make_map_2d;
 
 // ------------------------------------------------------------------ device
 constexpr int kMaxDevices = 64;
@@ -136,12 +138,13 @@ EncodeFn get_encode() {
   return fn;
 }
 
-// 2-D tensor [outer][inner] (inner contiguous) of fp16 (elem_bytes 2) or fp32
-// (elem_bytes 4), box {box_inner, box_outer}, swizzle chosen from the box's
-// row pitch (box_inner * elem_bytes); atom32: 128-byte rows swizzled in
-// 32-byte granules (the MN-major tf32 operand layout, layout.cuh).
-int make_map_2d(CUtensorMap* map, const void* ptr, uint64_t inner, uint64_t outer,
-                uint32_t box_inner, uint32_t box_outer, uint32_t elem_bytes = 2, bool atom32 = false) {
+}  // namespace
+
+namespace mlpk {
+namespace host {
+
+int make_map_2d(CUtensorMap* map, const void* ptr, uint64_t inner, uint64_t outer, uint32_t box_inner,
+                uint32_t box_outer, uint32_t elem_bytes, bool atom32) {
   EncodeFn enc = get_encode();
   if (!enc) return driver_status("cudaGetDriverEntryPoint(cuTensorMapEncodeTiled)", -1);
   const uint32_t pitch = box_inner * elem_bytes;
@@ -159,6 +162,23 @@ int make_map_2d(CUtensorMap* map, const void* ptr, uint64_t inner, uint64_t oute
                    CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return driver_status("cuTensorMapEncodeTiled", static_cast<int>(r));
 }
+
+int* device_status_word(int dev) {
+  static std::atomic<int*> known[kMaxDevices];  // found twice, it is the same
+  int* p = known[dev].load(std::memory_order_relaxed);
+  if (!p) {
+    void* found = nullptr;
+    if (cuda_status(cudaGetSymbolAddress(&found, mlpk::g_device_status))) return nullptr;
+    p = static_cast<int*>(found);
+    known[dev].store(p, std::memory_order_relaxed);
+  }
+  return p;
+}
+
+}  // namespace host
+}  // namespace mlpk
+
+namespace {
 
 // Raise a kernel's dynamic shared-memory limit once per (kernel, device).
 template <class Kern>

@@ -1,0 +1,8 @@
+// What stands behind a product in its epilogue (product_kernel.cuh).
+#pragma once
+
+namespace mlpk {
+
+enum Epi : int { kEpiPlain, kEpiPartial, kEpiLinear, kEpiGated, kEpiGatedBwd };
+
+}  // namespace mlpk

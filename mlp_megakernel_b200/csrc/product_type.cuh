@@ -1,0 +1,108 @@
+// The launches of one operand type (included by product_f16.cu and
+// product_bf16.cu alone).
+#pragma once
+#define MLPK_STATUS_BY_POINTER
+#include <algorithm>
+#include <atomic>
+#include <cstring>
+
+#include "product_kernel.cuh"
+#include "product_launch.cuh"
+
+namespace mlpk {
+namespace product {
+
+using namespace mlpk::host;
+
+// Pairs of CTAs that the device holds at a time.
+inline int pairs_at_once(const void* kern, int smem, int dev, int sm_count, std::atomic<int>* known) {
+  int n = known[dev].load(std::memory_order_relaxed);
+  if (n) return n;
+  if (!blocks_per_sm(kern, kProductThreads, smem, dev)) return 0;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(2 * (sm_count / 2));
+  cfg.blockDim = dim3(kProductThreads);
+  cfg.dynamicSmemBytes = smem;
+  if (cuda_status(cudaOccupancyMaxActiveClusters(&n, kern, &cfg))) return 0;
+  if (n < 1) {
+    cuda_status(cudaErrorLaunchOutOfResources);
+    return 0;
+  }
+  n = std::min(n, sm_count / 2);
+  known[dev].store(n, std::memory_order_relaxed);
+  return n;
+}
+
+inline int ceil_div_int(int64_t a, int64_t b) { return static_cast<int>((a + b - 1) / b); }
+
+template <class T, int EPI, int TN>
+int launch_tiles(const Product& c, cudaStream_t st) {
+  using Cfg = ProductCfg<EPI, TN>;
+  DevInfo di;
+  int dev = 0, rc = current_device_info(&di, &dev);
+  if (rc) return rc;
+  const auto kern = product_kernel<T, EPI, TN>;
+  static std::atomic<int> known[64];
+  const int pairs = pairs_at_once(reinterpret_cast<const void*>(kern), Cfg::SMEM, dev, di.sm_count, known);
+  if (!pairs) return MLPK_ERR_CUDA;
+
+  ProductArgs a;
+  std::memset(&a, 0, sizeof(a));
+  a.rows = static_cast<int>(c.rows);
+  a.cols = c.cols;
+  a.nk0 = ceil_div_int(c.k[0], kBlockK);
+  a.nk = a.nk0 + ceil_div_int(c.k[1], kBlockK);
+  a.tiles_m = ceil_div_int(c.rows, kPairRows);
+  a.tiles_n = ceil_div_int(c.cols, Cfg::OUT_COLS);
+  a.outputs = c.outputs;
+  a.splits = c.splits;
+  a.group = 8;
+  a.a_mn = c.a_mn;
+  a.b_mn = c.b_mn;
+  a.out_a = c.out_a;
+  a.idesc = make_idesc_f16(kPairRows, TN, c.a_mn, c.b_mn) |
+            (std::is_same_v<T, __nv_bfloat16> ? (1u << 7 | 1u << 10) : 0u);
+  a.act = c.act;
+  a.keep_kind = c.keep_kind;
+  a.residual = EPI == kEpiLinear && c.in[0] != nullptr;
+  a.bias = c.bias;
+  a.bias32 = c.bias32;
+  a.status = device_status_word(dev);
+  if (!a.status) return MLPK_ERR_CUDA;
+  a.partials = c.partials;
+  a.q_pitch = c.q_pitch;
+  a.scale_pitch = c.scale_pitch;
+  for (int i = 0; i < 2; ++i) {
+    a.q[i] = c.q[i];
+    a.scale[i] = c.scale[i];
+    const uint64_t k = i == 1 && c.k[1] > 0 ? c.k[1] : c.k[0];
+    const uint64_t rows = c.rows, cols = c.cols;
+    if (c.a[i] && (rc = c.a_mn ? make_map_2d(&a.a[i], c.a[i], rows, k, 64, kBlockK)
+                               : make_map_2d(&a.a[i], c.a[i], k, rows, kBlockK, 128)))
+      return rc;
+    if (c.b[i] && (rc = c.b_mn ? make_map_2d(&a.b[i], c.b[i], cols, k, 64, kBlockK)
+                               : make_map_2d(&a.b[i], c.b[i], k, cols, kBlockK, TN / 2)))
+      return rc;
+    if (c.in[i] && (rc = make_map_2d(&a.in[i], c.in[i], cols, rows, 32, 32))) return rc;
+    if (c.out[i] && EPI != kEpiPartial && (rc = make_map_2d(&a.out[i], c.out[i], cols, rows, 32, 32))) return rc;
+    if (c.keep[i] && (rc = make_map_2d(&a.keep[i], c.keep[i], cols, rows, 32, 32))) return rc;
+  }
+  const int64_t total = static_cast<int64_t>(a.tiles_m) * a.tiles_n * a.outputs * a.splits;
+  if (total > 0x7fffffff - 256) return MLPK_ERR_SHAPE;
+  return launch_kernel_early(kern, dim3(2 * static_cast<unsigned>(std::min<int64_t>(total, pairs))), kProductThreads,
+                             Cfg::SMEM, st, a);
+}
+
+template <class T>
+int launch_type(const Product& c, cudaStream_t st) {
+  switch (c.epi) {
+    case kEpiPlain: return launch_tiles<T, kEpiPlain, 256>(c, st);
+    case kEpiPartial: return launch_tiles<T, kEpiPartial, 256>(c, st);
+    case kEpiLinear: return launch_tiles<T, kEpiLinear, 256>(c, st);
+    case kEpiGated: return launch_tiles<T, kEpiGated, 256>(c, st);
+    default: return launch_tiles<T, kEpiGatedBwd, 256>(c, st);
+  }
+}
+
+}  // namespace product
+}  // namespace mlpk

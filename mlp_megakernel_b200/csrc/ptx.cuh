@@ -19,11 +19,13 @@
 
 namespace mlpk {
 
-// Device-global status word (0 = ok).  Set by bounded waits that expire.
-// mlpk_api.cu is the one translation unit that includes this header (the
-// kernels of the norm, the experts and AdamW have no such waits), so this is the
-// single definition.
+// Device-global status word (0 = ok).  Set by bounded waits that expire.  The
+// kernels of mlpk_api.cu and user kernels name it; a translation unit of the
+// library that defines MLPK_STATUS_BY_POINTER has no word of its own and hands
+// its kernels the address of mlpk_api.cu's (host.cuh, device_status_word).
+#ifndef MLPK_STATUS_BY_POINTER
 __device__ int g_device_status = 0;
+#endif
 
 enum DeviceStatus : int {
   kDevOk = 0,
@@ -83,8 +85,8 @@ __device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
 // Bounded wait for the phase with the given parity.  Returns false (and sets
 // the abort flag + device status) when the wait expires or another role of the
 // CTA already aborted.
-__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag,
-                                          int err_code) {
+__device__ __forceinline__ bool mbar_wait_to(uint32_t bar, uint32_t parity, volatile int* abort_flag, int err_code,
+                                             int* status) {
   if (mbar_try_wait(bar, parity)) return true;
   const uint64_t t0 = globaltimer_ns();
   while (true) {
@@ -93,12 +95,17 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
       if (mbar_try_wait(bar, parity)) return true;
     if (*abort_flag) return false;
     if (globaltimer_ns() - t0 > MLPK_WAIT_TIMEOUT_NS) {
-      atomicOr(&g_device_status, err_code);
+      atomicOr(status, err_code);
       *abort_flag = 1;
       return false;
     }
   }
 }
+#ifndef MLPK_STATUS_BY_POINTER
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int err_code) {
+  return mbar_wait_to(bar, parity, abort_flag, err_code, &g_device_status);
+}
+#endif
 
 // ---------------------------------------------------------------- fences
 __device__ __forceinline__ void fence_proxy_async_smem() {

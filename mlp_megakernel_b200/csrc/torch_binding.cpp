@@ -117,6 +117,13 @@ Tensor once(const Tensor& grad, std::initializer_list<const Tensor*> depends_on)
   return (*node)({grad.detach().requires_grad_(true)})[0];
 }
 
+// The same, where the node knows whether the gradient depends on such a tensor.
+Tensor once_if(const Tensor& grad, const Tensor& upstream, bool depends) {
+  if (!depends || !grad.defined() || !at::GradMode::is_enabled()) return once(grad, {&upstream});
+  const Tensor needing = upstream.detach().requires_grad_(true);
+  return once(grad, {&needing});
+}
+
 // ------------------------------------------------------------------ norm
 struct Normed {
   Tensor y, h, rstd;
@@ -396,6 +403,383 @@ py::object expert_combine(const Tensor& y, const std::optional<Tensor>& weights,
   return py::cast(out);
 }
 
+// ------------------------------------------------------------------ feed-forward
+constexpr int64_t kFfMaxRows = 0x7fffffff - 256, kFfMaxWidth = 1 << 20;
+constexpr int kActs = 6;
+
+bool operand_type(const Tensor& t) { return t.scalar_type() == at::kHalf || t.scalar_type() == at::kBFloat16; }
+bool ff_width(int64_t w) { return w >= 8 && w % 8 == 0 && w <= kFfMaxWidth; }
+int64_t rows_of(const Tensor& x) { return x.numel() / x.size(-1); }
+std::vector<int64_t> with_width(const Tensor& x, int64_t width) {
+  std::vector<int64_t> s(x.sizes().begin(), x.sizes().end());
+  s.back() = width;
+  return s;
+}
+
+// A weight [in][out] where it lies: contiguous, or the transpose of a contiguous
+// tensor; anything else is copied.
+struct Weight {
+  Tensor t;
+  int layout;
+};
+Weight weight_in(const Tensor& w, int layout) {
+  if (layout == MLPK_W_OUT_IN) return {aligned(w.t()), layout};
+  return {aligned(w), layout};
+}
+int layout_of(const Tensor& w) {
+  return !w.is_contiguous() && w.t().is_contiguous() ? MLPK_W_OUT_IN : MLPK_W_IN_OUT;
+}
+Weight weight_of(const Tensor& w) { return weight_in(w, layout_of(w)); }
+// A weight's gradient in its layout: [the memory, the tensor [in][out]].
+std::pair<Tensor, Tensor> grad_of(const Tensor& w, int layout) {
+  if (layout == MLPK_W_OUT_IN) {
+    const Tensor m = at::empty({w.size(1), w.size(0)}, w.options());
+    return {m, m.t()};
+  }
+  const Tensor m = at::empty({w.size(0), w.size(1)}, w.options());
+  return {m, m};
+}
+
+// Values that a forward keeps: of its type, or 8 bits and their scales.
+struct Kept {
+  Tensor v, scale;
+  int kind() const { return !v.defined() ? MLPK_KEEP_NONE : scale.defined() ? MLPK_KEEP_FP8 : MLPK_KEEP_16; }
+  float* scales() const { return static_cast<float*>(ptr(scale)); }
+};
+Kept keep_for(const Tensor& x, int64_t rows, int64_t width, int64_t keep) {
+  Kept k;
+  if (keep == MLPK_KEEP_16) k.v = at::empty({rows, width}, x.options());
+  if (keep == MLPK_KEEP_FP8) {
+    k.v = at::empty({rows, mlpk_fp8_pitch(static_cast<int>(width))}, x.options().dtype(at::kFloat8_e4m3fn));
+    k.scale = at::empty({rows, (width + 127) / 128}, x.options().dtype(at::kFloat));
+  }
+  return k;
+}
+
+Kept checkpoint(const Tensor& x_in) {
+  const c10::cuda::CUDAGuard guard(x_in.device());
+  const Tensor x = aligned(x_in);
+  const int64_t width = x.size(-1), rows = rows_of(x);
+  Kept k;
+  k.v = at::empty(x.sizes(), x.options().dtype(at::kFloat8_e4m3fn));
+  k.scale = at::empty(with_width(x, (width + 127) / 128), x.options().dtype(at::kFloat));
+  check("mlpk_fp8_checkpoint", mlpk_fp8_checkpoint(rows, static_cast<int>(width), code(x), ptr(x), ptr(k.v), k.scales(),
+                                                   stream_of(x)));
+  return k;
+}
+Tensor restore(const Tensor& q_in, const Tensor& scale_in, at::ScalarType type) {
+  const c10::cuda::CUDAGuard guard(q_in.device());
+  const Tensor q = aligned(q_in), scale = aligned(scale_in);
+  const int64_t width = q.size(-1);
+  Tensor x = at::empty(q.sizes(), q.options().dtype(type));
+  check("mlpk_fp8_restore", mlpk_fp8_restore(rows_of(q), static_cast<int>(width), code(type), ptr(q),
+                                             static_cast<float*>(ptr(scale)), ptr(x), stream_of(q)));
+  return x;
+}
+
+// out = act(x w + b) + r, and what is kept of x w + b.
+Tensor linear_forward(const Tensor& x_in, const Weight& w, int64_t n, const Tensor& b_in, const Tensor& r_in, int64_t act,
+                      Kept* z) {
+  const Tensor x = aligned(x_in), b = aligned(b_in), r = aligned(r_in);
+  Tensor out = at::empty(with_width(x, n), x.options());
+  check("mlpk_linear",
+        mlpk_linear(rows_of(x), static_cast<int>(x.size(-1)), static_cast<int>(n), code(x), ptr(x), ptr(w.t), w.layout,
+                    ptr(b), code(b.defined() ? b : x), static_cast<int>(act), ptr(r), ptr(out),
+                    z ? z->kind() : MLPK_KEEP_NONE, z ? ptr(z->v) : nullptr, z ? z->scales() : nullptr, stream_of(x)));
+  return out;
+}
+std::pair<Tensor, Kept> linear_kept(const Tensor& x, const Tensor& w, const Tensor& b, const Tensor& r, int64_t act,
+                                    int64_t keep) {
+  const c10::cuda::CUDAGuard guard(x.device());
+  Kept z = keep_for(x, rows_of(x), w.size(1), keep);
+  Tensor out = linear_forward(x, weight_of(w), w.size(1), b, r, act, &z);
+  return {std::move(out), std::move(z)};
+}
+
+Tensor workspace(int64_t bytes, const Tensor& like) {
+  return bytes > 0 ? at::empty({bytes}, like.options().dtype(at::kByte)) : Tensor();
+}
+// The gradients of x (of one product, or the sum of two) and of the weights.
+Tensor dx_of(const Tensor& shaped, std::initializer_list<Tensor> dz, std::initializer_list<Weight> w, int64_t d_in) {
+  const Tensor& first = *dz.begin();
+  Tensor dx = at::empty(with_width(shaped, d_in), first.options());
+  const void *zp[2], *wp[2];
+  int n = 0;
+  for (const Tensor& t : dz) zp[n++] = ptr(t);
+  n = 0;
+  for (const Weight& t : w) wp[n++] = ptr(t.t);
+  check("mlpk_linear_dx", mlpk_linear_dx(rows_of(first), static_cast<int>(d_in), static_cast<int>(first.size(-1)),
+                                         code(first), n, zp, wp, w.begin()->layout, ptr(dx), stream_of(first)));
+  return dx;
+}
+void dw_of(const Tensor& x_in, std::initializer_list<Tensor> dz, std::initializer_list<Tensor> dw, int layout) {
+  const Tensor x = aligned(x_in);
+  const void* zp[2];
+  void* wp[2];
+  int n = 0;
+  for (const Tensor& t : dz) zp[n++] = ptr(t);
+  n = 0;
+  for (const Tensor& t : dw) wp[n++] = ptr(t);
+  const int k = static_cast<int>(x.size(-1)), m = static_cast<int>(dz.begin()->size(-1));
+  const int64_t rows = rows_of(x), bytes = mlpk_linear_dw_workspace_size(rows, k, m, code(x), n);
+  const Tensor work = workspace(bytes, x);
+  check("mlpk_linear_dw",
+        mlpk_linear_dw(rows, k, m, code(x), n, ptr(x), zp, wp, layout, ptr(work), std::max<int64_t>(bytes, 0), stream_of(x)));
+}
+
+struct LinearGrads {
+  Tensor dx, dw, db;
+};
+LinearGrads linear_backward(const Tensor& go_in, const Kept& x, const Tensor& w_in, const Kept& z, int64_t act,
+                            at::ScalarType db_type, bool want_dx, bool want_dw, bool want_db) {
+  const c10::cuda::CUDAGuard guard(go_in.device());
+  const Tensor go = aligned(go_in);
+  const int64_t rows = rows_of(go), n = go.size(-1);
+  LinearGrads got;
+  Tensor dz = go;
+  if (act != MLPK_ACT_NONE || want_db) {
+    if (act != MLPK_ACT_NONE) dz = want_dx || want_dw ? at::empty_like(go) : Tensor();
+    Tensor work;
+    int64_t bytes = 0;
+    if (want_db) {
+      got.db = at::empty({n}, go.options().dtype(db_type));
+      bytes = mlpk_linear_dz_workspace_size(rows, static_cast<int>(n), code(go));
+      work = workspace(bytes, go);
+    }
+    check("mlpk_linear_dz",
+          mlpk_linear_dz(rows, static_cast<int>(n), code(go), static_cast<int>(act), ptr(go),
+                         act != MLPK_ACT_NONE ? z.kind() : MLPK_KEEP_NONE, ptr(z.v), z.scales(),
+                         act != MLPK_ACT_NONE ? ptr(dz) : nullptr, ptr(got.db), code(db_type), ptr(work),
+                         std::max<int64_t>(bytes, 0), stream_of(go)));
+  }
+  const Weight w = weight_of(w_in);
+  if (want_dx) got.dx = dx_of(go, {dz}, {w}, w_in.size(0));
+  if (want_dw) {
+    Tensor memory;
+    std::tie(memory, got.dw) = grad_of(w_in, w.layout);
+    dw_of(x.scale.defined() ? restore(x.v, x.scale, go.scalar_type()) : x.v, {dz}, {memory}, w.layout);
+  }
+  return got;
+}
+
+std::tuple<Tensor, Kept, Kept> gated_forward(const Tensor& x_in, const Tensor& wg_in, const Tensor& wu_in,
+                                             const Tensor& wd_in, const Tensor& r, int64_t act, int64_t keep) {
+  const c10::cuda::CUDAGuard guard(x_in.device());
+  const Tensor x = aligned(x_in);
+  const int64_t rows = rows_of(x), width = wg_in.size(1);
+  const int layout = layout_of(wg_in) == layout_of(wu_in) ? layout_of(wg_in) : MLPK_W_IN_OUT;
+  const Weight wg = weight_in(wg_in, layout), wu = weight_in(wu_in, layout);
+  Kept g = keep_for(x, rows, width, keep), u = keep_for(x, rows, width, keep);
+  const Tensor h = at::empty({rows, width}, x.options());
+  check("mlpk_gated", mlpk_gated(rows, static_cast<int>(x.size(-1)), static_cast<int>(width), code(x),
+                                 static_cast<int>(act), ptr(x), ptr(wg.t), ptr(wu.t), layout, ptr(h), g.kind(), ptr(g.v),
+                                 g.scales(), ptr(u.v), u.scales(), stream_of(x)));
+  Tensor out = linear_forward(h, weight_of(wd_in), wd_in.size(1), Tensor(), r, MLPK_ACT_NONE, nullptr);
+  return {out.view(with_width(x, wd_in.size(1))), std::move(g), std::move(u)};
+}
+
+struct GatedGrads {
+  Tensor dx, dwg, dwu, dwd;
+};
+GatedGrads gated_backward(const Tensor& go_in, const Kept& x, const Tensor& wg_in, const Tensor& wu_in, const Tensor& wd_in,
+                          const Kept& g, const Kept& u, int64_t act, bool want_dx, bool want_dgu, bool want_dd) {
+  const c10::cuda::CUDAGuard guard(go_in.device());
+  const Tensor go = aligned(go_in);
+  const int64_t rows = rows_of(go), width = wd_in.size(0);
+  const Weight wd = weight_of(wd_in);
+  Tensor dg = at::empty({rows, width}, go.options()), du = at::empty_like(dg), h = at::empty_like(dg);
+  check("mlpk_gated_bwd",
+        mlpk_gated_bwd(rows, static_cast<int>(width), static_cast<int>(go.size(-1)), code(go), static_cast<int>(act),
+                       ptr(go), ptr(wd.t), wd.layout, g.kind(), ptr(g.v), g.scales(), ptr(u.v), u.scales(), ptr(dg),
+                       ptr(du), ptr(h), stream_of(go)));
+  GatedGrads got;
+  Tensor memory, other;
+  if (want_dd) {
+    std::tie(memory, got.dwd) = grad_of(wd_in, wd.layout);
+    dw_of(h, {go}, {memory}, wd.layout);
+  }
+  h.reset();
+  const int layout = layout_of(wg_in) == layout_of(wu_in) ? layout_of(wg_in) : MLPK_W_IN_OUT;
+  if (want_dx) got.dx = dx_of(go, {dg, du}, {weight_in(wg_in, layout), weight_in(wu_in, layout)}, wg_in.size(0));
+  if (want_dgu) {
+    std::tie(memory, got.dwg) = grad_of(wg_in, layout);
+    std::tie(other, got.dwu) = grad_of(wu_in, layout);
+    dw_of(x.scale.defined() ? restore(x.v, x.scale, go.scalar_type()) : x.v, {dg, du}, {memory, other}, layout);
+  }
+  return got;
+}
+
+// What a node keeps of its input, if a weight's gradient needs it.
+Kept input_kept(const Tensor& x, bool wanted, bool fp8) {
+  if (!wanted) return {};
+  if (!fp8) return {x, Tensor()};
+  return checkpoint(x);
+}
+
+struct LinearNode : torch::autograd::Function<LinearNode> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const std::optional<Tensor>& bias,
+                               const std::optional<Tensor>& residual, int64_t act, bool fp8) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    const Tensor b = bias.value_or(Tensor()), r = residual.value_or(Tensor());
+    const bool any = x.requires_grad() || w.requires_grad() || (b.defined() && b.requires_grad());
+    auto [out, z] = linear_kept(x, w, b, r, act, act != MLPK_ACT_NONE && any ? (fp8 ? MLPK_KEEP_FP8 : MLPK_KEEP_16) : 0);
+    const Kept k = input_kept(x, w.requires_grad(), fp8);
+    ctx->saved_data["act"] = act;
+    ctx->saved_data["bias"] = static_cast<int64_t>(b.defined() ? b.scalar_type() : at::ScalarType::Undefined);
+    ctx->saved_data["residual"] = r.defined();
+    ctx->save_for_backward({k.v, k.scale, w, z.v, z.scale});
+    return {out};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const variable_list saved = ctx->get_saved_variables();
+    const Tensor &go = grads[0], &w = saved[2];
+    const int64_t act = ctx->saved_data["act"].toInt();
+    const auto db_type = static_cast<at::ScalarType>(ctx->saved_data["bias"].toInt());
+    const bool has_b = db_type != at::ScalarType::Undefined, has_r = ctx->saved_data["residual"].toBool();
+    const bool want_dx = ctx->needs_input_grad(0), want_dw = ctx->needs_input_grad(1);
+    const bool want_db = has_b && ctx->needs_input_grad(2), want_dr = has_r && ctx->needs_input_grad(has_b ? 3 : 2);
+    LinearGrads got;
+    if (!go.defined()) return variable_list(6);
+    if (want_dx || want_dw || want_db) {
+      const at::NoGradGuard no_grad;
+      const at::ScalarType type = has_b ? db_type : go.scalar_type();
+      if (direct({&go, &saved[0], &w})) {
+        got = linear_backward(go, {saved[0], saved[1]}, w, {saved[3], saved[4]}, act, type, want_dx, want_dw, want_db);
+      } else {
+        refuse_tangents({&go, &saved[0], &w});
+        const std::vector<Tensor> t =
+            operate("mlpk::linear_bwd", go, maybe(saved[0]), maybe(saved[1]), w, maybe(saved[3]), maybe(saved[4]), act,
+                    type, want_dx, want_dw, want_db)
+                .toTensorVector();
+        size_t i = 0;
+        if (want_dx) got.dx = t[i++];
+        if (want_dw) got.dw = t[i++];
+        if (want_db) got.db = t[i++];
+      }
+    }
+    // Whether a gradient depends on an input that needs one itself.
+    const bool by_z = act != MLPK_ACT_NONE && (want_dx || want_dw || want_db);
+    return {once_if(got.dx, go, by_z || want_dw), once_if(got.dw, go, by_z || want_dx), once_if(got.db, go, by_z),
+            want_dr ? go : Tensor(), Tensor(), Tensor()};
+  }
+};
+
+struct GatedNode : torch::autograd::Function<GatedNode> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& wg, const Tensor& wu, const Tensor& wd,
+                               const std::optional<Tensor>& residual, int64_t act, bool fp8) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    const Tensor r = residual.value_or(Tensor());
+    const bool any = x.requires_grad() || wg.requires_grad() || wu.requires_grad() || wd.requires_grad();
+    auto [out, g, u] = gated_forward(x, wg, wu, wd, r, act, any ? (fp8 ? MLPK_KEEP_FP8 : MLPK_KEEP_16) : 0);
+    const Kept k = input_kept(x, wg.requires_grad() || wu.requires_grad(), fp8);
+    ctx->saved_data["act"] = act;
+    ctx->saved_data["residual"] = r.defined();
+    ctx->save_for_backward({k.v, k.scale, wg, wu, wd, g.v, g.scale, u.v, u.scale});
+    return {out};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const variable_list saved = ctx->get_saved_variables();
+    const Tensor &go = grads[0], &x = saved[0], &wg = saved[2], &wu = saved[3], &wd = saved[4];
+    const int64_t act = ctx->saved_data["act"].toInt();
+    const bool want_dx = ctx->needs_input_grad(0), want_g = ctx->needs_input_grad(1), want_u = ctx->needs_input_grad(2);
+    const bool want_d = ctx->needs_input_grad(3), any = want_dx || want_g || want_u || want_d;
+    const bool want_dr = ctx->saved_data["residual"].toBool() && ctx->needs_input_grad(4);
+    GatedGrads got;
+    if (!go.defined()) return variable_list(7);
+    if (any) {
+      const at::NoGradGuard no_grad;
+      if (direct({&go, &x, &wg, &wu, &wd})) {
+        got = gated_backward(go, {x, saved[1]}, wg, wu, wd, {saved[5], saved[6]}, {saved[7], saved[8]}, act, want_dx,
+                             want_g || want_u, want_d);
+      } else {
+        refuse_tangents({&go, &x, &wg, &wu, &wd});
+        const std::vector<Tensor> t =
+            operate("mlpk::gated_mlp_bwd", go, maybe(x), maybe(saved[1]), wg, wu, wd, saved[5], maybe(saved[6]), saved[7],
+                    maybe(saved[8]), act, want_dx, want_g || want_u, want_d)
+                .toTensorVector();
+        size_t i = 0;
+        if (want_dx) got.dx = t[i++];
+        if (want_g || want_u) {
+          got.dwg = t[i++];
+          got.dwu = t[i++];
+        }
+        if (want_d) got.dwd = t[i++];
+      }
+    }
+    return {once_if(got.dx, go, any),  once_if(want_g ? got.dwg : Tensor(), go, any),
+            once_if(want_u ? got.dwu : Tensor(), go, any), once_if(got.dwd, go, any),
+            want_dr ? go : Tensor(),   Tensor(), Tensor()};
+  }
+};
+
+bool ff_x(const Tensor& x) {
+  return x.is_cuda() && operand_type(x) && x.dim() >= 1 && ff_width(x.size(-1)) && rows_of(x) <= kFfMaxRows;
+}
+bool ff_weight(const Tensor& w, const Tensor& x, int64_t d_in) {
+  return w.dim() == 2 && w.size(0) == d_in && ff_width(w.size(1)) && w.scalar_type() == x.scalar_type() &&
+         w.device() == x.device();
+}
+bool ff_residual(const Tensor& r, const Tensor& x, int64_t d_out) {
+  return !r.defined() || (r.sizes() == at::IntArrayRef(with_width(x, d_out)) && r.scalar_type() == x.scalar_type() &&
+                          r.device() == x.device());
+}
+
+py::object linear(const Tensor& x, const Tensor& w, const std::optional<Tensor>& bias,
+                  const std::optional<Tensor>& residual, int64_t act, bool fp8) {
+  const Tensor b = bias.value_or(Tensor()), r = residual.value_or(Tensor());
+  if (act < 0 || act >= kActs || !ff_x(x) || !ff_weight(w, x, x.size(-1)) || !ff_residual(r, x, w.size(1)) ||
+      (b.defined() && (b.dim() != 1 || b.size(0) != w.size(1) || b.device() != x.device() || !weight_type(b, x))) ||
+      !direct({&x, &w, &b, &r}))
+    return py::none();
+  Tensor out;
+  {
+    py::gil_scoped_release no_gil;
+    out = needs_grad({&x, &w, &b, &r}) ? LinearNode::apply(x, w, maybe(b), maybe(r), act, fp8)[0]
+                                       : linear_kept(x, w, b, r, act, MLPK_KEEP_NONE).first;
+  }
+  return py::cast(out);
+}
+
+py::object gated_mlp(const Tensor& x, const Tensor& wg, const Tensor& wu, const Tensor& wd,
+                     const std::optional<Tensor>& residual, int64_t act, bool fp8) {
+  const Tensor r = residual.value_or(Tensor());
+  if (act < 0 || act >= kActs || !ff_x(x) || !ff_weight(wg, x, x.size(-1)) || !ff_weight(wu, x, x.size(-1)) ||
+      wu.size(1) != wg.size(1) || !ff_weight(wd, x, wg.size(1)) || !ff_residual(r, x, wd.size(1)) ||
+      !direct({&x, &wg, &wu, &wd, &r}))
+    return py::none();
+  Tensor out;
+  {
+    py::gil_scoped_release no_gil;
+    out = needs_grad({&x, &wg, &wu, &wd, &r}) ? GatedNode::apply(x, wg, wu, wd, maybe(r), act, fp8)[0]
+                                              : std::get<0>(gated_forward(x, wg, wu, wd, r, act, MLPK_KEEP_NONE));
+  }
+  return py::cast(out);
+}
+
+py::object fp8_checkpoint(const Tensor& x) {
+  if (!x.is_cuda() || code(x) < 0 || x.dim() < 1 || x.size(-1) < 1 || x.size(-1) > 0x7fffffff || needs_grad({&x}) ||
+      !direct({&x}))
+    return py::none();
+  Kept k;
+  {
+    py::gil_scoped_release no_gil;
+    k = checkpoint(x);
+  }
+  return py::make_tuple(k.v, k.scale);
+}
+py::object fp8_restore(const Tensor& q, const Tensor& scale, at::ScalarType type) {
+  if (!q.is_cuda() || q.scalar_type() != at::kFloat8_e4m3fn || q.dim() < 1 || q.size(-1) < 1 ||
+      q.size(-1) > 0x7fffffff || scale.scalar_type() != at::kFloat || scale.device() != q.device() ||
+      scale.sizes() != at::IntArrayRef(with_width(q, (q.size(-1) + 127) / 128)) || !direct({&q, &scale}))
+    return py::none();
+  Tensor x;
+  {
+    py::gil_scoped_release no_gil;
+    x = restore(q, scale, type);
+  }
+  return py::cast(x);
+}
+
 // ------------------------------------------------------------------ AdamW
 // Some tensors of one type and device with their places in the flat state and
 // in its step counts.
@@ -538,6 +922,40 @@ PYBIND11_MODULE(mlpk_torch, m) {
                                const Tensor& offsets, bool want_dy, bool want_dw) {
     return combine_backward(g, y, w.value_or(Tensor()), row_of, offsets, want_dy, want_dw);
   });
+  m.def("linear", &linear);
+  m.def("gated_mlp", &gated_mlp);
+  m.def("fp8_checkpoint", &fp8_checkpoint);
+  m.def("fp8_restore", &fp8_restore);
+  using Maybe = std::optional<Tensor>;
+  m.def("linear_forward", [](const Tensor& x, const Tensor& w, const Maybe& b, const Maybe& r, int64_t act, int64_t keep) {
+    const auto [out, z] = linear_kept(x, w, b.value_or(Tensor()), r.value_or(Tensor()), act, keep);
+    return std::make_tuple(out, maybe(z.v), maybe(z.scale));
+  });
+  m.def("linear_backward", [](const Tensor& go, const Maybe& x, const Maybe& x_scale, const Tensor& w, const Maybe& z,
+                              const Maybe& z_scale, int64_t act, bool db32, bool want_dx, bool want_dw, bool want_db) {
+    const LinearGrads g = linear_backward(go, {x.value_or(Tensor()), x_scale.value_or(Tensor())}, w,
+                                          {z.value_or(Tensor()), z_scale.value_or(Tensor())}, act,
+                                          db32 ? at::kFloat : go.scalar_type(), want_dx, want_dw, want_db);
+    return std::make_tuple(maybe(g.dx), maybe(g.dw), maybe(g.db));
+  });
+  m.def("gated_forward", [](const Tensor& x, const Tensor& wg, const Tensor& wu, const Tensor& wd, const Maybe& r,
+                            int64_t act, int64_t keep) {
+    const auto [out, g, u] = gated_forward(x, wg, wu, wd, r.value_or(Tensor()), act, keep);
+    return std::make_tuple(out, maybe(g.v), maybe(g.scale), maybe(u.v), maybe(u.scale));
+  });
+  m.def("gated_backward", [](const Tensor& go, const Maybe& x, const Maybe& x_scale, const Tensor& wg, const Tensor& wu,
+                             const Tensor& wd, const Tensor& g, const Maybe& g_scale, const Tensor& u,
+                             const Maybe& u_scale, int64_t act, bool want_dx, bool want_dgu, bool want_dd) {
+    const GatedGrads t = gated_backward(go, {x.value_or(Tensor()), x_scale.value_or(Tensor())}, wg, wu, wd,
+                                        {g, g_scale.value_or(Tensor())}, {u, u_scale.value_or(Tensor())}, act, want_dx,
+                                        want_dgu, want_dd);
+    return std::make_tuple(maybe(t.dx), maybe(t.dwg), maybe(t.dwu), maybe(t.dwd));
+  });
+  m.def("checkpoint", [](const Tensor& x) {
+    const Kept k = checkpoint(x);
+    return std::make_tuple(k.v, k.scale);
+  });
+  m.def("restore", &restore);
   // Whether two lists hold the same objects in the same order.
   m.def("same_items", [](const py::list& a, const py::list& b) {
     const Py_ssize_t n = PyList_GET_SIZE(a.ptr());
