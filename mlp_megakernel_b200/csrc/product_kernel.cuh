@@ -219,7 +219,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kProductThreads, 1)
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < ST; ++s) {
-      mbar_init(bar_full(s), 2);
+      mbar_init(bar_full(s), 1);
       mbar_init(bar_empty(s), 1);
     }
     for (int b = 0; b < 2; ++b) {
@@ -243,8 +243,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kProductThreads, 1)
 
   if (warp == 0) {
     // ------------------------------------------------------------ loads
-    if (lane == 0) {
-      int issued = 0;
+    if (elect_one()) {
+      int issued = 0, s = 0;
+      uint32_t phase = 1;
       bool ok = true;
       for (int t = cluster_id(); ok && t < total; t += step) {
         const TileAt at = product_tile(t, p.tiles_m, p.tiles_n, p.outputs, p.group);
@@ -256,13 +257,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kProductThreads, 1)
         const int own_a = p.out_a ? at.output : 0;
         const int own_b = EPI == kEpiGated ? static_cast<int>(rank) : p.out_a ? 0 : at.output;
         for (int kb = k0; kb < k1; ++kb, ++issued) {
-          const int s = issued % ST;
-          if (!mbar_wait_cluster(bar_empty(s), ((issued / ST) & 1) ^ 1, abort_flag, kDevTimeoutEmpty, status)) {
+          if (!mbar_wait_to(bar_empty(s), phase, abort_flag, kDevTimeoutEmpty, status)) {
             ok = false;
             break;
           }
+          // The leader expects the bytes of both CTAs.  (An arrival of each CTA
+          // on the leader's barrier, with its own bytes, needs a release at
+          // cluster scope for every stage, and the products ran at half their
+          // rate: 8192 x 4096 x 4096 bf16 380 us.)
           const uint32_t full = mapa_shared(bar_full(s), 0);
-          mbar_arrive_expect_tx_cluster(full, Cfg::STAGE);
+          if (rank == 0) mbar_arrive_expect_tx(bar_full(s), 2 * Cfg::STAGE);
           const bool second = kb >= p.nk0;
           const int k = (second ? kb - p.nk0 : kb) * kBlockK;
           const CUtensorMap* ma = &p.a[second ? 1 : own_a];
@@ -280,58 +284,60 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kProductThreads, 1)
           } else {
             tma_load_2d_pair(sb, mb, full, k, col);
           }
+          if (++s == ST) s = 0, phase ^= 1;
         }
       }
       // After a wait that ran out: nothing of the loads may still be under way
       // when the CTAs end (the leader's barriers count both CTAs' bytes).
       if (!ok && rank == 0)
-        for (int s = 0; s < ST && s < issued; ++s) {
-          const int uses = (issued - s + ST - 1) / ST;
-          mbar_wait_cluster(bar_full(s), (uses - 1) & 1, &no_abort, kDevTimeoutFull, status);
+        for (int b = 0; b < ST && b < issued; ++b) {
+          const int uses = (issued - b + ST - 1) / ST;
+          mbar_wait_to(bar_full(b), (uses - 1) & 1, &no_abort, kDevTimeoutFull, status);
         }
     }
     __syncwarp();
   } else if (warp == 1) {
     // ------------------------------------------------------------ products (leader)
-    if (rank == 0) {
-      const bool issuer = lane == 0;
+    // One elected thread does all of it: a warp that meets at each stage (a vote
+    // on its wait, a __syncwarp behind its instructions) costs the products
+    // their run-ahead.
+    if (rank == 0 && elect_one()) {
       // K-step of 16: 32 bytes along a K-contiguous row, 16 rows of 128 bytes otherwise.
       const uint64_t a_step = p.a_mn ? 16 * 128 / 16 : 2, b_step = p.b_mn ? 16 * 128 / 16 : 2;
-      const uint64_t a_base = make_sdesc(0, p.a_mn ? kBlockK * 128 : 16, 1024, 2);
-      const uint64_t b_base = make_sdesc(0, p.b_mn ? kBlockK * 128 : 16, 1024, 2);
+      const uint64_t a_base = make_sdesc(s_stage, p.a_mn ? kBlockK * 128 : 16, 1024, 2);
+      const uint64_t b_base = make_sdesc(s_stage + Cfg::A_BYTES, p.b_mn ? kBlockK * 128 : 16, 1024, 2);
       const uint32_t idesc = p.idesc;
       bool ok = true;
-      int used = 0, mine = 0;
+      int s = 0, mine = 0;
+      uint32_t phase = 0;
       for (int t = cluster_id(); ok && t < total; t += step, ++mine) {
         const TileAt at = product_tile(t, p.tiles_m, p.tiles_n, p.outputs, p.group);
         const int k0 = static_cast<int>(static_cast<int64_t>(at.split) * p.nk / p.splits);
         const int k1 = static_cast<int>(static_cast<int64_t>(at.split + 1) * p.nk / p.splits);
         const int buf = mine & 1;
-        ok = __all_sync(0xffffffffu, mbar_wait_cluster(bar_free(buf), ((mine >> 1) & 1) ^ 1, abort_flag,
-                                                       kDevTimeoutMma, status));
+        const uint32_t d = tmem + buf * TN;
+        ok = mbar_wait_cluster(bar_free(buf), ((mine >> 1) & 1) ^ 1, abort_flag, kDevTimeoutMma, status);
         if (!ok) break;
         tc_fence_after();
-        for (int kb = k0; kb < k1; ++kb, ++used) {
-          const int s = used % ST;
-          ok = __all_sync(0xffffffffu,
-                          mbar_wait_cluster(bar_full(s), (used / ST) & 1, abort_flag, kDevTimeoutMma, status));
+        uint32_t more = 0;  // the first product of a tile overwrites the accumulator
+        for (int kb = k0; kb < k1; ++kb) {
+          ok = mbar_wait_to(bar_full(s), phase, abort_flag, kDevTimeoutMma, status);
           if (!ok) break;
           tc_fence_after();
-          if (issuer) {
-            const uint32_t sa = s_stage + s * Cfg::STAGE;
-            const uint64_t da = a_base + (sa >> 4), db = b_base + ((sa + Cfg::A_BYTES) >> 4);
+          const uint64_t da = a_base + s * (Cfg::STAGE >> 4), db = b_base + s * (Cfg::STAGE >> 4);
 #pragma unroll
-            for (int kk = 0; kk < kBlockK / 16; ++kk)
-              umma_f16_pair(tmem + buf * TN, da + kk * a_step, db + kk * b_step, idesc, (kb > k0 || kk > 0) ? 1u : 0u);
-            umma_commit_pair(bar_empty(s));
-            if (kb + 1 == k1) umma_commit_pair(bar_acc(buf));
+          for (int kk = 0; kk < kBlockK / 16; ++kk) {
+            umma_f16_pair(d, da + kk * a_step, db + kk * b_step, idesc, more);
+            more = 1;
           }
-          __syncwarp();
+          umma_commit_pair(bar_empty(s));
+          if (++s == ST) s = 0, phase ^= 1;
         }
+        if (ok) umma_commit_pair(bar_acc(buf));
       }
-      if (issuer) umma_commit_pair(bar_done);
-      __syncwarp();
+      umma_commit_pair(bar_done);
     }
+    __syncwarp();
   } else {
     // ------------------------------------------------------------ epilogue
     const int w = warp - 2, quarter = warp & 3, half = w >> 2;
@@ -381,8 +387,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kProductThreads, 1)
       int chunks = 0;
       if (row0 < p.rows && col0 < p.cols) chunks = min(Cfg::CHUNKS, (p.cols - col0 + 31) / 32);
       if (with_in && chunks > 0) fetch(it, col0, row0);
-      ok = __all_sync(0xffffffffu,
-                      mbar_wait_cluster(bar_acc(buf), (mine >> 1) & 1, abort_flag, kDevTimeoutEpi, status));
+      ok = __all_sync(0xffffffffu, mbar_wait_to(bar_acc(buf), (mine >> 1) & 1, abort_flag, kDevTimeoutEpi, status));
       if (!ok) break;
       tc_fence_after();
       const uint32_t t_acc = t_lane + buf * TN;
@@ -588,7 +593,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kProductThreads, 1)
   // Every product that writes this CTA's accumulators is complete (waited for
   // here, where the rest of the CTA is through: the wait's bound is no bound on
   // the kernel's time).
-  if (threadIdx.x == 32) mbar_wait_cluster(bar_done, 0, &no_abort, kDevTimeoutMma, status);
+  if (threadIdx.x == 32) mbar_wait_to(bar_done, 0, &no_abort, kDevTimeoutMma, status);
   __syncwarp();
   cluster_sync();  // neither CTA leaves while the other may still signal its barriers
   if (warp == 1) {
