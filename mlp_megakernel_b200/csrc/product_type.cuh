@@ -6,6 +6,7 @@
 #include <atomic>
 #include <cstring>
 
+#include "few_rows_kernel.cuh"
 #include "product_kernel.cuh"
 #include "product_launch.cuh"
 
@@ -32,6 +33,9 @@ inline int pairs_at_once(const void* kern, int smem, int dev, int sm_count, std:
   known[dev].store(n, std::memory_order_relaxed);
   return n;
 }
+
+// The operands' format in an instruction descriptor made for fp16.
+inline uint32_t type_bits(bool bf16) { return bf16 ? (1u << 7 | 1u << 10) : 0u; }
 
 inline int ceil_div_int(int64_t a, int64_t b) { return static_cast<int>((a + b - 1) / b); }
 
@@ -61,7 +65,7 @@ int launch_tiles(const Product& c, cudaStream_t st) {
   a.b_mn = c.b_mn;
   a.out_a = c.out_a;
   a.idesc = make_idesc_f16(kPairRows, TN, c.a_mn, c.b_mn) |
-            (std::is_same_v<T, __nv_bfloat16> ? (1u << 7 | 1u << 10) : 0u);
+            type_bits(std::is_same_v<T, __nv_bfloat16>);
   a.act = c.act;
   a.keep_kind = c.keep_kind;
   a.residual = EPI == kEpiLinear && c.in[0] != nullptr;
@@ -93,8 +97,76 @@ int launch_tiles(const Product& c, cudaStream_t st) {
                              Cfg::SMEM, st, a);
 }
 
+template <class T, int EPI>
+int launch_few(const Product& c, cudaStream_t st) {
+  DevInfo di;
+  int dev = 0, rc = current_device_info(&di, &dev);
+  if (rc) return rc;
+  constexpr bool GATED = EPI == kEpiGated;
+  FewArgs a;
+  std::memset(&a, 0, sizeof(a));
+  a.rows = static_cast<int>(c.rows);
+  a.cols = c.cols;
+  a.nk0 = ceil_div_int(c.k[0], kBlockK);
+  a.nk = a.nk0 + ceil_div_int(c.k[1], kBlockK);
+  const FewPlan plan = few_plan(c.rows, c.cols, a.nk, GATED ? 64 : 128, di.sm_count);
+  a.nt = plan.nt;
+  a.stages = plan.stages;
+  a.w_mn = c.b_mn;
+  a.idesc = make_idesc_f16(128, plan.nt, c.b_mn, 0) | type_bits(std::is_same_v<T, __nv_bfloat16>);
+  a.act = c.act;
+  a.keep_kind = c.keep_kind;
+  a.bias = c.bias;
+  a.bias32 = c.bias32;
+  a.q_pitch = c.q_pitch;
+  a.scale_pitch = c.scale_pitch;
+  a.status = device_status_word(dev);
+  if (!a.status) return MLPK_ERR_CUDA;
+  for (int i = 0; i < 2; ++i) {
+    a.in[i] = c.in[i];
+    a.out[i] = c.out[i];
+    a.keep[i] = c.keep[i];
+    a.q[i] = c.q[i];
+    a.scale[i] = c.scale[i];
+    const uint64_t k = i == 1 && c.k[1] > 0 ? c.k[1] : c.k[0];
+    if (c.a[i] && (rc = make_map_2d(&a.x[i], c.a[i], k, c.rows, kBlockK, plan.nt))) return rc;
+    if (c.b[i] && (rc = c.b_mn ? make_map_2d(&a.w[i], c.b[i], c.cols, k, 64, kBlockK)
+                               : make_map_2d(&a.w[i], c.b[i], k, c.cols, kBlockK, GATED ? 64 : 128)))
+      return rc;
+  }
+  const auto kern = few_rows_kernel<T, EPI>;
+  const int smem = few_smem(plan.nt, plan.stages);
+  if (!blocks_per_sm(reinterpret_cast<const void*>(kern), kFewThreads, smem, dev)) return MLPK_ERR_CUDA;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(plan.tiles * plan.ranks, plan.row_tiles);
+  cfg.blockDim = dim3(kFewThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = plan.ranks;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  return cuda_status(cudaLaunchKernelEx(&cfg, kern, a));
+}
+
+// Rows up to which a product goes to few_rows_kernel.
+constexpr int kFewRows = 256;
+
 template <class T>
 int launch_type(const Product& c, cudaStream_t st) {
+  // A gate's checkpoint group is wider than a tile of few_rows_kernel.
+  if (c.rows <= kFewRows && !c.a_mn && !(c.epi == kEpiGated && c.keep_kind == kKeep8)) {
+    switch (c.epi) {
+      case kEpiPlain: return launch_few<T, kEpiPlain>(c, st);
+      case kEpiLinear: return launch_few<T, kEpiLinear>(c, st);
+      case kEpiGated: return launch_few<T, kEpiGated>(c, st);
+      default: return launch_few<T, kEpiGatedBwd>(c, st);
+    }
+  }
   switch (c.epi) {
     case kEpiPlain: return launch_tiles<T, kEpiPlain, 256>(c, st);
     case kEpiPartial: return launch_tiles<T, kEpiPartial, 256>(c, st);
