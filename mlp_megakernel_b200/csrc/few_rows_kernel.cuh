@@ -16,15 +16,15 @@
 // partner's, so that act(g) u has both.
 //
 // Roles: warp 0 loads (a ring of 64-deep stages: 16 KB of weights, NT x 128 B of
-// rows), warp 1 issues, warps 2..5 empty the accumulator; all warps run the
-// epilogue.
+// rows), warp 1 issues, warps 2..9 empty the accumulator (two to a quarter of its
+// lanes); all warps run the epilogue.
 #pragma once
 #include "few_rows_plan.cuh"
 #include "product_kernel.cuh"
 
 namespace mlpk {
 
-constexpr int kFewThreads = 192;
+constexpr int kFewThreads = 320;
 struct alignas(64) FewArgs {
   CUtensorMap x[2], w[2];  // [1]: the second reduction range, or the gate's partner (w)
   int rows, cols;
@@ -180,7 +180,7 @@ __global__ void __launch_bounds__(kFewThreads) few_rows_kernel(const __grid_cons
       float* dst = reinterpret_cast<float*>(gbase) + quarter * 32 + lane;
       const int live = min(nt, p.rows - row0);
 #pragma unroll 1
-      for (int c = 0; c < live; c += 16) {
+      for (int c = (warp - 2) / 4 * 16; c < live; c += 32) {
         uint32_t r[16];
         tmem_ld_wait_x16(t_lane + c, r);
 #pragma unroll
@@ -198,102 +198,112 @@ __global__ void __launch_bounds__(kFewThreads) few_rows_kernel(const __grid_cons
   cluster_sync();
 
   // A warp takes a row of the tile: 128 columns, 4 a thread (the gate: 64, two
-  // rows a warp).
-  constexpr int PER_ROW = TILE_COLS / 4;
+  // rows a warp).  Four rows at once, so that their reads of the other CTAs'
+  // shared memory are under way together (one at a time: 128 x 256 x 256 took 12.6
+  // us instead of 7).
+  constexpr int PER_ROW = TILE_COLS / 4, ROWS = 4;
   const int live = min(nt, p.rows - row0);
-  const int sub = lane % PER_ROW, step = ranks * (kFewThreads / 32) * (32 / PER_ROW);
+  const int sub = lane % PER_ROW, own = lane / PER_ROW, step = ranks * (kFewThreads / 32) * (32 / PER_ROW);
   const int col = col0 + 4 * sub;
-  for (int r = (rank * (kFewThreads / 32) + warp) * (32 / PER_ROW) + lane / PER_ROW; r - lane / PER_ROW < live;
-       r += step) {
-    const bool here = r < live && col < p.cols;
-    float v[4] = {}, u[4] = {};
-    if (r < live) {
-      const uint32_t at = sbase + (r * 128 + 4 * sub) * 4;
-#pragma unroll 4
-      for (int k = 0; k < ranks; ++k) {
-        const uint32_t peer = mapa_shared(at, k);
-        const float4 f = peer_load4(peer);
-        v[0] += f.x, v[1] += f.y, v[2] += f.z, v[3] += f.w;
+  for (int base = (rank * (kFewThreads / 32) + warp) * (32 / PER_ROW); base < live; base += ROWS * step) {
+    float all[ROWS][4] = {}, partner[ROWS][4] = {};
+#pragma unroll 2
+    for (int k = 0; k < ranks; ++k) {
+      const uint32_t peer = mapa_shared(sbase + 16 * sub, k);
+#pragma unroll
+      for (int i = 0; i < ROWS; ++i) {
+        const int r = base + own + i * step;
+        if (r >= live) break;
+        const float4 f = peer_load4(peer + r * 512);
+        all[i][0] += f.x, all[i][1] += f.y, all[i][2] += f.z, all[i][3] += f.w;
         if (GATED) {
-          const float4 g = peer_load4(peer + 64 * 4);
-          u[0] += g.x, u[1] += g.y, u[2] += g.z, u[3] += g.w;
+          const float4 g = peer_load4(peer + r * 512 + 256);
+          partner[i][0] += g.x, partner[i][1] += g.y, partner[i][2] += g.z, partner[i][3] += g.w;
         }
       }
     }
-    const int64_t row = row0 + r, at = row * p.cols + col;
-    if constexpr (EPI == kEpiPlain) {
-      if (here) store4(static_cast<T*>(p.out[0]) + at, v);
-    } else if constexpr (EPI == kEpiLinear) {
-      if (here && p.bias) {
-        float b[4];
-        if (p.bias32) load4(static_cast<const float*>(p.bias) + col, b);
-        else load4(static_cast<const T*>(p.bias) + col, b);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] += b[e];
-      }
-      if (p.keep_kind == kKeep16 && here) store4(static_cast<T*>(p.keep[0]) + at, v);
-      if (p.keep_kind == kKeep8) {  // a whole warp has the row's 128 columns (zeros beyond the last)
-        float inv, most = max_abs(max_abs(0.0f, v[0], v[1]), v[2], v[3]);
-        if (!here) most = 0.0f;
-#pragma unroll
-        for (int o = 16; o; o >>= 1) most = max_nan(most, __shfl_xor_sync(0xffffffffu, most, o));
-        const float s = checkpoint_scale(most, &inv);
-        if (here) {
-          const uint32_t lo = to_fp8x2(make_float2(v[0] * inv, v[1] * inv));
-          const uint32_t hi = to_fp8x2(make_float2(v[2] * inv, v[3] * inv));
-          *reinterpret_cast<uint32_t*>(p.q[0] + row * p.q_pitch + col) = lo | hi << 16;
-          if (sub == 0) p.scale[0][row * p.scale_pitch + col0 / kKeepGroup] = s;
+    for (int i = 0; i < ROWS; ++i) {
+      if (base + i * step >= live) break;
+      const int r = base + own + i * step;
+      const bool here = r < live && col < p.cols;
+      float(&v)[4] = all[i];
+      float(&u)[4] = partner[i];
+      const int64_t row = row0 + r, at = row * p.cols + col;
+      if constexpr (EPI == kEpiPlain) {
+        if (here) store4(static_cast<T*>(p.out[0]) + at, v);
+      } else if constexpr (EPI == kEpiLinear) {
+        if (here && p.bias) {
+          float b[4];
+          if (p.bias32) load4(static_cast<const float*>(p.bias) + col, b);
+          else load4(static_cast<const T*>(p.bias) + col, b);
+  #pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] += b[e];
         }
-      }
-      with_act(p.act, [&](auto a) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = act_value<decltype(a)::value>(v[e]);
-      });
-      if (here) {
-        if (p.in[0]) {
-          float f[4];
-          load4(static_cast<const T*>(p.in[0]) + at, f);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) v[e] += f[e];
-        }
-        store4(static_cast<T*>(p.out[0]) + at, v);
-      }
-    } else if constexpr (EPI == kEpiGated) {
-      if (here) {
-        if (p.keep_kind == kKeep16) {
-          store4(static_cast<T*>(p.keep[0]) + at, v);
-          store4(static_cast<T*>(p.keep[1]) + at, u);
-        }
-        with_act(p.act, [&](auto a) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) v[e] = act_value<decltype(a)::value>(v[e]) * u[e];
-        });
-        store4(static_cast<T*>(p.out[0]) + at, v);
-      }
-    } else {  // kEpiGatedBwd
-      if (here) {
-        float g[4], h[4];
-        if (p.keep_kind == kKeep16) {
-          load4(static_cast<const T*>(p.in[0]) + at, g);
-          load4(static_cast<const T*>(p.in[1]) + at, u);
-        } else {
-          const int64_t s = row * p.scale_pitch + col / kKeepGroup;
-          load_fp8x4(p.q[0] + row * p.q_pitch + col, p.scale[0][s], g);
-          load_fp8x4(p.q[1] + row * p.q_pitch + col, p.scale[1][s], u);
-        }
-        with_act(p.act, [&](auto a) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            float slope;
-            const float value = act_both<decltype(a)::value>(g[e], slope);
-            g[e] = v[e] * (u[e] * slope);
-            h[e] = u[e] * value;
-            v[e] *= value;
+        if (p.keep_kind == kKeep16 && here) store4(static_cast<T*>(p.keep[0]) + at, v);
+        if (p.keep_kind == kKeep8) {  // a whole warp has the row's 128 columns (zeros beyond the last)
+          float inv, most = max_abs(max_abs(0.0f, v[0], v[1]), v[2], v[3]);
+          if (!here) most = 0.0f;
+  #pragma unroll
+          for (int o = 16; o; o >>= 1) most = max_nan(most, __shfl_xor_sync(0xffffffffu, most, o));
+          const float s = checkpoint_scale(most, &inv);
+          if (here) {
+            const uint32_t lo = to_fp8x2(make_float2(v[0] * inv, v[1] * inv));
+            const uint32_t hi = to_fp8x2(make_float2(v[2] * inv, v[3] * inv));
+            *reinterpret_cast<uint32_t*>(p.q[0] + row * p.q_pitch + col) = lo | hi << 16;
+            if (sub == 0) p.scale[0][row * p.scale_pitch + col0 / kKeepGroup] = s;
           }
+        }
+        with_act(p.act, [&](auto a) {
+  #pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] = act_value<decltype(a)::value>(v[e]);
         });
-        store4(static_cast<T*>(p.out[0]) + at, g);
-        store4(static_cast<T*>(p.out[1]) + at, v);
-        store4(static_cast<T*>(p.keep[0]) + at, h);
+        if (here) {
+          if (p.in[0]) {
+            float f[4];
+            load4(static_cast<const T*>(p.in[0]) + at, f);
+  #pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] += f[e];
+          }
+          store4(static_cast<T*>(p.out[0]) + at, v);
+        }
+      } else if constexpr (EPI == kEpiGated) {
+        if (here) {
+          if (p.keep_kind == kKeep16) {
+            store4(static_cast<T*>(p.keep[0]) + at, v);
+            store4(static_cast<T*>(p.keep[1]) + at, u);
+          }
+          with_act(p.act, [&](auto a) {
+  #pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = act_value<decltype(a)::value>(v[e]) * u[e];
+          });
+          store4(static_cast<T*>(p.out[0]) + at, v);
+        }
+      } else {  // kEpiGatedBwd
+        if (here) {
+          float g[4], h[4];
+          if (p.keep_kind == kKeep16) {
+            load4(static_cast<const T*>(p.in[0]) + at, g);
+            load4(static_cast<const T*>(p.in[1]) + at, u);
+          } else {
+            const int64_t s = row * p.scale_pitch + col / kKeepGroup;
+            load_fp8x4(p.q[0] + row * p.q_pitch + col, p.scale[0][s], g);
+            load_fp8x4(p.q[1] + row * p.q_pitch + col, p.scale[1][s], u);
+          }
+          with_act(p.act, [&](auto a) {
+  #pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              float slope;
+              const float value = act_both<decltype(a)::value>(g[e], slope);
+              g[e] = v[e] * (u[e] * slope);
+              h[e] = u[e] * value;
+              v[e] *= value;
+            }
+          });
+          store4(static_cast<T*>(p.out[0]) + at, g);
+          store4(static_cast<T*>(p.out[1]) + at, v);
+          store4(static_cast<T*>(p.keep[0]) + at, h);
+        }
       }
     }
   }

@@ -28,8 +28,10 @@ inline FewPlan few_plan(int64_t rows, int cols, int nk, int tile_cols, int sm_co
   FewPlan p;
   p.nt = 16;
   while (p.nt < rows && p.nt < kFewMostRows) p.nt *= 2;
-  // Two CTAs an SM, so that one loads while the other adds; wide tiles one.
-  const int each_sm = p.nt < kFewMostRows ? 2 : 1;
+  // Two CTAs an SM for the narrowest tiles, one for the others: a wide tile meets
+  // in more shared memory than it is worth to share it further (128 x 4096 x 4096
+  // bf16: 8 ranks 15.6 us, 4 ranks 11.4).
+  const int each_sm = p.nt <= 32 ? 2 : 1;
   p.stages = kFewMaxStages;
   while (p.stages > 2 && few_smem(p.nt, p.stages) > (each_sm == 2 ? 113 * 1024 : 226 * 1024)) --p.stages;
   p.tiles = (cols + tile_cols - 1) / tile_cols;

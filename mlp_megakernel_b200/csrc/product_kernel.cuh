@@ -11,8 +11,10 @@
 // blocks of 64 through a ring of TMA loads; operands are fp16 or bf16 in either
 // order (K contiguous, or the row / column index), chosen at run time by the
 // descriptors alone.  Roles of a CTA: warp 0 loads, warp 1 of the leader issues
-// the tcgen05 instructions, warps 2..9 are the epilogue (thread = row; two warps
-// share the 32 rows of a TMEM lane quarter and halve the columns).  Two
+// the tcgen05 instructions, warps 2..17 are the epilogue (thread = row; four warps
+// share the 32 rows of a TMEM lane quarter and quarter the columns: an epilogue is
+// a chain of waits, and eight warps left the gate's backward at twice the time of
+// its products).  Two
 // accumulators of TN columns, so the epilogue of a tile runs beside the products
 // of the next.  The kernel is persistent: tiles are taken in groups of `group`
 // row tiles over all column tiles, so that the pairs at work share rows and
@@ -35,23 +37,23 @@ enum Keep : int { kKeepNone = 0, kKeep16 = 1, kKeep8 = 2 };
 constexpr int kPairRows = 256;      // rows of a pair's tile
 constexpr int kBlockK = 64;         // reduction of a stage: one 128-byte row of 16-bit values
 constexpr int kKeepGroup = 128;     // columns that share a scale
-constexpr int kProductThreads = 320;
-constexpr int kEpiWarps = 8;
-constexpr int kTileBytes = 2048;    // 32 rows x 32 columns of 16-bit values, a warp's unit of TMA traffic
+constexpr int kEpiWarps = 16;
+constexpr int kProductThreads = 32 * (2 + kEpiWarps);
 
 struct alignas(64) ProductArgs {
   CUtensorMap a[2], b[2];  // [1]: the second reduction range (nk0 < nk), or the gate's partner / second output's B
-  CUtensorMap in[2];       // linear: residual; gated backward: g, u (16 bits)
   CUtensorMap out[2];      // plain: D (two of them with `outputs` 2); linear: out; gated: h; backward: dg, du
   CUtensorMap keep[2];     // linear: z; gated: g, u; backward: h
+  CUtensorMap in[2];       // backward: g, u (16 bits)
   int rows, cols;          // of each output
   int nk0, nk;             // blocks of the first reduction range, and of both
   int tiles_m, tiles_n, outputs, splits, group;
   int a_mn, b_mn;          // the operand's contiguous index is the row / column, not the reduction
   int out_a;               // with two outputs: A differs, not B
   uint32_t idesc;
-  int act, keep_kind, residual, bias32;
+  int act, keep_kind, bias32;
   const void* bias;
+  const void* residual;
   uint8_t* q[2];           // 8-bit values, rows of q_pitch bytes
   float* scale[2];         // [rows][scale_pitch]
   int64_t q_pitch;
@@ -65,21 +67,24 @@ struct ProductCfg {
   static constexpr int A_BYTES = 128 * kBlockK * 2;
   static constexpr int B_BYTES = TN / 2 * kBlockK * 2;
   static constexpr int STAGE = A_BYTES + B_BYTES;
-  // A warp's buffers of 2 KB: two for outputs in turn; residual / out and z, two
-  // of each; a ring of four for h, g, u; two pairs g / dg, u / du and one for h.
-  static constexpr int BUFS = EPI == kEpiPlain ? 2 : EPI == kEpiPartial ? 0 : EPI == kEpiGatedBwd ? 5 : 4;
+  static constexpr int OUT_COLS = EPI == kEpiGated ? TN / 2 : TN;  // columns of an output that a tile has
+  static constexpr int PART = OUT_COLS / 4;  // columns of an epilogue warp
+  // A warp's unit of TMA traffic: 32 rows of at most 32 columns, in two buffers
+  // in turn.
+  static constexpr int CHUNK = PART < 32 ? PART : 32;
+  static constexpr int PITCH = CHUNK * 2;
+  static constexpr int TILE = 32 * PITCH;
+  static constexpr int BUFS = EPI == kEpiPartial ? 0 : 2;
   static constexpr int OFF_EPI = 0;
-  static constexpr int EPI_BYTES = kEpiWarps * BUFS * kTileBytes;
+  static constexpr int EPI_BYTES = kEpiWarps * BUFS * TILE;
   static constexpr int STAGES_FIT = (227 * 1024 - 2048 - EPI_BYTES) / STAGE;
   static constexpr int STAGES = STAGES_FIT < 8 ? STAGES_FIT : 8;
   static constexpr int OFF_STAGE = EPI_BYTES;
   static constexpr int OFF_BAR = OFF_STAGE + STAGES * STAGE;
-  static constexpr int NUM_BARS = 2 * STAGES + 5 + 2 * kEpiWarps;
+  static constexpr int NUM_BARS = 2 * STAGES + 5 + kEpiWarps;
   static constexpr int OFF_MISC = OFF_BAR + 8 * NUM_BARS;
   static constexpr int SMEM = OFF_MISC + 16 + 1024;
-  static constexpr int OUT_COLS = EPI == kEpiGated ? TN / 2 : TN;  // columns of an output that a tile has
-  static constexpr int HALF = OUT_COLS / 2;
-  static constexpr int CHUNKS = HALF / 32;
+  static constexpr int CHUNKS = PART / CHUNK;
   static_assert(EPI_BYTES % 1024 == 0 && STAGE % 1024 == 0 && SMEM <= 227 * 1024, "shared memory");
   static_assert(STAGES >= 3 && (TN == 128 || TN == 256), "tile");
 };
@@ -102,39 +107,6 @@ __host__ __device__ inline TileAt product_tile(int t, int tiles_m, int tiles_n, 
   return at;
 }
 
-// 32 values as pairs of the type.
-template <class T>
-__device__ __forceinline__ void pack32(const float (&v)[32], uint32_t (&p)[16]) {
-#pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const typename Pair<T>::type x = Pair<T>::round(v[2 * i], v[2 * i + 1]);
-    p[i] = *reinterpret_cast<const uint32_t*>(&x);
-  }
-}
-template <class T>
-__device__ __forceinline__ void unpack32(const uint32_t (&p)[16], float (&v)[32]) {
-#pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const float2 f = to_float2(*reinterpret_cast<const typename Pair<T>::type*>(&p[i]));
-    v[2 * i] = f.x;
-    v[2 * i + 1] = f.y;
-  }
-}
-// A thread's row of a 32 x 32 tile in shared memory (64-byte rows, as a TMA box
-// with the 64-byte swizzle has them).
-__device__ __forceinline__ void tile_row_store(uint32_t tile, int lane, const uint32_t (&p)[16]) {
-#pragma unroll
-  for (int u = 0; u < 4; ++u)
-    st_shared_v4(tile + swz_off<64>(lane, u), p[4 * u], p[4 * u + 1], p[4 * u + 2], p[4 * u + 3]);
-}
-__device__ __forceinline__ void tile_row_load(uint32_t tile, int lane, uint32_t (&p)[16]) {
-#pragma unroll
-  for (int u = 0; u < 4; ++u)
-    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                 : "=r"(p[4 * u]), "=r"(p[4 * u + 1]), "=r"(p[4 * u + 2]), "=r"(p[4 * u + 3])
-                 : "r"(tile + swz_off<64>(lane, u))
-                 : "memory");
-}
 __device__ __forceinline__ void tmem_load32(uint32_t taddr, float (&v)[32]) {
   uint32_t r[32];
   tmem_ld_wait_x32(taddr, r);
@@ -142,7 +114,7 @@ __device__ __forceinline__ void tmem_load32(uint32_t taddr, float (&v)[32]) {
   for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
 }
 
-// 32 values of a row to 8 bits (q is 32-byte aligned) and back.
+// 32 values of a row to 8 bits (q is 32-byte aligned).
 __device__ __forceinline__ void store_fp8x32(uint8_t* q, const float (&v)[32], float inv) {
   uint32_t w[8];
 #pragma unroll
@@ -154,16 +126,15 @@ __device__ __forceinline__ void store_fp8x32(uint8_t* q, const float (&v)[32], f
   reinterpret_cast<uint4*>(q)[0] = make_uint4(w[0], w[1], w[2], w[3]);
   reinterpret_cast<uint4*>(q)[1] = make_uint4(w[4], w[5], w[6], w[7]);
 }
-__device__ __forceinline__ void load_fp8x32(const uint8_t* q, float scale, float (&v)[32]) {
-  const Raw<uint16_t, 8> a = load_raw<uint16_t, 8>(reinterpret_cast<const uint16_t*>(q));
-  const Raw<uint16_t, 8> b = load_raw<uint16_t, 8>(reinterpret_cast<const uint16_t*>(q) + 8);
+// 16 of a row's 8-bit values (4 words of them) as fp32.
+__device__ __forceinline__ void widen_fp8x16(const uint32_t* w, float scale, float (&v)[16]) {
+  Raw<uint16_t, 8> r;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r.v[2 * i] = static_cast<uint16_t>(w[i]), r.v[2 * i + 1] = static_cast<uint16_t>(w[i] >> 16);
   float2 f[8];
-  unpack_fp8<16>(a, f);
+  unpack_fp8<16>(r, f);
 #pragma unroll
   for (int i = 0; i < 8; ++i) v[2 * i] = f[i].x * scale, v[2 * i + 1] = f[i].y * scale;
-  unpack_fp8<16>(b, f);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) v[16 + 2 * i] = f[i].x * scale, v[17 + 2 * i] = f[i].y * scale;
 }
 
 // v += bias[col ..]; a vector of 8 columns is inside the tensor or outside.
@@ -184,6 +155,73 @@ __device__ __forceinline__ void add_bias(const ProductArgs& p, int col, float (&
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[8 * k + e] += b[e];
   }
+}
+
+// 32 values of a row, 16 bits each, from `at` on: those of `cols` columns (a
+// multiple of 8), zeros beyond.  A thread takes its own row: whole sectors of 32
+// bytes where the rows are aligned to them.
+template <class T>
+__device__ __forceinline__ void row_load32(const void* in, int64_t at, int cols, uint32_t (&p)[16]) {
+  const T* src = static_cast<const T*>(in) + at;
+  if (cols >= 32 && reinterpret_cast<uintptr_t>(src) % 32 == 0) {
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+      asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                   : "=r"(p[8 * k]), "=r"(p[8 * k + 1]), "=r"(p[8 * k + 2]), "=r"(p[8 * k + 3]), "=r"(p[8 * k + 4]),
+                     "=r"(p[8 * k + 5]), "=r"(p[8 * k + 6]), "=r"(p[8 * k + 7])
+                   : "l"(src + 16 * k)
+                   : "memory");
+    return;
+  }
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    uint4 v = make_uint4(0, 0, 0, 0);
+    if (8 * k < cols) v = *reinterpret_cast<const uint4*>(src + 8 * k);
+    p[4 * k] = v.x, p[4 * k + 1] = v.y, p[4 * k + 2] = v.z, p[4 * k + 3] = v.w;
+  }
+}
+// Pairs of the type as fp32.
+template <class T>
+__device__ __forceinline__ float2 widen(uint32_t p) {
+  return to_float2(*reinterpret_cast<const typename Pair<T>::type*>(&p));
+}
+// N values of a thread's row, from column `from` on, into and from its tile in
+// shared memory (as a TMA box with the row's swizzle has it).
+template <class T, int PITCH, int N>
+__device__ __forceinline__ void tile_store(uint32_t tile, int lane, int from, const float (&v)[N]) {
+#pragma unroll
+  for (int u = 0; u < N / 8; ++u) {
+    uint32_t p[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const typename Pair<T>::type x = Pair<T>::round(v[8 * u + 2 * i], v[8 * u + 2 * i + 1]);
+      p[i] = *reinterpret_cast<const uint32_t*>(&x);
+    }
+    st_shared_v4(tile + swz_off<PITCH>(lane, from / 8 + u), p[0], p[1], p[2], p[3]);
+  }
+}
+template <class T, int PITCH, int N>
+__device__ __forceinline__ void tile_load(uint32_t tile, int lane, int from, float (&v)[N]) {
+#pragma unroll
+  for (int u = 0; u < N / 8; ++u) {
+    uint32_t p[4];
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(p[0]), "=r"(p[1]), "=r"(p[2]), "=r"(p[3])
+                 : "r"(tile + swz_off<PITCH>(lane, from / 8 + u))
+                 : "memory");
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = widen<T>(p[i]);
+      v[8 * u + 2 * i] = f.x;
+      v[8 * u + 2 * i + 1] = f.y;
+    }
+  }
+}
+__device__ __forceinline__ void tmem_load16(uint32_t taddr, float (&v)[16]) {
+  uint32_t r[16];
+  tmem_ld_wait_x16(taddr, r);
+#pragma unroll
+  for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
 }
 
 __device__ __forceinline__ float most_of(float most, const float (&v)[32]) {
@@ -207,7 +245,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kProductThreads, 1)
   auto bar_acc = [&](int b) { return s_bar + 8u * (2 * ST + b); };       // both: accumulator b is complete
   auto bar_free = [&](int b) { return s_bar + 8u * (2 * ST + 2 + b); };  // leader: both epilogues have read it
   const uint32_t bar_done = s_bar + 8u * (2 * ST + 4);
-  auto bar_in = [&](int w, int b) { return s_bar + 8u * (2 * ST + 5 + 2 * w + b); };  // a warp's tiles of `in`
+  auto bar_in = [&](int w) { return s_bar + 8u * (2 * ST + 5 + w); };  // a warp's tiles of `in` have landed
   const uint32_t s_tmem = sbase + Cfg::OFF_MISC;
   volatile int* abort_flag = reinterpret_cast<volatile int*>(gbase + Cfg::OFF_MISC + 4);
   volatile int no_abort = 0;
@@ -227,7 +265,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kProductThreads, 1)
       mbar_init(bar_free(b), 2 * kEpiWarps);
     }
     mbar_init(bar_done, 1);
-    for (int w = 0; w < 2 * kEpiWarps; ++w) mbar_init(bar_in(0, w), 1);
+    for (int w = 0; w < kEpiWarps; ++w) mbar_init(bar_in(w), 1);
     *abort_flag = 0;
     fence_mbar_init();
   }
@@ -340,23 +378,22 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kProductThreads, 1)
     __syncwarp();
   } else {
     // ------------------------------------------------------------ epilogue
-    const int w = warp - 2, quarter = warp & 3, half = w >> 2;
+    const int w = warp - 2, quarter = warp & 3, part = w >> 2;
     const uint32_t t_lane = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
-    const uint32_t s_buf = sbase + Cfg::OFF_EPI + w * Cfg::BUFS * kTileBytes;
-    const bool with_in = (EPI == kEpiLinear && p.residual) || (EPI == kEpiGatedBwd && p.keep_kind == kKeep16);
+    constexpr int CHUNK = Cfg::CHUNK, PITCH = Cfg::PITCH;
+    const uint32_t s_buf = sbase + Cfg::OFF_EPI + w * Cfg::BUFS * Cfg::TILE;
+    const bool by_tma = EPI == kEpiGatedBwd && p.keep_kind == kKeep16;  // g and u come as tiles
     bool ok = true;
-    int it = 0;       // chunks so far: the turn of the buffers
-    int fetched = 0;  // chunks whose `in` has been asked for
-    int ring = 0;  // tiles stored so far (buffers in turn)
-    // A tile into the next buffer of the ring, and its store.
-    auto put = [&](const CUtensorMap* map, const float(&v)[32], int col, int row) {
-      constexpr int N = Cfg::BUFS > 0 ? Cfg::BUFS : 1;
-      const uint32_t tile = s_buf + (ring++ % N) * kTileBytes;
-      if (lane == 0) bulk_wait_group_read<N - 1>();
+    int turn = 0;  // tiles stored so far
+    // The next of the two buffers, once the store that used it last has read it;
+    // and its store.
+    auto begin_tile = [&]() -> uint32_t {
+      const uint32_t tile = s_buf + (turn++ & 1) * Cfg::TILE;
+      if (lane == 0) bulk_wait_group_read<1>();
       __syncwarp();
-      uint32_t packed[16];
-      pack32<T>(v, packed);
-      tile_row_store(tile, lane, packed);
+      return tile;
+    };
+    auto end_tile = [&](const CUtensorMap* map, uint32_t tile, int col, int row) {
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) {
@@ -364,50 +401,80 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kProductThreads, 1)
         bulk_commit_group();
       }
     };
-    // The tile(s) of `in` for the it-th chunk, into its turn's buffers, once
-    // every store so far has read its buffer.
-    auto fetch = [&](int turn, int col, int row) {
-      fetched = turn + 1;
-      if (lane == 0) {
-        bulk_wait_group_read<0>();
-        const uint32_t tile = s_buf + (turn & 1) * (EPI == kEpiGatedBwd ? 2 : 1) * kTileBytes;
-        mbar_arrive_expect_tx(bar_in(w, turn & 1), EPI == kEpiGatedBwd ? 2 * kTileBytes : kTileBytes);
-        tma_load_2d(tile, &p.in[0], bar_in(w, turn & 1), col, row);
-        if (EPI == kEpiGatedBwd) tma_load_2d(tile + kTileBytes, &p.in[1], bar_in(w, turn & 1), col, row);
-      }
-    };
     int mine = 0;
+    uint32_t in_phase = 0;
     for (int t = cluster_id(); ok && t < total; t += step, ++mine) {
       const TileAt at = product_tile(t, p.tiles_m, p.tiles_n, p.outputs, p.group);
       const int buf = mine & 1;
       const int row0 = at.m * kPairRows + static_cast<int>(rank) * 128 + quarter * 32;
       const int row = row0 + lane;
-      const int first = at.n * Cfg::OUT_COLS, col0 = first + half * Cfg::HALF;
+      const int first = at.n * Cfg::OUT_COLS, col0 = first + part * Cfg::PART;
       // Chunks with something to store.
       int chunks = 0;
-      if (row0 < p.rows && col0 < p.cols) chunks = min(Cfg::CHUNKS, (p.cols - col0 + 31) / 32);
-      if (with_in && chunks > 0) fetch(it, col0, row0);
+      if (row0 < p.rows && col0 < p.cols) chunks = min(Cfg::CHUNKS, (p.cols - col0 + CHUNK - 1) / CHUNK);
+      // g and u of a chunk into the two buffers, once every store has read them.
+      auto fetch_tiles = [&](int col) {
+        if (lane == 0) {
+          bulk_wait_group_read<0>();
+          mbar_arrive_expect_tx(bar_in(w), 2 * Cfg::TILE);
+          tma_load_2d(s_buf, &p.in[0], bar_in(w), col, row0);
+          tma_load_2d(s_buf + Cfg::TILE, &p.in[1], bar_in(w), col, row0);
+        }
+        __syncwarp();
+      };
+      // What the thread itself reads, 32 columns ahead.
+      uint32_t in0[16] = {}, in1[16] = {};
+      auto fetch_row = [&](int col) {
+        if (row >= p.rows || col >= p.cols) return;
+        if constexpr (EPI == kEpiGatedBwd) {
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const uint4* src = reinterpret_cast<const uint4*>(p.q[k] + row * p.q_pitch + col);
+            const uint4 x = src[0], y = src[1];
+            uint32_t(&in)[16] = k ? in1 : in0;
+            in[0] = x.x, in[1] = x.y, in[2] = x.z, in[3] = x.w, in[4] = y.x, in[5] = y.y, in[6] = y.z, in[7] = y.w;
+          }
+        } else {
+          row_load32<T>(p.residual, static_cast<int64_t>(row) * p.cols + col, p.cols - col, in0);
+        }
+      };
+      const bool by_row = (EPI == kEpiLinear && p.residual) || (EPI == kEpiGatedBwd && !by_tma);
+      float sg = 0.0f, su = 0.0f;  // the row's scales of a backward in 8 bits
+      if (by_tma && chunks > 0) fetch_tiles(col0);
+      if (by_row && chunks > 0) {
+        fetch_row(col0);
+        if (EPI == kEpiGatedBwd && row < p.rows) {
+          const int64_t o = static_cast<int64_t>(row) * p.scale_pitch + col0 / kKeepGroup;
+          sg = p.scale[0][o];
+          su = p.scale[1][o];
+        }
+      }
       ok = __all_sync(0xffffffffu, mbar_wait_to(bar_acc(buf), (mine >> 1) & 1, abort_flag, kDevTimeoutEpi, status));
-      if (!ok) break;
+      if (!ok) {
+        if (by_tma && chunks > 0) mbar_wait_to(bar_in(w), in_phase, &no_abort, kDevTimeoutEpi, status);
+        break;
+      }
       tc_fence_after();
-      const uint32_t t_acc = t_lane + buf * TN;
+      const uint32_t t_acc = t_lane + buf * TN, t_part = t_acc + part * Cfg::PART;
       if constexpr (EPI == kEpiPlain) {
 #pragma unroll 1
         for (int c = 0; c < chunks; ++c) {
           float v[32];
-          tmem_load32(t_acc + half * Cfg::HALF + 32 * c, v);
-          put(&p.out[at.output], v, col0 + 32 * c, row0);
+          tmem_load32(t_part + CHUNK * c, v);
+          const uint32_t tile = begin_tile();
+          tile_store<T, PITCH>(tile, lane, 0, v);
+          end_tile(&p.out[at.output], tile, col0 + CHUNK * c, row0);
         }
       } else if constexpr (EPI == kEpiPartial) {
         float* dst = p.partials + ((static_cast<int64_t>(at.split) * p.outputs + at.output) * p.rows + row) * p.cols;
 #pragma unroll 1
         for (int c = 0; c < chunks; ++c) {
           float v[32];
-          tmem_load32(t_acc + half * Cfg::HALF + 32 * c, v);
+          tmem_load32(t_part + CHUNK * c, v);
           if (row < p.rows) {
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-              const int col = col0 + 32 * c + 8 * k;
+              const int col = col0 + CHUNK * c + 8 * k;
               float2 f[4];
 #pragma unroll
               for (int e = 0; e < 4; ++e) f[e] = make_float2(v[8 * k + 2 * e], v[8 * k + 2 * e + 1]);
@@ -420,34 +487,34 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kProductThreads, 1)
         if (p.keep_kind == kKeep8 && chunks > 0) {
           // The largest magnitude of the row's 128 columns: a half of a wide
           // tile, or all of a narrow one.
-          const int g0 = TN == 256 ? col0 : first;
+          const int g0 = first + part * Cfg::PART / kKeepGroup * kKeepGroup;
           float most = 0.0f;
 #pragma unroll 1
-          for (int c = 0; c < 4 && g0 + 32 * c < p.cols; ++c) {
+          for (int c = 0; c < kKeepGroup && g0 + c < p.cols; c += 32) {
             float v[32];
-            tmem_load32(t_acc + (g0 - first) + 32 * c, v);
-            if (p.bias) add_bias<T>(p, g0 + 32 * c, v);
+            tmem_load32(t_acc + (g0 - first) + c, v);
+            if (p.bias) add_bias<T>(p, g0 + c, v);
             most = most_of(most, v);
           }
           const float s = checkpoint_scale(most, &inv);
           if (row < p.rows && g0 == col0) p.scale[0][static_cast<int64_t>(row) * p.scale_pitch + g0 / kKeepGroup] = s;
         }
 #pragma unroll 1
-        for (int c = 0; c < chunks; ++c, ++it) {
-          const int col = col0 + 32 * c;
-          if (with_in && c + 1 < chunks) fetch(it + 1, col + 32, row0);
-          if (!with_in) {
-            if (lane == 0) bulk_wait_group_read<1>();
-            __syncwarp();
-          }
-          const uint32_t tile = s_buf + (it & 1) * kTileBytes, ztile = tile + 2 * kTileBytes;
+        for (int c = 0; c < chunks; ++c) {
+          const int col = col0 + CHUNK * c;
           float v[32];
-          uint32_t packed[16];
-          tmem_load32(t_acc + half * Cfg::HALF + 32 * c, v);
+          uint32_t r[16];
+          tmem_load32(t_part + CHUNK * c, v);
+          if (p.residual) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) r[i] = in0[i];
+            if (c + 1 < chunks) fetch_row(col + CHUNK);
+          }
           if (p.bias) add_bias<T>(p, col, v);
           if (p.keep_kind == kKeep16) {
-            pack32<T>(v, packed);
-            tile_row_store(ztile, lane, packed);
+            const uint32_t tile = begin_tile();
+            tile_store<T, PITCH>(tile, lane, 0, v);
+            end_tile(&p.keep[0], tile, col, row0);
           } else if (p.keep_kind == kKeep8 && row < p.rows) {
             store_fp8x32(p.q[0] + row * p.q_pitch + col, v, inv);
           }
@@ -455,25 +522,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kProductThreads, 1)
 #pragma unroll
             for (int i = 0; i < 32; ++i) v[i] = act_value<decltype(a)::value>(v[i]);
           });
-          if (with_in) {
-            ok = __all_sync(0xffffffffu,
-                            mbar_wait_to(bar_in(w, it & 1), (it >> 1) & 1, abort_flag, kDevTimeoutEpi, status));
-            if (!ok) break;
-            float r[32];
-            tile_row_load(tile, lane, packed);
-            unpack32<T>(packed, r);
+          if (p.residual) {
 #pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] += r[i];
+            for (int i = 0; i < 16; ++i) {
+              const float2 f = widen<T>(r[i]);
+              v[2 * i] += f.x;
+              v[2 * i + 1] += f.y;
+            }
           }
-          pack32<T>(v, packed);
-          tile_row_store(tile, lane, packed);
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) {
-            tma_store_2d(&p.out[0], tile, col, row0);
-            if (p.keep_kind == kKeep16) tma_store_2d(&p.keep[0], ztile, col, row0);
-            bulk_commit_group();
-          }
+          const uint32_t tile = begin_tile();
+          tile_store<T, PITCH>(tile, lane, 0, v);
+          end_tile(&p.out[0], tile, col, row0);
         }
       } else if constexpr (EPI == kEpiGated) {
         // The gate's columns come first, its partner's after them.
@@ -481,110 +540,119 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kProductThreads, 1)
         if (p.keep_kind == kKeep8 && chunks > 0) {
           float most_g = 0.0f, most_u = 0.0f;
 #pragma unroll 1
-          for (int c = 0; c < Cfg::OUT_COLS / 32; ++c) {
+          for (int c = 0; c < Cfg::OUT_COLS; c += 32) {
             float v[32];
-            tmem_load32(t_acc + 32 * c, v);
+            tmem_load32(t_acc + c, v);
             most_g = most_of(most_g, v);
-            tmem_load32(t_acc + TN / 2 + 32 * c, v);
+            tmem_load32(t_acc + TN / 2 + c, v);
             most_u = most_of(most_u, v);
           }
-          const float sg = checkpoint_scale(most_g, &inv_g), su = checkpoint_scale(most_u, &inv_u);
-          if (row < p.rows && half == 0) {
+          const float s_g = checkpoint_scale(most_g, &inv_g), s_u = checkpoint_scale(most_u, &inv_u);
+          if (row < p.rows && part == 0) {
             const int64_t o = static_cast<int64_t>(row) * p.scale_pitch + first / kKeepGroup;
-            p.scale[0][o] = sg;
-            p.scale[1][o] = su;
+            p.scale[0][o] = s_g;
+            p.scale[1][o] = s_u;
           }
         }
-#pragma unroll 1
-        for (int c = 0; c < chunks; ++c) {
-          const int col = col0 + 32 * c;
-          float g[32], u[32];
-          tmem_load32(t_acc + half * Cfg::HALF + 32 * c, g);
-          tmem_load32(t_acc + TN / 2 + half * Cfg::HALF + 32 * c, u);
+        if (chunks > 0) {  // one: a warp's part is a chunk
+          float g[CHUNK], u[CHUNK];
+#pragma unroll
+          for (int from = 0; from < CHUNK; from += 16) {
+            float v[16];
+            tmem_load16(t_part + from, v);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) g[from + i] = v[i];
+            tmem_load16(t_part + TN / 2 + from, v);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) u[from + i] = v[i];
+          }
           if (p.keep_kind == kKeep16) {
-            put(&p.keep[0], g, col, row0);
-            put(&p.keep[1], u, col, row0);
-          } else if (p.keep_kind == kKeep8 && row < p.rows) {
-            store_fp8x32(p.q[0] + row * p.q_pitch + col, g, inv_g);
-            store_fp8x32(p.q[1] + row * p.q_pitch + col, u, inv_u);
+            uint32_t tile = begin_tile();
+            tile_store<T, PITCH>(tile, lane, 0, g);
+            end_tile(&p.keep[0], tile, col0, row0);
+            tile = begin_tile();
+            tile_store<T, PITCH>(tile, lane, 0, u);
+            end_tile(&p.keep[1], tile, col0, row0);
+          }
+          if constexpr (CHUNK == 32) {
+            if (p.keep_kind == kKeep8 && row < p.rows) {
+              store_fp8x32(p.q[0] + row * p.q_pitch + col0, g, inv_g);
+              store_fp8x32(p.q[1] + row * p.q_pitch + col0, u, inv_u);
+            }
           }
           with_act(p.act, [&](auto a) {
 #pragma unroll
-            for (int i = 0; i < 32; ++i) g[i] = act_value<decltype(a)::value>(g[i]) * u[i];
+            for (int i = 0; i < CHUNK; ++i) g[i] = act_value<decltype(a)::value>(g[i]) * u[i];
           });
-          put(&p.out[0], g, col, row0);
+          const uint32_t tile = begin_tile();
+          tile_store<T, PITCH>(tile, lane, 0, g);
+          end_tile(&p.out[0], tile, col0, row0);
         }
       } else {  // kEpiGatedBwd
-        float sg = 0.0f, su = 0.0f;
-        if (p.keep_kind == kKeep8 && chunks > 0 && row < p.rows && TN == 256) {
-          const int64_t o = static_cast<int64_t>(row) * p.scale_pitch + col0 / kKeepGroup;
-          sg = p.scale[0][o];
-          su = p.scale[1][o];
-        }
 #pragma unroll 1
-        for (int c = 0; c < chunks; ++c, ++it) {
-          const int col = col0 + 32 * c;
-          const uint32_t tile = s_buf + (it & 1) * 2 * kTileBytes, htile = s_buf + 4 * kTileBytes;
-          float g[32], u[32], d[32];
-          uint32_t packed[16];
-          if (with_in) {
-            if (c + 1 < chunks) fetch(it + 1, col + 32, row0);
-            else if (lane == 0) bulk_wait_group_read<0>();
-            ok = __all_sync(0xffffffffu,
-                            mbar_wait_to(bar_in(w, it & 1), (it >> 1) & 1, abort_flag, kDevTimeoutEpi, status));
-            if (!ok) break;
-            tile_row_load(tile, lane, packed);
-            unpack32<T>(packed, g);
-            tile_row_load(tile + kTileBytes, lane, packed);
-            unpack32<T>(packed, u);
-          } else {
-            if (row < p.rows) {
-              load_fp8x32(p.q[0] + row * p.q_pitch + col, sg, g);
-              load_fp8x32(p.q[1] + row * p.q_pitch + col, su, u);
-            } else {
-#pragma unroll
-              for (int i = 0; i < 32; ++i) g[i] = u[i] = 0.0f;
+        for (int c = 0; c < chunks; ++c) {
+          const int col = col0 + CHUNK * c;
+          const uint32_t tile_g = s_buf, tile_u = s_buf + Cfg::TILE;
+          if (by_tma) {
+            ok = __all_sync(0xffffffffu, mbar_wait_to(bar_in(w), in_phase, abort_flag, kDevTimeoutEpi, status));
+            if (!ok) {
+              mbar_wait_to(bar_in(w), in_phase, &no_abort, kDevTimeoutEpi, status);
+              break;
             }
+            in_phase ^= 1;
+          } else {
             if (lane == 0) bulk_wait_group_read<0>();
             __syncwarp();
           }
-          tmem_load32(t_acc + half * Cfg::HALF + 32 * c, d);
-          with_act(p.act, [&](auto a) {
+          // dg and du take g's and u's places; h waits in registers for a free
+          // buffer.  16 columns at a time, for the registers' sake.
+          uint32_t h[CHUNK / 2];
 #pragma unroll
-            for (int i = 0; i < 32; ++i) {
-              float slope;
-              const float v = act_both<decltype(a)::value>(g[i], slope);
-              g[i] = d[i] * (u[i] * slope);  // dg
-              d[i] *= v;                     // du
-              u[i] *= v;                     // h
+          for (int from = 0; from < CHUNK; from += 16) {
+            float g[16], u[16], d[16];
+            tmem_load16(t_part + CHUNK * c + from, d);
+            if (by_tma) {
+              tile_load<T, PITCH>(tile_g, lane, from, g);
+              tile_load<T, PITCH>(tile_u, lane, from, u);
+            } else {
+              widen_fp8x16(in0 + from / 4, sg, g);
+              widen_fp8x16(in1 + from / 4, su, u);
+              if (from + 16 == CHUNK && c + 1 < chunks) fetch_row(col + CHUNK);
             }
-          });
-          pack32<T>(g, packed);
-          tile_row_store(tile, lane, packed);
-          pack32<T>(d, packed);
-          tile_row_store(tile + kTileBytes, lane, packed);
-          pack32<T>(u, packed);
-          tile_row_store(htile, lane, packed);
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) {
-            tma_store_2d(&p.out[0], tile, col, row0);
-            tma_store_2d(&p.out[1], tile + kTileBytes, col, row0);
-            tma_store_2d(&p.keep[0], htile, col, row0);
-            bulk_commit_group();
+            with_act(p.act, [&](auto a) {
+#pragma unroll
+              for (int i = 0; i < 16; ++i) {
+                float slope;
+                const float v = act_both<decltype(a)::value>(g[i], slope);
+                g[i] = d[i] * (u[i] * slope);  // dg
+                d[i] *= v;                     // du
+                u[i] *= v;                     // h
+              }
+            });
+            tile_store<T, PITCH>(tile_g, lane, from, g);
+            tile_store<T, PITCH>(tile_u, lane, from, d);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const typename Pair<T>::type x = Pair<T>::round(u[2 * i], u[2 * i + 1]);
+              h[from / 2 + i] = *reinterpret_cast<const uint32_t*>(&x);
+            }
           }
+          end_tile(&p.out[0], tile_g, col, row0);
+          end_tile(&p.out[1], tile_u, col, row0);
+          if (lane == 0) bulk_wait_group_read<1>();
+          __syncwarp();
+#pragma unroll
+          for (int u = 0; u < CHUNK / 8; ++u)
+            st_shared_v4(tile_g + swz_off<PITCH>(lane, u), h[4 * u], h[4 * u + 1], h[4 * u + 2], h[4 * u + 3]);
+          end_tile(&p.keep[0], tile_g, col, row0);
+          if (by_tma && c + 1 < chunks) fetch_tiles(col + CHUNK);
         }
       }
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive_cluster(mapa_shared(bar_free(buf), 0));
     }
-    if (lane == 0) {
-      // After a wait that ran out: no load may still be under way.
-      for (; !ok && it < fetched; ++it)
-        mbar_wait_to(bar_in(w, it & 1), (it >> 1) & 1, &no_abort, kDevTimeoutEpi, status);
-      bulk_wait_group<0>();
-    }
+    if (lane == 0) bulk_wait_group<0>();
     __syncwarp();
   }
 

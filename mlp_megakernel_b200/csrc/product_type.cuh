@@ -5,6 +5,7 @@
 #include <algorithm>
 #include <atomic>
 #include <cstring>
+#include <utility>
 
 #include "few_rows_kernel.cuh"
 #include "product_kernel.cuh"
@@ -68,12 +69,12 @@ int launch_tiles(const Product& c, cudaStream_t st) {
             type_bits(std::is_same_v<T, __nv_bfloat16>);
   a.act = c.act;
   a.keep_kind = c.keep_kind;
-  a.residual = EPI == kEpiLinear && c.in[0] != nullptr;
   a.bias = c.bias;
   a.bias32 = c.bias32;
   a.status = device_status_word(dev);
   if (!a.status) return MLPK_ERR_CUDA;
   a.partials = c.partials;
+  a.residual = EPI == kEpiLinear ? c.in[0] : nullptr;
   a.q_pitch = c.q_pitch;
   a.scale_pitch = c.scale_pitch;
   for (int i = 0; i < 2; ++i) {
@@ -87,9 +88,10 @@ int launch_tiles(const Product& c, cudaStream_t st) {
     if (c.b[i] && (rc = c.b_mn ? make_map_2d(&a.b[i], c.b[i], cols, k, 64, kBlockK)
                                : make_map_2d(&a.b[i], c.b[i], k, cols, kBlockK, TN / 2)))
       return rc;
-    if (c.in[i] && (rc = make_map_2d(&a.in[i], c.in[i], cols, rows, 32, 32))) return rc;
-    if (c.out[i] && EPI != kEpiPartial && (rc = make_map_2d(&a.out[i], c.out[i], cols, rows, 32, 32))) return rc;
-    if (c.keep[i] && (rc = make_map_2d(&a.keep[i], c.keep[i], cols, rows, 32, 32))) return rc;
+    for (const auto& [map, v] : {std::make_pair(&a.in[i], EPI == kEpiGatedBwd ? c.in[i] : nullptr),
+                                 std::make_pair(&a.out[i], const_cast<const void*>(EPI == kEpiPartial ? nullptr : c.out[i])),
+                                 std::make_pair(&a.keep[i], const_cast<const void*>(c.keep[i]))})
+      if (v && (rc = make_map_2d(map, v, cols, rows, Cfg::CHUNK, 32))) return rc;
   }
   const int64_t total = static_cast<int64_t>(a.tiles_m) * a.tiles_n * a.outputs * a.splits;
   if (total > 0x7fffffff - 256) return MLPK_ERR_SHAPE;
@@ -153,13 +155,45 @@ int launch_few(const Product& c, cudaStream_t st) {
   return cuda_status(cudaLaunchKernelEx(&cfg, kern, a));
 }
 
-// Rows up to which a product goes to few_rows_kernel.
-constexpr int kFewRows = 256;
+// Tiles of 256 columns, or of 128 where that ends earlier: a narrow tile takes
+// about 0.7 of a wide one's time (its rows are read for half the products), so it
+// pays where the wide tiles leave pairs of CTAs idle (512 x 4096 x 4096 bf16: 64
+// narrow tiles 19.7 us, 32 wide ones 25.3; 1024 x 4096 x 4096: 128 narrow ones in
+// two goes 34.2, 64 wide ones in one 26.3).  A gate's checkpoint needs the wide
+// tile's 128 columns, and so does what reads it.
+template <class T, int EPI>
+int launch_best(const Product& c, int pairs, cudaStream_t st) {
+  if (c.keep_kind != kKeep8 || EPI == kEpiLinear) {
+    const int64_t each = static_cast<int64_t>(ceil_div_int(c.rows, kPairRows)) * c.outputs * c.splits;
+    const int64_t wide = each * ceil_div_int(c.cols, ProductCfg<EPI, 256>::OUT_COLS);
+    const int64_t narrow = each * ceil_div_int(c.cols, ProductCfg<EPI, 128>::OUT_COLS);
+    if (7 * ceil_div_int(narrow, pairs) < 10 * ceil_div_int(wide, pairs)) return launch_tiles<T, EPI, 128>(c, st);
+  }
+  return launch_tiles<T, EPI, 256>(c, st);
+}
+
+// Whether a product goes to few_rows_kernel.  Up to 128 rows it does, but for
+// short reductions of more than 64 (bf16, us, here and in tiles of 256 rows: 1 x
+// 4096 x 4096 8.5 and 24, 64 x 4096 x 14336 24.1 and 30.5, 128 x 4096 x 4096 11.4
+// and 19.0; 128 x 256 x 256 8.0 and 6.2).  Up to 256 rows it does where a long
+// reduction would leave half of the pairs of CTAs without a tile (256 x 4096 x 4096
+// 16.3 and 19.2; 256 x 4096 x 8192 27.0 and 25.6, 256 x 2048 x 4096 14.7 and 13.3).
+// The rows must be read along the reduction, and a gate's checkpoint group is wider
+// than a tile.
+inline bool few_rows(const Product& c, int pairs) {
+  if (c.rows > kFewMostRows || c.a_mn || c.outputs > 1 || (c.epi == kEpiGated && c.keep_kind == kKeep8)) return false;
+  const int nk = ceil_div_int(c.k[0], kBlockK) + ceil_div_int(c.k[1], kBlockK);
+  if (c.rows <= 128) return c.rows <= 64 || nk >= 16;
+  return nk >= 48 && 2 * ceil_div_int(c.cols, c.epi == kEpiGated ? 64 : 128) <= pairs;
+}
 
 template <class T>
 int launch_type(const Product& c, cudaStream_t st) {
-  // A gate's checkpoint group is wider than a tile of few_rows_kernel.
-  if (c.rows <= kFewRows && !c.a_mn && !(c.epi == kEpiGated && c.keep_kind == kKeep8)) {
+  DevInfo di;
+  const int rc = current_device_info(&di, nullptr);
+  if (rc) return rc;
+  const int pairs = di.sm_count / 2;
+  if (few_rows(c, pairs)) {
     switch (c.epi) {
       case kEpiPlain: return launch_few<T, kEpiPlain>(c, st);
       case kEpiLinear: return launch_few<T, kEpiLinear>(c, st);
@@ -168,11 +202,11 @@ int launch_type(const Product& c, cudaStream_t st) {
     }
   }
   switch (c.epi) {
-    case kEpiPlain: return launch_tiles<T, kEpiPlain, 256>(c, st);
-    case kEpiPartial: return launch_tiles<T, kEpiPartial, 256>(c, st);
-    case kEpiLinear: return launch_tiles<T, kEpiLinear, 256>(c, st);
-    case kEpiGated: return launch_tiles<T, kEpiGated, 256>(c, st);
-    default: return launch_tiles<T, kEpiGatedBwd, 256>(c, st);
+    case kEpiPlain: return launch_best<T, kEpiPlain>(c, pairs, st);
+    case kEpiPartial: return launch_best<T, kEpiPartial>(c, pairs, st);
+    case kEpiLinear: return launch_best<T, kEpiLinear>(c, pairs, st);
+    case kEpiGated: return launch_best<T, kEpiGated>(c, pairs, st);
+    default: return launch_best<T, kEpiGatedBwd>(c, pairs, st);
   }
 }
 
