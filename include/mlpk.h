@@ -373,12 +373,16 @@ int64_t mlpk_linear_dz_workspace_size(int64_t rows, int width, int dtype);
 int mlpk_linear_dz(int64_t rows, int width, int dtype, int act, const void* grad_out, int keep, const void* z,
                    const float* z_scale, void* dz, void* db, int db_dtype, void* workspace, int64_t workspace_bytes,
                    mlpk_stream_t stream);
-/* dx = the sum over i < count (1 or 2) of dz[i] w[i]^T; dz[i]: [rows][d_out]. */
+/* dx = the sum over i < count (1 or 2) of dz[i] w[i]^T; dz[i]: [rows][d_out].
+ * This and the next call need a workspace of the size that theirs gives (often
+ * 0): the last tiles of a product are shared out over all SMs. */
+int64_t mlpk_linear_dx_workspace_size(int64_t rows, int d_in, int d_out, int dtype, int count, int w_layout);
 int mlpk_linear_dx(int64_t rows, int d_in, int d_out, int dtype, int count, const void* const* dz,
-                   const void* const* w, int w_layout, void* dx, mlpk_stream_t stream);
+                   const void* const* w, int w_layout, void* dx, void* workspace, int64_t workspace_bytes,
+                   mlpk_stream_t stream);
 /* dw[i] = x^T dz[i] for i < count (1 or 2), summed over the rows in fp32 in a
  * fixed order, stored in w_layout. */
-int64_t mlpk_linear_dw_workspace_size(int64_t rows, int d_in, int d_out, int dtype, int count);
+int64_t mlpk_linear_dw_workspace_size(int64_t rows, int d_in, int d_out, int dtype, int count, int w_layout);
 int mlpk_linear_dw(int64_t rows, int d_in, int d_out, int dtype, int count, const void* x, const void* const* dz,
                    void* const* dw, int w_layout, void* workspace, int64_t workspace_bytes, mlpk_stream_t stream);
 

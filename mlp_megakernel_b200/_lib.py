@@ -97,8 +97,9 @@ SIGNATURES = {
     "mlpk_linear": (_i32, [_i64, _i32, _i32, _i32, _vp, _vp, _i32, _vp, _i32, _i32, _vp, _vp, _i32, _vp, _vp, _vp]),
     "mlpk_linear_dz_workspace_size": (_i64, [_i64, _i32, _i32]),
     "mlpk_linear_dz": (_i32, [_i64, _i32, _i32, _i32, _vp, _i32, _vp, _vp, _vp, _vp, _i32, _vp, _i64, _vp]),
-    "mlpk_linear_dx": (_i32, [_i64, _i32, _i32, _i32, _i32, _VPP, _VPP, _i32, _vp, _vp]),
-    "mlpk_linear_dw_workspace_size": (_i64, [_i64, _i32, _i32, _i32, _i32]),
+    "mlpk_linear_dx_workspace_size": (_i64, [_i64, _i32, _i32, _i32, _i32, _i32]),
+    "mlpk_linear_dx": (_i32, [_i64, _i32, _i32, _i32, _i32, _VPP, _VPP, _i32, _vp, _vp, _i64, _vp]),
+    "mlpk_linear_dw_workspace_size": (_i64, [_i64, _i32, _i32, _i32, _i32, _i32]),
     "mlpk_linear_dw": (_i32, [_i64, _i32, _i32, _i32, _i32, _vp, _VPP, _VPP, _i32, _vp, _i64, _vp]),
     "mlpk_gated": (_i32, [_i64, _i32, _i32, _i32, _i32, _vp, _vp, _vp, _i32, _vp, _i32, _vp, _vp, _vp, _vp, _vp]),
     "mlpk_gated_bwd": (_i32, [_i64, _i32, _i32, _i32, _i32, _vp, _vp, _i32, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp,

@@ -30,7 +30,7 @@ SOURCES = {
     "expert_api.cu": ["host.cuh", "pdl.cuh", "vec.cuh", "expert_plan.cuh", "expert_kernel.cuh"],
     **{f"product_{part}.cu": ["host.cuh", "pdl.cuh", "ptx.cuh", "pair.cuh", "layout.cuh", "softplus.cuh", "vec.cuh",
                               "act.cuh", "product_epi.cuh", "product_kernel.cuh", "product_launch.cuh",
-                              "few_rows_plan.cuh", "few_rows_kernel.cuh", "product_type.cuh"] for part in ("f16", "bf16")},
+                              "product_plan.cuh", "tail_kernel.cuh", "few_rows_plan.cuh", "few_rows_kernel.cuh", "product_type.cuh"] for part in ("f16", "bf16")},
     "ff_api.cu": ["host.cuh", "pdl.cuh", "ptx.cuh", "softplus.cuh", "vec.cuh", "act.cuh", "product_epi.cuh",
                   "product_launch.cuh", "ff_kernel.cuh"],
     "adamw_api.cu": ["host.cuh", "pdl.cuh", "vec.cuh", "adamw_kernel.cuh"],

@@ -63,12 +63,32 @@ void set_keep(Product* c, int keep, int width, void* const (&v)[2], float* const
   }
 }
 
-// Shares of a product's reduction: as many as bring the tiles to about one for
-// each pair of CTAs, 16 blocks of 64 in each at least.
-int dw_splits(int64_t rows, int d_in, int d_out, int count, int sm_count) {
-  const int64_t tiles = ceil_to(d_in, 256) * ceil_to(d_out, 256) * count;
-  const int64_t want = (sm_count / 2) / std::max<int64_t>(tiles, 1);
-  return static_cast<int>(std::max<int64_t>(1, std::min(want, ceil_to(rows, 64) / 16)));
+// dx and dw as products, their operands aside.
+Product dx_product(int64_t rows, int d_in, int d_out, int count, int w_layout) {
+  Product c;
+  c.epi = kEpiPlain;
+  c.rows = rows;
+  c.cols = d_in;
+  for (int i = 0; i < count; ++i) c.k[i] = d_out;
+  c.b_mn = w_layout == MLPK_W_OUT_IN;
+  return c;
+}
+Product dw_product(int64_t rows, int d_in, int d_out, int count, int w_layout) {
+  Product c;
+  c.epi = kEpiPlain;
+  c.outputs = count;
+  c.k[0] = rows;
+  c.a_mn = c.b_mn = true;
+  const bool in_out = w_layout == MLPK_W_IN_OUT;
+  c.out_a = !in_out;
+  c.rows = in_out ? d_in : d_out;
+  c.cols = in_out ? d_out : d_in;
+  return c;
+}
+int64_t product_workspace(const Product& c) {
+  DevInfo di;
+  if (c.rows == 0 || c.k[0] == 0) return 0;
+  return current_device_info(&di, nullptr) ? -1 : product::workspace_bytes(c, di.sm_count);
 }
 
 template <class F>
@@ -163,34 +183,34 @@ int mlpk_linear_dz(int64_t rows, int width, int dtype, int act, const void* grad
   });
 }
 
+int64_t mlpk_linear_dx_workspace_size(int64_t rows, int d_in, int d_out, int dtype, int count, int w_layout) {
+  if (check_call(rows, {d_in, d_out}, dtype, 0, 0) || check_layout(w_layout) || count < 1 || count > 2) return -1;
+  return product_workspace(dx_product(rows, d_in, d_out, count, w_layout));
+}
+
 int mlpk_linear_dx(int64_t rows, int d_in, int d_out, int dtype, int count, const void* const* dz,
-                   const void* const* w, int w_layout, void* dx, mlpk_stream_t stream) {
+                   const void* const* w, int w_layout, void* dx, void* workspace, int64_t workspace_bytes,
+                   mlpk_stream_t stream) {
   int rc = check_call(rows, {d_in, d_out}, dtype, 0, 0);
   if (rc || (rc = check_layout(w_layout))) return rc;
   if (count != 1 && count != 2) return MLPK_ERR_SHAPE;
   if (!dz || !w) return MLPK_ERR_NULL;
   if (rows == 0) return MLPK_OK;
-  if ((rc = check_ptrs({dx, dz[0], w[0], dz[count - 1], w[count - 1]}))) return rc;
-  Product c;
-  c.epi = kEpiPlain;
-  c.rows = rows;
-  c.cols = d_in;
+  if ((rc = check_ptrs({dx, dz[0], w[0], dz[count - 1], w[count - 1]}, {workspace}))) return rc;
+  Product c = dx_product(rows, d_in, d_out, count, w_layout);
   for (int i = 0; i < count; ++i) {
-    c.k[i] = d_out;
     c.a[i] = dz[i];
     c.b[i] = w[i];
   }
-  c.b_mn = w_layout == MLPK_W_OUT_IN;
   c.out[0] = dx;
+  c.workspace = workspace;
+  c.workspace_bytes = workspace_bytes;
   return run(c, dtype, stream);
 }
 
-int64_t mlpk_linear_dw_workspace_size(int64_t rows, int d_in, int d_out, int dtype, int count) {
-  if (check_call(rows, {d_in, d_out}, dtype, 0, 0) || count < 1 || count > 2) return -1;
-  DevInfo di;
-  if (current_device_info(&di, nullptr)) return -1;
-  const int splits = dw_splits(rows, d_in, d_out, count, di.sm_count);
-  return splits == 1 ? 0 : static_cast<int64_t>(splits) * count * d_in * d_out * static_cast<int64_t>(sizeof(float));
+int64_t mlpk_linear_dw_workspace_size(int64_t rows, int d_in, int d_out, int dtype, int count, int w_layout) {
+  if (check_call(rows, {d_in, d_out}, dtype, 0, 0) || check_layout(w_layout) || count < 1 || count > 2) return -1;
+  return product_workspace(dw_product(rows, d_in, d_out, count, w_layout));
 }
 
 int mlpk_linear_dw(int64_t rows, int d_in, int d_out, int dtype, int count, const void* x, const void* const* dz,
@@ -199,46 +219,24 @@ int mlpk_linear_dw(int64_t rows, int d_in, int d_out, int dtype, int count, cons
   if (rc || (rc = check_layout(w_layout))) return rc;
   if (count != 1 && count != 2) return MLPK_ERR_SHAPE;
   if (!dz || !dw) return MLPK_ERR_NULL;
-  const int64_t each = static_cast<int64_t>(d_in) * d_out;
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (rows == 0) {
+    const size_t bytes = static_cast<size_t>(d_in) * d_out * 2;
     for (int i = 0; i < count; ++i)
       if (!dw[i]) return MLPK_ERR_NULL;
-      else if ((rc = cuda_status(cudaMemsetAsync(dw[i], 0, static_cast<size_t>(each) * 2, st)))) return rc;
+      else if ((rc = cuda_status(cudaMemsetAsync(dw[i], 0, bytes, static_cast<cudaStream_t>(stream))))) return rc;
     return MLPK_OK;
   }
   if ((rc = check_ptrs({x, dz[0], dz[count - 1], dw[0], dw[count - 1]}, {workspace}))) return rc;
-  DevInfo di;
-  if ((rc = current_device_info(&di, nullptr))) return rc;
-  const int splits = dw_splits(rows, d_in, d_out, count, di.sm_count);
-  if (splits > 1) {
-    if (!workspace) return MLPK_ERR_NULL;
-    if (workspace_bytes < splits * count * each * static_cast<int64_t>(sizeof(float))) return MLPK_ERR_SCRATCH;
-  }
-  Product c;
-  c.epi = splits > 1 ? kEpiPartial : kEpiPlain;
-  c.splits = splits;
-  c.partials = static_cast<float*>(workspace);
-  c.outputs = count;
-  c.k[0] = rows;
-  c.a_mn = c.b_mn = true;
+  Product c = dw_product(rows, d_in, d_out, count, w_layout);
   const bool in_out = w_layout == MLPK_W_IN_OUT;
-  c.out_a = !in_out;
-  c.rows = in_out ? d_in : d_out;
-  c.cols = in_out ? d_out : d_in;
   (in_out ? c.a : c.b)[0] = x;
   for (int i = 0; i < count; ++i) {
     (in_out ? c.b : c.a)[i] = dz[i];
     c.out[i] = dw[i];
   }
-  if ((rc = run(c, dtype, stream)) || splits == 1) return rc;
-  const int64_t n = each * count;
-  const dim3 grid(stream_blocks(ceil_to(n, 8 * kStreamThreads), di.sm_count, 16));
-  return with_value_type(dtype, [&](auto t) {
-    using T = decltype(t);
-    return launch_kernel_early(split_sum_kernel<T>, grid, kStreamThreads, 0, st, n, each, splits,
-                               static_cast<const float*>(workspace), static_cast<T*>(dw[0]), static_cast<T*>(dw[count - 1]));
-  });
+  c.workspace = workspace;
+  c.workspace_bytes = workspace_bytes;
+  return run(c, dtype, stream);
 }
 
 int mlpk_gated(int64_t rows, int d_in, int hidden, int dtype, int act, const void* x, const void* w_gate,

@@ -1,5 +1,5 @@
 // What stands beside the products (product_kernel.cuh): checkpoints in 8 bits,
-// the activation's backward with the bias gradient, the sum of a split product.
+// and the activation's backward with the bias gradient.
 // All of them are streams over memory, bound by it.
 #pragma once
 #include "act.cuh"
@@ -218,26 +218,6 @@ __global__ void __launch_bounds__(kStreamThreads)
 #pragma unroll
     for (int k = 0; k < kStreamThreads / 32; ++k) all += s_sum[k][lane];
     db[col] = from_float<W>(all);
-  }
-}
-
-// ---------------------------------------------------------------- the sum of a split product
-// D = the sum over s of partials[s], in the order of s.  n: values of all outputs
-// (a multiple of 8); output o has `each` of them.
-template <class T>
-__global__ void __launch_bounds__(kStreamThreads)
-    split_sum_kernel(int64_t n, int64_t each, int splits, const float* __restrict__ partials, T* d0, T* d1) {
-  pdl_enter();
-  const int64_t step = static_cast<int64_t>(gridDim.x) * kStreamThreads * 8;
-  for (int64_t i = (static_cast<int64_t>(blockIdx.x) * kStreamThreads + threadIdx.x) * 8; i < n; i += step) {
-    float f[8] = {};
-#pragma unroll 4
-    for (int s = 0; s < splits; ++s) {
-      const Raw<float, 8> r = load_32b(partials + s * n + i);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) f[e] += r.v[e];
-    }
-    store8(i < each ? d0 + i : d1 + (i - each), f);
   }
 }
 

@@ -3,6 +3,6 @@
 
 namespace mlpk {
 
-enum Epi : int { kEpiPlain, kEpiPartial, kEpiLinear, kEpiGated, kEpiGatedBwd };
+enum Epi : int { kEpiPlain, kEpiLinear, kEpiGated, kEpiGatedBwd };
 
 }  // namespace mlpk

@@ -2,7 +2,6 @@
 // stands behind each product in its epilogue:
 //
 //   kEpiPlain     D = A B                                     (dx, dW)
-//   kEpiPartial   the same in fp32, of a share of the reduction (dW, split)
 //   kEpiLinear    z = A B + bias; out = act(z) + residual; z kept for the backward
 //   kEpiGated     g = A Bg, u = A Bu; h = act(g) u; g and u kept for the backward
 //   kEpiGatedBwd  dh = A B; dg = dh u act'(g), du = dh act(g), h = act(g) u again
@@ -18,7 +17,9 @@
 // accumulators of TN columns, so the epilogue of a tile runs beside the products
 // of the next.  The kernel is persistent: tiles are taken in groups of `group`
 // row tiles over all column tiles, so that the pairs at work share rows and
-// columns in L2.
+// columns in L2.  The tiles behind the last full turn of the pairs may be shared
+// out (kEpiPlain alone): an item is then a share of a tile's reduction, whose fp32
+// values go to a workspace, and tail_sum_kernel adds them in order.
 //
 // Everything between the operands and the stored values is fp32: accumulators,
 // bias, activation, residual.  What is kept for the backward is rounded once, to
@@ -29,6 +30,7 @@
 #include "layout.cuh"
 #include "pair.cuh"
 #include "product_epi.cuh"
+#include "product_plan.cuh"
 
 namespace mlpk {
 
@@ -47,7 +49,8 @@ struct alignas(64) ProductArgs {
   CUtensorMap in[2];       // backward: g, u (16 bits)
   int rows, cols;          // of each output
   int nk0, nk;             // blocks of the first reduction range, and of both
-  int tiles_m, tiles_n, outputs, splits, group;
+  int tiles_m, tiles_n, outputs, group;
+  int full, splits, items; // tiles computed whole, shares of each of the others, and both together
   int a_mn, b_mn;          // the operand's contiguous index is the row / column, not the reduction
   int out_a;               // with two outputs: A differs, not B
   uint32_t idesc;
@@ -58,7 +61,7 @@ struct alignas(64) ProductArgs {
   float* scale[2];         // [rows][scale_pitch]
   int64_t q_pitch;
   int scale_pitch;
-  float* partials;         // [splits][outputs][rows][cols]
+  float* partials;         // [shares][256 x TN], each as share_unit says
   int* status;
 };
 
@@ -74,7 +77,7 @@ struct ProductCfg {
   static constexpr int CHUNK = PART < 32 ? PART : 32;
   static constexpr int PITCH = CHUNK * 2;
   static constexpr int TILE = 32 * PITCH;
-  static constexpr int BUFS = EPI == kEpiPartial ? 0 : 2;
+  static constexpr int BUFS = 2;
   static constexpr int OFF_EPI = 0;
   static constexpr int EPI_BYTES = kEpiWarps * BUFS * TILE;
   static constexpr int STAGES_FIT = (227 * 1024 - 2048 - EPI_BYTES) / STAGE;
@@ -89,24 +92,31 @@ struct ProductCfg {
   static_assert(STAGES >= 3 && (TN == 128 || TN == 256), "tile");
 };
 
-struct TileAt {
-  int m, n, output, split;
+// The tile and the blocks of the t-th item.
+struct ItemAt {
+  TileAt tile;
+  int k0, k1, share;  // share: below 0 for a whole tile
 };
-__host__ __device__ inline TileAt product_tile(int t, int tiles_m, int tiles_n, int outputs, int group) {
-  const int wide = tiles_n * outputs, each = tiles_m * wide;
-  TileAt at;
-  at.split = t / each;
-  t -= at.split * each;
-  const int first = t / (group * wide) * group;
-  const int high = tiles_m - first < group ? tiles_m - first : group;
-  t -= first * wide;
-  at.m = first + t % high;
-  const int n = t / high;
-  at.output = n / tiles_n;
-  at.n = n - at.output * tiles_n;
-  return at;
+__device__ __forceinline__ ItemAt product_item(const ProductArgs& p, int t) {
+  ItemAt it;
+  it.share = t - p.full;
+  int tile = t;
+  it.k0 = 0;
+  it.k1 = p.nk;
+  if (it.share >= 0) {
+    tile = p.full + it.share / p.splits;
+    const int s = it.share % p.splits;
+    it.k0 = static_cast<int>(static_cast<int64_t>(s) * p.nk / p.splits);
+    it.k1 = static_cast<int>(static_cast<int64_t>(s + 1) * p.nk / p.splits);
+  }
+  it.tile = product_tile(tile, p.tiles_m, p.tiles_n, p.outputs, p.group);
+  return it;
 }
 
+// Shared memory to consecutive global memory (16-byte units).
+__device__ __forceinline__ void bulk_store(void* dst, uint32_t src, uint32_t bytes) {
+  asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst), "r"(src), "r"(bytes) : "memory");
+}
 __device__ __forceinline__ void tmem_load32(uint32_t taddr, float (&v)[32]) {
   uint32_t r[32];
   tmem_ld_wait_x32(taddr, r);
@@ -251,7 +261,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kProductThreads, 1)
   volatile int no_abort = 0;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_ctarank();
-  const int total = p.tiles_m * p.tiles_n * p.outputs * p.splits;
+  const int total = p.items;
   const int step = static_cast<int>(cluster_count());
   int* const status = p.status;
 
@@ -286,9 +296,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kProductThreads, 1)
       uint32_t phase = 1;
       bool ok = true;
       for (int t = cluster_id(); ok && t < total; t += step) {
-        const TileAt at = product_tile(t, p.tiles_m, p.tiles_n, p.outputs, p.group);
-        const int k0 = static_cast<int>(static_cast<int64_t>(at.split) * p.nk / p.splits);
-        const int k1 = static_cast<int>(static_cast<int64_t>(at.split + 1) * p.nk / p.splits);
+        const ItemAt item = product_item(p, t);
+        const TileAt at = item.tile;
+        const int k0 = item.k0, k1 = item.k1;
         const int row = at.m * kPairRows + static_cast<int>(rank) * 128;
         // A pair's half of B: columns, or for the gate its own matrix.
         const int col = EPI == kEpiGated ? at.n * (TN / 2) : at.n * TN + static_cast<int>(rank) * (TN / 2);
@@ -349,9 +359,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kProductThreads, 1)
       int s = 0, mine = 0;
       uint32_t phase = 0;
       for (int t = cluster_id(); ok && t < total; t += step, ++mine) {
-        const TileAt at = product_tile(t, p.tiles_m, p.tiles_n, p.outputs, p.group);
-        const int k0 = static_cast<int>(static_cast<int64_t>(at.split) * p.nk / p.splits);
-        const int k1 = static_cast<int>(static_cast<int64_t>(at.split + 1) * p.nk / p.splits);
+        const ItemAt item = product_item(p, t);
+        const int k0 = item.k0, k1 = item.k1;
         const int buf = mine & 1;
         const uint32_t d = tmem + buf * TN;
         ok = mbar_wait_cluster(bar_free(buf), ((mine >> 1) & 1) ^ 1, abort_flag, kDevTimeoutMma, status);
@@ -404,7 +413,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kProductThreads, 1)
     int mine = 0;
     uint32_t in_phase = 0;
     for (int t = cluster_id(); ok && t < total; t += step, ++mine) {
-      const TileAt at = product_tile(t, p.tiles_m, p.tiles_n, p.outputs, p.group);
+      const ItemAt item = product_item(p, t);
+      const TileAt at = item.tile;
       const int buf = mine & 1;
       const int row0 = at.m * kPairRows + static_cast<int>(rank) * 128 + quarter * 32;
       const int row = row0 + lane;
@@ -457,6 +467,32 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kProductThreads, 1)
       tc_fence_after();
       const uint32_t t_acc = t_lane + buf * TN, t_part = t_acc + part * Cfg::PART;
       if constexpr (EPI == kEpiPlain) {
+        if (item.share >= 0) {
+          // Both buffers together: 32 rows x 32 columns of fp32, a run of the
+          // workspace (share_unit; with what lies outside the output, as zeros).
+          static_assert(2 * Cfg::TILE == 4096 && CHUNK == 32, "a share's run");
+          float* dst = p.partials + (static_cast<int64_t>(item.share) * 32 + rank * 16 + w) * (Cfg::CHUNKS * 1024);
+#pragma unroll 1
+          for (int c = 0; c < Cfg::CHUNKS; ++c) {
+            float v[32];
+            tmem_load32(t_part + CHUNK * c, v);
+            if (lane == 0) bulk_wait_group_read<0>();
+            __syncwarp();
+#pragma unroll
+            for (int u = 0; u < 8; ++u)
+              st_shared_v4(s_buf + lane * 128 + ((u ^ (lane & 7)) << 4), __float_as_uint(v[4 * u]),
+                           __float_as_uint(v[4 * u + 1]), __float_as_uint(v[4 * u + 2]), __float_as_uint(v[4 * u + 3]));
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+              bulk_store(dst + c * 1024, s_buf, 4096);
+              bulk_commit_group();
+            }
+          }
+          if (lane == 0) bulk_wait_group_read<0>();
+          __syncwarp();
+          chunks = 0;
+        }
 #pragma unroll 1
         for (int c = 0; c < chunks; ++c) {
           float v[32];
@@ -464,23 +500,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kProductThreads, 1)
           const uint32_t tile = begin_tile();
           tile_store<T, PITCH>(tile, lane, 0, v);
           end_tile(&p.out[at.output], tile, col0 + CHUNK * c, row0);
-        }
-      } else if constexpr (EPI == kEpiPartial) {
-        float* dst = p.partials + ((static_cast<int64_t>(at.split) * p.outputs + at.output) * p.rows + row) * p.cols;
-#pragma unroll 1
-        for (int c = 0; c < chunks; ++c) {
-          float v[32];
-          tmem_load32(t_part + CHUNK * c, v);
-          if (row < p.rows) {
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const int col = col0 + CHUNK * c + 8 * k;
-              float2 f[4];
-#pragma unroll
-              for (int e = 0; e < 4; ++e) f[e] = make_float2(v[8 * k + 2 * e], v[8 * k + 2 * e + 1]);
-              if (col < p.cols) store_32b(dst + col, f);
-            }
-          }
         }
       } else if constexpr (EPI == kEpiLinear) {
         float inv = 0.0f;

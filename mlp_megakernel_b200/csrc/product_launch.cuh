@@ -28,9 +28,12 @@ struct Product {
   float* scale[2] = {nullptr, nullptr};
   int64_t q_pitch = 0;
   int scale_pitch = 0;
-  float* partials = nullptr;
-  int splits = 1;
+  void* workspace = nullptr;  // of a plain product's shares
+  int64_t workspace_bytes = 0;
 };
+
+// The workspace that a plain product needs: from its rows, cols, outputs, k, a_mn.
+__attribute__((visibility("hidden"))) int64_t workspace_bytes(const Product& p, int sm_count);
 
 __attribute__((visibility("hidden"))) int launch_f16(const Product& p, cudaStream_t st);
 __attribute__((visibility("hidden"))) int launch_bf16(const Product& p, cudaStream_t st);

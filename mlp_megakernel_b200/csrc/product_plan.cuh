@@ -1,0 +1,95 @@
+// How a product in tiles of 256 rows is laid out over the pairs of CTAs
+// (product_kernel.cuh): host arithmetic alone, so that it can be gone over without
+// a GPU.
+#pragma once
+#include <cstdint>
+
+#ifdef __CUDACC__
+#define MLPK_HOST_DEVICE __host__ __device__
+#else
+#define MLPK_HOST_DEVICE
+#endif
+
+namespace mlpk {
+
+struct ProductPlan {
+  int cols = 256;     // columns of a tile: 256, or 128
+  int64_t full = 0;   // tiles computed whole, the first ones
+  int64_t tail = 0;   // tiles that `splits` items share, the last ones
+  int splits = 1;     // shares of a tail tile's reduction; 1: it is computed whole too
+  int64_t items() const { return full + tail * splits; }
+  // fp32 values that the shares leave in the workspace.
+  int64_t partials() const { return splits > 1 ? tail * splits * 256 * cols : 0; }
+};
+
+// rows, cols: of each output; out_cols: columns of an output that a wide tile has
+// (half of a narrow one's is its); nk: blocks of 64 of the reduction; may_split,
+// may_narrow: whether the product's epilogue allows it.
+//
+// The tiles go over the pairs in turns; a turn takes nk blocks' time, 0.7 of that
+// for narrow tiles (their rows are read for half the products).  What is left
+// behind the last full turn may be shared out over all pairs in shares of the
+// reduction: ceil(tail splits / pairs) turns of nk / splits blocks, and the
+// traffic of the shares (0.25 us a megabyte, written and read) and of a second
+// kernel (4 us).  A block takes 0.3 us.
+inline ProductPlan product_plan(int64_t rows, int cols, int outputs, int out_cols, int nk, int pairs, bool may_split,
+                                bool may_narrow) {
+  ProductPlan best;
+  double best_us = 0.0;
+  for (int narrow = 0; narrow <= (may_narrow ? 1 : 0); ++narrow) {
+    const int each = narrow ? out_cols / 2 : out_cols;
+    const int64_t tiles = (rows + 255) / 256 * ((cols + each - 1) / each) * outputs;
+    const double block_us = narrow ? 0.21 : 0.3;
+    const int64_t left = tiles % pairs;
+    const double full_us = static_cast<double>(tiles / pairs) * nk * block_us;
+    const int most = may_split && left ? (nk / 4 < 32 ? nk / 4 : 32) : 1;
+    for (int splits = 1; splits <= (most > 1 ? most : 1); ++splits) {
+      ProductPlan p;
+      p.cols = narrow ? 128 : 256;
+      p.splits = splits;
+      p.tail = splits > 1 ? left : 0;
+      p.full = tiles - p.tail;
+      double us = full_us;
+      if (left) us += static_cast<double>((left * splits + pairs - 1) / pairs) * ((nk + splits - 1) / splits) * block_us;
+      if (splits > 1) us += 4.0 + 0.25 * 4e-6 * static_cast<double>(p.partials());
+      if (best_us == 0.0 || us < best_us) {
+        best_us = us;
+        best = p;
+      }
+    }
+  }
+  return best;
+}
+
+// The t-th tile: row tiles in groups of `group`, over all column tiles of all
+// outputs.
+struct TileAt {
+  int m, n, output;
+};
+MLPK_HOST_DEVICE inline TileAt product_tile(int t, int tiles_m, int tiles_n, int outputs, int group) {
+  const int wide = tiles_n * outputs;
+  TileAt at;
+  const int first = t / (group * wide) * group;
+  const int high = tiles_m - first < group ? tiles_m - first : group;
+  t -= first * wide;
+  at.m = first + t % high;
+  const int n = t / high;
+  at.output = n / tiles_n;
+  at.n = n - at.output * tiles_n;
+  return at;
+}
+
+// Where the share of an item's value in `row` (of 256) and the 4 columns from
+// `col` (a multiple of 4) lies among the item's values, in units of 4: each
+// epilogue warp has runs of 32 rows x 32 columns, the 8 units of a row turned
+// around by the row (as its shared memory has them, against bank conflicts).
+// Epilogue warp w has the rows from 32 ((w + 2) % 4) on of its CTA's 128, and a quarter
+// of the columns, w / 4.
+MLPK_HOST_DEVICE inline int share_unit(int row, int col, int tile_cols) {
+  const int part_cols = tile_cols / 4, chunks = part_cols / 32;
+  const int rank = row / 128, quarter = row % 128 / 32, lane = row % 32;
+  const int warp = col / part_cols * 4 + (quarter + 2) % 4, chunk = col % part_cols / 32;
+  return ((rank * 16 + warp) * chunks + chunk) * 256 + lane * 8 + ((col % 32 / 4) ^ (lane % 8));
+}
+
+}  // namespace mlpk

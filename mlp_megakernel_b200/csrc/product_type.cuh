@@ -10,6 +10,7 @@
 #include "few_rows_kernel.cuh"
 #include "product_kernel.cuh"
 #include "product_launch.cuh"
+#include "tail_kernel.cuh"
 
 namespace mlpk {
 namespace product {
@@ -41,11 +42,9 @@ inline uint32_t type_bits(bool bf16) { return bf16 ? (1u << 7 | 1u << 10) : 0u; 
 inline int ceil_div_int(int64_t a, int64_t b) { return static_cast<int>((a + b - 1) / b); }
 
 template <class T, int EPI, int TN>
-int launch_tiles(const Product& c, cudaStream_t st) {
+int launch_tiles(const Product& c, const ProductPlan& plan, const DevInfo& di, int dev, cudaStream_t st) {
   using Cfg = ProductCfg<EPI, TN>;
-  DevInfo di;
-  int dev = 0, rc = current_device_info(&di, &dev);
-  if (rc) return rc;
+  int rc;
   const auto kern = product_kernel<T, EPI, TN>;
   static std::atomic<int> known[64];
   const int pairs = pairs_at_once(reinterpret_cast<const void*>(kern), Cfg::SMEM, dev, di.sm_count, known);
@@ -60,8 +59,11 @@ int launch_tiles(const Product& c, cudaStream_t st) {
   a.tiles_m = ceil_div_int(c.rows, kPairRows);
   a.tiles_n = ceil_div_int(c.cols, Cfg::OUT_COLS);
   a.outputs = c.outputs;
-  a.splits = c.splits;
   a.group = 8;
+  if (plan.items() > 0x7fffffff - 256) return MLPK_ERR_SHAPE;
+  a.full = static_cast<int>(plan.full);
+  a.splits = plan.splits;
+  a.items = static_cast<int>(plan.items());
   a.a_mn = c.a_mn;
   a.b_mn = c.b_mn;
   a.out_a = c.out_a;
@@ -73,7 +75,7 @@ int launch_tiles(const Product& c, cudaStream_t st) {
   a.bias32 = c.bias32;
   a.status = device_status_word(dev);
   if (!a.status) return MLPK_ERR_CUDA;
-  a.partials = c.partials;
+  a.partials = static_cast<float*>(c.workspace);
   a.residual = EPI == kEpiLinear ? c.in[0] : nullptr;
   a.q_pitch = c.q_pitch;
   a.scale_pitch = c.scale_pitch;
@@ -89,21 +91,23 @@ int launch_tiles(const Product& c, cudaStream_t st) {
                                : make_map_2d(&a.b[i], c.b[i], k, cols, kBlockK, TN / 2)))
       return rc;
     for (const auto& [map, v] : {std::make_pair(&a.in[i], EPI == kEpiGatedBwd ? c.in[i] : nullptr),
-                                 std::make_pair(&a.out[i], const_cast<const void*>(EPI == kEpiPartial ? nullptr : c.out[i])),
+                                 std::make_pair(&a.out[i], const_cast<const void*>(c.out[i])),
                                  std::make_pair(&a.keep[i], const_cast<const void*>(c.keep[i]))})
       if (v && (rc = make_map_2d(map, v, cols, rows, Cfg::CHUNK, 32))) return rc;
   }
-  const int64_t total = static_cast<int64_t>(a.tiles_m) * a.tiles_n * a.outputs * a.splits;
-  if (total > 0x7fffffff - 256) return MLPK_ERR_SHAPE;
-  return launch_kernel_early(kern, dim3(2 * static_cast<unsigned>(std::min<int64_t>(total, pairs))), kProductThreads,
-                             Cfg::SMEM, st, a);
+  rc = launch_kernel_early(kern, dim3(2 * static_cast<unsigned>(std::min(a.items, pairs))), kProductThreads, Cfg::SMEM, st, a);
+  if (rc || plan.splits == 1) return rc;
+  if constexpr (EPI == kEpiPlain) {
+    TailArgs t = {a.partials, {c.out[0], c.out[1]}, a.rows, a.cols, a.tiles_m, a.tiles_n, a.outputs, a.group, a.full, a.splits};
+    rc = launch_kernel_early(tail_sum_kernel<T, TN>, dim3(256 * TN / 8 / kTailThreads, static_cast<unsigned>(plan.tail)),
+                             kTailThreads, 0, st, t);
+  }
+  return rc;
 }
 
 template <class T, int EPI>
-int launch_few(const Product& c, cudaStream_t st) {
-  DevInfo di;
-  int dev = 0, rc = current_device_info(&di, &dev);
-  if (rc) return rc;
+int launch_few(const Product& c, const DevInfo& di, int dev, cudaStream_t st) {
+  int rc;
   constexpr bool GATED = EPI == kEpiGated;
   FewArgs a;
   std::memset(&a, 0, sizeof(a));
@@ -155,23 +159,6 @@ int launch_few(const Product& c, cudaStream_t st) {
   return cuda_status(cudaLaunchKernelEx(&cfg, kern, a));
 }
 
-// Tiles of 256 columns, or of 128 where that ends earlier: a narrow tile takes
-// about 0.7 of a wide one's time (its rows are read for half the products), so it
-// pays where the wide tiles leave pairs of CTAs idle (512 x 4096 x 4096 bf16: 64
-// narrow tiles 19.7 us, 32 wide ones 25.3; 1024 x 4096 x 4096: 128 narrow ones in
-// two goes 34.2, 64 wide ones in one 26.3).  A gate's checkpoint needs the wide
-// tile's 128 columns, and so does what reads it.
-template <class T, int EPI>
-int launch_best(const Product& c, int pairs, cudaStream_t st) {
-  if (c.keep_kind != kKeep8 || EPI == kEpiLinear) {
-    const int64_t each = static_cast<int64_t>(ceil_div_int(c.rows, kPairRows)) * c.outputs * c.splits;
-    const int64_t wide = each * ceil_div_int(c.cols, ProductCfg<EPI, 256>::OUT_COLS);
-    const int64_t narrow = each * ceil_div_int(c.cols, ProductCfg<EPI, 128>::OUT_COLS);
-    if (7 * ceil_div_int(narrow, pairs) < 10 * ceil_div_int(wide, pairs)) return launch_tiles<T, EPI, 128>(c, st);
-  }
-  return launch_tiles<T, EPI, 256>(c, st);
-}
-
 // Whether a product goes to few_rows_kernel.  Up to 128 rows it does, but for
 // short reductions of more than 64 (bf16, us, here and in tiles of 256 rows: 1 x
 // 4096 x 4096 8.5 and 24, 64 x 4096 x 14336 24.1 and 30.5, 128 x 4096 x 4096 11.4
@@ -187,26 +174,35 @@ inline bool few_rows(const Product& c, int pairs) {
   return nk >= 48 && 2 * ceil_div_int(c.cols, c.epi == kEpiGated ? 64 : 128) <= pairs;
 }
 
+// The tiles of a product (product_plan.cuh).  A gate's checkpoint needs the wide
+// tile's 128 columns, and so does what reads it.
+inline ProductPlan plan_of(const Product& c, int pairs) {
+  const int nk = ceil_div_int(c.k[0], kBlockK) + ceil_div_int(c.k[1], kBlockK);
+  return product_plan(c.rows, c.cols, c.outputs, c.epi == kEpiGated ? 128 : 256, nk, pairs, c.epi == kEpiPlain,
+                      c.keep_kind != kKeep8 || c.epi == kEpiLinear);
+}
+
+template <class T, int EPI>
+int launch_epi(const Product& c, cudaStream_t st) {
+  DevInfo di;
+  int dev = 0;
+  const int rc = current_device_info(&di, &dev);
+  if (rc) return rc;
+  if (few_rows(c, di.sm_count / 2)) return launch_few<T, EPI>(c, di, dev, st);
+  const ProductPlan plan = plan_of(c, di.sm_count / 2);
+  const int64_t bytes = plan.partials() * static_cast<int64_t>(sizeof(float));
+  if (bytes && !c.workspace) return MLPK_ERR_NULL;
+  if (c.workspace_bytes < bytes) return MLPK_ERR_SCRATCH;
+  return plan.cols == 128 ? launch_tiles<T, EPI, 128>(c, plan, di, dev, st) : launch_tiles<T, EPI, 256>(c, plan, di, dev, st);
+}
+
 template <class T>
 int launch_type(const Product& c, cudaStream_t st) {
-  DevInfo di;
-  const int rc = current_device_info(&di, nullptr);
-  if (rc) return rc;
-  const int pairs = di.sm_count / 2;
-  if (few_rows(c, pairs)) {
-    switch (c.epi) {
-      case kEpiPlain: return launch_few<T, kEpiPlain>(c, st);
-      case kEpiLinear: return launch_few<T, kEpiLinear>(c, st);
-      case kEpiGated: return launch_few<T, kEpiGated>(c, st);
-      default: return launch_few<T, kEpiGatedBwd>(c, st);
-    }
-  }
   switch (c.epi) {
-    case kEpiPlain: return launch_best<T, kEpiPlain>(c, pairs, st);
-    case kEpiPartial: return launch_best<T, kEpiPartial>(c, pairs, st);
-    case kEpiLinear: return launch_best<T, kEpiLinear>(c, pairs, st);
-    case kEpiGated: return launch_best<T, kEpiGated>(c, pairs, st);
-    default: return launch_best<T, kEpiGatedBwd>(c, pairs, st);
+    case kEpiPlain: return launch_epi<T, kEpiPlain>(c, st);
+    case kEpiLinear: return launch_epi<T, kEpiLinear>(c, st);
+    case kEpiGated: return launch_epi<T, kEpiGated>(c, st);
+    default: return launch_epi<T, kEpiGatedBwd>(c, st);
   }
 }
 

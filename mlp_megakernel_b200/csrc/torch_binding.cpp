@@ -508,8 +508,11 @@ Tensor dx_of(const Tensor& shaped, std::initializer_list<Tensor> dz, std::initia
   for (const Tensor& t : dz) zp[n++] = ptr(t);
   n = 0;
   for (const Weight& t : w) wp[n++] = ptr(t.t);
-  check("mlpk_linear_dx", mlpk_linear_dx(rows_of(first), static_cast<int>(d_in), static_cast<int>(first.size(-1)),
-                                         code(first), n, zp, wp, w.begin()->layout, ptr(dx), stream_of(first)));
+  const int k = static_cast<int>(d_in), m = static_cast<int>(first.size(-1)), layout = w.begin()->layout;
+  const int64_t rows = rows_of(first), bytes = mlpk_linear_dx_workspace_size(rows, k, m, code(first), n, layout);
+  const Tensor work = workspace(bytes, first);
+  check("mlpk_linear_dx", mlpk_linear_dx(rows, k, m, code(first), n, zp, wp, layout, ptr(dx), ptr(work),
+                                         std::max<int64_t>(bytes, 0), stream_of(first)));
   return dx;
 }
 void dw_of(const Tensor& x_in, std::initializer_list<Tensor> dz, std::initializer_list<Tensor> dw, int layout) {
@@ -521,7 +524,7 @@ void dw_of(const Tensor& x_in, std::initializer_list<Tensor> dz, std::initialize
   n = 0;
   for (const Tensor& t : dw) wp[n++] = ptr(t);
   const int k = static_cast<int>(x.size(-1)), m = static_cast<int>(dz.begin()->size(-1));
-  const int64_t rows = rows_of(x), bytes = mlpk_linear_dw_workspace_size(rows, k, m, code(x), n);
+  const int64_t rows = rows_of(x), bytes = mlpk_linear_dw_workspace_size(rows, k, m, code(x), n, layout);
   const Tensor work = workspace(bytes, x);
   check("mlpk_linear_dw",
         mlpk_linear_dw(rows, k, m, code(x), n, ptr(x), zp, wp, layout, ptr(work), std::max<int64_t>(bytes, 0), stream_of(x)));
