@@ -99,16 +99,21 @@ int with_value_type(int dtype, F&& f) {
     default: return f(float{});
   }
 }
-unsigned stream_blocks(int64_t work, int sm_count, int each_sm) {
-  return static_cast<unsigned>(std::max<int64_t>(1, std::min<int64_t>(work, static_cast<int64_t>(sm_count) * each_sm)));
+// Blocks of a kernel that goes over its work in turns: as many as the SMs hold at
+// a time (0: a failure).
+template <class K>
+unsigned stream_blocks(K kern, int64_t work, const DevInfo& di, int dev) {
+  const int64_t most =
+      static_cast<int64_t>(di.sm_count) * blocks_per_sm(reinterpret_cast<const void*>(kern), kStreamThreads, 0, dev);
+  return static_cast<unsigned>(std::min(std::max<int64_t>(work, 1), most));
 }
 
-// Blocks of linear_dz_kernel over the rows: enough for every SM, each with at
-// least 8 turns.
+// Blocks of linear_dz_kernel over the rows: enough for every SM, each thread with
+// the 4 rows of a turn at least.
 int dz_parts(int64_t rows, int width, int sm_count) {
   const int64_t across = ceil_to(width, 8 * kDzVectors);
-  const int64_t want = std::max<int64_t>(1, static_cast<int64_t>(sm_count) * 8 / across);
-  return static_cast<int>(std::max<int64_t>(1, std::min(want, ceil_to(rows, 8 * kDzRows))));
+  const int64_t want = std::max<int64_t>(1, static_cast<int64_t>(sm_count) * 4 / across);
+  return static_cast<int>(std::max<int64_t>(1, std::min(want, ceil_to(rows, 4 * kDzRows))));
 }
 
 }  // namespace
@@ -304,16 +309,18 @@ int mlpk_fp8_checkpoint(int64_t rows, int width, int dtype, const void* x, void*
   int rc = check_ptrs({x, q, scale});
   if (rc) return rc;
   DevInfo di;
-  if ((rc = current_device_info(&di, nullptr))) return rc;
+  int dev;
+  if ((rc = current_device_info(&di, &dev))) return rc;
   const int groups = static_cast<int>(ceil_to(width, kGroupCols));
   if (rows > INT64_MAX / width) return MLPK_ERR_SHAPE;
   const bool vectors = width % 8 == 0;
-  const int team = vectors ? 16 : 32;
-  const dim3 grid(stream_blocks(ceil_to(rows * groups, kStreamThreads / team), di.sm_count, 16));
+  const int team = vectors ? 8 : 32;
   return with_value_type(dtype, [&](auto t) {
     using T = decltype(t);
     const auto kern = vectors ? checkpoint_kernel<T, true> : checkpoint_kernel<T, false>;
-    return launch_kernel_early(kern, grid, kStreamThreads, 0, static_cast<cudaStream_t>(stream), rows, width, groups,
+    const unsigned blocks = stream_blocks(kern, ceil_to(rows * groups, 2 * (kStreamThreads / team)), di, dev);
+    if (!blocks) return static_cast<int>(MLPK_ERR_CUDA);
+    return launch_kernel_early(kern, dim3(blocks), kStreamThreads, 0, static_cast<cudaStream_t>(stream), rows, width, groups,
                                static_cast<const T*>(x), static_cast<uint8_t*>(q), scale);
   });
 }
@@ -326,16 +333,17 @@ int mlpk_fp8_restore(int64_t rows, int width, int dtype, const void* q, const fl
   int rc = check_ptrs({q, scale, x});
   if (rc) return rc;
   DevInfo di;
-  if ((rc = current_device_info(&di, nullptr))) return rc;
+  int dev;
+  if ((rc = current_device_info(&di, &dev))) return rc;
   if (rows > INT64_MAX / width) return MLPK_ERR_SHAPE;
   const int groups = static_cast<int>(ceil_to(width, kGroupCols));
-  const bool vectors = width % 8 == 0;
-  const dim3 grid(stream_blocks(ceil_to(rows * (vectors ? width / 8 : width), kStreamThreads), di.sm_count, 16));
+  const int64_t total = rows * width;
   return with_value_type(dtype, [&](auto t) {
     using T = decltype(t);
-    const auto kern = vectors ? restore_kernel<T, true> : restore_kernel<T, false>;
-    return launch_kernel_early(kern, grid, kStreamThreads, 0, static_cast<cudaStream_t>(stream), rows, width, groups,
-                               static_cast<const uint8_t*>(q), scale, static_cast<T*>(x));
+    const unsigned blocks = stream_blocks(restore_kernel<T>, ceil_to(total, 16 * 2 * kStreamThreads), di, dev);
+    if (!blocks) return static_cast<int>(MLPK_ERR_CUDA);
+    return launch_kernel_early(restore_kernel<T>, dim3(blocks), kStreamThreads, 0, static_cast<cudaStream_t>(stream), total, width,
+                               groups, static_cast<const uint8_t*>(q), scale, static_cast<T*>(x));
   });
 }
 

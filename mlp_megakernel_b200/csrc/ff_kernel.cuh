@@ -11,7 +11,7 @@ constexpr int kStreamThreads = 256;
 constexpr int kGroupCols = 128;  // columns that share a scale
 
 // ---------------------------------------------------------------- checkpoints
-// A group of 128 columns of a row is taken by 16 threads, 8 values each, in
+// A group of 128 columns of a row is taken by 8 threads, 16 values each, in
 // vectors; or, where the rows are of no whole number of vectors, by a warp, in
 // single values (neighbouring threads take neighbouring values).
 template <class T>
@@ -34,58 +34,95 @@ __device__ __forceinline__ void store8(T* p, const float (&f)[8]) {
   }
 }
 
+// Where a team's or thread's work lies, step by step: the divisions are done once
+// (one for each item of 8 values cost more than the rest of it).
+struct Steps {
+  int64_t major, major_step;
+  int minor, minor_step, minors;
+  __device__ Steps(int64_t first, int64_t step, int minors_) : minors(minors_) {
+    major = first / minors;
+    minor = static_cast<int>(first - major * minors);
+    major_step = step / minors;
+    minor_step = static_cast<int>(step - major_step * minors);
+  }
+  __device__ __forceinline__ void next() {
+    major += major_step;
+    minor += minor_step;
+    if (minor >= minors) {
+      minor -= minors;
+      ++major;
+    }
+  }
+};
+
+// Groups of a team under way together: one at a time left memory waiting
+// (16384 x 8192 bf16, both ways: 167 us).
+template <bool VECTORS>
+constexpr int kGroupsAtOnce = VECTORS ? 2 : 4;
+
 template <class T, bool VECTORS>
 __global__ void __launch_bounds__(kStreamThreads)
     checkpoint_kernel(int64_t rows, int width, int groups, const T* __restrict__ x, uint8_t* __restrict__ q,
                       float* __restrict__ scale) {
   pdl_enter();
-  constexpr int TEAM = VECTORS ? 16 : 32;
+  constexpr int TEAM = VECTORS ? 8 : 32, N = VECTORS ? 16 : 4, AT_ONCE = kGroupsAtOnce<VECTORS>;
+  const bool wide = width % 16 == 0;  // 16-byte vectors of 8-bit values
   const int64_t teams = static_cast<int64_t>(gridDim.x) * (kStreamThreads / TEAM);
-  const int64_t work = rows * groups, id = threadIdx.x % TEAM;
+  const int id = threadIdx.x % TEAM;
+  const int64_t block_first = static_cast<int64_t>(blockIdx.x) * (kStreamThreads / TEAM);
+  Steps at(block_first + threadIdx.x / TEAM, teams, groups);
   // All threads of a warp take the same number of turns (they exchange values).
-  for (int64_t base = static_cast<int64_t>(blockIdx.x) * (kStreamThreads / TEAM); base < work; base += teams) {
-    const int64_t i = base + threadIdx.x / TEAM;
-    const bool live = i < work;
-    const int64_t row = live ? i / groups : 0;
-    const int g = static_cast<int>(live ? i - row * groups : 0);
-    const int64_t at = row * width + g * kGroupCols;
-    const int cols = min(kGroupCols, width - g * kGroupCols);
-    float inv, most = 0.0f;
-    if constexpr (VECTORS) {
-      float f[8];
-      const bool here = live && id * 8 < cols;
-      if (here) load8(x + at + id * 8, f);
+  for (int64_t base = block_first; base < rows * groups; base += AT_ONCE * teams) {
+    float f[AT_ONCE][N];
+    int64_t first[AT_ONCE], group[AT_ONCE];
+    int cols[AT_ONCE];  // of the group; 0: there is none
 #pragma unroll
-      for (int e = 0; e < 8; ++e) f[e] = here ? f[e] : 0.0f;
+    for (int k = 0; k < AT_ONCE; ++k) {
+      cols[k] = at.major < rows ? min(kGroupCols, width - at.minor * kGroupCols) : 0;
+      first[k] = at.major * width + at.minor * kGroupCols;
+      group[k] = at.major * groups + at.minor;
+      at.next();
 #pragma unroll
-      for (int e = 0; e < 8; e += 2) most = max_abs(most, f[e], f[e + 1]);
+      for (int e = 0; e < N; ++e) f[k][e] = 0.0f;
+      if constexpr (VECTORS) {
 #pragma unroll
-      for (int o = 8; o; o >>= 1) most = max_nan(most, __shfl_xor_sync(0xffffffffu, most, o));
-      const float s = checkpoint_scale(most, &inv);
-      if (here) {
-        uint32_t w[2];
+        for (int v = 0; v < 2; ++v)
+          if (id * 16 + 8 * v < cols[k])
+            load8(x + first[k] + id * 16 + 8 * v, *reinterpret_cast<float(*)[8]>(&f[k][8 * v]));
+      } else {
 #pragma unroll
-        for (int k = 0; k < 2; ++k)
-          w[k] = to_fp8x2(make_float2(f[4 * k] * inv, f[4 * k + 1] * inv)) |
-                 static_cast<uint32_t>(to_fp8x2(make_float2(f[4 * k + 2] * inv, f[4 * k + 3] * inv))) << 16;
-        *reinterpret_cast<uint2*>(q + at + id * 8) = make_uint2(w[0], w[1]);
-        if (id == 0) scale[i] = s;
+        for (int e = 0; e < N; ++e)
+          if (id + 32 * e < cols[k]) f[k][e] = to_float(x[first[k] + id + 32 * e]);
       }
-    } else {
-      float f[4];
+    }
 #pragma unroll
-      for (int e = 0; e < 4; ++e) f[e] = live && id + 32 * e < cols ? to_float(x[at + id + 32 * e]) : 0.0f;
-      most = max_abs(max_abs(0.0f, f[0], f[1]), f[2], f[3]);
+    for (int k = 0; k < AT_ONCE; ++k) {
+      float inv, most = 0.0f;
 #pragma unroll
-      for (int o = 16; o; o >>= 1) most = max_nan(most, __shfl_xor_sync(0xffffffffu, most, o));
+      for (int e = 0; e < N; e += 2) most = max_abs(most, f[k][e], f[k][e + 1]);
+#pragma unroll
+      for (int o = TEAM / 2; o; o >>= 1) most = max_nan(most, __shfl_xor_sync(0xffffffffu, most, o));
       const float s = checkpoint_scale(most, &inv);
-      if (live) {
+      uint32_t w[N / 4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (id + 32 * e < cols)
-            q[at + id + 32 * e] = static_cast<uint8_t>(to_fp8x2(make_float2(f[e] * inv, 0.0f)));
-        if (id == 0) scale[i] = s;
+      for (int v = 0; v < N / 4; ++v)
+        w[v] = to_fp8x2(make_float2(f[k][4 * v] * inv, f[k][4 * v + 1] * inv)) |
+               static_cast<uint32_t>(to_fp8x2(make_float2(f[k][4 * v + 2] * inv, f[k][4 * v + 3] * inv))) << 16;
+      if constexpr (VECTORS) {
+        uint8_t* to = q + first[k] + id * 16;
+        if (wide && id * 16 < cols[k]) {
+          *reinterpret_cast<uint4*>(to) = make_uint4(w[0], w[1], w[2], w[3]);
+        } else {
+#pragma unroll
+          for (int v = 0; v < 2; ++v)
+            if (id * 16 + 8 * v < cols[k]) *reinterpret_cast<uint2*>(to + 8 * v) = make_uint2(w[2 * v], w[2 * v + 1]);
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < N; ++e)
+          if (id + 32 * e < cols[k]) q[first[k] + id + 32 * e] = static_cast<uint8_t>(w[0] >> 8 * e);
       }
+      if (id == 0 && cols[k] > 0) scale[group[k]] = s;
     }
   }
 }
@@ -99,34 +136,81 @@ __device__ __forceinline__ float clip(float v, float most) {  // a NaN stays
   return v > most ? most : v < -most ? -most : v;
 }
 
-template <class T, bool VECTORS>
+// 16 values of the flat tensor at a time, whatever the width: they have one
+// scale, or each looks up its own (at a group's end where 16 does not divide the
+// width).
+template <class T>
 __global__ void __launch_bounds__(kStreamThreads)
-    restore_kernel(int64_t rows, int width, int groups, const uint8_t* __restrict__ q,
+    restore_kernel(int64_t total, int width, int groups, const uint8_t* __restrict__ q,
                    const float* __restrict__ scale, T* __restrict__ x) {
   pdl_enter();
-  constexpr int EACH = VECTORS ? 8 : 1;
-  const int per_row = width / EACH;
-  const int64_t total = rows * per_row, step = static_cast<int64_t>(gridDim.x) * kStreamThreads;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * kStreamThreads + threadIdx.x; i < total; i += step) {
-    const int64_t row = i / per_row;
-    const int col = static_cast<int>(i - row * per_row) * EACH;
-    const float s = scale[row * groups + col / kGroupCols];
-    if constexpr (VECTORS) {
-      float2 f[4];
-      float v[8];
-      unpack_fp8<8>(load_raw<uint16_t, 4>(reinterpret_cast<const uint16_t*>(q + i * 8)), f);
+  constexpr int AT_ONCE = 2, N = 16;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * kStreamThreads * N;
+  int64_t i = (static_cast<int64_t>(blockIdx.x) * kStreamThreads + threadIdx.x) * N;
+  Steps at(i, step, width);
+  for (; i < total; i += AT_ONCE * step) {
+    Raw<uint16_t, N / 2> raw[AT_ONCE];
+    float s[AT_ONCE];
+    int64_t row[AT_ONCE];
+    int col[AT_ONCE];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        v[2 * e] = clip(f[e].x * s, finite_max<T>());
-        v[2 * e + 1] = clip(f[e].y * s, finite_max<T>());
+    for (int k = 0; k < AT_ONCE; ++k) {
+      row[k] = at.major;
+      col[k] = at.minor;
+      at.next();
+      const int64_t p = i + k * step;
+      if (p + N <= total) {
+        raw[k] = load_raw<uint16_t, N / 2>(reinterpret_cast<const uint16_t*>(q + p));
+        s[k] = scale[row[k] * groups + col[k] / kGroupCols];
       }
-      store8(x + i * 8, v);
-    } else {
-      Raw<uint16_t, 1> r;
-      r.v[0] = q[i];
-      float2 f[1];
-      unpack_fp8<2>(r, f);
-      x[i] = from_float<T>(clip(f[0].x * s, finite_max<T>()));
+    }
+#pragma unroll
+    for (int k = 0; k < AT_ONCE; ++k) {
+      const int64_t p = i + k * step;
+      int64_t r = row[k];
+      int c = col[k];
+      if (p + N <= total) {
+        const bool one = c + N <= width && c % kGroupCols + N <= kGroupCols;
+        float2 f[N / 2];
+        float v[N];
+        unpack_fp8<N>(raw[k], f);
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+          if (!one && e > 0) {
+            if (++c == width) c = 0, ++r;
+            if (c % kGroupCols == 0) s[k] = scale[r * groups + c / kGroupCols];
+          }
+          v[e] = clip((e % 2 ? f[e / 2].y : f[e / 2].x) * s[k], finite_max<T>());
+        }
+        if constexpr (sizeof(T) == 2) {
+          uint32_t w[N / 2];
+#pragma unroll
+          for (int e = 0; e < N / 2; ++e) {
+            const typename Pair<T>::type y = Pair<T>::round(v[2 * e], v[2 * e + 1]);
+            w[e] = *reinterpret_cast<const uint32_t*>(&y);
+          }
+          if (reinterpret_cast<uintptr_t>(x) % 32 == 0) {
+            asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(x + p), "r"(w[0]), "r"(w[1]),
+                         "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                         : "memory");
+          } else {
+            reinterpret_cast<uint4*>(x + p)[0] = make_uint4(w[0], w[1], w[2], w[3]);
+            reinterpret_cast<uint4*>(x + p)[1] = make_uint4(w[4], w[5], w[6], w[7]);
+          }
+        } else {
+          store8(x + p, *reinterpret_cast<const float(*)[8]>(&v[0]));
+          store8(x + p + 8, *reinterpret_cast<const float(*)[8]>(&v[8]));
+        }
+      } else {
+        for (int64_t e = p; e < total; ++e) {
+          Raw<uint16_t, 1> one_value;
+          one_value.v[0] = q[e];
+          float2 f[1];
+          unpack_fp8<2>(one_value, f);
+          x[e] = from_float<T>(clip(f[0].x * scale[r * groups + c / kGroupCols], finite_max<T>()));
+          if (++c == width) c = 0, ++r;
+        }
+      }
     }
   }
 }
@@ -152,41 +236,58 @@ constexpr int kDzVectors = 32, kDzRows = kStreamThreads / kDzVectors;
 template <class T>
 __global__ void __launch_bounds__(kStreamThreads) linear_dz_kernel(const DzArgs a) {
   pdl_enter();
+  constexpr int AT_ONCE = 4;  // rows under way (one: 16384 x 8192 bf16 with z in 8 bits 180 us)
   const int v = threadIdx.x % kDzVectors, r = threadIdx.x / kDzVectors;
   const int col = (blockIdx.x * kDzVectors + v) * 8;
-  const bool live = col < a.width;
+  const int64_t step = static_cast<int64_t>(gridDim.y) * kDzRows;
+  const bool fp8 = a.keep_kind == 2;
   float sum[8] = {};
-  if (live)
-    for (int64_t row = static_cast<int64_t>(blockIdx.y) * kDzRows + r; row < a.rows;
-         row += static_cast<int64_t>(gridDim.y) * kDzRows) {
-      const int64_t at = row * a.width + col;
-      float d[8];
-      load8(static_cast<const T*>(a.grad) + at, d);
-      if (a.act != kActNone) {
-        float z[8];
-        if (a.keep_kind == 2) {
-          const float s = a.scale[row * a.scale_pitch + col / kGroupCols];
-          float2 f[4];
-          unpack_fp8<8>(load_raw<uint16_t, 4>(reinterpret_cast<const uint16_t*>(
-                            static_cast<const uint8_t*>(a.z) + row * a.q_pitch + col)),
-                        f);
+  if (col < a.width)
+    for (int64_t first = static_cast<int64_t>(blockIdx.y) * kDzRows + r; first < a.rows; first += AT_ONCE * step) {
+      Raw<T, 8> graw[AT_ONCE], zraw[AT_ONCE];
+      float s[AT_ONCE];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) z[2 * e] = f[e].x * s, z[2 * e + 1] = f[e].y * s;
-        } else {
-          load8(static_cast<const T*>(a.z) + at, z);
+      for (int k = 0; k < AT_ONCE; ++k) {
+        const int64_t row = first + k * step, at = row * a.width + col;
+        if (row >= a.rows) break;
+        graw[k] = load_raw<T, 8>(static_cast<const T*>(a.grad) + at);
+        if (a.act != kActNone && fp8) {
+          s[k] = a.scale[row * a.scale_pitch + col / kGroupCols];
+          *reinterpret_cast<Raw<uint16_t, 4>*>(&zraw[k]) = load_raw<uint16_t, 4>(
+              reinterpret_cast<const uint16_t*>(static_cast<const uint8_t*>(a.z) + row * a.q_pitch + col));
+        } else if (a.act != kActNone) {
+          zraw[k] = load_raw<T, 8>(static_cast<const T*>(a.z) + at);
         }
-        with_act(a.act, [&](auto act) {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            float slope;
-            act_both<decltype(act)::value>(z[e], slope);
-            d[e] *= slope;
-          }
-        });
       }
-      if (a.dz) store8(static_cast<T*>(a.dz) + at, d);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) sum[e] += d[e];
+      for (int k = 0; k < AT_ONCE; ++k) {
+        const int64_t row = first + k * step;
+        if (row >= a.rows) break;
+        float d[8];
+        unpack<T, 8>(graw[k], d);
+        if (a.act != kActNone) {
+          float z[8];
+          if (fp8) {
+            float2 f[4];
+            unpack_fp8<8>(*reinterpret_cast<const Raw<uint16_t, 4>*>(&zraw[k]), f);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) z[2 * e] = f[e].x * s[k], z[2 * e + 1] = f[e].y * s[k];
+          } else {
+            unpack<T, 8>(zraw[k], z);
+          }
+          with_act(a.act, [&](auto act) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              float slope;
+              act_both<decltype(act)::value>(z[e], slope);
+              d[e] *= slope;
+            }
+          });
+        }
+        if (a.dz) store8(static_cast<T*>(a.dz) + row * a.width + col, d);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sum[e] += d[e];
+      }
     }
   if (!a.partial) return;
   __shared__ float s_sum[kDzRows][kDzVectors * 8 + 4];
