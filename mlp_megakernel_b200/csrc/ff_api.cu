@@ -108,12 +108,24 @@ unsigned stream_blocks(K kern, int64_t work, const DevInfo& di, int dev) {
   return static_cast<unsigned>(std::min(std::max<int64_t>(work, 1), most));
 }
 
-// Blocks of linear_dz_kernel over the rows: enough for every SM, each thread with
-// the 4 rows of a turn at least.
+// Blocks of linear_dz_kernel over the rows: what the SMs hold at a time, each
+// thread with the 4 rows of a turn at least.
 int dz_parts(int64_t rows, int width, int sm_count) {
   const int64_t across = ceil_to(width, 8 * kDzVectors);
-  const int64_t want = std::max<int64_t>(1, static_cast<int64_t>(sm_count) * 4 / across);
+  const int64_t want = std::max<int64_t>(1, static_cast<int64_t>(sm_count) * kDzBlocks / across);
   return static_cast<int>(std::max<int64_t>(1, std::min(want, ceil_to(rows, 4 * kDzRows))));
+}
+
+template <class T, bool FP8>
+auto dz_kernel(int act) -> void (*)(DzArgs) {
+  switch (act) {
+    case kActRelu: return linear_dz_kernel<T, kActRelu, FP8>;
+    case kActSilu: return linear_dz_kernel<T, kActSilu, FP8>;
+    case kActGeluTanh: return linear_dz_kernel<T, kActGeluTanh, FP8>;
+    case kActSoftplus: return linear_dz_kernel<T, kActSoftplus, FP8>;
+    case kActSigmoid: return linear_dz_kernel<T, kActSigmoid, FP8>;
+    default: return linear_dz_kernel<T, kActNone, false>;
+  }
 }
 
 }  // namespace
@@ -175,11 +187,13 @@ int mlpk_linear_dz(int64_t rows, int width, int dtype, int act, const void* grad
   const int parts = dz_parts(rows, width, di.sm_count);
   if (db && workspace_bytes < static_cast<int64_t>(parts) * width * static_cast<int64_t>(sizeof(float)))
     return MLPK_ERR_SCRATCH;
-  DzArgs a = {rows, width, act, keep, static_cast<int>(ceil_to(width, kGroupCols)), mlpk_fp8_pitch(width), grad_out, z,
+  DzArgs a = {rows, width, static_cast<int>(ceil_to(width, kGroupCols)), mlpk_fp8_pitch(width), grad_out, z,
               z_scale, dz, db ? static_cast<float*>(workspace) : nullptr};
   const dim3 grid(static_cast<unsigned>(ceil_to(width, 8 * kDzVectors)), parts);
-  rc = dtype == MLPK_DT_F16 ? launch_kernel_early(linear_dz_kernel<__half>, grid, kStreamThreads, 0, st, a)
-                            : launch_kernel_early(linear_dz_kernel<__nv_bfloat16>, grid, kStreamThreads, 0, st, a);
+  const bool fp8 = keep == MLPK_KEEP_FP8;
+  const auto kern = dtype == MLPK_DT_F16 ? (fp8 ? dz_kernel<__half, true>(act) : dz_kernel<__half, false>(act))
+                                         : (fp8 ? dz_kernel<__nv_bfloat16, true>(act) : dz_kernel<__nv_bfloat16, false>(act));
+  rc = launch_kernel_early(kern, grid, kStreamThreads, 0, st, a);
   if (rc || !db) return rc;
   return with_value_type(db_dtype, [&](auto t) {
     using W = decltype(t);

@@ -223,7 +223,7 @@ __global__ void __launch_bounds__(kStreamThreads)
 // bias_grad_kernel adds in order.
 struct DzArgs {
   int64_t rows;
-  int width, act, keep_kind, scale_pitch;
+  int width, scale_pitch;
   int64_t q_pitch;
   const void* grad;
   const void* z;         // 16 bits, or 8
@@ -232,61 +232,65 @@ struct DzArgs {
   float* partial;        // NULL: not wanted
 };
 constexpr int kDzVectors = 32, kDzRows = kStreamThreads / kDzVectors;
+constexpr int kDzBlocks = 4;  // of an SM
 
-template <class T>
-__global__ void __launch_bounds__(kStreamThreads) linear_dz_kernel(const DzArgs a) {
+template <class T, int ACT, bool FP8>
+__global__ void __launch_bounds__(kStreamThreads, kDzBlocks) linear_dz_kernel(const DzArgs a) {
   pdl_enter();
-  constexpr int AT_ONCE = 4;  // rows under way (one: 16384 x 8192 bf16 with z in 8 bits 180 us)
+  constexpr int AT_ONCE = 2;  // rows under way
   const int v = threadIdx.x % kDzVectors, r = threadIdx.x / kDzVectors;
   const int col = (blockIdx.x * kDzVectors + v) * 8;
   const int64_t step = static_cast<int64_t>(gridDim.y) * kDzRows;
-  const bool fp8 = a.keep_kind == 2;
   float sum[8] = {};
   if (col < a.width)
     for (int64_t first = static_cast<int64_t>(blockIdx.y) * kDzRows + r; first < a.rows; first += AT_ONCE * step) {
-      Raw<T, 8> graw[AT_ONCE], zraw[AT_ONCE];
+      uint4 graw[AT_ONCE], zraw[AT_ONCE];
       float s[AT_ONCE];
 #pragma unroll
       for (int k = 0; k < AT_ONCE; ++k) {
-        const int64_t row = first + k * step, at = row * a.width + col;
-        if (row >= a.rows) break;
-        graw[k] = load_raw<T, 8>(static_cast<const T*>(a.grad) + at);
-        if (a.act != kActNone && fp8) {
-          s[k] = a.scale[row * a.scale_pitch + col / kGroupCols];
-          *reinterpret_cast<Raw<uint16_t, 4>*>(&zraw[k]) = load_raw<uint16_t, 4>(
-              reinterpret_cast<const uint16_t*>(static_cast<const uint8_t*>(a.z) + row * a.q_pitch + col));
-        } else if (a.act != kActNone) {
-          zraw[k] = load_raw<T, 8>(static_cast<const T*>(a.z) + at);
+        const int64_t row = first + k * step;
+        graw[k] = zraw[k] = make_uint4(0, 0, 0, 0);
+        s[k] = 0.0f;
+        if (row < a.rows) {
+          graw[k] = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.grad) + row * a.width + col);
+          if constexpr (ACT != kActNone && FP8) {
+            s[k] = a.scale[row * a.scale_pitch + col / kGroupCols];
+            const uint2 x = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(a.z) + row * a.q_pitch + col);
+            zraw[k].x = x.x;
+            zraw[k].y = x.y;
+          } else if constexpr (ACT != kActNone) {
+            zraw[k] = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.z) + row * a.width + col);
+          }
         }
       }
 #pragma unroll
       for (int k = 0; k < AT_ONCE; ++k) {
         const int64_t row = first + k * step;
-        if (row >= a.rows) break;
         float d[8];
-        unpack<T, 8>(graw[k], d);
-        if (a.act != kActNone) {
+        unpack<T, 8>(*reinterpret_cast<const Raw<T, 8>*>(&graw[k]), d);
+        if constexpr (ACT != kActNone) {
           float z[8];
-          if (fp8) {
+          if constexpr (FP8) {
+            const uint2 x = make_uint2(zraw[k].x, zraw[k].y);
             float2 f[4];
-            unpack_fp8<8>(*reinterpret_cast<const Raw<uint16_t, 4>*>(&zraw[k]), f);
+            unpack_fp8<8>(*reinterpret_cast<const Raw<uint16_t, 4>*>(&x), f);
 #pragma unroll
             for (int e = 0; e < 4; ++e) z[2 * e] = f[e].x * s[k], z[2 * e + 1] = f[e].y * s[k];
           } else {
-            unpack<T, 8>(zraw[k], z);
+            unpack<T, 8>(*reinterpret_cast<const Raw<T, 8>*>(&zraw[k]), z);
           }
-          with_act(a.act, [&](auto act) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              float slope;
-              act_both<decltype(act)::value>(z[e], slope);
-              d[e] *= slope;
-            }
-          });
+          for (int e = 0; e < 8; ++e) {
+            float slope;
+            act_both<ACT>(z[e], slope);
+            d[e] *= slope;
+          }
         }
-        if (a.dz) store8(static_cast<T*>(a.dz) + row * a.width + col, d);
+        if (row < a.rows) {
+          if (a.dz) store8(static_cast<T*>(a.dz) + row * a.width + col, d);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) sum[e] += d[e];
+          for (int e = 0; e < 8; ++e) sum[e] += d[e];
+        }
       }
     }
   if (!a.partial) return;
