@@ -363,7 +363,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kProductThreads, 1)
         const int k0 = item.k0, k1 = item.k1;
         const int buf = mine & 1;
         const uint32_t d = tmem + buf * TN;
-        ok = mbar_wait_cluster(bar_free(buf), ((mine >> 1) & 1) ^ 1, abort_flag, kDevTimeoutMma, status);
+        ok = mbar_wait_to(bar_free(buf), ((mine >> 1) & 1) ^ 1, abort_flag, kDevTimeoutMma, status);
         if (!ok) break;
         tc_fence_after();
         uint32_t more = 0;  // the first product of a tile overwrites the accumulator
@@ -656,9 +656,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kProductThreads, 1)
               h[from / 2 + i] = *reinterpret_cast<const uint32_t*>(&x);
             }
           }
-          end_tile(&p.out[0], tile_g, col, row0);
-          end_tile(&p.out[1], tile_u, col, row0);
-          if (lane == 0) bulk_wait_group_read<1>();
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            tma_store_2d(&p.out[0], tile_g, col, row0);
+            bulk_commit_group();
+            tma_store_2d(&p.out[1], tile_u, col, row0);
+            bulk_commit_group();
+            bulk_wait_group_read<1>();
+          }
           __syncwarp();
 #pragma unroll
           for (int u = 0; u < CHUNK / 8; ++u)
@@ -669,7 +675,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kProductThreads, 1)
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive_cluster(mapa_shared(bar_free(buf), 0));
+      if (lane == 0) mbar_arrive_remote(mapa_shared(bar_free(buf), 0));
     }
     if (lane == 0) bulk_wait_group<0>();
     __syncwarp();
