@@ -64,10 +64,9 @@ def _check_kept_type(activation_dtype) -> None:
         raise TypeError(f"activation_dtype must be None (the operands' type) or {FP8}, got {activation_dtype}")
 
 
-def _require_cuda(*ts) -> None:
-    for t in ts:
-        if isinstance(t, Tensor) and not t.is_cuda:
-            raise RuntimeError("the feed-forward operators run on CUDA (sm_100) only; got a CPU tensor")
+def _require_cuda(t) -> None:
+    if isinstance(t, Tensor) and not t.is_cuda:
+        raise RuntimeError("the feed-forward operators run on CUDA (sm_100) only; got a CPU tensor")
 
 
 def _check_x(x, what="x") -> None:
@@ -213,7 +212,7 @@ def _kept_fake(ref, rows, width, keep):
 def _linear_op(x: Tensor, weight: Tensor, bias: Optional[Tensor], residual: Optional[Tensor], act: int,
                keep: int) -> list[Tensor]:
     """[out], and z (with its scales) as `keep` says: 0 not, 1 in x's type, 2 in 8 bits."""
-    _require_cuda(x, weight, bias, residual)
+    _require_cuda(x)
     _check_linear(x, weight, bias, residual)
     _check_act(act)
     _check_keep(keep)
@@ -240,7 +239,7 @@ def _linear_bwd_op(grad_out: Tensor, x: Optional[Tensor], x_scale: Optional[Tens
                    z_scale: Optional[Tensor], act: int, db_dtype: torch.dtype, want_dx: bool, want_dw: bool,
                    want_db: bool) -> list[Tensor]:
     """[dx], [dw] and [db], as wanted.  x with x_scale: its checkpoint."""
-    _require_cuda(grad_out, x, x_scale, weight, z, z_scale)
+    _require_cuda(grad_out)
     _check_linear_bwd(grad_out, x, x_scale, weight, z, z_scale, act, db_dtype, (want_dx, want_dw, want_db))
     got = native().linear_backward(grad_out, x, x_scale, weight, z, z_scale, act, db_dtype == torch.float32, want_dx,
                                    want_dw, want_db)
@@ -259,7 +258,7 @@ def _linear_bwd_fake(grad_out, x, x_scale, weight, z, z_scale, act, db_dtype, wa
 def _gated_op(x: Tensor, w_gate: Tensor, w_up: Tensor, w_down: Tensor, residual: Optional[Tensor], act: int,
               keep: int) -> list[Tensor]:
     """[out], and g (with its scales) and u (with its) as `keep` says."""
-    _require_cuda(x, w_gate, w_up, w_down, residual)
+    _require_cuda(x)
     _check_gated(x, w_gate, w_up, w_down, residual)
     _check_act(act)
     _check_keep(keep)
@@ -280,7 +279,7 @@ def _gated_bwd_op(grad_out: Tensor, x: Optional[Tensor], x_scale: Optional[Tenso
                   w_down: Tensor, g: Tensor, g_scale: Optional[Tensor], u: Tensor, u_scale: Optional[Tensor], act: int,
                   want_dx: bool, want_dgu: bool, want_dd: bool) -> list[Tensor]:
     """[dx], [dw_gate, dw_up] and [dw_down], as wanted."""
-    _require_cuda(grad_out, x, x_scale, w_gate, w_up, w_down, g, g_scale, u, u_scale)
+    _require_cuda(grad_out)
     _check_gated_bwd(grad_out, x, x_scale, w_gate, w_up, w_down, g, g_scale, u, u_scale, act, (want_dx, want_dgu, want_dd))
     got = native().gated_backward(grad_out, x, x_scale, w_gate, w_up, w_down, g, g_scale, u, u_scale, act, want_dx,
                                   want_dgu, want_dd)
@@ -312,7 +311,7 @@ def _checkpoint_fake(x):
 
 @torch.library.custom_op("mlpk::fp8_restore", mutates_args=())
 def _restore_op(q: Tensor, scale: Tensor, dtype: torch.dtype) -> Tensor:
-    _require_cuda(q, scale)
+    _require_cuda(q)
     _check_quantized(q, scale)
     _check_restored(dtype)
     return native().restore(q, scale, dtype)
@@ -412,7 +411,7 @@ def fused_linear(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, *, ac
         if got is not None:
             return got
     _refuse_transforms("fused_linear", x, weight, bias, residual)
-    _require_cuda(x, weight, bias, residual)
+    _require_cuda(x)
     _check_linear(x, weight, bias, residual)
     if _needs_grad(x, weight, bias, residual):
         return _LinearFn.apply(x, weight, bias, residual, act, fp8)
@@ -438,7 +437,7 @@ def fused_gated_mlp(x: Tensor, w_gate: Tensor, w_up: Tensor, w_down: Tensor, *, 
         if got is not None:
             return got
     _refuse_transforms("fused_gated_mlp", x, w_gate, w_up, w_down, residual)
-    _require_cuda(x, w_gate, w_up, w_down, residual)
+    _require_cuda(x)
     _check_gated(x, w_gate, w_up, w_down, residual)
     if _needs_grad(x, w_gate, w_up, w_down, residual):
         return _GatedFn.apply(x, w_gate, w_up, w_down, residual, act, fp8)
@@ -476,7 +475,7 @@ def fp8_restore(q: Tensor, scale: Tensor, dtype: torch.dtype = torch.bfloat16) -
         if got is not None:
             return got
     _refuse_transforms("fp8_restore", q, scale)
-    _require_cuda(q, scale)
+    _require_cuda(q)
     _check_quantized(q, scale)
     _check_restored(dtype)
     return torch.ops.mlpk.fp8_restore(q, scale, dtype)
