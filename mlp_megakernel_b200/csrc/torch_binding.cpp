@@ -630,6 +630,7 @@ struct LinearNode : torch::autograd::Function<LinearNode> {
     ctx->saved_data["act"] = act;
     ctx->saved_data["bias"] = static_cast<int64_t>(b.defined() ? b.scalar_type() : at::ScalarType::Undefined);
     ctx->saved_data["residual"] = r.defined();
+    ctx->saved_data["x_needs"] = x.requires_grad();
     ctx->save_for_backward({k.v, k.scale, w, z.v, z.scale});
     return {out};
   }
@@ -660,9 +661,11 @@ struct LinearNode : torch::autograd::Function<LinearNode> {
         if (want_db) got.db = t[i++];
       }
     }
-    // Whether a gradient depends on an input that needs one itself.
-    const bool by_z = act != MLPK_ACT_NONE && (want_dx || want_dw || want_db);
-    return {once_if(got.dx, go, by_z || want_dw), once_if(got.dw, go, by_z || want_dx), once_if(got.db, go, by_z),
+    // Whether a gradient depends on an input that needs one itself (wanted in this
+    // pass or not): through z on x, w and b, which are not all without one.
+    const bool by_z = act != MLPK_ACT_NONE;
+    return {once_if(got.dx, go, by_z || w.requires_grad()),
+            once_if(got.dw, go, by_z || ctx->saved_data["x_needs"].toBool()), once_if(got.db, go, by_z),
             want_dr ? go : Tensor(), Tensor(), Tensor()};
   }
 };
@@ -677,6 +680,7 @@ struct GatedNode : torch::autograd::Function<GatedNode> {
     const Kept k = input_kept(x, wg.requires_grad() || wu.requires_grad(), fp8);
     ctx->saved_data["act"] = act;
     ctx->saved_data["residual"] = r.defined();
+    ctx->saved_data["x_needs"] = x.requires_grad();
     ctx->save_for_backward({k.v, k.scale, wg, wu, wd, g.v, g.scale, u.v, u.scale});
     return {out};
   }
@@ -709,9 +713,16 @@ struct GatedNode : torch::autograd::Function<GatedNode> {
         if (want_d) got.dwd = t[i++];
       }
     }
-    return {once_if(got.dx, go, any),  once_if(want_g ? got.dwg : Tensor(), go, any),
-            once_if(want_u ? got.dwu : Tensor(), go, any), once_if(got.dwd, go, any),
-            want_dr ? go : Tensor(),   Tensor(), Tensor()};
+    // Whether a gradient depends on an input that needs one itself: w_up's does not
+    // on w_up, w_down's not on w_down.
+    const bool x_or_g = ctx->saved_data["x_needs"].toBool() || wg.requires_grad();
+    return {once_if(got.dx, go, true),
+            once_if(want_g ? got.dwg : Tensor(), go, true),
+            once_if(want_u ? got.dwu : Tensor(), go, x_or_g || wd.requires_grad()),
+            once_if(got.dwd, go, x_or_g || wu.requires_grad()),
+            want_dr ? go : Tensor(),
+            Tensor(),
+            Tensor()};
   }
 };
 
