@@ -2,6 +2,7 @@
 // alone, so that it can be gone over without a GPU.
 #pragma once
 #include <cstdint>
+#include <initializer_list>
 
 namespace mlpk {
 
@@ -14,6 +15,7 @@ struct FewPlan {
   int nt = 0;      // rows of a tile
   int stages = 0;  // depth of the ring
   int ranks = 0;   // CTAs that share a tile's reduction
+  int each_sm = 0; // CTAs that an SM is to hold
   int tiles = 0, row_tiles = 0;
 };
 
@@ -28,19 +30,32 @@ inline FewPlan few_plan(int64_t rows, int cols, int nk, int tile_cols, int sm_co
   FewPlan p;
   p.nt = 16;
   while (p.nt < rows && p.nt < kFewMostRows) p.nt *= 2;
-  // Two CTAs an SM for the narrowest tiles, one for the others: a wide tile meets
-  // in more shared memory than it is worth to share it further (128 x 4096 x 4096
-  // bf16: 8 ranks 15.6 us, 4 ranks 11.4).
-  const int each_sm = p.nt <= 32 ? 2 : 1;
-  p.stages = kFewMaxStages;
-  while (p.stages > 2 && few_smem(p.nt, p.stages) > (each_sm == 2 ? 113 * 1024 : 226 * 1024)) --p.stages;
   p.tiles = (cols + tile_cols - 1) / tile_cols;
   p.row_tiles = static_cast<int>((rows + p.nt - 1) / p.nt);
-  // As many shares as fill the SMs in one go, 4 blocks in each at least.
-  p.ranks = 1;
-  while (p.ranks < kFewMaxRanks && static_cast<int64_t>(p.tiles) * p.row_tiles * p.ranks * 2 <= each_sm * sm_count &&
-         nk >= p.ranks * 2 * 4)
-    p.ranks *= 2;
+  // Shares of a tile's reduction: as many as fill the SMs in one go with `each`
+  // CTAs, 4 blocks in each at least.  A cluster has its SMs from one part of the
+  // chip, so larger ones leave some out, a ninth of them at most (clusters of 8, two
+  // an SM: 264 of 296 CTAs); of 7, or of 3 with one CTA an SM, they ended in two
+  // goes (8 x 5120 x 5120 bf16: 7 shares 15.1 us, 4 shares 10.6; 64 x 2048 x 5120: 3
+  // shares 17.2, 2 shares 10.1).
+  const int64_t tiles = static_cast<int64_t>(p.tiles) * p.row_tiles;
+  const auto shares = [&](int each) {
+    for (int n : {8, 4, 3, 2})
+      if ((n != 3 || each == 2) && tiles * n * (n > 2 ? 9 : 8) <= static_cast<int64_t>(each) * sm_count * 8 && nk >= 4 * n)
+        return n;
+    return 1;
+  };
+  // One CTA an SM with a deep ring, where two would not have more of the SMs at
+  // work: a tile of many rows meets in more shared memory than it is worth to share
+  // it further (128 x 4096 x 4096 bf16: 8 shares 15.6 us, 4 shares 11.4; 48 x 4096 x
+  // 14336, gated, 224 tiles: one an SM 45.0, two 39.5; 64 x 4096 x 11008, 86 tiles:
+  // one share 21.1, three 17.1).  Tiles of few rows always two.
+  const int64_t one = tiles * shares(1), two = tiles * shares(2);
+  const bool fuller = 20 * two > 23 * 2 * (one < sm_count ? one : sm_count) || one > sm_count;
+  p.each_sm = p.nt <= 32 || (p.nt < kFewMostRows && fuller) ? 2 : 1;
+  p.ranks = shares(p.each_sm);
+  p.stages = kFewMaxStages;
+  while (p.stages > 2 && few_smem(p.nt, p.stages) > (p.each_sm == 2 ? 113 * 1024 : 226 * 1024)) --p.stages;
   return p;
 }
 

@@ -34,6 +34,11 @@ constexpr int kMaxBlockSmem = 227 * 1024;  // dynamic shared memory of a block
 // status is kept for mlpk_last_cuda_error.
 __attribute__((visibility("hidden"))) int blocks_per_sm(const void* kern, int threads, size_t smem, int dev);
 
+// Clusters of `ranks` blocks of a kernel that the device holds at a time (found
+// once for each size, after blocks_per_sm of the same); 0 on a failure.
+__attribute__((visibility("hidden"))) int clusters_at_once(const void* kern, int threads, size_t smem, int ranks,
+                                                           int dev);
+
 // The tensor map of a 2-D tensor [outer][inner] (inner contiguous) of 16-bit
 // elements (elem_bytes 2) or fp32 (4), box {box_inner, box_outer}, swizzled in the
 // box's row pitch (128, 64 or 32 bytes).  atom32: 128-byte rows swizzled in

@@ -111,6 +111,31 @@ int blocks_per_sm(const void* kern, int threads, size_t smem, int dev) try {
   return 0;
 }
 
+int clusters_at_once(const void* kern, int threads, size_t smem, int ranks, int dev) try {
+  static std::mutex mu;
+  static std::map<std::tuple<const void*, int, size_t, int, int>, int> known;
+  std::lock_guard<std::mutex> lk(mu);
+  int& n = known[{kern, threads, smem, ranks, dev}];
+  if (n == 0) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(ranks);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = ranks;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    if (cuda_status(cudaOccupancyMaxActiveClusters(&n, kern, &cfg))) n = 0;
+    else if (n == 0) cuda_status(cudaErrorLaunchOutOfResources);
+  }
+  return n;
+} catch (...) {  // the map's memory; no exception may leave a C entry point
+  cuda_status(cudaErrorMemoryAllocation);
+  return 0;
+}
+
 }  // namespace host
 }  // namespace mlpk
 

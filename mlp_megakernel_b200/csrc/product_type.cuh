@@ -3,7 +3,6 @@
 #pragma once
 #define MLPK_STATUS_BY_POINTER
 #include <algorithm>
-#include <atomic>
 #include <cstring>
 #include <utility>
 
@@ -17,25 +16,6 @@ namespace product {
 
 using namespace mlpk::host;
 
-// Pairs of CTAs that the device holds at a time.
-inline int pairs_at_once(const void* kern, int smem, int dev, int sm_count, std::atomic<int>* known) {
-  int n = known[dev].load(std::memory_order_relaxed);
-  if (n) return n;
-  if (!blocks_per_sm(kern, kProductThreads, smem, dev)) return 0;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(2 * (sm_count / 2));
-  cfg.blockDim = dim3(kProductThreads);
-  cfg.dynamicSmemBytes = smem;
-  if (cuda_status(cudaOccupancyMaxActiveClusters(&n, kern, &cfg))) return 0;
-  if (n < 1) {
-    cuda_status(cudaErrorLaunchOutOfResources);
-    return 0;
-  }
-  n = std::min(n, sm_count / 2);
-  known[dev].store(n, std::memory_order_relaxed);
-  return n;
-}
-
 // The operands' format in an instruction descriptor made for fp16.
 inline uint32_t type_bits(bool bf16) { return bf16 ? (1u << 7 | 1u << 10) : 0u; }
 
@@ -46,9 +26,10 @@ int launch_tiles(const Product& c, const ProductPlan& plan, const DevInfo& di, i
   using Cfg = ProductCfg<EPI, TN>;
   int rc;
   const auto kern = product_kernel<T, EPI, TN>;
-  static std::atomic<int> known[64];
-  const int pairs = pairs_at_once(reinterpret_cast<const void*>(kern), Cfg::SMEM, dev, di.sm_count, known);
-  if (!pairs) return MLPK_ERR_CUDA;
+  const void* entry = reinterpret_cast<const void*>(kern);
+  if (!blocks_per_sm(entry, kProductThreads, Cfg::SMEM, dev)) return MLPK_ERR_CUDA;
+  const int pairs = std::min(clusters_at_once(entry, kProductThreads, Cfg::SMEM, 2, dev), di.sm_count / 2);
+  if (pairs < 1) return MLPK_ERR_CUDA;
 
   ProductArgs a;
   std::memset(&a, 0, sizeof(a));
@@ -142,7 +123,8 @@ int launch_few(const Product& c, const DevInfo& di, int dev, cudaStream_t st) {
   }
   const auto kern = few_rows_kernel<T, EPI>;
   const int smem = few_smem(plan.nt, plan.stages);
-  if (!blocks_per_sm(reinterpret_cast<const void*>(kern), kFewThreads, smem, dev)) return MLPK_ERR_CUDA;
+  const void* entry = reinterpret_cast<const void*>(kern);
+  if (!blocks_per_sm(entry, kFewThreads, smem, dev)) return MLPK_ERR_CUDA;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(plan.tiles * plan.ranks, plan.row_tiles);
   cfg.blockDim = dim3(kFewThreads);

@@ -95,8 +95,8 @@ int main() {
           for (int tile : {64, 128}) {
             const FewPlan p = few_plan(rows, cols, nk, tile, sms);
             // The instruction's N, a power of two of TMEM columns of which 512 are there for the CTAs of an SM.
-            const int at_once = p.nt <= 32 ? 2 : 1, columns = p.nt < 32 ? 32 : p.nt;
-            bool ok = p.nt >= 16 && p.nt <= 256 && (p.nt & (p.nt - 1)) == 0 && int64_t(p.nt) * p.row_tiles >= rows &&
+            const int at_once = p.each_sm, columns = p.nt < 32 ? 32 : p.nt;
+            bool ok = (at_once == 1 || at_once == 2) && p.nt >= 16 && p.nt <= 256 && (p.nt & (p.nt - 1)) == 0 && int64_t(p.nt) * p.row_tiles >= rows &&
                       columns * at_once <= 512 && p.stages >= 2 && p.stages <= kFewMaxStages &&
                       few_smem(p.nt, p.stages) * at_once <= 227 * 1024 && int64_t(p.tiles) * tile >= cols &&
                       int64_t(p.tiles - 1) * tile < cols;
