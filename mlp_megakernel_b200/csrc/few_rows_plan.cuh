@@ -34,25 +34,29 @@ inline FewPlan few_plan(int64_t rows, int cols, int nk, int tile_cols, int sm_co
   p.row_tiles = static_cast<int>((rows + p.nt - 1) / p.nt);
   // Shares of a tile's reduction: as many as fill the SMs in one go with `each`
   // CTAs, 4 blocks in each at least.  A cluster has its SMs from one part of the
-  // chip, so larger ones leave some out, a ninth of them at most (clusters of 8, two
-  // an SM: 264 of 296 CTAs); of 7, or of 3 with one CTA an SM, they ended in two
-  // goes (8 x 5120 x 5120 bf16: 7 shares 15.1 us, 4 shares 10.6; 64 x 2048 x 5120: 3
-  // shares 17.2, 2 shares 10.1).
+  // chip, so larger ones leave some out: a ninth of them, or a fifth with clusters
+  // of 8 that have an SM a CTA (15 of them on 148 SMs); beyond that, and with
+  // clusters of 7, or of 3 with an SM a CTA, they ended in two goes (8 x 5120 x 5120
+  // bf16: 7 shares 15.1 us, 4 shares 10.6; 64 x 2048 x 5120: 3 shares 17.2, 2 shares
+  // 10.1).
   const int64_t tiles = static_cast<int64_t>(p.tiles) * p.row_tiles;
   const auto shares = [&](int each) {
-    for (int n : {8, 4, 3, 2})
-      if ((n != 3 || each == 2) && tiles * n * (n > 2 ? 9 : 8) <= static_cast<int64_t>(each) * sm_count * 8 && nk >= 4 * n)
-        return n;
+    for (int n : {8, 4, 3, 2}) {
+      const int left_out = n == 2 ? 8 : n == 8 && each == 1 ? 10 : 9;  // in eighths
+      if ((n != 3 || each == 2) && tiles * n * left_out <= static_cast<int64_t>(each) * sm_count * 8 && nk >= 4 * n) return n;
+    }
     return 1;
   };
-  // One CTA an SM with a deep ring, where two would not have more of the SMs at
-  // work: a tile of many rows meets in more shared memory than it is worth to share
-  // it further (128 x 4096 x 4096 bf16: 8 shares 15.6 us, 4 shares 11.4; 48 x 4096 x
-  // 14336, gated, 224 tiles: one an SM 45.0, two 39.5; 64 x 4096 x 11008, 86 tiles:
-  // one share 21.1, three 17.1).  Tiles of few rows always two.
+  // One CTA an SM with a deep ring, which also leaves room for the next kernel's
+  // CTAs to begin, where two would not have more of the SMs at work (weights from
+  // memory: 1 x 4096 x 4096 bf16 10.5 us with two of 8 shares, 9.8 with one of 4; 1 x
+  // 14336 x 4096, gated, 39.5 and 37.4; 128 x 4096 x 4096 15.6 and 11.4, where the
+  // shares meet in more shared memory than it is worth.  But 48 x 4096 x 14336, gated,
+  // 224 tiles: two an SM 39.5, one 45.0; 64 x 4096 x 11008, 86 tiles: three shares
+  // 17.1, one 21.1).
   const int64_t one = tiles * shares(1), two = tiles * shares(2);
   const bool fuller = 20 * two > 23 * 2 * (one < sm_count ? one : sm_count) || one > sm_count;
-  p.each_sm = p.nt <= 32 || (p.nt < kFewMostRows && fuller) ? 2 : 1;
+  p.each_sm = p.nt < kFewMostRows && fuller ? 2 : 1;
   p.ranks = shares(p.each_sm);
   p.stages = kFewMaxStages;
   while (p.stages > 2 && few_smem(p.nt, p.stages) > (p.each_sm == 2 ? 113 * 1024 : 226 * 1024)) --p.stages;
