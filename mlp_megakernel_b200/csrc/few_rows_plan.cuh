@@ -33,7 +33,8 @@ inline FewPlan few_plan(int64_t rows, int cols, int nk, int tile_cols, int sm_co
   p.tiles = (cols + tile_cols - 1) / tile_cols;
   p.row_tiles = static_cast<int>((rows + p.nt - 1) / p.nt);
   // Shares of a tile's reduction: as many as fill the SMs in one go with `each`
-  // CTAs, 4 blocks in each at least.  A cluster has its SMs from one part of the
+  // CTAs, 4 blocks in each at least, 2 where that is few CTAs (64 x 256 x 256 fp16: 4
+  // shares of one tile's 4 blocks 6.2 us, 2 shares 6.0, one 6.7).  A cluster has its SMs from one part of the
   // chip, so larger ones leave some out: a ninth of them, or a fifth with clusters
   // of 8 that have an SM a CTA (15 of them on 148 SMs); beyond that, and with
   // clusters of 7, or of 3 with an SM a CTA, they ended in two goes (8 x 5120 x 5120
@@ -43,7 +44,8 @@ inline FewPlan few_plan(int64_t rows, int cols, int nk, int tile_cols, int sm_co
   const auto shares = [&](int each) {
     for (int n : {8, 4, 3, 2}) {
       const int left_out = n == 2 ? 8 : n == 8 && each == 1 ? 10 : 9;  // in eighths
-      if ((n != 3 || each == 2) && tiles * n * left_out <= static_cast<int64_t>(each) * sm_count * 8 && nk >= 4 * n) return n;
+      if ((n != 3 || each == 2) && tiles * n * left_out <= static_cast<int64_t>(each) * sm_count * 8 && nk >= (tiles * n <= 64 ? 2 : 4) * n)
+        return n;
     }
     return 1;
   };
