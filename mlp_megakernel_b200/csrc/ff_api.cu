@@ -354,9 +354,10 @@ int mlpk_fp8_restore(int64_t rows, int width, int dtype, const void* q, const fl
   const int64_t total = rows * width;
   return with_value_type(dtype, [&](auto t) {
     using T = decltype(t);
-    const unsigned blocks = stream_blocks(restore_kernel<T>, ceil_to(total, 16 * 2 * kStreamThreads), di, dev);
+    const auto kern = width % 16 == 0 ? restore_kernel<T, true> : restore_kernel<T, false>;
+    const unsigned blocks = stream_blocks(kern, ceil_to(total, 16 * 2 * kStreamThreads), di, dev);
     if (!blocks) return static_cast<int>(MLPK_ERR_CUDA);
-    return launch_kernel_early(restore_kernel<T>, dim3(blocks), kStreamThreads, 0, static_cast<cudaStream_t>(stream), total, width,
+    return launch_kernel_early(kern, dim3(blocks), kStreamThreads, 0, static_cast<cudaStream_t>(stream), total, width,
                                groups, static_cast<const uint8_t*>(q), scale, static_cast<T*>(x));
   });
 }

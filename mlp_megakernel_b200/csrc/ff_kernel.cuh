@@ -137,9 +137,10 @@ __device__ __forceinline__ float clip(float v, float most) {  // a NaN stays
 }
 
 // 16 values of the flat tensor at a time, whatever the width: they have one
-// scale, or each looks up its own (at a group's end where 16 does not divide the
-// width).
-template <class T>
+// scale (always where 16 divides the width, ONE: what follows costs 16384 x 8192
+// bf16 84 -> 100 us), or two (the rest of a group and the beginning of the next),
+// or, where a row's last group is shorter than that, each looks up its own.
+template <class T, bool ONE>
 __global__ void __launch_bounds__(kStreamThreads)
     restore_kernel(int64_t total, int width, int groups, const uint8_t* __restrict__ q,
                    const float* __restrict__ scale, T* __restrict__ x) {
@@ -150,18 +151,27 @@ __global__ void __launch_bounds__(kStreamThreads)
   Steps at(i, step, width);
   for (; i < total; i += AT_ONCE * step) {
     Raw<uint16_t, N / 2> raw[AT_ONCE];
-    float s[AT_ONCE];
+    float s[AT_ONCE], next[AT_ONCE];
     int64_t row[AT_ONCE];
-    int col[AT_ONCE];
+    int col[AT_ONCE], here[AT_ONCE], there[AT_ONCE];  // values of this group, and of the next, from the first on
 #pragma unroll
     for (int k = 0; k < AT_ONCE; ++k) {
       row[k] = at.major;
       col[k] = at.minor;
       at.next();
       const int64_t p = i + k * step;
+      here[k] = min(kGroupCols - col[k] % kGroupCols, width - col[k]);
+      there[k] = N;
+      next[k] = 0.0f;
       if (p + N <= total) {
         raw[k] = load_raw<uint16_t, N / 2>(reinterpret_cast<const uint16_t*>(q + p));
-        s[k] = scale[row[k] * groups + col[k] / kGroupCols];
+        const int64_t group = row[k] * groups + col[k] / kGroupCols;  // the next one follows it, on the next row too
+        s[k] = scale[group];
+        if (!ONE && here[k] < N) {
+          const int begin = col[k] + here[k] == width ? 0 : col[k] + here[k];
+          there[k] = min(kGroupCols, width - begin);
+          next[k] = scale[group + 1];
+        }
       }
     }
 #pragma unroll
@@ -170,17 +180,18 @@ __global__ void __launch_bounds__(kStreamThreads)
       int64_t r = row[k];
       int c = col[k];
       if (p + N <= total) {
-        const bool one = c + N <= width && c % kGroupCols + N <= kGroupCols;
         float2 f[N / 2];
         float v[N];
         unpack_fp8<N>(raw[k], f);
+        const bool two = ONE || here[k] + there[k] >= N;
 #pragma unroll
         for (int e = 0; e < N; ++e) {
-          if (!one && e > 0) {
+          float each = ONE || e < here[k] ? s[k] : next[k];
+          if (!two) {
+            each = scale[r * groups + c / kGroupCols];
             if (++c == width) c = 0, ++r;
-            if (c % kGroupCols == 0) s[k] = scale[r * groups + c / kGroupCols];
           }
-          v[e] = clip((e % 2 ? f[e / 2].y : f[e / 2].x) * s[k], finite_max<T>());
+          v[e] = clip((e % 2 ? f[e / 2].y : f[e / 2].x) * each, finite_max<T>());
         }
         if constexpr (sizeof(T) == 2) {
           uint32_t w[N / 2];
