@@ -362,10 +362,13 @@ int64_t mlpk_fp8_pitch(int width); /* width rounded up to 128 */
 
 /* out = act(z) + residual, z = x w + bias.  x: [rows][d_in]; w: [d_in][d_out]
  * in w_layout; bias: [d_out] or NULL; residual: [rows][d_out] or NULL; z (and
- * z_scale) as `keep` says. */
+ * z_scale) as `keep` says.  This call, _dx and _dw need a workspace of the size
+ * that theirs gives (often 0): the last tiles of a product are shared out over all
+ * SMs. */
+int64_t mlpk_linear_workspace_size(int64_t rows, int d_in, int d_out, int dtype, int w_layout, int keep);
 int mlpk_linear(int64_t rows, int d_in, int d_out, int dtype, const void* x, const void* w, int w_layout,
                 const void* bias, int bias_dtype, int act, const void* residual, void* out, int keep, void* z,
-                float* z_scale, mlpk_stream_t stream);
+                float* z_scale, void* workspace, int64_t workspace_bytes, mlpk_stream_t stream);
 /* dz = grad_out act'(z) (NULL: not wanted) and db, the sum of dz over the rows
  * before its rounding, in a fixed order (of dtype or fp32; NULL: not wanted; it
  * alone needs the workspace).  z as `keep` says; unused without an activation. */
@@ -373,9 +376,7 @@ int64_t mlpk_linear_dz_workspace_size(int64_t rows, int width, int dtype);
 int mlpk_linear_dz(int64_t rows, int width, int dtype, int act, const void* grad_out, int keep, const void* z,
                    const float* z_scale, void* dz, void* db, int db_dtype, void* workspace, int64_t workspace_bytes,
                    mlpk_stream_t stream);
-/* dx = the sum over i < count (1 or 2) of dz[i] w[i]^T; dz[i]: [rows][d_out].
- * This and the next call need a workspace of the size that theirs gives (often
- * 0): the last tiles of a product are shared out over all SMs. */
+/* dx = the sum over i < count (1 or 2) of dz[i] w[i]^T; dz[i]: [rows][d_out]. */
 int64_t mlpk_linear_dx_workspace_size(int64_t rows, int d_in, int d_out, int dtype, int count, int w_layout);
 int mlpk_linear_dx(int64_t rows, int d_in, int d_out, int dtype, int count, const void* const* dz,
                    const void* const* w, int w_layout, void* dx, void* workspace, int64_t workspace_bytes,

@@ -94,7 +94,9 @@ SIGNATURES = {
     "mlpk_expert_combine": (_i32, [_i64, _i32, _i32, _i32, _vp, _vp, _i32, _vp, _vp, _vp, _vp]),
     "mlpk_expert_combine_bwd": (_i32, [_i64, _i32, _i32, _i32, _vp, _vp, _vp, _i32, _vp, _vp, _vp, _vp, _vp]),
     "mlpk_fp8_pitch": (_i64, [_i32]),
-    "mlpk_linear": (_i32, [_i64, _i32, _i32, _i32, _vp, _vp, _i32, _vp, _i32, _i32, _vp, _vp, _i32, _vp, _vp, _vp]),
+    "mlpk_linear_workspace_size": (_i64, [_i64, _i32, _i32, _i32, _i32, _i32]),
+    "mlpk_linear": (_i32, [_i64, _i32, _i32, _i32, _vp, _vp, _i32, _vp, _i32, _i32, _vp, _vp, _i32, _vp, _vp, _vp, _i64,
+                           _vp]),
     "mlpk_linear_dz_workspace_size": (_i64, [_i64, _i32, _i32]),
     "mlpk_linear_dz": (_i32, [_i64, _i32, _i32, _i32, _vp, _i32, _vp, _vp, _vp, _vp, _i32, _vp, _i64, _vp]),
     "mlpk_linear_dx_workspace_size": (_i64, [_i64, _i32, _i32, _i32, _i32, _i32]),

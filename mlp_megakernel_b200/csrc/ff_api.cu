@@ -63,7 +63,17 @@ void set_keep(Product* c, int keep, int width, void* const (&v)[2], float* const
   }
 }
 
-// dx and dw as products, their operands aside.
+// The calls as products, their operands aside.
+Product linear_product(int64_t rows, int d_in, int d_out, int w_layout, int keep) {
+  Product c;
+  c.epi = kEpiLinear;
+  c.keep_kind = keep;
+  c.rows = rows;
+  c.cols = d_out;
+  c.k[0] = d_in;
+  c.b_mn = w_layout == MLPK_W_IN_OUT;
+  return c;
+}
 Product dx_product(int64_t rows, int d_in, int d_out, int count, int w_layout) {
   Product c;
   c.epi = kEpiPlain;
@@ -134,24 +144,26 @@ extern "C" {
 
 int64_t mlpk_fp8_pitch(int width) { return width < 1 ? -1 : ceil_to(width, kGroupCols) * kGroupCols; }
 
+int64_t mlpk_linear_workspace_size(int64_t rows, int d_in, int d_out, int dtype, int w_layout, int keep) {
+  if (check_call(rows, {d_in, d_out}, dtype, 0, keep) || check_layout(w_layout)) return -1;
+  return product_workspace(linear_product(rows, d_in, d_out, w_layout, keep));
+}
+
 int mlpk_linear(int64_t rows, int d_in, int d_out, int dtype, const void* x, const void* w, int w_layout,
                 const void* bias, int bias_dtype, int act, const void* residual, void* out, int keep, void* z,
-                float* z_scale, mlpk_stream_t stream) {
+                float* z_scale, void* workspace, int64_t workspace_bytes, mlpk_stream_t stream) {
   int rc = check_call(rows, {d_in, d_out}, dtype, act, keep);
   if (rc || (rc = check_layout(w_layout))) return rc;
   if (bias && bias_dtype != dtype && bias_dtype != MLPK_DT_F32) return MLPK_ERR_UNSUPPORTED;
   if (rows == 0) return MLPK_OK;
-  if ((rc = check_ptrs({x, w, out}, {bias, residual, z}))) return rc;
+  if ((rc = check_ptrs({x, w, out}, {bias, residual, z, workspace}))) return rc;
   if ((keep != MLPK_KEEP_NONE && !z) || (keep == MLPK_KEEP_FP8 && !z_scale)) return MLPK_ERR_NULL;
-  Product c;
-  c.epi = kEpiLinear;
+  Product c = linear_product(rows, d_in, d_out, w_layout, keep);
   c.act = act;
-  c.rows = rows;
-  c.cols = d_out;
-  c.k[0] = d_in;
   c.a[0] = x;
   c.b[0] = w;
-  c.b_mn = w_layout == MLPK_W_IN_OUT;
+  c.workspace = workspace;
+  c.workspace_bytes = workspace_bytes;
   c.bias = bias;
   c.bias32 = bias_dtype == MLPK_DT_F32;
   c.in[0] = residual;

@@ -18,8 +18,9 @@
 // of the next.  The kernel is persistent: tiles are taken in groups of `group`
 // row tiles over all column tiles, so that the pairs at work share rows and
 // columns in L2.  The tiles behind the last full turn of the pairs may be shared
-// out (kEpiPlain alone): an item is then a share of a tile's reduction, whose fp32
-// values go to a workspace, and tail_sum_kernel adds them in order.
+// out (kEpiPlain, and kEpiLinear that keeps nothing): an item is then a share of a
+// tile's reduction, whose fp32 values go to a workspace, and tail_sum_kernel adds
+// them in order and runs the epilogue.
 //
 // Everything between the operands and the stored values is fp32: accumulators,
 // bias, activation, residual.  What is kept for the backward is rounded once, to
@@ -448,7 +449,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kProductThreads, 1)
           row_load32<T>(p.residual, static_cast<int64_t>(row) * p.cols + col, p.cols - col, in0);
         }
       };
-      const bool by_row = (EPI == kEpiLinear && p.residual) || (EPI == kEpiGatedBwd && !by_tma);
+      const bool by_row = (EPI == kEpiLinear && p.residual && item.share < 0) || (EPI == kEpiGatedBwd && !by_tma);
       float sg = 0.0f, su = 0.0f;  // the row's scales of a backward in 8 bits
       if (by_tma && chunks > 0) fetch_tiles(col0);
       if (by_row && chunks > 0) {
@@ -466,7 +467,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kProductThreads, 1)
       }
       tc_fence_after();
       const uint32_t t_acc = t_lane + buf * TN, t_part = t_acc + part * Cfg::PART;
-      if constexpr (EPI == kEpiPlain) {
+      if constexpr (EPI == kEpiPlain || EPI == kEpiLinear) {
         if (item.share >= 0) {
           // Both buffers together: 32 rows x 32 columns of fp32, a run of the
           // workspace (share_unit; with what lies outside the output, as zeros).
@@ -491,8 +492,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kProductThreads, 1)
           }
           if (lane == 0) bulk_wait_group_read<0>();
           __syncwarp();
-          chunks = 0;
+          chunks = 0;  // the rest of the epilogue is tail_sum_kernel's
         }
+      }
+      if constexpr (EPI == kEpiPlain) {
 #pragma unroll 1
         for (int c = 0; c < chunks; ++c) {
           float v[32];

@@ -28,11 +28,11 @@ struct Product {
   float* scale[2] = {nullptr, nullptr};
   int64_t q_pitch = 0;
   int scale_pitch = 0;
-  void* workspace = nullptr;  // of a plain product's shares
+  void* workspace = nullptr;  // of the shares
   int64_t workspace_bytes = 0;
 };
 
-// The workspace that a plain product needs: from its rows, cols, outputs, k, a_mn.
+// The workspace that a product needs: from its epi, keep_kind, rows, cols, outputs, k, a_mn.
 __attribute__((visibility("hidden"))) int64_t workspace_bytes(const Product& p, int sm_count);
 
 __attribute__((visibility("hidden"))) int launch_f16(const Product& p, cudaStream_t st);

@@ -78,8 +78,9 @@ int launch_tiles(const Product& c, const ProductPlan& plan, const DevInfo& di, i
   }
   rc = launch_kernel_early(kern, dim3(2 * static_cast<unsigned>(std::min(a.items, pairs))), kProductThreads, Cfg::SMEM, st, a);
   if (rc || plan.splits == 1) return rc;
-  if constexpr (EPI == kEpiPlain) {
-    TailArgs t = {a.partials, {c.out[0], c.out[1]}, a.rows, a.cols, a.tiles_m, a.tiles_n, a.outputs, a.group, a.full, a.splits};
+  if constexpr (EPI == kEpiPlain || EPI == kEpiLinear) {
+    const TailArgs t = {a.partials, {c.out[0], c.out[1]}, a.rows, a.cols, a.tiles_m, a.tiles_n, a.outputs, a.group,
+                        a.full,     a.splits,             a.act,  a.bias32, a.bias,  a.residual};
     rc = launch_kernel_early(tail_sum_kernel<T, TN>, dim3(256 * TN / 8 / kTailThreads, static_cast<unsigned>(plan.tail)),
                              kTailThreads, 0, st, t);
   }
@@ -160,7 +161,8 @@ inline bool few_rows(const Product& c, int pairs) {
 // tile's 128 columns, and so does what reads it.
 inline ProductPlan plan_of(const Product& c, int pairs) {
   const int nk = ceil_div_int(c.k[0], kBlockK) + ceil_div_int(c.k[1], kBlockK);
-  return product_plan(c.rows, c.cols, c.outputs, c.epi == kEpiGated ? 128 : 256, nk, pairs, c.epi == kEpiPlain,
+  return product_plan(c.rows, c.cols, c.outputs, c.epi == kEpiGated ? 128 : 256, nk, pairs,
+                      c.epi == kEpiPlain || (c.epi == kEpiLinear && c.keep_kind == kKeepNone),
                       c.keep_kind != kKeep8 || c.epi == kEpiLinear);
 }
 

@@ -1,7 +1,9 @@
-// The sum of the shares of a product's last tiles (product_kernel.cuh): D = the
-// sum over s of share s, in the order of s, rounded once.  Bound by reading the
-// shares; a thread takes 8 columns of a row, four shares under way at a time.
+// The sum of the shares of a product's last tiles (product_kernel.cuh): z = the
+// sum over s of share s, in the order of s; out = act(z + bias) + residual,
+// rounded once.  Bound by reading the shares; a thread takes 8 columns of a row,
+// four shares under way at a time.
 #pragma once
+#include "act.cuh"
 #include "pdl.cuh"
 #include "product_plan.cuh"
 #include "vec.cuh"
@@ -16,6 +18,9 @@ struct TailArgs {
   int rows, cols;
   int tiles_m, tiles_n, outputs, group;
   int full, splits;
+  int act, bias32;
+  const void* bias;      // NULL: none
+  const void* residual;  // NULL: none
 };
 
 template <class T, int TN>
@@ -36,7 +41,29 @@ __global__ void __launch_bounds__(kTailThreads) tail_sum_kernel(const TailArgs a
     f[0] += x.x, f[1] += x.y, f[2] += x.z, f[3] += x.w;
     f[4] += y.x, f[5] += y.y, f[6] += y.z, f[7] += y.w;
   }
-  store_vec<T, 8>(static_cast<T*>(a.out[at.output]) + out_row * a.cols + out_col, f);
+  const int64_t o = out_row * a.cols + out_col;
+  if (a.bias && a.bias32) {
+    const float4* b = reinterpret_cast<const float4*>(static_cast<const float*>(a.bias) + out_col);
+    const float4 x = b[0], y = b[1];
+    f[0] += x.x, f[1] += x.y, f[2] += x.z, f[3] += x.w;
+    f[4] += y.x, f[5] += y.y, f[6] += y.z, f[7] += y.w;
+  } else if (a.bias) {
+    float b[8];
+    unpack<T, 8>(load_raw<T, 8>(static_cast<const T*>(a.bias) + out_col), b);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] += b[e];
+  }
+  with_act(a.act, [&](auto act) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] = act_value<decltype(act)::value>(f[e]);
+  });
+  if (a.residual) {
+    float r[8];
+    unpack<T, 8>(load_raw<T, 8>(static_cast<const T*>(a.residual) + o), r);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] += r[e];
+  }
+  store_vec<T, 8>(static_cast<T*>(a.out[at.output]) + o, f);
 }
 
 }  // namespace mlpk

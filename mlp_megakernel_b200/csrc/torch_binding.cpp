@@ -477,15 +477,20 @@ Tensor restore(const Tensor& q_in, const Tensor& scale_in, at::ScalarType type) 
   return x;
 }
 
+Tensor workspace(int64_t bytes, const Tensor& like) {
+  return bytes > 0 ? at::empty({bytes}, like.options().dtype(at::kByte)) : Tensor();
+}
 // out = act(x w + b) + r, and what is kept of x w + b.
 Tensor linear_forward(const Tensor& x_in, const Weight& w, int64_t n, const Tensor& b_in, const Tensor& r_in, int64_t act,
                       Kept* z) {
   const Tensor x = aligned(x_in), b = aligned(b_in), r = aligned(r_in);
   Tensor out = at::empty(with_width(x, n), x.options());
-  check("mlpk_linear",
-        mlpk_linear(rows_of(x), static_cast<int>(x.size(-1)), static_cast<int>(n), code(x), ptr(x), ptr(w.t), w.layout,
-                    ptr(b), code(b.defined() ? b : x), static_cast<int>(act), ptr(r), ptr(out),
-                    z ? z->kind() : MLPK_KEEP_NONE, z ? ptr(z->v) : nullptr, z ? z->scales() : nullptr, stream_of(x)));
+  const int k = static_cast<int>(x.size(-1)), m = static_cast<int>(n), keep = z ? z->kind() : MLPK_KEEP_NONE;
+  const int64_t rows = rows_of(x), bytes = mlpk_linear_workspace_size(rows, k, m, code(x), w.layout, keep);
+  const Tensor work = workspace(bytes, x);
+  check("mlpk_linear", mlpk_linear(rows, k, m, code(x), ptr(x), ptr(w.t), w.layout, ptr(b), code(b.defined() ? b : x),
+                                   static_cast<int>(act), ptr(r), ptr(out), keep, z ? ptr(z->v) : nullptr,
+                                   z ? z->scales() : nullptr, ptr(work), std::max<int64_t>(bytes, 0), stream_of(x)));
   return out;
 }
 std::pair<Tensor, Kept> linear_kept(const Tensor& x, const Tensor& w, const Tensor& b, const Tensor& r, int64_t act,
@@ -496,9 +501,6 @@ std::pair<Tensor, Kept> linear_kept(const Tensor& x, const Tensor& w, const Tens
   return {std::move(out), std::move(z)};
 }
 
-Tensor workspace(int64_t bytes, const Tensor& like) {
-  return bytes > 0 ? at::empty({bytes}, like.options().dtype(at::kByte)) : Tensor();
-}
 // The gradients of x (of one product, or the sum of two) and of the weights.
 Tensor dx_of(const Tensor& shaped, std::initializer_list<Tensor> dz, std::initializer_list<Weight> w, int64_t d_in) {
   const Tensor& first = *dz.begin();

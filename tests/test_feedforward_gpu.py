@@ -154,6 +154,16 @@ def test_linear_activations(act, keep, dtype):
     linear_case(333, 192, 456, dtype, act, dtype, True, keep=keep if act else 0, scale=3.0)
 
 
+@pytest.mark.parametrize("shape", [(300, 4096, 128), (257, 2056, 136), (1000, 4096, 1032), (700, 5000, 264)])
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("dtype", list(U))
+def test_linear_whose_last_tiles_are_shared_out(shape, act, dtype):
+    """Long reductions of few tiles: shares of a tile meet in a second kernel, which runs the epilogue."""
+    assert _lib.lib().mlpk_linear_workspace_size(*shape, 0 if dtype == torch.float16 else 2, 0, 0) > 0
+    linear_case(*shape, dtype, act, dtype, True)
+    linear_case(*shape, dtype, act, torch.float32, False, transposed=True)
+
+
 def gated_case(rows, k, h, n, dtype, act, residual, keep, transposed=(False, False, False)):
     u = U[dtype]
     x = make(rows, k, dtype=dtype, seed=1)

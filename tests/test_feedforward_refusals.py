@@ -124,7 +124,7 @@ def test_c_calls_refuse_before_they_touch_the_device(built_lib):
     one, two, none, odd = (_lib.ptr_array(p) for p in ([a], [a, a], [0], [a + 2]))
 
     def linear(rows=4, k=16, n=24, dt=2, x=a, w=a, layout=0, b=None, bdt=2, act=0, r=None, out=a, keep=0, z=None, zs=None):
-        return lib.mlpk_linear(rows, k, n, dt, x, w, layout, b, bdt, act, r, out, keep, z, zs, None)
+        return lib.mlpk_linear(rows, k, n, dt, x, w, layout, b, bdt, act, r, out, keep, z, zs, None, 0, None)
 
     for want, more in ((sh, dict(rows=-1)), (sh, dict(rows=2 ** 31)), (sh, dict(k=0)), (un, dict(k=12)), (un, dict(n=20)),
                        (un, dict(dt=1)), (un, dict(layout=2)), (un, dict(act=6)), (un, dict(act=-1)), (un, dict(keep=3)),
