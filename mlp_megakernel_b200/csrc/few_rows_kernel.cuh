@@ -91,7 +91,7 @@ __global__ void __launch_bounds__(kFewThreads) few_rows_kernel(const __grid_cons
   const int col0 = tile * TILE_COLS;
   const int k0 = static_cast<int>(static_cast<int64_t>(rank) * p.nk / ranks);
   const int k1 = static_cast<int>(static_cast<int64_t>(rank + 1) * p.nk / ranks);
-  const uint32_t columns = nt < 32 ? 32 : nt;  // of TMEM: 32, 64, 128 or 256
+  const uint32_t columns = nt <= 32 ? 32 : nt <= 64 ? 64 : nt <= 128 ? 128 : 256;  // of TMEM
   int* const status = p.status;
 
   if (threadIdx.x == 0) {

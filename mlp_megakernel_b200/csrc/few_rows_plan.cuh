@@ -12,11 +12,12 @@ constexpr int kFewWBytes = 128 * 64 * 2;  // a stage's weights
 constexpr int kFewMaxRanks = 8;      // the portable cluster size
 
 struct FewPlan {
-  int nt = 0;      // rows of a tile
+  int nt = 0;      // rows of a tile, a multiple of 16 up to 256
   int stages = 0;  // depth of the ring
   int ranks = 0;   // CTAs that share a tile's reduction
   int each_sm = 0; // CTAs that an SM is to hold
   int tiles = 0, row_tiles = 0;
+  double us = 0.0;  // about what it takes, where the weights are in L2
 };
 
 // Bytes of dynamic shared memory: the ring (which the fp32 tile reuses), barriers.
@@ -28,18 +29,18 @@ inline int few_smem(int nt, int stages) {
 // tile_cols: weight columns of a tile; nk: blocks of 64 of the reduction.
 inline FewPlan few_plan(int64_t rows, int cols, int nk, int tile_cols, int sm_count) {
   FewPlan p;
-  p.nt = 16;
-  while (p.nt < rows && p.nt < kFewMostRows) p.nt *= 2;
+  // As few tiles of rows as their most allows, alike, of a multiple of 16.
+  p.row_tiles = static_cast<int>((rows + kFewMostRows - 1) / kFewMostRows);
+  p.nt = static_cast<int>((rows + 16 * p.row_tiles - 1) / (16 * p.row_tiles)) * 16;
   p.tiles = (cols + tile_cols - 1) / tile_cols;
-  p.row_tiles = static_cast<int>((rows + p.nt - 1) / p.nt);
   // Shares of a tile's reduction: as many as fill the SMs in one go with `each`
   // CTAs, 4 blocks in each at least, 2 where that is few CTAs (64 x 256 x 256 fp16: 4
-  // shares of one tile's 4 blocks 6.2 us, 2 shares 6.0, one 6.7).  A cluster has its SMs from one part of the
-  // chip, so larger ones leave some out: a ninth of them, or a fifth with clusters
-  // of 8 that have an SM a CTA (15 of them on 148 SMs); beyond that, and with
-  // clusters of 7, or of 3 with an SM a CTA, they ended in two goes (8 x 5120 x 5120
-  // bf16: 7 shares 15.1 us, 4 shares 10.6; 64 x 2048 x 5120: 3 shares 17.2, 2 shares
-  // 10.1).
+  // shares of one tile's 4 blocks 6.2 us, 2 shares 6.0, one 6.7).  A cluster has its
+  // SMs from one part of the chip, so larger ones leave some out: a ninth of them, or
+  // a fifth with clusters of 8 that have an SM a CTA (15 of them on 148 SMs); beyond
+  // that, and with clusters of 7, or of 3 with an SM a CTA, they ended in two goes (8
+  // x 5120 x 5120 bf16: 7 shares 15.1 us, 4 shares 10.6; 64 x 2048 x 5120: 3 shares
+  // 17.2, 2 shares 10.1).
   const int64_t tiles = static_cast<int64_t>(p.tiles) * p.row_tiles;
   const auto shares = [&](int each) {
     for (int n : {8, 4, 3, 2}) {
@@ -58,10 +59,16 @@ inline FewPlan few_plan(int64_t rows, int cols, int nk, int tile_cols, int sm_co
   // 17.1, one 21.1).
   const int64_t one = tiles * shares(1), two = tiles * shares(2);
   const bool fuller = 20 * two > 23 * 2 * (one < sm_count ? one : sm_count) || one > sm_count;
-  p.each_sm = p.nt < kFewMostRows && fuller ? 2 : 1;
+  p.each_sm = p.nt <= 128 && fuller ? 2 : 1;
   p.ranks = shares(p.each_sm);
   p.stages = kFewMaxStages;
   while (p.stages > 2 && few_smem(p.nt, p.stages) > (p.each_sm == 2 ? 113 * 1024 : 226 * 1024)) --p.stages;
+  // Shares of the blocks at 115 GB/s an SM, the tile's way through shared memory
+  // at 45 GB/s (its own and the others'), where an SM has several CTAs one after
+  // the other.
+  const double turns = static_cast<double>(tiles) * p.ranks / sm_count;
+  const double block = (kFewWBytes + 128.0 * p.nt) / 115e3, meet = 512.0 * p.nt * (2.0 - 1.0 / p.ranks) / 45e3;
+  p.us = 3.5 + (turns > 1.0 ? turns : 1.0) * ((nk + p.ranks - 1) / p.ranks * block + 1.0 + meet);
   return p;
 }
 

@@ -5,7 +5,7 @@ namespace mlpk {
 namespace product {
 
 int64_t workspace_bytes(const Product& p, int sm_count) {  // the same for both types
-  if (few_rows(p, sm_count / 2)) return 0;
+  if (few_rows(p, sm_count)) return 0;
   return plan_of(p, sm_count / 2).partials() * static_cast<int64_t>(sizeof(float));
 }
 

@@ -17,6 +17,7 @@ struct ProductPlan {
   int64_t full = 0;   // tiles computed whole, the first ones
   int64_t tail = 0;   // tiles that `splits` items share, the last ones
   int splits = 1;     // shares of a tail tile's reduction; 1: it is computed whole too
+  double us = 0.0;    // about what it takes
   int64_t items() const { return full + tail * splits; }
   // fp32 values that the shares leave in the workspace.
   int64_t partials() const { return splits > 1 ? tail * splits * 256 * cols : 0; }
@@ -31,17 +32,16 @@ struct ProductPlan {
 // behind the last full turn may be shared out over all pairs in shares of the
 // reduction: ceil(tail splits / pairs) turns of nk / splits blocks, and the
 // traffic of the shares (0.25 us a megabyte, written and read) and of a second
-// kernel (4 us).  A block takes 0.3 us.
+// kernel (4 us).  A block takes 0.3 us, a kernel's beginning and end 5.
 inline ProductPlan product_plan(int64_t rows, int cols, int outputs, int out_cols, int nk, int pairs, bool may_split,
                                 bool may_narrow) {
   ProductPlan best;
-  double best_us = 0.0;
   for (int narrow = 0; narrow <= (may_narrow ? 1 : 0); ++narrow) {
     const int each = narrow ? out_cols / 2 : out_cols;
     const int64_t tiles = (rows + 255) / 256 * ((cols + each - 1) / each) * outputs;
     const double block_us = narrow ? 0.21 : 0.3;
     const int64_t left = tiles % pairs;
-    const double full_us = static_cast<double>(tiles / pairs) * nk * block_us;
+    const double full_us = 5.0 + static_cast<double>(tiles / pairs) * nk * block_us;
     const int most = may_split && left ? (nk / 4 < 32 ? nk / 4 : 32) : 1;
     for (int splits = 1; splits <= (most > 1 ? most : 1); ++splits) {
       ProductPlan p;
@@ -52,10 +52,8 @@ inline ProductPlan product_plan(int64_t rows, int cols, int outputs, int out_col
       double us = full_us;
       if (left) us += static_cast<double>((left * splits + pairs - 1) / pairs) * ((nk + splits - 1) / splits) * block_us;
       if (splits > 1) us += 4.0 + 0.25 * 4e-6 * static_cast<double>(p.partials());
-      if (best_us == 0.0 || us < best_us) {
-        best_us = us;
-        best = p;
-      }
+      p.us = us;
+      if (best.us == 0.0 || us < best.us) best = p;
     }
   }
   return best;

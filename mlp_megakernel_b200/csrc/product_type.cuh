@@ -87,6 +87,19 @@ int launch_tiles(const Product& c, const ProductPlan& plan, const DevInfo& di, i
   return rc;
 }
 
+inline int blocks_of(const Product& c) { return ceil_div_int(c.k[0], kBlockK) + ceil_div_int(c.k[1], kBlockK); }
+
+// The tiles of a product (product_plan.cuh).  A gate's checkpoint needs the wide
+// tile's 128 columns, and so does what reads it.
+inline ProductPlan plan_of(const Product& c, int pairs) {
+  return product_plan(c.rows, c.cols, c.outputs, c.epi == kEpiGated ? 128 : 256, blocks_of(c), pairs,
+                      c.epi == kEpiPlain || (c.epi == kEpiLinear && c.keep_kind == kKeepNone),
+                      c.keep_kind != kKeep8 || c.epi == kEpiLinear);
+}
+inline FewPlan few_plan_of(const Product& c, int sm_count) {
+  return few_plan(c.rows, c.cols, blocks_of(c), c.epi == kEpiGated ? 64 : 128, sm_count);
+}
+
 template <class T, int EPI>
 int launch_few(const Product& c, const DevInfo& di, int dev, cudaStream_t st) {
   int rc;
@@ -97,7 +110,7 @@ int launch_few(const Product& c, const DevInfo& di, int dev, cudaStream_t st) {
   a.cols = c.cols;
   a.nk0 = ceil_div_int(c.k[0], kBlockK);
   a.nk = a.nk0 + ceil_div_int(c.k[1], kBlockK);
-  const FewPlan plan = few_plan(c.rows, c.cols, a.nk, GATED ? 64 : 128, di.sm_count);
+  const FewPlan plan = few_plan_of(c, di.sm_count);
   a.nt = plan.nt;
   a.stages = plan.stages;
   a.w_mn = c.b_mn;
@@ -142,28 +155,16 @@ int launch_few(const Product& c, const DevInfo& di, int dev, cudaStream_t st) {
   return cuda_status(cudaLaunchKernelEx(&cfg, kern, a));
 }
 
-// Whether a product goes to few_rows_kernel.  Up to 128 rows it does, but for
-// short reductions of more than 64 (bf16, us, here and in tiles of 256 rows: 1 x
-// 4096 x 4096 8.5 and 24, 64 x 4096 x 14336 24.1 and 30.5, 128 x 4096 x 4096 11.4
-// and 19.0; 128 x 256 x 256 8.0 and 6.2).  Up to 256 rows it does where a long
-// reduction would leave half of the pairs of CTAs without a tile (256 x 4096 x 4096
-// 16.3 and 19.2; 256 x 4096 x 8192 27.0 and 25.6, 256 x 2048 x 4096 14.7 and 13.3).
+// Whether a product goes to few_rows_kernel: up to 64 rows, and up to 512 where its
+// plan says that it ends earlier (a linear layer with a residual, bf16, us, there and
+// in tiles of 256 rows: 128 x 4096 x 14336 31.3 and 33.1, 136 x 4096 x 8192 16.3 and
+// 20.4, 200 x 4096 x 4096 15.0 and 17.9, 320 x 8192 x 2048 16.1 and 23.0; 128 x 256 x
+// 256 8.6 and 6.8, 256 x 4096 x 14336 49.3 and 34.2, 512 x 8192 x 1024 21.3 and 17.9).
 // The rows must be read along the reduction, and a gate's checkpoint group is wider
 // than a tile.
-inline bool few_rows(const Product& c, int pairs) {
-  if (c.rows > kFewMostRows || c.a_mn || c.outputs > 1 || (c.epi == kEpiGated && c.keep_kind == kKeep8)) return false;
-  const int nk = ceil_div_int(c.k[0], kBlockK) + ceil_div_int(c.k[1], kBlockK);
-  if (c.rows <= 128) return c.rows <= 64 || nk >= 16;
-  return nk >= 48 && 2 * ceil_div_int(c.cols, c.epi == kEpiGated ? 64 : 128) <= pairs;
-}
-
-// The tiles of a product (product_plan.cuh).  A gate's checkpoint needs the wide
-// tile's 128 columns, and so does what reads it.
-inline ProductPlan plan_of(const Product& c, int pairs) {
-  const int nk = ceil_div_int(c.k[0], kBlockK) + ceil_div_int(c.k[1], kBlockK);
-  return product_plan(c.rows, c.cols, c.outputs, c.epi == kEpiGated ? 128 : 256, nk, pairs,
-                      c.epi == kEpiPlain || (c.epi == kEpiLinear && c.keep_kind == kKeepNone),
-                      c.keep_kind != kKeep8 || c.epi == kEpiLinear);
+inline bool few_rows(const Product& c, int sm_count) {
+  if (c.rows > 512 || c.a_mn || c.outputs > 1 || (c.epi == kEpiGated && c.keep_kind == kKeep8)) return false;
+  return c.rows <= 64 || few_plan_of(c, sm_count).us <= plan_of(c, sm_count / 2).us + 0.5;
 }
 
 template <class T, int EPI>
@@ -172,7 +173,7 @@ int launch_epi(const Product& c, cudaStream_t st) {
   int dev = 0;
   const int rc = current_device_info(&di, &dev);
   if (rc) return rc;
-  if (few_rows(c, di.sm_count / 2)) return launch_few<T, EPI>(c, di, dev, st);
+  if (few_rows(c, di.sm_count)) return launch_few<T, EPI>(c, di, dev, st);
   const ProductPlan plan = plan_of(c, di.sm_count / 2);
   const int64_t bytes = plan.partials() * static_cast<int64_t>(sizeof(float));
   if (bytes && !c.workspace) return MLPK_ERR_NULL;

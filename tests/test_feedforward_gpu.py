@@ -154,14 +154,29 @@ def test_linear_activations(act, keep, dtype):
     linear_case(333, 192, 456, dtype, act, dtype, True, keep=keep if act else 0, scale=3.0)
 
 
-@pytest.mark.parametrize("shape", [(300, 4096, 128), (257, 2056, 136), (1000, 4096, 1032), (700, 5000, 264)])
+@pytest.mark.parametrize("shape", [(300, 4096, 128), (257, 2056, 136), (520, 4096, 128), (513, 2056, 136), (1000, 4096, 1032),
+                                   (700, 5000, 264)])
 @pytest.mark.parametrize("act", ACTS)
 @pytest.mark.parametrize("dtype", list(U))
 def test_linear_whose_last_tiles_are_shared_out(shape, act, dtype):
     """Long reductions of few tiles: shares of a tile meet in a second kernel, which runs the epilogue."""
-    assert _lib.lib().mlpk_linear_workspace_size(*shape, 0 if dtype == torch.float16 else 2, 0, 0) > 0
+    if shape[0] > 512:  # fewer rows go to the kernel for few rows
+        assert _lib.lib().mlpk_linear_workspace_size(*shape, 0 if dtype == torch.float16 else 2, 0, 0) > 0
     linear_case(*shape, dtype, act, dtype, True)
     linear_case(*shape, dtype, act, torch.float32, False, transposed=True)
+
+
+@pytest.mark.parametrize("shape", [(129, 2056, 520), (145, 4096, 264), (208, 1032, 1000), (257, 4096, 136), (300, 2048, 1000),
+                                   (400, 4104, 264), (512, 4096, 136)])
+@pytest.mark.parametrize("dtype", list(U))
+def test_long_reductions_of_some_hundred_rows(shape, dtype):
+    """Rows that fill one or two tiles of the kernel for few rows, the last one partly."""
+    rows, k, n = shape
+    linear_case(rows, k, n, dtype, None, None, False)
+    linear_case(rows, k, n, dtype, "gelu_tanh", dtype, True, keep=1)
+    linear_case(rows, k, n, dtype, "silu", torch.float32, False, keep=2, transposed=True)
+    gated_case(rows, k, n, 136, dtype, "silu", True, 0)
+    gated_case(rows, k, n, 136, dtype, "gelu_tanh", False, 1, transposed=(True, False, True))
 
 
 def gated_case(rows, k, h, n, dtype, act, residual, keep, transposed=(False, False, False)):

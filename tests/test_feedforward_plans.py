@@ -89,14 +89,15 @@ using namespace mlpk;
 int main() {
   long bad = 0, seen = 0;
   for (int sms : {2, 16, 74, 132, 148, 160})
-    for (int64_t rows = 1; rows <= kFewMostRows; ++rows)
+    for (int64_t rows = 1; rows <= 3 * kFewMostRows; ++rows)
       for (int cols : {8, 64, 72, 128, 136, 4096, 14336, 65536})
         for (int nk : {1, 2, 3, 4, 5, 7, 8, 16, 31, 32, 64, 224, 1000})
           for (int tile : {64, 128}) {
             const FewPlan p = few_plan(rows, cols, nk, tile, sms);
-            // The instruction's N, a power of two of TMEM columns of which 512 are there for the CTAs of an SM.
-            const int at_once = p.each_sm, columns = p.nt < 32 ? 32 : p.nt;
-            bool ok = (at_once == 1 || at_once == 2) && p.nt >= 16 && p.nt <= 256 && (p.nt & (p.nt - 1)) == 0 && int64_t(p.nt) * p.row_tiles >= rows &&
+            // The instruction's N (a multiple of 16), its columns of TMEM (512 for the CTAs of an SM).
+            const int at_once = p.each_sm, columns = p.nt <= 32 ? 32 : p.nt <= 64 ? 64 : p.nt <= 128 ? 128 : 256;
+            bool ok = (at_once == 1 || at_once == 2) && p.nt >= 16 && p.nt <= 256 && p.nt % 16 == 0 && int64_t(p.nt) * p.row_tiles >= rows &&
+                      int64_t(p.nt) * (p.row_tiles - 1) < rows &&
                       columns * at_once <= 512 && p.stages >= 2 && p.stages <= kFewMaxStages &&
                       few_smem(p.nt, p.stages) * at_once <= 227 * 1024 && int64_t(p.tiles) * tile >= cols &&
                       int64_t(p.tiles - 1) * tile < cols;
