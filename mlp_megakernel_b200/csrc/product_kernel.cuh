@@ -50,6 +50,7 @@ struct alignas(64) ProductArgs {
   CUtensorMap in[2];       // backward: g, u (16 bits)
   int rows, cols;          // of each output
   int nk0, nk;             // blocks of the first reduction range, and of both
+  int tile_cols, b_bytes;  // columns of a tile (at most TN), bytes of a CTA's loads of B in a stage
   int tiles_m, tiles_n, outputs, group;
   int full, splits, items; // tiles computed whole, shares of each of the others, and both together
   int a_mn, b_mn;          // the operand's contiguous index is the row / column, not the reduction
@@ -62,7 +63,7 @@ struct alignas(64) ProductArgs {
   float* scale[2];         // [rows][scale_pitch]
   int64_t q_pitch;
   int scale_pitch;
-  float* partials;         // [shares][256 x TN], each as share_unit says
+  float* partials;         // of the shares, each as share_unit says
   int* status;
 };
 
@@ -302,7 +303,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kProductThreads, 1)
         const int k0 = item.k0, k1 = item.k1;
         const int row = at.m * kPairRows + static_cast<int>(rank) * 128;
         // A pair's half of B: columns, or for the gate its own matrix.
-        const int col = EPI == kEpiGated ? at.n * (TN / 2) : at.n * TN + static_cast<int>(rank) * (TN / 2);
+        const int col = EPI == kEpiGated ? at.n * (TN / 2) : at.n * p.tile_cols + static_cast<int>(rank) * (p.tile_cols / 2);
         const int own_a = p.out_a ? at.output : 0;
         const int own_b = EPI == kEpiGated ? static_cast<int>(rank) : p.out_a ? 0 : at.output;
         for (int kb = k0; kb < k1; ++kb, ++issued) {
@@ -315,7 +316,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kProductThreads, 1)
           // cluster scope for every stage, and the products ran at half their
           // rate: 8192 x 4096 x 4096 bf16 380 us.)
           const uint32_t full = mapa_shared(bar_full(s), 0);
-          if (rank == 0) mbar_arrive_expect_tx(bar_full(s), 2 * Cfg::STAGE);
+          if (rank == 0) mbar_arrive_expect_tx(bar_full(s), 2 * (Cfg::A_BYTES + p.b_bytes));
           const bool second = kb >= p.nk0;
           const int k = (second ? kb - p.nk0 : kb) * kBlockK;
           const CUtensorMap* ma = &p.a[second ? 1 : own_a];
@@ -392,6 +393,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kProductThreads, 1)
     const uint32_t t_lane = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
     constexpr int CHUNK = Cfg::CHUNK, PITCH = Cfg::PITCH;
     const uint32_t s_buf = sbase + Cfg::OFF_EPI + w * Cfg::BUFS * Cfg::TILE;
+    // A warp's chunks: together where a group of columns has a scale, otherwise
+    // every fourth, so that a tile may have any number of them.
+    const bool together = EPI == kEpiGated || EPI == kEpiGatedBwd || p.keep_kind == kKeep8;
+    const int apart = together ? Cfg::PART : CHUNK, next = together ? CHUNK : 4 * CHUNK;
     const bool by_tma = EPI == kEpiGatedBwd && p.keep_kind == kKeep16;  // g and u come as tiles
     bool ok = true;
     int turn = 0;  // tiles stored so far
@@ -419,10 +424,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kProductThreads, 1)
       const int buf = mine & 1;
       const int row0 = at.m * kPairRows + static_cast<int>(rank) * 128 + quarter * 32;
       const int row = row0 + lane;
-      const int first = at.n * Cfg::OUT_COLS, col0 = first + part * Cfg::PART;
+      const int first = EPI == kEpiGated ? at.n * (TN / 2) : at.n * p.tile_cols;
+      const int col0 = first + part * apart, last = min(p.cols, first + (EPI == kEpiGated ? TN / 2 : p.tile_cols));
       // Chunks with something to store.
       int chunks = 0;
-      if (row0 < p.rows && col0 < p.cols) chunks = min(Cfg::CHUNKS, (p.cols - col0 + CHUNK - 1) / CHUNK);
+      if (row0 < p.rows && col0 < last) chunks = min(Cfg::CHUNKS, (last - col0 + next - 1) / next);
       // g and u of a chunk into the two buffers, once every store has read them.
       auto fetch_tiles = [&](int col) {
         if (lane == 0) {
@@ -466,7 +472,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kProductThreads, 1)
         break;
       }
       tc_fence_after();
-      const uint32_t t_acc = t_lane + buf * TN, t_part = t_acc + part * Cfg::PART;
+      const uint32_t t_acc = t_lane + buf * TN, t_part = t_acc + part * apart;
       if constexpr (EPI == kEpiPlain || EPI == kEpiLinear) {
         if (item.share >= 0) {
           // Both buffers together: 32 rows x 32 columns of fp32, a run of the
@@ -474,9 +480,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kProductThreads, 1)
           static_assert(2 * Cfg::TILE == 4096 && CHUNK == 32, "a share's run");
           float* dst = p.partials + (static_cast<int64_t>(item.share) * 32 + rank * 16 + w) * (Cfg::CHUNKS * 1024);
 #pragma unroll 1
-          for (int c = 0; c < Cfg::CHUNKS; ++c) {
+          for (int c = 0; c < Cfg::CHUNKS && part * apart + c * next < p.tile_cols; ++c) {
             float v[32];
-            tmem_load32(t_part + CHUNK * c, v);
+            tmem_load32(t_part + next * c, v);
             if (lane == 0) bulk_wait_group_read<0>();
             __syncwarp();
 #pragma unroll
@@ -499,17 +505,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kProductThreads, 1)
 #pragma unroll 1
         for (int c = 0; c < chunks; ++c) {
           float v[32];
-          tmem_load32(t_part + CHUNK * c, v);
+          tmem_load32(t_part + next * c, v);
           const uint32_t tile = begin_tile();
           tile_store<T, PITCH>(tile, lane, 0, v);
-          end_tile(&p.out[at.output], tile, col0 + CHUNK * c, row0);
+          end_tile(&p.out[at.output], tile, col0 + next * c, row0);
         }
       } else if constexpr (EPI == kEpiLinear) {
         float inv = 0.0f;
         if (p.keep_kind == kKeep8 && chunks > 0) {
           // The largest magnitude of the row's 128 columns: a half of a wide
           // tile, or all of a narrow one.
-          const int g0 = first + part * Cfg::PART / kKeepGroup * kKeepGroup;
+          const int g0 = first + part * apart / kKeepGroup * kKeepGroup;
           float most = 0.0f;
 #pragma unroll 1
           for (int c = 0; c < kKeepGroup && g0 + c < p.cols; c += 32) {
@@ -523,14 +529,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kProductThreads, 1)
         }
 #pragma unroll 1
         for (int c = 0; c < chunks; ++c) {
-          const int col = col0 + CHUNK * c;
+          const int col = col0 + next * c;
           float v[32];
           uint32_t r[16];
-          tmem_load32(t_part + CHUNK * c, v);
+          tmem_load32(t_part + next * c, v);
           if (p.residual) {
 #pragma unroll
             for (int i = 0; i < 16; ++i) r[i] = in0[i];
-            if (c + 1 < chunks) fetch_row(col + CHUNK);
+            if (c + 1 < chunks) fetch_row(col + next);
           }
           if (p.bias) add_bias<T>(p, col, v);
           if (p.keep_kind == kKeep16) {

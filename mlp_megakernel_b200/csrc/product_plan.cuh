@@ -12,40 +12,43 @@
 
 namespace mlpk {
 
+// Units of 4 fp32 values of a share in the workspace: 256 rows x 128 or 256 columns.
+MLPK_HOST_DEVICE constexpr int share_units(int tile_cols) { return (tile_cols + 127) / 128 * 8192; }
+
 struct ProductPlan {
-  int cols = 256;     // columns of a tile: 256, or 128
+  int cols = 256;     // columns of a tile, of both matrices together for the gate
   int64_t full = 0;   // tiles computed whole, the first ones
   int64_t tail = 0;   // tiles that `splits` items share, the last ones
   int splits = 1;     // shares of a tail tile's reduction; 1: it is computed whole too
   double us = 0.0;    // about what it takes
   int64_t items() const { return full + tail * splits; }
   // fp32 values that the shares leave in the workspace.
-  int64_t partials() const { return splits > 1 ? tail * splits * 256 * cols : 0; }
+  int64_t partials() const { return splits > 1 ? tail * splits * 4 * share_units(cols) : 0; }
 };
 
-// rows, cols: of each output; out_cols: columns of an output that a wide tile has
-// (half of a narrow one's is its); nk: blocks of 64 of the reduction; may_split,
-// may_narrow: whether the product's epilogue allows it.
+// rows, cols: of each output; out_cols: columns of an output that a tile of 256 has;
+// nk: blocks of 64 of the reduction; may_split, may_narrow, may_any: whether the
+// product's epilogue allows shares, tiles of 128 columns, tiles of 160 to 224.
 //
-// The tiles go over the pairs in turns; a turn takes nk blocks' time, 0.7 of that
-// for narrow tiles (their rows are read for half the products).  What is left
+// The tiles go over the pairs in turns; a turn takes nk blocks' time.  What is left
 // behind the last full turn may be shared out over all pairs in shares of the
 // reduction: ceil(tail splits / pairs) turns of nk / splits blocks, and the
 // traffic of the shares (0.25 us a megabyte, written and read) and of a second
 // kernel (4 us).  A block takes 0.3 us, a kernel's beginning and end 5.
 inline ProductPlan product_plan(int64_t rows, int cols, int outputs, int out_cols, int nk, int pairs, bool may_split,
-                                bool may_narrow) {
+                                bool may_narrow, bool may_any) {
   ProductPlan best;
-  for (int narrow = 0; narrow <= (may_narrow ? 1 : 0); ++narrow) {
-    const int each = narrow ? out_cols / 2 : out_cols;
+  for (int wide = 256; wide >= 128; wide -= 32) {
+    if (wide == 128 ? !may_narrow : wide < 256 && !may_any) continue;
+    const int each = wide * out_cols / 256;
     const int64_t tiles = (rows + 255) / 256 * ((cols + each - 1) / each) * outputs;
-    const double block_us = narrow ? 0.21 : 0.3;
+    const double block_us = wide == 128 ? 0.21 : 0.3 * (512 + wide) / 768.0;
     const int64_t left = tiles % pairs;
     const double full_us = 5.0 + static_cast<double>(tiles / pairs) * nk * block_us;
     const int most = may_split && left ? (nk / 4 < 32 ? nk / 4 : 32) : 1;
     for (int splits = 1; splits <= (most > 1 ? most : 1); ++splits) {
       ProductPlan p;
-      p.cols = narrow ? 128 : 256;
+      p.cols = wide;
       p.splits = splits;
       p.tail = splits > 1 ? left : 0;
       p.full = tiles - p.tail;
@@ -81,12 +84,12 @@ MLPK_HOST_DEVICE inline TileAt product_tile(int t, int tiles_m, int tiles_n, int
 // `col` (a multiple of 4) lies among the item's values, in units of 4: each
 // epilogue warp has runs of 32 rows x 32 columns, the 8 units of a row turned
 // around by the row (as its shared memory has them, against bank conflicts).
-// Epilogue warp w has the rows from 32 ((w + 2) % 4) on of its CTA's 128, and a quarter
-// of the columns, w / 4.
+// Epilogue warp w has the rows from 32 ((w + 2) % 4) on of its CTA's 128, and every
+// fourth run of columns from the (w / 4)-th on.
 MLPK_HOST_DEVICE inline int share_unit(int row, int col, int tile_cols) {
-  const int part_cols = tile_cols / 4, chunks = part_cols / 32;
+  const int chunks = (tile_cols + 127) / 128;
   const int rank = row / 128, quarter = row % 128 / 32, lane = row % 32;
-  const int warp = col / part_cols * 4 + (quarter + 2) % 4, chunk = col % part_cols / 32;
+  const int warp = col / 32 % 4 * 4 + (quarter + 2) % 4, chunk = col / 128;
   return ((rank * 16 + warp) * chunks + chunk) * 256 + lane * 8 + ((col % 32 / 4) ^ (lane % 8));
 }
 

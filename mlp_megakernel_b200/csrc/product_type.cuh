@@ -38,7 +38,9 @@ int launch_tiles(const Product& c, const ProductPlan& plan, const DevInfo& di, i
   a.nk0 = ceil_div_int(c.k[0], kBlockK);
   a.nk = a.nk0 + ceil_div_int(c.k[1], kBlockK);
   a.tiles_m = ceil_div_int(c.rows, kPairRows);
-  a.tiles_n = ceil_div_int(c.cols, Cfg::OUT_COLS);
+  a.tile_cols = plan.cols;
+  a.b_bytes = c.b_mn ? Cfg::B_BYTES : plan.cols / 2 * kBlockK * 2;
+  a.tiles_n = ceil_div_int(c.cols, EPI == kEpiGated ? plan.cols / 2 : plan.cols);
   a.outputs = c.outputs;
   a.group = 8;
   if (plan.items() > 0x7fffffff - 256) return MLPK_ERR_SHAPE;
@@ -48,7 +50,7 @@ int launch_tiles(const Product& c, const ProductPlan& plan, const DevInfo& di, i
   a.a_mn = c.a_mn;
   a.b_mn = c.b_mn;
   a.out_a = c.out_a;
-  a.idesc = make_idesc_f16(kPairRows, TN, c.a_mn, c.b_mn) |
+  a.idesc = make_idesc_f16(kPairRows, plan.cols, c.a_mn, c.b_mn) |
             type_bits(std::is_same_v<T, __nv_bfloat16>);
   a.act = c.act;
   a.keep_kind = c.keep_kind;
@@ -69,7 +71,7 @@ int launch_tiles(const Product& c, const ProductPlan& plan, const DevInfo& di, i
                                : make_map_2d(&a.a[i], c.a[i], k, rows, kBlockK, 128)))
       return rc;
     if (c.b[i] && (rc = c.b_mn ? make_map_2d(&a.b[i], c.b[i], cols, k, 64, kBlockK)
-                               : make_map_2d(&a.b[i], c.b[i], k, cols, kBlockK, TN / 2)))
+                               : make_map_2d(&a.b[i], c.b[i], k, cols, kBlockK, plan.cols / 2)))
       return rc;
     for (const auto& [map, v] : {std::make_pair(&a.in[i], EPI == kEpiGatedBwd ? c.in[i] : nullptr),
                                  std::make_pair(&a.out[i], const_cast<const void*>(c.out[i])),
@@ -81,8 +83,15 @@ int launch_tiles(const Product& c, const ProductPlan& plan, const DevInfo& di, i
   if constexpr (EPI == kEpiPlain || EPI == kEpiLinear) {
     const TailArgs t = {a.partials, {c.out[0], c.out[1]}, a.rows, a.cols, a.tiles_m, a.tiles_n, a.outputs, a.group,
                         a.full,     a.splits,             a.act,  a.bias32, a.bias,  a.residual};
-    rc = launch_kernel_early(tail_sum_kernel<T, TN>, dim3(256 * TN / 8 / kTailThreads, static_cast<unsigned>(plan.tail)),
-                             kTailThreads, 0, st, t);
+    const auto sum = [&](auto cols) {
+      return launch_kernel_early(tail_sum_kernel<T, cols()>, dim3(256 * cols() / 8 / kTailThreads, static_cast<unsigned>(plan.tail)),
+                                 kTailThreads, 0, st, t);
+    };
+    if constexpr (TN == 128) return sum(std::integral_constant<int, 128>{});
+    rc = plan.cols == 256   ? sum(std::integral_constant<int, 256>{})
+         : plan.cols == 224 ? sum(std::integral_constant<int, 224>{})
+         : plan.cols == 192 ? sum(std::integral_constant<int, 192>{})
+                            : sum(std::integral_constant<int, 160>{});
   }
   return rc;
 }
@@ -94,7 +103,8 @@ inline int blocks_of(const Product& c) { return ceil_div_int(c.k[0], kBlockK) + 
 inline ProductPlan plan_of(const Product& c, int pairs) {
   return product_plan(c.rows, c.cols, c.outputs, c.epi == kEpiGated ? 128 : 256, blocks_of(c), pairs,
                       c.epi == kEpiPlain || (c.epi == kEpiLinear && c.keep_kind == kKeepNone),
-                      c.keep_kind != kKeep8 || c.epi == kEpiLinear);
+                      c.keep_kind != kKeep8 || c.epi == kEpiLinear,
+                      c.epi == kEpiPlain || (c.epi == kEpiLinear && c.keep_kind != kKeep8));
 }
 inline FewPlan few_plan_of(const Product& c, int sm_count) {
   return few_plan(c.rows, c.cols, blocks_of(c), c.epi == kEpiGated ? 64 : 128, sm_count);

@@ -22,16 +22,16 @@ int main() {
       for (int cols : some_cols)
         for (int nk : {1, 2, 3, 4, 7, 8, 16, 33, 64, 344, 15626})
           for (int outputs : {1, 2})
-            for (int mode = 0; mode < 4; ++mode) {
+            for (int mode = 0; mode < 5; ++mode) {
               const int out_cols = mode & 1 ? 128 : 256;
-              const bool split = mode == 0 || mode == 2, narrow = mode < 2;
-              const ProductPlan p = product_plan(rows, cols, outputs, out_cols, nk, pairs, split, narrow);
-              const int each = p.cols == 128 ? out_cols / 2 : out_cols;
+              const bool split = mode == 0 || mode >= 2, narrow = mode < 2 || mode == 4, any = mode == 4;
+              const ProductPlan p = product_plan(rows, cols, outputs, out_cols, nk, pairs, split, narrow, any);
+              const int each = out_cols * p.cols / 256;
               const int64_t tm = (rows + 255) / 256, tn = (cols + each - 1) / each;
-              bool ok = (p.cols == 256 || (p.cols == 128 && narrow)) && p.full + p.tail == tm * tn * outputs &&
+              bool ok = (p.cols == 256 || (p.cols == 128 && narrow) || (any && p.cols > 128 && p.cols < 256 && p.cols % 32 == 0)) && p.full + p.tail == tm * tn * outputs &&
                         p.splits >= 1 && (split || p.splits == 1) && (p.splits > 1 || p.tail == 0) && p.tail < pairs &&
                         (p.splits == 1 || nk / p.splits >= 4) &&
-                        p.partials() == (p.splits > 1 ? p.tail * p.splits * 256 * p.cols : 0);
+                        p.partials() == (p.splits > 1 ? p.tail * p.splits * 4 * share_units(p.cols) : 0);
               if (p.tail) ok = ok && p.full % pairs == 0;  // whole turns of whole tiles, then the shares
               // A share's blocks, as the kernel cuts them.
               int64_t covered = 0;
@@ -59,22 +59,25 @@ int main() {
         ++seen;
       }
   // Every value of a share at its own place, and where the kernel's warps put it.
-  for (int cols : {128, 256}) {
-    std::vector<int> hit(64 * cols);
-    const int part = cols / 4, chunks = part / 32;
+  for (int cols : {128, 160, 192, 224, 256}) {
+    std::vector<int> hit(share_units(cols));
+    const int chunks = (cols + 127) / 128;
+    int units = 0;
     for (int rank = 0; rank < 2; ++rank)
       for (int w = 0; w < 16; ++w)
-        for (int c = 0; c < chunks; ++c)
+        for (int c = 0; c < chunks && w / 4 * 32 + c * 128 < cols; ++c)
           for (int lane = 0; lane < 32; ++lane)
             for (int u = 0; u < 8; ++u) {
               const int quarter = (w + 2) & 3;  // warp w + 2 of the CTA reads this quarter of its TMEM lanes
-              const int row = rank * 128 + quarter * 32 + lane, col = w / 4 * part + c * 32 + u * 4;
+              const int row = rank * 128 + quarter * 32 + lane, col = w / 4 * 32 + c * 128 + u * 4;
               const int there = ((rank * 16 + w) * chunks + c) * 256 + lane * 8 + (u ^ (lane & 7));
               const int unit = share_unit(row, col, cols);
-              if (unit != there || unit < 0 || unit >= 64 * cols) { ++bad; continue; }
+              if (unit != there || unit < 0 || unit >= share_units(cols)) { ++bad; continue; }
               ++hit[unit];
+              ++units;
             }
-    for (int h : hit) bad += h != 1;
+    bad += units != 64 * cols;
+    for (int h : hit) bad += h > 1;
     ++seen;
   }
   std::printf("%ld seen, %ld bad\\n", seen, bad);
