@@ -63,12 +63,15 @@ inline FewPlan few_plan(int64_t rows, int cols, int nk, int tile_cols, int sm_co
   p.ranks = shares(p.each_sm);
   p.stages = kFewMaxStages;
   while (p.stages > 2 && few_smem(p.nt, p.stages) > (p.each_sm == 2 ? 113 * 1024 : 226 * 1024)) --p.stages;
-  // Shares of the blocks at 115 GB/s an SM, the tile's way through shared memory
-  // at 45 GB/s (its own and the others'), where an SM has several CTAs one after
-  // the other.
-  const double turns = static_cast<double>(tiles) * p.ranks / sm_count;
-  const double block = (kFewWBytes + 128.0 * p.nt) / 115e3, meet = 512.0 * p.nt * (2.0 - 1.0 / p.ranks) / 45e3;
-  p.us = 3.5 + (turns > 1.0 ? turns : 1.0) * ((nk + p.ranks - 1) / p.ranks * block + 1.0 + meet);
+  // Shares of the blocks at 115 GB/s an SM and the tile's way through shared memory
+  // at 45 GB/s (its own and the others'; longer where 8 meet: 1500 x 2048
+  // x 256 bf16 15.1 us), for each CTA that an SM has.
+  const int64_t ctas = tiles * p.ranks, room = static_cast<int64_t>(p.each_sm) * sm_count;
+  const double turns = ctas <= sm_count ? 1.0
+                       : ctas <= room   ? static_cast<double>(ctas) / sm_count
+                                        : static_cast<double>((ctas + room - 1) / room * p.each_sm);
+  const double block = (kFewWBytes + 128.0 * p.nt) / 115e3, meet = 512.0 * p.nt * (p.ranks == 8 ? 3.0 : 2.0 - 1.0 / p.ranks) / 45e3;
+  p.us = 3.5 + turns * ((nk + p.ranks - 1) / p.ranks * block + 1.0 + meet);
   return p;
 }
 

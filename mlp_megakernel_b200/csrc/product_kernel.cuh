@@ -106,8 +106,8 @@ __device__ __forceinline__ ItemAt product_item(const ProductArgs& p, int t) {
   it.k0 = 0;
   it.k1 = p.nk;
   if (it.share >= 0) {
-    tile = p.full + it.share / p.splits;
-    const int s = it.share % p.splits;
+    const int tail = (p.items - p.full) / p.splits, s = it.share / tail;
+    tile = p.full + it.share - s * tail;
     it.k0 = static_cast<int>(static_cast<int64_t>(s) * p.nk / p.splits);
     it.k1 = static_cast<int>(static_cast<int64_t>(s + 1) * p.nk / p.splits);
   }
@@ -480,7 +480,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kProductThreads, 1)
           static_assert(2 * Cfg::TILE == 4096 && CHUNK == 32, "a share's run");
           float* dst = p.partials + (static_cast<int64_t>(item.share) * 32 + rank * 16 + w) * (Cfg::CHUNKS * 1024);
 #pragma unroll 1
-          for (int c = 0; c < Cfg::CHUNKS && part * apart + c * next < p.tile_cols; ++c) {
+          for (int c = 0; c < Cfg::CHUNKS; ++c) {
             float v[32];
             tmem_load32(t_part + next * c, v);
             if (lane == 0) bulk_wait_group_read<0>();

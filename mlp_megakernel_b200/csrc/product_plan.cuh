@@ -12,9 +12,6 @@
 
 namespace mlpk {
 
-// Units of 4 fp32 values of a share in the workspace: 256 rows x 128 or 256 columns.
-MLPK_HOST_DEVICE constexpr int share_units(int tile_cols) { return (tile_cols + 127) / 128 * 8192; }
-
 struct ProductPlan {
   int cols = 256;     // columns of a tile, of both matrices together for the gate
   int64_t full = 0;   // tiles computed whole, the first ones
@@ -23,7 +20,7 @@ struct ProductPlan {
   double us = 0.0;    // about what it takes
   int64_t items() const { return full + tail * splits; }
   // fp32 values that the shares leave in the workspace.
-  int64_t partials() const { return splits > 1 ? tail * splits * 4 * share_units(cols) : 0; }
+  int64_t partials() const { return splits > 1 ? tail * splits * 256 * cols : 0; }
 };
 
 // rows, cols: of each output; out_cols: columns of an output that a tile of 256 has;
@@ -31,9 +28,9 @@ struct ProductPlan {
 // product's epilogue allows shares, tiles of 128 columns, tiles of 160 to 224.
 //
 // The tiles go over the pairs in turns; a turn takes nk blocks' time.  What is left
-// behind the last full turn may be shared out over all pairs in shares of the
-// reduction: ceil(tail splits / pairs) turns of nk / splits blocks, and the
-// traffic of the shares (0.25 us a megabyte, written and read) and of a second
+// behind the last full turn of tiles of 256 or 128 columns may be shared out over
+// all pairs in shares of the reduction: ceil(tail splits / pairs) turns of nk / splits blocks, and the
+// traffic of the shares (0.5 us a megabyte, written and read) and of a second
 // kernel (4 us).  A block takes 0.3 us, a kernel's beginning and end 5.
 inline ProductPlan product_plan(int64_t rows, int cols, int outputs, int out_cols, int nk, int pairs, bool may_split,
                                 bool may_narrow, bool may_any) {
@@ -45,7 +42,7 @@ inline ProductPlan product_plan(int64_t rows, int cols, int outputs, int out_col
     const double block_us = wide == 128 ? 0.21 : 0.3 * (512 + wide) / 768.0;
     const int64_t left = tiles % pairs;
     const double full_us = 5.0 + static_cast<double>(tiles / pairs) * nk * block_us;
-    const int most = may_split && left ? (nk / 4 < 32 ? nk / 4 : 32) : 1;
+    const int most = may_split && left && wide % 128 == 0 ? (nk / 4 < 32 ? nk / 4 : 32) : 1;
     for (int splits = 1; splits <= (most > 1 ? most : 1); ++splits) {
       ProductPlan p;
       p.cols = wide;
@@ -54,7 +51,7 @@ inline ProductPlan product_plan(int64_t rows, int cols, int outputs, int out_col
       p.full = tiles - p.tail;
       double us = full_us;
       if (left) us += static_cast<double>((left * splits + pairs - 1) / pairs) * ((nk + splits - 1) / splits) * block_us;
-      if (splits > 1) us += 4.0 + 0.25 * 4e-6 * static_cast<double>(p.partials());
+      if (splits > 1) us += 4.0 + 0.5 * 4e-6 * static_cast<double>(p.partials());
       p.us = us;
       if (best.us == 0.0 || us < best.us) best = p;
     }
@@ -87,7 +84,7 @@ MLPK_HOST_DEVICE inline TileAt product_tile(int t, int tiles_m, int tiles_n, int
 // Epilogue warp w has the rows from 32 ((w + 2) % 4) on of its CTA's 128, and every
 // fourth run of columns from the (w / 4)-th on.
 MLPK_HOST_DEVICE inline int share_unit(int row, int col, int tile_cols) {
-  const int chunks = (tile_cols + 127) / 128;
+  const int chunks = tile_cols / 128;
   const int rank = row / 128, quarter = row % 128 / 32, lane = row % 32;
   const int warp = col / 32 % 4 * 4 + (quarter + 2) % 4, chunk = col / 128;
   return ((rank * 16 + warp) * chunks + chunk) * 256 + lane * 8 + ((col % 32 / 4) ^ (lane % 8));

@@ -83,15 +83,8 @@ int launch_tiles(const Product& c, const ProductPlan& plan, const DevInfo& di, i
   if constexpr (EPI == kEpiPlain || EPI == kEpiLinear) {
     const TailArgs t = {a.partials, {c.out[0], c.out[1]}, a.rows, a.cols, a.tiles_m, a.tiles_n, a.outputs, a.group,
                         a.full,     a.splits,             a.act,  a.bias32, a.bias,  a.residual};
-    const auto sum = [&](auto cols) {
-      return launch_kernel_early(tail_sum_kernel<T, cols()>, dim3(256 * cols() / 8 / kTailThreads, static_cast<unsigned>(plan.tail)),
-                                 kTailThreads, 0, st, t);
-    };
-    if constexpr (TN == 128) return sum(std::integral_constant<int, 128>{});
-    rc = plan.cols == 256   ? sum(std::integral_constant<int, 256>{})
-         : plan.cols == 224 ? sum(std::integral_constant<int, 224>{})
-         : plan.cols == 192 ? sum(std::integral_constant<int, 192>{})
-                            : sum(std::integral_constant<int, 160>{});
+    rc = launch_kernel_early(tail_sum_kernel<T, TN>, dim3(256 * TN / 8 / kTailThreads, static_cast<unsigned>(plan.tail)),
+                             kTailThreads, 0, st, t);
   }
   return rc;
 }
@@ -165,15 +158,15 @@ int launch_few(const Product& c, const DevInfo& di, int dev, cudaStream_t st) {
   return cuda_status(cudaLaunchKernelEx(&cfg, kern, a));
 }
 
-// Whether a product goes to few_rows_kernel: up to 64 rows, and up to 512 where its
+// Whether a product goes to few_rows_kernel: up to 64 rows, and up to 2048 where its
 // plan says that it ends earlier (a linear layer with a residual, bf16, us, there and
 // in tiles of 256 rows: 128 x 4096 x 14336 31.3 and 33.1, 136 x 4096 x 8192 16.3 and
-// 20.4, 200 x 4096 x 4096 15.0 and 17.9, 320 x 8192 x 2048 16.1 and 23.0; 128 x 256 x
-// 256 8.6 and 6.8, 256 x 4096 x 14336 49.3 and 34.2, 512 x 8192 x 1024 21.3 and 17.9).
-// The rows must be read along the reduction, and a gate's checkpoint group is wider
-// than a tile.
+// 20.4, 320 x 8192 x 2048 16.1 and 23.0, 1024 x 8192 x 1024 22.4 and 25.3, 2000 x 4096
+// x 512 17.5 and 19.7; 128 x 256 x 256 8.6 and 6.8, 256 x 4096 x 14336 49.3 and 34.2,
+// 512 x 8192 x 1024 21.3 and 17.9).  The rows must be read along the reduction, and a
+// gate's checkpoint group is wider than a tile.
 inline bool few_rows(const Product& c, int sm_count) {
-  if (c.rows > 512 || c.a_mn || c.outputs > 1 || (c.epi == kEpiGated && c.keep_kind == kKeep8)) return false;
+  if (c.rows > 2048 || c.a_mn || c.outputs > 1 || (c.epi == kEpiGated && c.keep_kind == kKeep8)) return false;
   return c.rows <= 64 || few_plan_of(c, sm_count).us <= plan_of(c, sm_count / 2).us + 0.5;
 }
 

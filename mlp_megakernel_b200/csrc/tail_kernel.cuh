@@ -32,12 +32,13 @@ __global__ void __launch_bounds__(kTailThreads) tail_sum_kernel(const TailArgs a
   const int64_t out_row = static_cast<int64_t>(at.m) * 256 + row;
   const int out_col = at.n * TN + col;
   if (out_row >= a.rows || out_col >= a.cols) return;
-  const float4* p = reinterpret_cast<const float4*>(a.partials) + static_cast<int64_t>(blockIdx.y) * a.splits * share_units(TN);
+  const float4* p = reinterpret_cast<const float4*>(a.partials) + static_cast<int64_t>(blockIdx.y) * (64 * TN);
   const int first = share_unit(row, col, TN), second = share_unit(row, col + 4, TN);
+  const int64_t apart = static_cast<int64_t>(gridDim.y) * (64 * TN);
   float f[8] = {};
 #pragma unroll 4
   for (int s = 0; s < a.splits; ++s) {
-    const float4 x = p[static_cast<int64_t>(s) * share_units(TN) + first], y = p[static_cast<int64_t>(s) * share_units(TN) + second];
+    const float4 x = p[s * apart + first], y = p[s * apart + second];
     f[0] += x.x, f[1] += x.y, f[2] += x.z, f[3] += x.w;
     f[4] += y.x, f[5] += y.y, f[6] += y.z, f[7] += y.w;
   }

@@ -155,22 +155,32 @@ def test_linear_activations(act, keep, dtype):
 
 
 @pytest.mark.parametrize("shape", [(300, 4096, 128), (257, 2056, 136), (520, 4096, 128), (513, 2056, 136), (1000, 4096, 1032),
-                                   (700, 5000, 264)])
+                                   (700, 5000, 264), (2100, 4096, 136), (2305, 5000, 264), (4000, 4096, 520)])
 @pytest.mark.parametrize("act", ACTS)
 @pytest.mark.parametrize("dtype", list(U))
 def test_linear_whose_last_tiles_are_shared_out(shape, act, dtype):
     """Long reductions of few tiles: shares of a tile meet in a second kernel, which runs the epilogue."""
-    if shape[0] > 512:  # fewer rows go to the kernel for few rows
+    if shape in ((2100, 4096, 136), (2305, 5000, 264)):  # others may go elsewhere, or end earlier whole
         assert _lib.lib().mlpk_linear_workspace_size(*shape, 0 if dtype == torch.float16 else 2, 0, 0) > 0
     linear_case(*shape, dtype, act, dtype, True)
     linear_case(*shape, dtype, act, torch.float32, False, transposed=True)
 
 
+@pytest.mark.parametrize("shape", [(513, 136, 3088), (513, 136, 3872), (600, 200, 4600), (769, 520, 4656), (2000, 264, 1288),
+                                   (2500, 72, 1400)])
+@pytest.mark.parametrize("transposed", [False, True])
+@pytest.mark.parametrize("dtype", list(U))
+def test_tiles_of_any_width(shape, transposed, dtype):
+    """One turn of tiles of 160, 192 and 224 columns, the last one cut off by the edge."""
+    linear_case(*shape, dtype, None, None, False, transposed=transposed)
+    linear_case(*shape, dtype, "gelu_tanh", dtype, True, keep=1, transposed=transposed)
+
+
 @pytest.mark.parametrize("shape", [(129, 2056, 520), (145, 4096, 264), (208, 1032, 1000), (257, 4096, 136), (300, 2048, 1000),
-                                   (400, 4104, 264), (512, 4096, 136)])
+                                   (400, 4104, 264), (512, 4096, 136), (1000, 4096, 1000), (1999, 4096, 520)])
 @pytest.mark.parametrize("dtype", list(U))
 def test_long_reductions_of_some_hundred_rows(shape, dtype):
-    """Rows that fill one or two tiles of the kernel for few rows, the last one partly."""
+    """Rows that fill one tile or several of the kernel for few rows, the last one partly."""
     rows, k, n = shape
     linear_case(rows, k, n, dtype, None, None, False)
     linear_case(rows, k, n, dtype, "gelu_tanh", dtype, True, keep=1)

@@ -30,8 +30,8 @@ int main() {
               const int64_t tm = (rows + 255) / 256, tn = (cols + each - 1) / each;
               bool ok = (p.cols == 256 || (p.cols == 128 && narrow) || (any && p.cols > 128 && p.cols < 256 && p.cols % 32 == 0)) && p.full + p.tail == tm * tn * outputs &&
                         p.splits >= 1 && (split || p.splits == 1) && (p.splits > 1 || p.tail == 0) && p.tail < pairs &&
-                        (p.splits == 1 || nk / p.splits >= 4) &&
-                        p.partials() == (p.splits > 1 ? p.tail * p.splits * 4 * share_units(p.cols) : 0);
+                        (p.splits == 1 || (nk / p.splits >= 4 && p.cols % 128 == 0)) &&
+                        p.partials() == (p.splits > 1 ? p.tail * p.splits * 256 * p.cols : 0);
               if (p.tail) ok = ok && p.full % pairs == 0;  // whole turns of whole tiles, then the shares
               // A share's blocks, as the kernel cuts them.
               int64_t covered = 0;
@@ -59,25 +59,22 @@ int main() {
         ++seen;
       }
   // Every value of a share at its own place, and where the kernel's warps put it.
-  for (int cols : {128, 160, 192, 224, 256}) {
-    std::vector<int> hit(share_units(cols));
-    const int chunks = (cols + 127) / 128;
-    int units = 0;
+  for (int cols : {128, 256}) {
+    std::vector<int> hit(64 * cols);
+    const int chunks = cols / 128;
     for (int rank = 0; rank < 2; ++rank)
       for (int w = 0; w < 16; ++w)
-        for (int c = 0; c < chunks && w / 4 * 32 + c * 128 < cols; ++c)
+        for (int c = 0; c < chunks; ++c)
           for (int lane = 0; lane < 32; ++lane)
             for (int u = 0; u < 8; ++u) {
               const int quarter = (w + 2) & 3;  // warp w + 2 of the CTA reads this quarter of its TMEM lanes
               const int row = rank * 128 + quarter * 32 + lane, col = w / 4 * 32 + c * 128 + u * 4;
               const int there = ((rank * 16 + w) * chunks + c) * 256 + lane * 8 + (u ^ (lane & 7));
               const int unit = share_unit(row, col, cols);
-              if (unit != there || unit < 0 || unit >= share_units(cols)) { ++bad; continue; }
+              if (unit != there || unit < 0 || unit >= 64 * cols) { ++bad; continue; }
               ++hit[unit];
-              ++units;
             }
-    bad += units != 64 * cols;
-    for (int h : hit) bad += h > 1;
+    for (int h : hit) bad += h != 1;
     ++seen;
   }
   std::printf("%ld seen, %ld bad\\n", seen, bad);
