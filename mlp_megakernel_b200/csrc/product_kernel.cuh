@@ -6,21 +6,23 @@
 //   kEpiGated     g = A Bg, u = A Bu; h = act(g) u; g and u kept for the backward
 //   kEpiGatedBwd  dh = A B; dg = dh u act'(g), du = dh act(g), h = act(g) u again
 //
-// A tile of D is 256 rows x TN columns of a pair of CTAs (pair.cuh), reduced in
+// A tile of D is 256 rows x TN columns (kEpiPlain, and kEpiLinear without 8-bit
+// values: any multiple of 32 up to TN) of a pair of CTAs (pair.cuh), reduced in
 // blocks of 64 through a ring of TMA loads; operands are fp16 or bf16 in either
 // order (K contiguous, or the row / column index), chosen at run time by the
 // descriptors alone.  Roles of a CTA: warp 0 loads, warp 1 of the leader issues
 // the tcgen05 instructions, warps 2..17 are the epilogue (thread = row; four warps
-// share the 32 rows of a TMEM lane quarter and quarter the columns: an epilogue is
-// a chain of waits, and eight warps left the gate's backward at twice the time of
-// its products).  Two
-// accumulators of TN columns, so the epilogue of a tile runs beside the products
-// of the next.  The kernel is persistent: tiles are taken in groups of `group`
-// row tiles over all column tiles, so that the pairs at work share rows and
-// columns in L2.  The tiles behind the last full turn of the pairs may be shared
-// out (kEpiPlain, and kEpiLinear that keeps nothing): an item is then a share of a
-// tile's reduction, whose fp32 values go to a workspace, and tail_sum_kernel adds
-// them in order and runs the epilogue.
+// share the 32 rows of a TMEM lane quarter and have a quarter of the runs of 32
+// columns each: an epilogue is a chain of waits, and eight warps left the gate's
+// backward at twice the time of its products).  Two accumulators of TN columns, so
+// the epilogue of a tile runs beside the products of the next.  The kernel is
+// persistent: tiles are taken in groups of `group` row tiles over all column tiles,
+// so that the pairs at work share rows and columns in L2.  The tiles behind the
+// last full turn of the pairs may be shared out (kEpiPlain, and kEpiLinear that
+// keeps nothing): an item is then a share of a tile's reduction, whose fp32 values
+// go to a workspace, and tail_sum_kernel adds them in order and runs the epilogue.
+// All tiles' first shares come first: the pairs at work then read one part of the
+// operands (2816 x 20011 x 1024: 309 MB from memory tile by tile, 177 so).
 //
 // Everything between the operands and the stored values is fp32: accumulators,
 // bias, activation, residual.  What is kept for the backward is rounded once, to

@@ -27,11 +27,17 @@ struct ProductPlan {
 // nk: blocks of 64 of the reduction; may_split, may_narrow, may_any: whether the
 // product's epilogue allows shares, tiles of 128 columns, tiles of 160 to 224.
 //
-// The tiles go over the pairs in turns; a turn takes nk blocks' time.  What is left
-// behind the last full turn of tiles of 256 or 128 columns may be shared out over
-// all pairs in shares of the reduction: ceil(tail splits / pairs) turns of nk / splits blocks, and the
-// traffic of the shares (0.5 us a megabyte, written and read) and of a second
-// kernel (4 us).  A block takes 0.3 us, a kernel's beginning and end 5.
+// The tiles go over the pairs in turns; a turn takes nk blocks' time: 0.3 us each at
+// 256 columns, less for narrower tiles, but not in their proportion (their rows are
+// loaded for fewer products).  Narrower ones pay where they fill the last turn
+// better (a linear layer, bf16, us: 2000 x 5120 x 1280 in 40 tiles of 256 columns
+// 33.4, in 64 of 160 26.3; 3000 x 2048 x 5120 in 240 of 256 55.9, in 276 of 224 52.4;
+// 8192 x 1024 x 4096 in 512 of 256 58, in 1024 of 128 85).  What is left behind the
+// last full turn of tiles of 256 or 128 columns may be shared out over all pairs in
+// shares of the reduction: ceil(tail splits / pairs) turns of nk / splits blocks,
+// the traffic of the shares (0.5 us a megabyte, written and read) and a second
+// kernel (4 us); dw of 20011 x 1024 x 2816: 136 whole, 119 so.  A kernel's beginning
+// and end are 5 us.
 inline ProductPlan product_plan(int64_t rows, int cols, int outputs, int out_cols, int nk, int pairs, bool may_split,
                                 bool may_narrow, bool may_any) {
   ProductPlan best;
