@@ -167,7 +167,7 @@ def test_linear_whose_last_tiles_are_shared_out(shape, act, dtype):
 
 
 @pytest.mark.parametrize("shape", [(513, 136, 3088), (513, 136, 3872), (600, 200, 4600), (769, 520, 4656), (2000, 264, 1288),
-                                   (2500, 72, 1400)])
+                                   (2500, 72, 1400), (520, 2000, 1288), (20000, 264, 136)])
 @pytest.mark.parametrize("transposed", [False, True])
 @pytest.mark.parametrize("dtype", list(U))
 def test_tiles_of_any_width(shape, transposed, dtype):
@@ -236,6 +236,16 @@ def test_gated(shape, dtype):
     gated_case(*shape, dtype, "silu", True, 1)
     gated_case(*shape, dtype, "gelu_tanh", False, 2, (True, True, False))
     gated_case(*shape, dtype, "silu", True, 0, (True, False, True))
+
+
+@pytest.mark.parametrize("shape", [(100, 72, 264, 4096), (300, 72, 520, 4104), (1000, 136, 264, 8192), (300, 136, 4104, 72),
+                                   (1001, 264, 4096, 136), (9001, 264, 136, 72)])
+@pytest.mark.parametrize("keep", [1, 2])
+@pytest.mark.parametrize("dtype", list(U))
+def test_gated_long_reductions(shape, keep, dtype):
+    """Of the gate's backward, of dx over both projections, and of dw, some in the kernel for few rows, some in shares."""
+    gated_case(*shape, dtype, "silu", True, keep)
+    gated_case(*shape, dtype, "softplus", False, keep, (False, True, True))
 
 
 @pytest.mark.parametrize("act", ACTS)
