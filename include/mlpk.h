@@ -403,7 +403,7 @@ int mlpk_gated_bwd(int64_t rows, int hidden, int d_out, int dtype, int act, cons
  * two (2^-126 at least) with max|x| / scale <= 448 over a row's 128 columns (the
  * last group may be shorter), NaN where a value is not finite; and back, x = q
  * scale (exact in fp32 and bf16; clipped to dtype's largest finite value, which
- * rounding up may pass).  x: fp16, bf16 or fp32 [rows][width], any width; q:
+ * rounding up may pass).  x: fp16, bf16 or fp32 [rows][width], width from 1 on; q:
  * [rows][width]; scale: [rows][ceil(width / 128)]. */
 int mlpk_fp8_checkpoint(int64_t rows, int width, int dtype, const void* x, void* q, float* scale,
                         mlpk_stream_t stream);

@@ -122,6 +122,7 @@ ADAMW_CHUNK = 2048  # MLPK_ADAMW_CHUNK: the unit of the step counts, in elements
 EXPERT_MAX = 1024
 FF_MAX_ROWS = 2 ** 31 - 1 - 256
 FF_MAX_WIDTH = 2 ** 20
+FP8_MAX_WIDTH = 2 ** 31 - 1
 NORM_MAX_WIDTH = 32768
 NORM_GROUP = 128  # columns that share a scale of the 8-bit norm
 PEER_HANDLE_BYTES = 64

@@ -185,16 +185,23 @@ def _check_gated_bwd(grad_out, x, x_scale, w_gate, w_up, w_down, g, g_scale, u, 
         _check_saved_x(x, x_scale, grad_out, w_gate.shape[0])
 
 
+def _check_columns(x) -> None:
+    if x.shape[-1] > _lib.FP8_MAX_WIDTH:  # the C calls' int
+        raise ValueError(f"rows must have at most {_lib.FP8_MAX_WIDTH} columns, got {x.shape[-1]}: view them as more rows")
+
+
 def _check_values(x) -> None:
     if not isinstance(x, Tensor) or x.dim() < 1 or x.shape[-1] < 1:
         raise ValueError("x must be a tensor [..., width]")
     if x.dtype not in DTYPES:
         raise TypeError(f"fp8_checkpoint takes fp16, bf16 or fp32, got {x.dtype}")
+    _check_columns(x)
 
 
 def _check_quantized(q, scale) -> None:
     if not isinstance(q, Tensor) or q.dim() < 1 or q.shape[-1] < 1 or q.dtype != FP8:
         raise ValueError(f"q must be a {FP8} tensor [..., width]")
+    _check_columns(q)
     want = (*q.shape[:-1], -(-q.shape[-1] // 128))
     if not isinstance(scale, Tensor) or scale.shape != want or scale.dtype != torch.float32 or scale.device != q.device:
         raise ValueError(f"scale must be a {want} float32 tensor on {q.device}")
@@ -447,7 +454,7 @@ def fused_gated_mlp(x: Tensor, w_gate: Tensor, w_up: Tensor, w_down: Tensor, *, 
 def fp8_checkpoint(x: Tensor):
     """``(q, scale)``: x in 8 bits, for a backward pass or a cache of the caller's.
 
-    ``x`` is fp16, bf16 or fp32 ``[..., width]`` of any width; ``q`` is
+    ``x`` is fp16, bf16 or fp32 ``[..., width]`` of any width below 2^31; ``q`` is
     float8_e4m3fn of its shape, ``scale`` fp32 ``[..., ceil(width / 128)]``: the
     smallest power of two (2^-126 at least) with ``max|x| / scale <= 448`` over
     its 128 columns, NaN where one of them is not finite.  A value is off by 1/16
