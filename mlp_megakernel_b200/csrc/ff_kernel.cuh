@@ -39,19 +39,18 @@ __device__ __forceinline__ void store8(T* p, const float (&f)[8]) {
 struct Steps {
   int64_t major, major_step;
   int minor, minor_step, minors;
-  __device__ Steps(int64_t first, int64_t step, int minors_) : minors(minors_) {
+  __host__ __device__ Steps(int64_t first, int64_t step, int minors_) : minors(minors_) {
     major = first / minors;
     minor = static_cast<int>(first - major * minors);
     major_step = step / minors;
     minor_step = static_cast<int>(step - major_step * minors);
   }
-  __device__ __forceinline__ void next() {
-    major += major_step;
-    minor += minor_step;
-    if (minor >= minors) {
-      minor -= minors;
-      ++major;
-    }
+  __host__ __device__ __forceinline__ void next() {
+    // Unsigned: both are below 2^31, their sum need not be.
+    const uint32_t next = static_cast<uint32_t>(minor) + static_cast<uint32_t>(minor_step);
+    const bool over = next >= static_cast<uint32_t>(minors);
+    minor = static_cast<int>(over ? next - static_cast<uint32_t>(minors) : next);
+    major += major_step + over;
   }
 };
 
