@@ -353,7 +353,8 @@ int mlpk_adamw_step(int count, const int64_t* numel, void* const* params, const 
 #define MLPK_ACT_SOFTPLUS 4
 #define MLPK_ACT_SIGMOID 5
 /* What a forward call keeps for the backward: nothing, values of dtype
- * [rows][width], or 8-bit values [rows][mlpk_fp8_pitch(width)] with fp32 scales
+ * [rows][width] (a finite value beyond dtype's largest is kept as that: fp16's
+ * 65504), or 8-bit values [rows][mlpk_fp8_pitch(width)] with fp32 scales
  * [rows][ceil(width / 128)] (see mlpk_fp8_checkpoint). */
 #define MLPK_KEEP_NONE 0
 #define MLPK_KEEP_16 1
@@ -393,7 +394,8 @@ int mlpk_gated(int64_t rows, int d_in, int hidden, int dtype, int act, const voi
                const void* w_up, int w_layout, void* h, int keep, void* g, float* g_scale, void* u, float* u_scale,
                mlpk_stream_t stream);
 /* Its backward behind out = h w_down: dh = grad_out w_down^T, dg = dh u act'(g),
- * du = dh act(g), and h = act(g) u again (for w_down's gradient), in one kernel.
+ * du = dh act(g), and h = act(g) u again (for w_down's gradient; finite values
+ * beyond dtype's largest as that), in one kernel.
  * w_down: [hidden][d_out] in w_layout. */
 int mlpk_gated_bwd(int64_t rows, int hidden, int d_out, int dtype, int act, const void* grad_out, const void* w_down,
                    int w_layout, int keep, const void* g, const float* g_scale, const void* u, const float* u_scale,

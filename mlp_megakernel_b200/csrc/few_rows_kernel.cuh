@@ -61,6 +61,10 @@ template <class T>
 __device__ __forceinline__ void store4(T* p, const float (&f)[4]) {
   store_vec<T, 4>(p, f);
 }
+template <class T>
+__device__ __forceinline__ void store_kept4(T* p, const float (&f)[4]) {
+  *reinterpret_cast<uint2*>(p) = make_uint2(kept_pair<T>(f[0], f[1]), kept_pair<T>(f[2], f[3]));
+}
 __device__ __forceinline__ void load_fp8x4(const uint8_t* q, float scale, float (&f)[4]) {
   float2 v[2];
   unpack_fp8<4>(load_raw<uint16_t, 2>(reinterpret_cast<const uint16_t*>(q)), v);
@@ -240,7 +244,7 @@ __global__ void __launch_bounds__(kFewThreads) few_rows_kernel(const __grid_cons
   #pragma unroll
           for (int e = 0; e < 4; ++e) v[e] += b[e];
         }
-        if (p.keep_kind == kKeep16 && here) store4(static_cast<T*>(p.keep[0]) + at, v);
+        if (p.keep_kind == kKeep16 && here) store_kept4(static_cast<T*>(p.keep[0]) + at, v);
         if (p.keep_kind == kKeep8) {  // a whole warp has the row's 128 columns (zeros beyond the last)
           float inv, most = max_abs(max_abs(0.0f, v[0], v[1]), v[2], v[3]);
           if (!here) most = 0.0f;
@@ -270,8 +274,8 @@ __global__ void __launch_bounds__(kFewThreads) few_rows_kernel(const __grid_cons
       } else if constexpr (EPI == kEpiGated) {
         if (here) {
           if (p.keep_kind == kKeep16) {
-            store4(static_cast<T*>(p.keep[0]) + at, v);
-            store4(static_cast<T*>(p.keep[1]) + at, u);
+            store_kept4(static_cast<T*>(p.keep[0]) + at, v);
+            store_kept4(static_cast<T*>(p.keep[1]) + at, u);
           }
           with_act(p.act, [&](auto a) {
   #pragma unroll
@@ -302,7 +306,7 @@ __global__ void __launch_bounds__(kFewThreads) few_rows_kernel(const __grid_cons
           });
           store4(static_cast<T*>(p.out[0]) + at, g);
           store4(static_cast<T*>(p.out[1]) + at, v);
-          store4(static_cast<T*>(p.keep[0]) + at, h);
+          store_kept4(static_cast<T*>(p.keep[0]) + at, h);
         }
       }
     }

@@ -26,8 +26,9 @@
 //
 // Everything between the operands and the stored values is fp32: accumulators,
 // bias, activation, residual.  What is kept for the backward is rounded once, to
-// the operands' type (as a 16-bit activation is anywhere else in training) or to
-// 8 bits with a scale for each row and 128 columns (act.cuh).
+// the operands' type (as a 16-bit activation is anywhere else in training; a finite
+// value beyond the type's largest becomes that, vec.cuh's kept_pair) or to 8 bits
+// with a scale for each row and 128 columns (act.cuh).
 #pragma once
 #include "act.cuh"
 #include "layout.cuh"
@@ -200,16 +201,22 @@ __device__ __forceinline__ float2 widen(uint32_t p) {
   return to_float2(*reinterpret_cast<const typename Pair<T>::type*>(&p));
 }
 // N values of a thread's row, from column `from` on, into and from its tile in
-// shared memory (as a TMA box with the row's swizzle has it).
-template <class T, int PITCH, int N>
+// shared memory (as a TMA box with the row's swizzle has it).  KEPT: for a backward
+// pass to read (kept_pair).
+template <class T, int PITCH, bool KEPT = false, int N>
 __device__ __forceinline__ void tile_store(uint32_t tile, int lane, int from, const float (&v)[N]) {
 #pragma unroll
   for (int u = 0; u < N / 8; ++u) {
     uint32_t p[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const typename Pair<T>::type x = Pair<T>::round(v[8 * u + 2 * i], v[8 * u + 2 * i + 1]);
-      p[i] = *reinterpret_cast<const uint32_t*>(&x);
+      const float a = v[8 * u + 2 * i], b = v[8 * u + 2 * i + 1];
+      if constexpr (KEPT) {
+        p[i] = kept_pair<T>(a, b);
+      } else {
+        const typename Pair<T>::type x = Pair<T>::round(a, b);
+        p[i] = *reinterpret_cast<const uint32_t*>(&x);
+      }
     }
     st_shared_v4(tile + swz_off<PITCH>(lane, from / 8 + u), p[0], p[1], p[2], p[3]);
   }
@@ -543,7 +550,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kProductThreads, 1)
           if (p.bias) add_bias<T>(p, col, v);
           if (p.keep_kind == kKeep16) {
             const uint32_t tile = begin_tile();
-            tile_store<T, PITCH>(tile, lane, 0, v);
+            tile_store<T, PITCH, true>(tile, lane, 0, v);
             end_tile(&p.keep[0], tile, col, row0);
           } else if (p.keep_kind == kKeep8 && row < p.rows) {
             store_fp8x32(p.q[0] + row * p.q_pitch + col, v, inv);
@@ -598,10 +605,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kProductThreads, 1)
           }
           if (p.keep_kind == kKeep16) {
             uint32_t tile = begin_tile();
-            tile_store<T, PITCH>(tile, lane, 0, g);
+            tile_store<T, PITCH, true>(tile, lane, 0, g);
             end_tile(&p.keep[0], tile, col0, row0);
             tile = begin_tile();
-            tile_store<T, PITCH>(tile, lane, 0, u);
+            tile_store<T, PITCH, true>(tile, lane, 0, u);
             end_tile(&p.keep[1], tile, col0, row0);
           }
           if constexpr (CHUNK == 32) {
@@ -662,10 +669,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kProductThreads, 1)
             tile_store<T, PITCH>(tile_g, lane, from, g);
             tile_store<T, PITCH>(tile_u, lane, from, d);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const typename Pair<T>::type x = Pair<T>::round(u[2 * i], u[2 * i + 1]);
-              h[from / 2 + i] = *reinterpret_cast<const uint32_t*>(&x);
-            }
+            for (int i = 0; i < 8; ++i) h[from / 2 + i] = kept_pair<T>(u[2 * i], u[2 * i + 1]);
           }
           fence_proxy_async_smem();
           __syncwarp();

@@ -8,6 +8,7 @@
 #include <cuda_fp8.h>
 
 #include <cstdint>
+#include <type_traits>
 
 namespace mlpk {
 
@@ -56,6 +57,22 @@ struct Pair<__nv_bfloat16> {
   using type = __nv_bfloat162;
   static __device__ __forceinline__ type round(float a, float b) { return __floats2bfloat162_rn(a, b); }
 };
+
+// Two values rounded for a backward pass to read, as they lie in memory: a finite
+// one beyond the type's largest becomes that (rounded to infinity, it would make
+// a NaN of a derivative that is 0 there); infinities and NaN stay.  Infinity less
+// one, as a whole number, is the largest value of its sign.
+template <class T>
+__device__ __forceinline__ uint32_t kept_pair(float a, float b) {
+  const typename Pair<T>::type v = Pair<T>::round(a, b);
+  uint32_t p = *reinterpret_cast<const uint32_t*>(&v);
+  // The least magnitude that rounds to infinity.
+  constexpr float over = std::is_same_v<T, __half> ? 65520.0f : 3.3961775292304601e+38f;
+  const float infinity = __uint_as_float(0x7f800000u);
+  if (fabsf(a) >= over && fabsf(a) < infinity) p -= 1;
+  if (fabsf(b) >= over && fabsf(b) < infinity) p -= 0x10000u;
+  return p;
+}
 
 template <class T, int VEC>
 __device__ __forceinline__ void unpack(const Raw<T, VEC>& r, float (&f)[VEC]) {

@@ -409,7 +409,9 @@ def fused_linear(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, *, ac
     weight's and the bias's gradients are summed over the rows in fp32 in a fixed
     order.  ``activation_dtype`` is the precision of what the backward keeps (x
     where the weight needs a gradient, the values before the activation): x's
-    type, or ``torch.float8_e4m3fn`` (fp8_checkpoint).
+    type, or ``torch.float8_e4m3fn`` (fp8_checkpoint).  In x's type a finite value
+    beyond its largest (65504 in fp16) is kept as that; the gradients are the same,
+    since every derivative is constant out there.
     """
     act = _act_code(activation)
     fp8 = _keeps_fp8(activation_dtype, getattr(x, "dtype", None))
@@ -435,7 +437,9 @@ def fused_gated_mlp(x: Tensor, w_gate: Tensor, w_up: Tensor, w_down: Tensor, *, 
     values are rounded to x's type between them.  Differentiable in all of them:
     the backward forms both hidden gradients and the hidden values again in the
     epilogue of one product.  ``activation`` and ``activation_dtype`` as in
-    fused_linear (kept: x, and both projections).
+    fused_linear (kept: x, and both projections).  Where a projection is beyond the
+    largest value of x's type (65504 in fp16), the gradients are those of a
+    projection of that value; kept in 8 bits it stays within 1/16 of itself.
     """
     act = _act_code(activation)
     fp8 = _keeps_fp8(activation_dtype, getattr(x, "dtype", None))
