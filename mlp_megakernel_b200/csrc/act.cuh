@@ -44,7 +44,8 @@ __device__ __forceinline__ float act_both(float z, float& slope) {
     const float s = sigmoid_f32(ACT == kActSilu ? z : kGeluA * fmaf(kGeluB * z, zz, z));
     const float v = z * s;
     const float rest = fmaf(-v, s, v);  // z s (1 - s)
-    slope = ACT == kActSilu ? s + rest : fmaf(rest, fmaf(3.0f * kGeluA * kGeluB, zz, kGeluA), s);
+    // p' stays finite (zz does not, above |z| = 1.8e19): z s (1 - s) is 0 long before.
+    slope = ACT == kActSilu ? s + rest : fmaf(rest, fmaf(3.0f * kGeluA * kGeluB, fminf(zz, 1e30f), kGeluA), s);
     return v;
   }
   if constexpr (ACT == kActSoftplus) {

@@ -76,6 +76,49 @@ def test_linear_beyond_bf16(rows, act):
     linear(rows, act, 1, BF16, x, w, b, r, 3.39618e38)
 
 
+@pytest.mark.parametrize("rows", ROWS)
+@pytest.mark.parametrize("top", [2e19, 1e22, 3e38])
+@pytest.mark.parametrize("keep", [1, 2])
+def test_gelu_where_the_square_overflows(rows, top, keep):
+    """z^2 leaves fp32 above 1.8e19: the derivative is 1 or 0 there."""
+    x, w = make(rows, 72, dtype=BF16, seed=1), make(72, 264, dtype=BF16, seed=2, scale=0.1)
+    b, r = make(264, dtype=F32, seed=3), make(rows, 264, dtype=BF16, seed=4)
+    b[3], b[200] = top, -top
+    n, z = 264, x.double() @ w.double() + b.double()
+    out, *kept = ops.linear(x, w, b, r, ff.ACTIVATIONS["gelu_tanh"], keep)
+    v, s = (kept + [None])[:2]
+    go = make(rows, n, dtype=BF16, seed=5)
+    dx, dw, db = ops.linear_bwd(go, x, None, w, v, s, ff.ACTIVATIONS["gelu_tanh"], F32, True, True, True)
+    assert torch.isfinite(out).all() and all(torch.isfinite(t).all() for t in (dx, dw, db))
+    far = z.abs() > 1e19
+    assert far[:, 3].all() and far[:, 200].all() and not far[:, :3].any()
+    near = torch.where(far, z, kept64(v, s, n))
+    _, slope, rel = act64("gelu_tanh", near)
+    assert (slope[:, 3] == 1).all() and (slope[:, 200] == 0).all()
+    dz, u = go.double() * slope, U[BF16]
+    room = torch.where(far, 0.0, rel * go.double().abs() * slope.abs().clamp(min=0.01)) + ACC * go.double().abs()
+    close(db, dz.sum(0), room.sum(0) + (rows + 20) * ACC * dz.abs().sum(0), ACC, "db")
+    room = room * (1 + u) + u * dz.abs() + TINY
+    close(dx, *product(dz, w.double().t(), ea=room), u, "dx")
+    close(dw, *product(x.double().t(), dz, eb=room), u, "dw")
+
+
+@pytest.mark.parametrize("rows", ROWS)
+@pytest.mark.parametrize("keep", [1, 2])
+def test_a_gelu_gate_where_the_square_overflows(rows, keep):
+    """A gate of -1e22 is shut: no gradient of its column, and none that is not finite."""
+    x, wg, wu = make(rows, 72, dtype=BF16, seed=1), make(72, 264, dtype=BF16, seed=2, scale=0.1), make(72, 264, dtype=BF16, seed=3, scale=0.1)
+    wd, go = make(264, 136, dtype=BF16, seed=4, scale=0.1), make(rows, 136, dtype=BF16, seed=5)
+    x[:, 0], wg[0] = 1e12, 0
+    wg[0, 7] = -1e10
+    wu[0] = 0
+    out, *kept = ops.gated_mlp(x, wg, wu, wd, None, ff.ACTIVATIONS["gelu_tanh"], keep)
+    gk, sg, uk, su = kept if keep == 2 else (kept[0], None, kept[1], None)
+    dx, dwg, dwu, dwd = ops.gated_mlp_bwd(go, x, None, wg, wu, wd, gk, sg, uk, su, ff.ACTIVATIONS["gelu_tanh"], True, True, True)
+    assert all(torch.isfinite(t).all() for t in (out, dx, dwg, dwu, dwd))
+    assert not dwg[:, 7].any() and not dwu[:, 7].any() and not dwd[7].any()
+
+
 def stored(ref, off, u):
     return off * (1 + u) + u * ref.abs() + TINY
 
