@@ -92,4 +92,18 @@ __device__ __forceinline__ float checkpoint_scale(float most, float* inv) {
   return __uint_as_float(biased << 23);
 }
 
+__device__ __forceinline__ float clip(float v, float most) {  // a NaN stays
+  return v > most ? most : v < -most ? -most : v;
+}
+// Values read back, q scale in fp32: next to fp32's largest value e4m3 rounds up to
+// 256 x 2^120, which is that value here too.  The largest scale is 2^120, and no
+// other group has anything to clip.
+template <int N>
+__device__ __forceinline__ void clip_restored(float (&v)[N], float scale) {
+  if (scale >= 1.329227995784916e+36f) {  // 2^120
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = clip(v[i], 3.402823466e+38f);
+  }
+}
+
 }  // namespace mlpk

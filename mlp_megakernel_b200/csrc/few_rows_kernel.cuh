@@ -69,6 +69,7 @@ __device__ __forceinline__ void load_fp8x4(const uint8_t* q, float scale, float 
   float2 v[2];
   unpack_fp8<4>(load_raw<uint16_t, 2>(reinterpret_cast<const uint16_t*>(q)), v);
   f[0] = v[0].x * scale, f[1] = v[0].y * scale, f[2] = v[1].x * scale, f[3] = v[1].y * scale;
+  clip_restored(f, scale);
 }
 
 template <class T, int EPI>

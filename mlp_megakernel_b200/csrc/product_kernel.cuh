@@ -150,6 +150,7 @@ __device__ __forceinline__ void widen_fp8x16(const uint32_t* w, float scale, flo
   unpack_fp8<16>(r, f);
 #pragma unroll
   for (int i = 0; i < 8; ++i) v[2 * i] = f[i].x * scale, v[2 * i + 1] = f[i].y * scale;
+  clip_restored(v, scale);
 }
 
 // v += bias[col ..]; a vector of 8 columns is inside the tensor or outside.

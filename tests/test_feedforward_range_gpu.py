@@ -76,11 +76,7 @@ def test_linear_beyond_bf16(rows, act):
     linear(rows, act, 1, BF16, x, w, b, r, 3.39618e38)
 
 
-@pytest.mark.parametrize("rows", ROWS)
-@pytest.mark.parametrize("top", [2e19, 1e22, 3e38])
-@pytest.mark.parametrize("keep", [1, 2])
-def test_gelu_where_the_square_overflows(rows, top, keep):
-    """z^2 leaves fp32 above 1.8e19: the derivative is 1 or 0 there."""
+def gelu_far_out(rows, top, keep):
     x, w = make(rows, 72, dtype=BF16, seed=1), make(72, 264, dtype=BF16, seed=2, scale=0.1)
     b, r = make(264, dtype=F32, seed=3), make(rows, 264, dtype=BF16, seed=4)
     b[3], b[200] = top, -top
@@ -101,6 +97,44 @@ def test_gelu_where_the_square_overflows(rows, top, keep):
     room = room * (1 + u) + u * dz.abs() + TINY
     close(dx, *product(dz, w.double().t(), ea=room), u, "dx")
     close(dw, *product(x.double().t(), dz, eb=room), u, "dw")
+
+
+@pytest.mark.parametrize("rows", ROWS)
+@pytest.mark.parametrize("top", [2e19, 1e22, 3e38])
+@pytest.mark.parametrize("keep", [1, 2])
+def test_gelu_where_the_square_overflows(rows, top, keep):
+    """z^2 leaves fp32 above 1.8e19: the derivative is 1 or 0 there."""
+    gelu_far_out(rows, top, keep)
+
+
+@pytest.mark.parametrize("rows", ROWS)
+@pytest.mark.parametrize("keep", [1, 2])
+def test_gelu_next_to_the_largest_value(rows, keep):
+    """3.38e38 in 8 bits is 256 x 2^120, beyond fp32: read back, it is fp32's largest value."""
+    gelu_far_out(rows, 3.38e38, keep)
+
+
+@pytest.mark.parametrize("rows", ROWS)
+@pytest.mark.parametrize("act", [a for a in ACTS if a != "gelu_tanh"])
+def test_linear_from_8_bits_next_to_the_largest_value(rows, act):
+    x, w = make(rows, 72, dtype=BF16, seed=1), make(72, 264, dtype=BF16, seed=2, scale=0.1)
+    b, r = make(264, dtype=F32, seed=3), make(rows, 264, dtype=BF16, seed=4)
+    b[3], b[200] = 3.35e38, -3.35e38
+    linear(rows, act, 2, BF16, x, w, b, r, 3.3e38)
+
+
+@pytest.mark.parametrize("rows", ROWS)
+@pytest.mark.parametrize("act", ["silu", "gelu_tanh"])
+def test_a_gate_from_8_bits_next_to_the_largest_value(rows, act):
+    """A shut gate whose 8-bit value would be minus infinity in fp32."""
+    x, wg, wu = make(rows, 72, dtype=BF16, seed=1), make(72, 264, dtype=BF16, seed=2, scale=0.1), make(72, 264, dtype=BF16, seed=3, scale=0.1)
+    wd, go = make(264, 136, dtype=BF16, seed=4, scale=0.1), make(rows, 136, dtype=BF16, seed=5)
+    x[:, 0], wg[0], wu[0] = 2.0 ** 64, 0, 0
+    wg[0, 7] = -1.9765625 * 2.0 ** 63  # g is -3.36e38
+    out, gk, sg, uk, su = ops.gated_mlp(x, wg, wu, wd, None, ff.ACTIVATIONS[act], 2)
+    assert (kept64(gk, sg, 264)[:, 7] == -2.0 ** 128).all()
+    got = ops.gated_mlp_bwd(go, None, None, wg, wu, wd, gk, sg, uk, su, ff.ACTIVATIONS[act], True, False, True)
+    assert all(torch.isfinite(t).all() for t in (out, *got)) and not got[1][7].any()
 
 
 @pytest.mark.parametrize("rows", ROWS)
