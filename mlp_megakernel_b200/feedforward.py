@@ -505,7 +505,8 @@ def _operand_type(x: Tensor) -> torch.dtype:
 
 class FusedLinear(nn.Module):
     """``activation(x @ weight + bias) + residual`` with ``weight`` ``[in, out]``.
-    Parameters of another type (fp32 ones, say) are cast to x's, or autocast's."""
+    Parameters of another type (fp32 ones, say) are cast to x's, or autocast's; an
+    fp32 bias is added as it is."""
 
     def __init__(self, in_features: int, out_features: int, bias: bool = True, activation: Optional[str] = None,
                  activation_dtype: Optional[torch.dtype] = None):
@@ -520,7 +521,8 @@ class FusedLinear(nn.Module):
 
     def forward(self, x: Tensor, residual: Optional[Tensor] = None) -> Tensor:
         t = _operand_type(x)
-        return fused_linear(x.to(t), self.weight.to(t), self.bias, activation=self.activation,
+        bias = self.bias if self.bias is None or self.bias.dtype == torch.float32 else self.bias.to(t)
+        return fused_linear(x.to(t), self.weight.to(t), bias, activation=self.activation,
                             residual=None if residual is None else residual.to(t),
                             activation_dtype=self.activation_dtype)
 
