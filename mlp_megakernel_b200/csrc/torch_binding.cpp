@@ -446,6 +446,23 @@ struct Kept {
   int kind() const { return !v.defined() ? MLPK_KEEP_NONE : scale.defined() ? MLPK_KEEP_FP8 : MLPK_KEEP_16; }
   float* scales() const { return static_cast<float*>(ptr(scale)); }
 };
+// As the kernels take it: a hook on saved tensors may give back other strides.
+Kept aligned(const Kept& k) { return {aligned(k.v), aligned(k.scale)}; }
+// Whether values [..., width] of that many rows are what a forward keeps for `go`'s
+// backward, in all but the layout: of its type, or in 8 bits with scales (the
+// values in rows of `pitch`).
+bool kept_for(const Kept& k, const Tensor& go, int64_t rows, int64_t width, int64_t pitch) {
+  const Tensor &v = k.v, &s = k.scale;
+  if (!v.defined() || v.device() != go.device() || v.dim() < 1) return false;
+  if (!s.defined()) return v.scalar_type() == go.scalar_type() && v.size(-1) == width && v.numel() == rows * width;
+  return v.scalar_type() == at::kFloat8_e4m3fn && v.size(-1) == pitch && v.numel() == rows * pitch &&
+         s.scalar_type() == at::kFloat && s.device() == go.device() && s.dim() >= 1 && s.size(-1) == (width + 127) / 128 &&
+         s.numel() == rows * s.size(-1);
+}
+bool weight_for(const Tensor& w, const Tensor& go) {
+  return w.dim() == 2 && w.scalar_type() == go.scalar_type() && w.device() == go.device();
+}
+void check_saved(bool ok) { TORCH_CHECK(ok, "a saved tensor is not what the forward saved (a hook changed its shape, type or device)"); }
 Kept keep_for(const Tensor& x, int64_t rows, int64_t width, int64_t keep) {
   Kept k;
   if (keep == MLPK_KEEP_16) k.v = at::empty({rows, width}, x.options());
@@ -535,11 +552,15 @@ void dw_of(const Tensor& x_in, std::initializer_list<Tensor> dz, std::initialize
 struct LinearGrads {
   Tensor dx, dw, db;
 };
-LinearGrads linear_backward(const Tensor& go_in, const Kept& x, const Tensor& w_in, const Kept& z, int64_t act,
+LinearGrads linear_backward(const Tensor& go_in, const Kept& x, const Tensor& w_in, const Kept& z_in, int64_t act,
                             at::ScalarType db_type, bool want_dx, bool want_dw, bool want_db) {
   const c10::cuda::CUDAGuard guard(go_in.device());
   const Tensor go = aligned(go_in);
   const int64_t rows = rows_of(go), n = go.size(-1);
+  check_saved(weight_for(w_in, go) && w_in.size(1) == n &&
+              (act == MLPK_ACT_NONE || kept_for(z_in, go, rows, n, mlpk_fp8_pitch(static_cast<int>(n)))) &&
+              (!want_dw || kept_for(x, go, rows, w_in.size(0), w_in.size(0))));
+  const Kept z = aligned(z_in);
   LinearGrads got;
   Tensor dz = go;
   if (act != MLPK_ACT_NONE || want_db) {
@@ -587,10 +608,15 @@ struct GatedGrads {
   Tensor dx, dwg, dwu, dwd;
 };
 GatedGrads gated_backward(const Tensor& go_in, const Kept& x, const Tensor& wg_in, const Tensor& wu_in, const Tensor& wd_in,
-                          const Kept& g, const Kept& u, int64_t act, bool want_dx, bool want_dgu, bool want_dd) {
+                          const Kept& g_in, const Kept& u_in, int64_t act, bool want_dx, bool want_dgu, bool want_dd) {
   const c10::cuda::CUDAGuard guard(go_in.device());
   const Tensor go = aligned(go_in);
-  const int64_t rows = rows_of(go), width = wd_in.size(0);
+  check_saved(weight_for(wd_in, go) && wd_in.size(1) == go.size(-1) && weight_for(wg_in, go) && weight_for(wu_in, go));
+  const int64_t rows = rows_of(go), width = wd_in.size(0), pitch = mlpk_fp8_pitch(static_cast<int>(width));
+  check_saved(wg_in.size(1) == width && wu_in.sizes() == wg_in.sizes() && kept_for(g_in, go, rows, width, pitch) &&
+              kept_for(u_in, go, rows, width, pitch) && g_in.kind() == u_in.kind() &&
+              (!want_dgu || kept_for(x, go, rows, wg_in.size(0), wg_in.size(0))));
+  const Kept g = aligned(g_in), u = aligned(u_in);
   const Weight wd = weight_of(wd_in);
   Tensor dg = at::empty({rows, width}, go.options()), du = at::empty_like(dg), h = at::empty_like(dg);
   check("mlpk_gated_bwd",
@@ -649,7 +675,7 @@ struct LinearNode : torch::autograd::Function<LinearNode> {
     if (want_dx || want_dw || want_db) {
       const at::NoGradGuard no_grad;
       const at::ScalarType type = has_b ? db_type : go.scalar_type();
-      if (direct({&go, &saved[0], &w})) {
+      if (direct({&go, &saved[0], &saved[1], &w, &saved[3], &saved[4]})) {
         got = linear_backward(go, {saved[0], saved[1]}, w, {saved[3], saved[4]}, act, type, want_dx, want_dw, want_db);
       } else {
         refuse_tangents({&go, &saved[0], &w});
@@ -697,7 +723,7 @@ struct GatedNode : torch::autograd::Function<GatedNode> {
     if (!go.defined()) return variable_list(7);
     if (any) {
       const at::NoGradGuard no_grad;
-      if (direct({&go, &x, &wg, &wu, &wd})) {
+      if (direct({&go, &x, &saved[1], &wg, &wu, &wd, &saved[5], &saved[6], &saved[7], &saved[8]})) {
         got = gated_backward(go, {x, saved[1]}, wg, wu, wd, {saved[5], saved[6]}, {saved[7], saved[8]}, act, want_dx,
                              want_g || want_u, want_d);
       } else {
