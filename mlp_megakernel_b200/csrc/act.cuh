@@ -7,7 +7,7 @@
 //   gelu_tanh z s            s + z s (1 - s) p'(z),  s = sigmoid(p), p = 2 sqrt(2 / pi) (z + 0.044715 z^3),
 //             which is 0.5 z (1 + tanh(p / 2))
 //   softplus  max(z, 0) + log1p(e^-|z|)  (softplus.cuh's polynomial, 1/8 of fp16's half step)
-// A NaN stays a NaN.
+// relu's derivative is 0 at 0.  A NaN stays a NaN, in values and derivatives.
 #pragma once
 #include <type_traits>
 
@@ -36,7 +36,7 @@ __device__ __forceinline__ float act_value(float z) {
 template <int ACT>
 __device__ __forceinline__ float act_both(float z, float& slope) {
   if constexpr (ACT == kActRelu) {
-    slope = z > 0.0f ? 1.0f : 0.0f;
+    slope = z > 0.0f ? 1.0f : z <= 0.0f ? 0.0f : z;
     return z < 0.0f ? 0.0f : z;
   }
   if constexpr (ACT == kActSilu || ACT == kActGeluTanh) {
