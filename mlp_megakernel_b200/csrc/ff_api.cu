@@ -119,7 +119,7 @@ unsigned stream_blocks(K kern, int64_t work, const DevInfo& di, int dev) {
 }
 
 // Blocks of linear_dz_kernel over the rows: what the SMs hold at a time, each
-// thread with the 4 rows of a turn at least.
+// thread with 4 rows (two turns) at least.
 int dz_parts(int64_t rows, int width, int sm_count) {
   const int64_t across = ceil_to(width, 8 * kDzVectors);
   const int64_t want = std::max<int64_t>(1, static_cast<int64_t>(sm_count) * kDzBlocks / across);

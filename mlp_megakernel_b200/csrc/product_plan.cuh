@@ -38,6 +38,11 @@ struct ProductPlan {
 // the traffic of the shares (0.5 us a megabyte, written and read) and a second
 // kernel (4 us); dw of 20011 x 1024 x 2816: 136 whole, 119 so.  A kernel's beginning
 // and end are 5 us.
+//
+// The estimate compares tiles of one product; it has no term for the epilogue.  One
+// that keeps z, adds a residual and evaluates an activation beside a short reduction
+// takes longer than it says (5003 x 1000 x 2056 fp16, bias, gelu, residual, z kept:
+// 32 us, the estimate 18).
 inline ProductPlan product_plan(int64_t rows, int cols, int outputs, int out_cols, int nk, int pairs, bool may_split,
                                 bool may_narrow, bool may_any) {
   ProductPlan best;

@@ -163,7 +163,8 @@ int launch_few(const Product& c, const DevInfo& di, int dev, cudaStream_t st) {
 // in tiles of 256 rows: 128 x 4096 x 14336 31.3 and 33.1, 136 x 4096 x 8192 16.3 and
 // 20.4, 320 x 8192 x 2048 16.1 and 23.0, 1024 x 8192 x 1024 22.4 and 25.3, 2000 x 4096
 // x 512 17.5 and 19.7; 128 x 256 x 256 8.6 and 6.8, 256 x 4096 x 14336 49.3 and 34.2,
-// 512 x 8192 x 1024 21.3 and 17.9).  The rows must be read along the reduction, and a
+// 512 x 8192 x 1024 21.3 and 17.9; other epilogues were not measured for it, and
+// neither estimate knows of them).  The rows must be read along the reduction, and a
 // gate's checkpoint group is wider than a tile.
 inline bool few_rows(const Product& c, int sm_count) {
   if (c.rows > 2048 || c.a_mn || c.outputs > 1 || (c.epi == kEpiGated && c.keep_kind == kKeep8)) return false;

@@ -433,7 +433,7 @@ def fused_gated_mlp(x: Tensor, w_gate: Tensor, w_up: Tensor, w_down: Tensor, *, 
 
     ``x`` is fp16 or bf16 ``[..., in]``, ``w_gate`` and ``w_up`` ``[in, hidden]``,
     ``w_down`` ``[hidden, out]`` of its type (each contiguous or the transpose of
-    a contiguous tensor), ``residual`` ``[..., out]``.  Two kernels; the hidden
+    a contiguous tensor), ``residual`` ``[..., out]``.  Two products; the hidden
     values are rounded to x's type between them.  Differentiable in all of them:
     the backward forms both hidden gradients and the hidden values again in the
     epilogue of one product.  ``activation`` and ``activation_dtype`` as in
