@@ -67,9 +67,10 @@ __device__ __forceinline__ void store_kept4(T* p, const float (&f)[4]) {
 }
 __device__ __forceinline__ void load_fp8x4(const uint8_t* q, float scale, float (&f)[4]) {
   float2 v[2];
-  unpack_fp8<4>(load_raw<uint16_t, 2>(reinterpret_cast<const uint16_t*>(q)), v);
+  uint32_t w = *reinterpret_cast<const uint32_t*>(q);
+  if (scale >= kLargestScale) w = below_256(w);
+  unpack_fp8<4>(*reinterpret_cast<const Raw<uint16_t, 2>*>(&w), v);
   f[0] = v[0].x * scale, f[1] = v[0].y * scale, f[2] = v[1].x * scale, f[3] = v[1].y * scale;
-  clip_restored(f, scale);
 }
 
 template <class T, int EPI>

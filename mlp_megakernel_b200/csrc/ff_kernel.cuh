@@ -132,6 +132,10 @@ __device__ __forceinline__ float finite_max() {
   return sizeof(T) == 4 ? 3.402823466e+38f : std::is_same_v<T, __half> ? 65504.0f : 3.3895313892515355e+38f;
 }
 
+__device__ __forceinline__ float clip(float v, float most) {  // a NaN stays
+  return v > most ? most : v < -most ? -most : v;
+}
+
 // 16 values of the flat tensor at a time, whatever the width: they have one
 // scale (always where 16 divides the width, ONE: what follows costs 16384 x 8192
 // bf16 84 -> 100 us), or two (the rest of a group and the beginning of the next),
@@ -270,6 +274,11 @@ __global__ void __launch_bounds__(kStreamThreads, kDzBlocks) linear_dz_kernel(co
           }
         }
       }
+      if constexpr (ACT != kActNone && FP8) {
+#pragma unroll
+        for (int k = 0; k < AT_ONCE; ++k)
+          if (s[k] >= kLargestScale) zraw[k].x = below_256(zraw[k].x), zraw[k].y = below_256(zraw[k].y);
+      }
 #pragma unroll
       for (int k = 0; k < AT_ONCE; ++k) {
         const int64_t row = first + k * step;
@@ -283,7 +292,6 @@ __global__ void __launch_bounds__(kStreamThreads, kDzBlocks) linear_dz_kernel(co
             unpack_fp8<8>(*reinterpret_cast<const Raw<uint16_t, 4>*>(&x), f);
 #pragma unroll
             for (int e = 0; e < 4; ++e) z[2 * e] = f[e].x * s[k], z[2 * e + 1] = f[e].y * s[k];
-            clip_restored(z, s[k]);
           } else {
             unpack<T, 8>(*reinterpret_cast<const Raw<T, 8>*>(&zraw[k]), z);
           }

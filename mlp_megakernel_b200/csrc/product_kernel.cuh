@@ -150,7 +150,6 @@ __device__ __forceinline__ void widen_fp8x16(const uint32_t* w, float scale, flo
   unpack_fp8<16>(r, f);
 #pragma unroll
   for (int i = 0; i < 8; ++i) v[2 * i] = f[i].x * scale, v[2 * i + 1] = f[i].y * scale;
-  clip_restored(v, scale);
 }
 
 // v += bias[col ..]; a vector of 8 columns is inside the tensor or outside.
@@ -202,9 +201,9 @@ __device__ __forceinline__ float2 widen(uint32_t p) {
   return to_float2(*reinterpret_cast<const typename Pair<T>::type*>(&p));
 }
 // N values of a thread's row, from column `from` on, into and from its tile in
-// shared memory (as a TMA box with the row's swizzle has it).  KEPT: for a backward
-// pass to read (kept_pair).
-template <class T, int PITCH, bool KEPT = false, int N>
+// shared memory (as a TMA box with the row's swizzle has it).  CLIP: kept_pair for
+// each pair; tile_keep: for a backward pass to read.
+template <class T, int PITCH, bool CLIP = false, int N>
 __device__ __forceinline__ void tile_store(uint32_t tile, int lane, int from, const float (&v)[N]) {
 #pragma unroll
   for (int u = 0; u < N / 8; ++u) {
@@ -212,15 +211,15 @@ __device__ __forceinline__ void tile_store(uint32_t tile, int lane, int from, co
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const float a = v[8 * u + 2 * i], b = v[8 * u + 2 * i + 1];
-      if constexpr (KEPT) {
-        p[i] = kept_pair<T>(a, b);
-      } else {
-        const typename Pair<T>::type x = Pair<T>::round(a, b);
-        p[i] = *reinterpret_cast<const uint32_t*>(&x);
-      }
+      p[i] = CLIP ? kept_pair<T>(a, b) : round_pair<T>(a, b);
     }
     st_shared_v4(tile + swz_off<PITCH>(lane, from / 8 + u), p[0], p[1], p[2], p[3]);
   }
+}
+template <class T, int PITCH, int N>
+__device__ __forceinline__ void tile_keep(uint32_t tile, int lane, int from, const float (&v)[N]) {
+  if (some_round_to_infinity<T>(v)) tile_store<T, PITCH, true>(tile, lane, from, v);
+  else tile_store<T, PITCH>(tile, lane, from, v);
 }
 template <class T, int PITCH, int N>
 __device__ __forceinline__ void tile_load(uint32_t tile, int lane, int from, float (&v)[N]) {
@@ -551,7 +550,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kProductThreads, 1)
           if (p.bias) add_bias<T>(p, col, v);
           if (p.keep_kind == kKeep16) {
             const uint32_t tile = begin_tile();
-            tile_store<T, PITCH, true>(tile, lane, 0, v);
+            tile_keep<T, PITCH>(tile, lane, 0, v);
             end_tile(&p.keep[0], tile, col, row0);
           } else if (p.keep_kind == kKeep8 && row < p.rows) {
             store_fp8x32(p.q[0] + row * p.q_pitch + col, v, inv);
@@ -606,10 +605,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kProductThreads, 1)
           }
           if (p.keep_kind == kKeep16) {
             uint32_t tile = begin_tile();
-            tile_store<T, PITCH, true>(tile, lane, 0, g);
+            tile_keep<T, PITCH>(tile, lane, 0, g);
             end_tile(&p.keep[0], tile, col0, row0);
             tile = begin_tile();
-            tile_store<T, PITCH, true>(tile, lane, 0, u);
+            tile_keep<T, PITCH>(tile, lane, 0, u);
             end_tile(&p.keep[1], tile, col0, row0);
           }
           if constexpr (CHUNK == 32) {
@@ -639,6 +638,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kProductThreads, 1)
             }
             in_phase ^= 1;
           } else {
+            if (fmaxf(sg, su) >= kLargestScale) {
+#pragma unroll
+              for (int i = 0; i < 8; ++i) in0[i] = below_256(in0[i]), in1[i] = below_256(in1[i]);
+            }
             if (lane == 0) bulk_wait_group_read<0>();
             __syncwarp();
           }
@@ -670,7 +673,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kProductThreads, 1)
             tile_store<T, PITCH>(tile_g, lane, from, g);
             tile_store<T, PITCH>(tile_u, lane, from, d);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) h[from / 2 + i] = kept_pair<T>(u[2 * i], u[2 * i + 1]);
+            for (int i = 0; i < 8; ++i) h[from / 2 + i] = round_pair<T>(u[2 * i], u[2 * i + 1]);
+            if (some_round_to_infinity<T>(u)) {
+#pragma unroll
+              for (int i = 0; i < 8; ++i) h[from / 2 + i] = kept_pair<T>(u[2 * i], u[2 * i + 1]);
+            }
           }
           fence_proxy_async_smem();
           __syncwarp();
